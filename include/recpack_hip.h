@@ -538,6 +538,72 @@ int rphip_predict_topk_dist(rphip_ctx* ctx, rphip_comm* comm, const rphip_model*
  * (every pair of rounds gives every rank the same share of the lower triangle), item = that panel * panel + l % panel.  Otherwise
  * col_begin + l.  n_local_cols of the local columns are items (the rest is padding). */
 int rphip_model_dense_layout(const rphip_model* m, int64_t* n_local_cols, int64_t* panel, int32_t* world, int32_t* rank, int64_t* col_begin);
+
+/* ---- 4-bit matrices (MXFP4) and sampling: operators on caller-owned device arrays ---------------------------------------------------
+ * A compressed item-item model, its scores, an answer drawn from them (no counterpart in the reference, whose similarity matrices are
+ * float64 and whose answers are the best K).  Conventions of this section:
+ *  - `stream` is the hipStream_t the call is ordered on, NULL = the device's default stream; the context gives the device, the lock
+ *    and the error message (its own stream is not touched, the caller's current device is left as it was).  Nothing is allocated,
+ *    copied to the host or waited for: every call can be captured into a graph.  Scratch memory is the caller's (`workspace`, 256-byte
+ *    aligned; each captured graph and each stream needs its own while it may run);
+ *  - matrices are row-major with leading dimensions in ELEMENTS (codes and scales: bytes);
+ *  - element types of the dense operands: */
+#define RPHIP_F32 0
+#define RPHIP_F16 1
+#define RPHIP_BF16 2
+#define RPHIP_MXFP4 3 /* rphip_mxfp4_gemm_nt's A only */
+/* MXFP4 (OCP Microscaling Formats 1.0): blocks of 32 consecutive elements of a row share one scale byte s = 2^(s - 127) and hold E2M1
+ * elements {0, .5, 1, 1.5, 2, 3, 4, 6} with a sign.  codes: 16 bytes per block, the even element in the low nibble, ceil(cols / 32) blocks a
+ * row, base and leading dimension multiples of 16; codes beyond the last column are 0.  scales: one byte per block.
+ *   quantise: s - 127 = floor(log2(max |v| of the block)) - 2, at least -127; v / 2^(s - 127) rounded to nearest even, saturating at 6.
+ *             A block with an infinity or a NaN gets s = 255 and reads back as NaN; a block of zeros s = 0.
+ *             transpose != 0: x (rows x cols) is quantised DOWN its columns, codes and scales are those of the cols x rows transpose.
+ *   dequantize: the values, rounded once to out_type (float32 holds them exactly). */
+int rphip_mxfp4_quantize(rphip_ctx* ctx, void* stream, int64_t rows, int64_t cols, const void* x_dev, int32_t x_type, int64_t ldx, int32_t transpose,
+                         uint8_t* codes_dev, int64_t ld_codes, uint8_t* scales_dev, int64_t ld_scales);
+int rphip_mxfp4_dequantize(rphip_ctx* ctx, void* stream, int64_t rows, int64_t cols, const uint8_t* codes_dev, int64_t ld_codes,
+                           const uint8_t* scales_dev, int64_t ld_scales, void* out_dev, int32_t out_type, int64_t ld_out);
+/* C[M,N] = A[M,K] W[N,K]^T, W in MXFP4 with its blocks along K: dense rows (user profiles) against a quantised matrix, beside
+ * rphip_gemm_nt_f32.  A: RPHIP_F32 / F16 / BF16 with every product exact (A is cut into 3 / 2 / 1 bf16 planes, 2 bytes each per element of
+ * workspace), or RPHIP_MXFP4 (A_dev = codes, lda in bytes, a_scales; ignored otherwise).  Sums in float32, one rounding to c_type.
+ * M <= 65 535 * 16, N <= 2^28. */
+int rphip_mxfp4_gemm_nt_workspace(rphip_ctx* ctx, int64_t M, int64_t N, int64_t K, int32_t a_type, int64_t* bytes_out);
+int rphip_mxfp4_gemm_nt(rphip_ctx* ctx, void* stream, int64_t M, int64_t N, int64_t K, const void* A_dev, int32_t a_type, int64_t lda,
+                        const uint8_t* a_scales_dev, int64_t ld_a_scales, const uint8_t* w_codes_dev, int64_t ld_w, const uint8_t* w_scales_dev,
+                        int64_t ld_w_scales, void* C_dev, int32_t c_type, int64_t ldc, void* workspace_dev, int64_t workspace_bytes);
+/* Scores of histories against a quantised item-item matrix W (rows x cols, blocks along the columns): X @ similarity_matrix_
+ * (recpack/algorithms/base.py:248) for n_users CSR rows,
+ *   out[u, :] = sum over e in [indptr[u], indptr[u + 1]) of weights[e] * W[indices[e], :]     (weights NULL: 1)
+ * in float32, one rounding to out_type.  Repeated entries count as often as they stand; entries outside [0, rows) count nothing and
+ * indptr is read no further than nnz.  exclude_history != 0 (needs rows = cols; history removal of pipelines/pipeline.py:174-175): the
+ * history's own items get -inf.  item_keep (cols bytes, NULL = all): items with 0 get -inf (postprocessing/filters.py:58-101). */
+int rphip_mxfp4_scores(rphip_ctx* ctx, void* stream, int64_t n_users, int64_t nnz, const int32_t* indptr_dev, const int32_t* indices_dev,
+                       const float* weights_dev, int64_t rows, int64_t cols, const uint8_t* codes_dev, int64_t ld_codes, const uint8_t* scales_dev,
+                       int64_t ld_scales, int32_t exclude_history, const uint8_t* item_keep_dev, void* out_dev, int32_t out_type, int64_t ld_out);
+/* Items drawn from score rows.  Candidates of a row: index < length (lengths NULL: width), score neither NaN nor -inf; ranked by score
+ * descending, then index ascending; mass m_j = exp((score_j - best) / temperature).  Kept: the leading ranks that pass all of
+ *   top_k  the first k (0: all),
+ *   top_p  the shortest prefix with at least top_p of the mass of the first k,
+ *   min_p  m_j >= min_p (the best one has 1).
+ * Draw d = 0 .. draws - 1 is WITHOUT replacement: of the kept and not yet drawn, in rank order, the first whose cumulative mass
+ * exceeds u[d] times their total; prob = its share of that total (the propensity of the draw).  u in [0, 1) (values outside are moved to
+ * the nearest end, NaN to 0).  temperature 0: the first k in rank order, prob 1; top_p, min_p and u are not used.
+ * Out: idx (index, or ids[row, index]; -1 where nothing was left), prob (0 there), nnz = number drawn (may be NULL): rows x draws and
+ * rows, contiguous.  Masses are summed in 64 bits; the result does not depend on the launch.
+ * params: scalars, or one value per row where a device array is given (values out of range are moved into it; top_k_dev needs top_k > 0 as
+ * its upper bound, entries <= 0 mean that bound).  draws > 1 needs min(top_k, width) <= 1024. */
+typedef struct rphip_sample_params {
+  float temperature, top_p, min_p;
+  int32_t top_k;
+  const float* temperature_dev;
+  const float* top_p_dev;
+  const float* min_p_dev;
+  const int32_t* top_k_dev;
+} rphip_sample_params;
+int rphip_sample_workspace(rphip_ctx* ctx, int64_t rows, int64_t width, int32_t draws, int32_t top_k, int64_t* bytes_out);
+int rphip_sample(rphip_ctx* ctx, void* stream, int64_t rows, int64_t width, const void* scores_dev, int32_t type, int64_t ld, const int32_t* lengths_dev,
+                 const int32_t* ids_dev, int64_t ld_ids, int32_t draws, const float* u_dev, int64_t ld_u, const rphip_sample_params* params,
+                 int32_t* idx_dev, float* prob_dev, int32_t* nnz_dev, void* workspace_dev, int64_t workspace_bytes);
 #ifdef __cplusplus
 }
 #endif

@@ -127,6 +127,20 @@ PROTOTYPES = {
     "rphip_predict_topk_dist": (C.c_int, [_p, _p, _p, _p, _i32, _i32, C.POINTER(_i64), C.POINTER(_i64), _p, _p, _p]),
     "rphip_comm_selftest": (C.c_int, [_p, _p, _i32, _i64, C.POINTER(_i64), C.POINTER(_f64)]),
 }
+class SampleParams(C.Structure):
+    _fields_ = [("temperature", C.c_float), ("top_p", C.c_float), ("min_p", C.c_float), ("top_k", C.c_int32), ("temperature_dev", C.c_void_p),
+                ("top_p_dev", C.c_void_p), ("min_p_dev", C.c_void_p), ("top_k_dev", C.c_void_p)]
+
+
+PROTOTYPES.update({
+    "rphip_mxfp4_quantize": (C.c_int, [_p, _p, _i64, _i64, _p, _i32, _i64, _i32, _p, _i64, _p, _i64]),
+    "rphip_mxfp4_dequantize": (C.c_int, [_p, _p, _i64, _i64, _p, _i64, _p, _i64, _p, _i32, _i64]),
+    "rphip_mxfp4_gemm_nt_workspace": (C.c_int, [_p, _i64, _i64, _i64, _i32, C.POINTER(_i64)]),
+    "rphip_mxfp4_gemm_nt": (C.c_int, [_p, _p, _i64, _i64, _i64, _p, _i32, _i64, _p, _i64, _p, _i64, _p, _i64, _p, _i32, _i64, _p, _i64]),
+    "rphip_mxfp4_scores": (C.c_int, [_p, _p, _i64, _i64, _p, _p, _p, _i64, _i64, _p, _i64, _p, _i64, _i32, _p, _p, _i32, _i64]),
+    "rphip_sample_workspace": (C.c_int, [_p, _i64, _i64, _i32, _i32, C.POINTER(_i64)]),
+    "rphip_sample": (C.c_int, [_p, _p, _i64, _i64, _p, _i32, _i64, _p, _p, _i64, _i32, _p, _i64, C.POINTER(SampleParams), _p, _p, _p, _p, _i64]),
+})
 # include/recpack_hip_diag.h: measuring instruments and test hooks (tools/, tests/), not the drop-in boundary
 DIAG_PROTOTYPES = {
     "rphip_model_adopt_gather": (C.c_int, [_p, _p]),

@@ -1,0 +1,292 @@
+// MXFP4 matrices (microscaled 4-bit floating point): quantisation of rows or columns, reading back, and the scores of histories
+// against a quantised item-item matrix.  C ABI: include/recpack_hip.h, section "4-bit matrices".
+#include "rp_ops.h"
+
+#include <algorithm>
+
+int rp_mx_check(const char* who, int64_t rows, int64_t cols, const uint8_t* codes, int64_t ld_codes, const uint8_t* scales, int64_t ld_scales) {
+  const int64_t nb = rp_cdiv(cols, RP_MX);
+  if (rows < 0 || cols < 0 || rows > INT32_MAX || cols > INT32_MAX) RP_FAIL(RPHIP_EINVAL, "%s: %lld x %lld is no matrix size", who, (long long)rows, (long long)cols);
+  if (rows == 0 || cols == 0) return RPHIP_OK;
+  if (!codes || !scales) RP_FAIL(RPHIP_EINVAL, "%s: NULL codes or scales", who);
+  if (((uintptr_t)codes & 15) || (ld_codes & 15)) RP_FAIL(RPHIP_EINVAL, "%s: codes and their leading dimension must be multiples of 16 bytes", who);
+  if (ld_codes < nb * 16 || ld_scales < nb)
+    RP_FAIL(RPHIP_EINVAL, "%s: leading dimensions %lld / %lld bytes are too small for %lld columns (%lld blocks)", who, (long long)ld_codes, (long long)ld_scales,
+            (long long)cols, (long long)nb);
+  return RPHIP_OK;
+}
+
+// ---- quantise --------------------------------------------------------------------------------------------------------------------
+// Four lanes per block of 32, eight elements each: the block's largest magnitude is two exchanges inside the quad.  Bound by HBM
+// (4 or 2 bytes read, 0.53 written per element).
+template <class T>
+__global__ __launch_bounds__(256) void k_mx_quantize(const T* __restrict__ x, int64_t ldx, int rows, int cols, int nb, uint8_t* __restrict__ codes,
+                                                     int64_t ldc, uint8_t* __restrict__ scales, int64_t lds) {
+  const int upr = nb * 4;  // units (eight elements) of a row
+  const int64_t unit = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  const int64_t r64 = unit / upr;
+  if (r64 >= rows) return;  // (upr is a multiple of 4: a quad leaves together)
+  const int q = (int)(unit - r64 * upr);
+  const T* p = x + r64 * ldx + (int64_t)q * 8;
+  float v[8];
+  if (q * 8 + 8 <= cols) {
+    const rp_vec<T, 8> t = rp_load_vec<T, 8>(p);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = rp_to_f32(t.v[i]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = q * 8 + i < cols ? rp_to_f32(p[i]) : 0.0f;
+  }
+  uint32_t a = 0;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) a = max(a, __float_as_uint(v[i]) & 0x7fffffffu);  // as integers: NaN above Inf above every number
+  a = max(a, (uint32_t)__shfl_xor((int)a, 1));
+  a = max(a, (uint32_t)__shfl_xor((int)a, 2));
+  const uint32_t byte = rp_mx_scale_byte(a);
+  const uint32_t w = byte == 255u ? 0u : rp_mx_pack8(v, rp_mx_scale(byte));
+  *(uint32_t*)(codes + r64 * ldc + (int64_t)q * 4) = w;
+  if ((q & 3) == 0) scales[r64 * lds + (q >> 2)] = (uint8_t)byte;
+}
+
+// The transpose: out row = column of x, blocks down the rows.  A wave takes 32 rows x 64 columns (a lane: one column, its block in
+// registers; loads of a row are contiguous over the lanes); eight waves take 256 rows, so that a line of 128 code bytes is written
+// whole, through LDS (16-byte pieces scattered over the lines otherwise).
+constexpr int MXT_WAVES = 8, MXT_COLS = 64, MXT_LD = MXT_WAVES * 4 + 1;  // (LDS words of a column, odd: conflict-free either way)
+template <class T>
+__global__ __launch_bounds__(MXT_WAVES * 64) void k_mx_quantize_t(const T* __restrict__ x, int64_t ldx, int rows, int cols, int nb, uint8_t* __restrict__ codes,
+                                                                  int64_t ldc, uint8_t* __restrict__ scales, int64_t lds) {
+  __shared__ uint32_t tile[MXT_COLS * MXT_LD];
+  __shared__ uint8_t sbyte[MXT_COLS * MXT_WAVES];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int b0 = blockIdx.y * MXT_WAVES;          // first block (of 32 rows)
+  const int c0 = blockIdx.x * MXT_COLS, c = c0 + lane;
+  const int r0 = (b0 + wave) * RP_MX;
+  if (r0 < rows) {
+    float v[32];
+    const T* p = x + (int64_t)r0 * ldx + c;
+    if (r0 + 32 <= rows && c < cols) {
+#pragma unroll
+      for (int i = 0; i < 32; ++i) v[i] = rp_to_f32(p[i * ldx]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 32; ++i) v[i] = (r0 + i < rows && c < cols) ? rp_to_f32(p[i * ldx]) : 0.0f;
+    }
+    uint32_t a = 0;
+#pragma unroll
+    for (int i = 0; i < 32; ++i) a = max(a, __float_as_uint(v[i]) & 0x7fffffffu);
+    const uint32_t byte = rp_mx_scale_byte(a);
+    const float s = rp_mx_scale(byte);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) tile[lane * MXT_LD + wave * 4 + i] = byte == 255u ? 0u : rp_mx_pack8(v + 8 * i, s);
+    sbyte[lane * MXT_WAVES + wave] = (uint8_t)byte;
+  }
+  __syncthreads();
+  // thread: one block (16 bytes) of one column, eight neighbouring lanes write one line
+  const int col = threadIdx.x >> 3, b = threadIdx.x & 7;
+  if (c0 + col < cols && b0 + b < nb) {
+    uint4 w;
+    w.x = tile[col * MXT_LD + b * 4];
+    w.y = tile[col * MXT_LD + b * 4 + 1];
+    w.z = tile[col * MXT_LD + b * 4 + 2];
+    w.w = tile[col * MXT_LD + b * 4 + 3];
+    *(uint4*)(codes + (int64_t)(c0 + col) * ldc + (int64_t)(b0 + b) * 16) = w;
+    scales[(int64_t)(c0 + col) * lds + b0 + b] = sbyte[col * MXT_WAVES + b];
+  }
+}
+
+static int mx_type_ok(const char* who, int32_t type) {
+  if (type != RPHIP_F32 && type != RPHIP_F16 && type != RPHIP_BF16) RP_FAIL(RPHIP_EINVAL, "%s: element type %d: RPHIP_F32, RPHIP_F16 or RPHIP_BF16 expected", who, type);
+  return RPHIP_OK;
+}
+
+extern "C" int rphip_mxfp4_quantize(rphip_ctx* ctx, void* stream, int64_t rows, int64_t cols, const void* x_dev, int32_t x_type, int64_t ldx, int32_t transpose,
+                                    uint8_t* codes_dev, int64_t ld_codes, uint8_t* scales_dev, int64_t ld_scales) {
+  rp_op_scope scope;
+  RP_TRY(mx_type_ok("mxfp4_quantize", x_type));
+  RP_TRY(rp_mx_check("mxfp4_quantize", transpose ? cols : rows, transpose ? rows : cols, codes_dev, ld_codes, scales_dev, ld_scales));
+  if (rows == 0 || cols == 0) return RPHIP_OK;
+  if (!x_dev) RP_FAIL(RPHIP_EINVAL, "mxfp4_quantize: x is NULL");
+  if ((uintptr_t)x_dev % rp_type_bytes(x_type)) RP_FAIL(RPHIP_EINVAL, "mxfp4_quantize: x is not aligned to its elements");
+  if (ldx < cols) RP_FAIL(RPHIP_EINVAL, "mxfp4_quantize: ldx %lld < cols %lld", (long long)ldx, (long long)cols);
+  if (transpose && cols > ((int64_t)1 << 28)) RP_FAIL(RPHIP_ELIMIT, "mxfp4_quantize: the transpose takes at most 2^28 columns");
+  RP_TRY(scope.enter(ctx));
+  const int nb = (int)rp_cdiv(transpose ? rows : cols, RP_MX);
+  return rp_by_type(x_type, [&](auto tag) -> int {
+    using T = typename decltype(tag)::T;
+    if (transpose) {
+      const int64_t gy = rp_cdiv(nb, MXT_WAVES), gx = rp_cdiv(cols, MXT_COLS);
+      // (grid.y is 16 bits wide: 65 535 * 256 rows; larger inputs go in strips of rows)
+      for (int64_t y0 = 0; y0 < gy; y0 += 65535) {
+        const int64_t r0 = y0 * MXT_WAVES * RP_MX, b0 = y0 * MXT_WAVES;
+        k_mx_quantize_t<T><<<dim3((unsigned)gx, (unsigned)std::min<int64_t>(gy - y0, 65535)), MXT_WAVES * 64, 0, (hipStream_t)stream>>>(
+            (const T*)x_dev + r0 * ldx, ldx, (int)(rows - r0), (int)cols, (int)(nb - b0), codes_dev + b0 * 16, ld_codes, scales_dev + b0, ld_scales);
+        RP_LAUNCHED();
+      }
+    } else {
+      // strips of rows keep a launch below 2^32 threads
+      const int64_t strip = std::max<int64_t>(1, ((int64_t)1 << 31) / ((int64_t)nb * 4));
+      for (int64_t r0 = 0; r0 < rows; r0 += strip) {
+        const int64_t n = std::min(strip, rows - r0);
+        k_mx_quantize<T><<<(unsigned)rp_cdiv(n * nb * 4, 256), 256, 0, (hipStream_t)stream>>>((const T*)x_dev + r0 * ldx, ldx, (int)n, (int)cols, nb,
+                                                                                            codes_dev + r0 * ld_codes, ld_codes, scales_dev + r0 * ld_scales, ld_scales);
+        RP_LAUNCHED();
+      }
+    }
+    return RPHIP_OK;
+  });
+}
+
+// ---- reading back ------------------------------------------------------------------------------------------------------------------
+template <class T>
+__global__ __launch_bounds__(256) void k_mx_dequantize(const uint8_t* __restrict__ codes, int64_t ldc, const uint8_t* __restrict__ scales, int64_t lds, int rows,
+                                                       int cols, int upr, T* __restrict__ out, int64_t ldo) {
+  const int64_t unit = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  const int64_t r = unit / upr;
+  if (r >= rows) return;
+  const int q = (int)(unit - r * upr);
+  const uint32_t w = *(const uint32_t*)(codes + r * ldc + (int64_t)q * 4);
+  float v[8];
+  rp_mx_unpack8(w, rp_mx_scale(scales[r * lds + (q >> 2)]), v);
+  T* p = out + r * ldo + (int64_t)q * 8;
+  if (q * 8 + 8 <= cols) {
+    rp_vec<T, 8> t;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) t.v[i] = rp_from_f32<T>(v[i]);
+    rp_store_vec<T, 8>(p, t);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (q * 8 + i < cols) p[i] = rp_from_f32<T>(v[i]);
+  }
+}
+
+extern "C" int rphip_mxfp4_dequantize(rphip_ctx* ctx, void* stream, int64_t rows, int64_t cols, const uint8_t* codes_dev, int64_t ld_codes, const uint8_t* scales_dev,
+                                      int64_t ld_scales, void* out_dev, int32_t out_type, int64_t ld_out) {
+  rp_op_scope scope;
+  RP_TRY(mx_type_ok("mxfp4_dequantize", out_type));
+  RP_TRY(rp_mx_check("mxfp4_dequantize", rows, cols, codes_dev, ld_codes, scales_dev, ld_scales));
+  if (rows == 0 || cols == 0) return RPHIP_OK;
+  if (!out_dev) RP_FAIL(RPHIP_EINVAL, "mxfp4_dequantize: out is NULL");
+  if ((uintptr_t)out_dev % rp_type_bytes(out_type)) RP_FAIL(RPHIP_EINVAL, "mxfp4_dequantize: out is not aligned to its elements");
+  if (ld_out < cols) RP_FAIL(RPHIP_EINVAL, "mxfp4_dequantize: ld_out %lld < cols %lld", (long long)ld_out, (long long)cols);
+  RP_TRY(scope.enter(ctx));
+  const int upr = (int)rp_cdiv(cols, 8);
+  return rp_by_type(out_type, [&](auto tag) -> int {
+    using T = typename decltype(tag)::T;
+    const int64_t strip = std::max<int64_t>(1, ((int64_t)1 << 31) / upr);
+    for (int64_t r0 = 0; r0 < rows; r0 += strip) {
+      const int64_t n = std::min(strip, rows - r0);
+      k_mx_dequantize<T><<<(unsigned)rp_cdiv(n * upr, 256), 256, 0, (hipStream_t)stream>>>(codes_dev + r0 * ld_codes, ld_codes, scales_dev + r0 * ld_scales, ld_scales,
+                                                                                         (int)n, (int)cols, upr, (T*)out_dev + r0 * ld_out, ld_out);
+      RP_LAUNCHED();
+    }
+    return RPHIP_OK;
+  });
+}
+
+// ---- scores of histories -----------------------------------------------------------------------------------------------------------
+// out[u, :] = sum over the entries e of user u of w_e * W[idx_e, :], in f32, in the history's order: the rows of a history are
+// contiguous, their blocks run along the output, so a lane owns one block of 32 columns (16 code bytes, one scale) of every row and
+// keeps its 32 sums in registers.  One wave per (user, 2048 columns).
+constexpr int MXS_COLS = 64 * RP_MX;
+template <class T, bool WEIGHTED>
+__global__ __launch_bounds__(64) void k_mx_scores(const int32_t* __restrict__ indptr, const int32_t* __restrict__ indices, const float* __restrict__ weights, int64_t nnz,
+                                                  int rows, int cols, int nb, const uint8_t* __restrict__ codes, int64_t ldc, const uint8_t* __restrict__ scales,
+                                                  int64_t lds, int exclude, const uint8_t* __restrict__ keep, T* __restrict__ out, int64_t ldo, int64_t user0) {
+  __shared__ uint32_t drop[64];  // bit c of word l: column 32 l + c of the tile gets -inf
+  const int lane = threadIdx.x;
+  const int64_t u = user0 + blockIdx.y;
+  const int b = blockIdx.x * 64 + lane;  // this lane's block of columns
+  const int c0 = blockIdx.x * MXS_COLS;
+  const bool mine = b < nb;
+  drop[lane] = 0;
+  __syncthreads();
+  float acc[32];
+#pragma unroll
+  for (int i = 0; i < 32; ++i) acc[i] = 0.0f;
+  const int64_t e1 = min((int64_t)indptr[u + 1], nnz);
+  for (int64_t e0 = max((int64_t)indptr[u], (int64_t)0); e0 < e1; e0 += 64) {
+    const int n = (int)min((int64_t)64, e1 - e0);
+    int idx = -1;
+    float wgt = 0.0f;
+    if (lane < n) {
+      idx = indices[e0 + lane];
+      if ((unsigned)idx >= (unsigned)rows) idx = -1;
+      if (WEIGHTED) wgt = weights[e0 + lane];
+      if (exclude && idx >= c0 && idx < c0 + MXS_COLS) atomicOr(&drop[(idx - c0) >> 5], 1u << (idx & 31));
+    }
+    for (int k = 0; k < n; ++k) {
+      const int row = __builtin_amdgcn_readlane(idx, k);
+      if (row < 0) continue;
+      uint4 w = make_uint4(0, 0, 0, 0);
+      uint32_t byte = 0;
+      if (mine) {
+        w = *(const uint4*)(codes + (int64_t)row * ldc + (int64_t)b * 16);
+        byte = scales[(int64_t)row * lds + b];
+      }
+      const float s = rp_mx_scale(byte);
+      const float f = WEIGHTED ? __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(wgt), k)) : 1.0f;
+      float v[32];
+      rp_mx_unpack8(w.x, s, v);
+      rp_mx_unpack8(w.y, s, v + 8);
+      rp_mx_unpack8(w.z, s, v + 16);
+      rp_mx_unpack8(w.w, s, v + 24);
+#pragma unroll
+      for (int i = 0; i < 32; ++i) acc[i] = WEIGHTED ? fmaf(f, v[i], acc[i]) : acc[i] + v[i];
+    }
+  }
+  __syncthreads();
+  if (!mine) return;
+  uint32_t m = drop[lane];
+  const int c = b * RP_MX;
+  const int left = min(RP_MX, cols - c);
+  if (keep)
+    for (int i = 0; i < left; ++i) m |= keep[c + i] ? 0u : 1u << i;
+  T* p = out + u * ldo + c;
+#pragma unroll
+  for (int i = 0; i < 32; ++i)
+    if ((m >> i) & 1) acc[i] = -INFINITY;
+  if (left == RP_MX) {
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      rp_vec<T, 8> t;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) t.v[i] = rp_from_f32<T>(acc[g * 8 + i]);
+      rp_store_vec<T, 8>(p + g * 8, t);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 32; ++i)
+      if (i < left) p[i] = rp_from_f32<T>(acc[i]);
+  }
+}
+
+extern "C" int rphip_mxfp4_scores(rphip_ctx* ctx, void* stream, int64_t n_users, int64_t nnz, const int32_t* indptr_dev, const int32_t* indices_dev,
+                                  const float* weights_dev, int64_t rows, int64_t cols, const uint8_t* codes_dev, int64_t ld_codes, const uint8_t* scales_dev,
+                                  int64_t ld_scales, int32_t exclude_history, const uint8_t* item_keep_dev, void* out_dev, int32_t out_type, int64_t ld_out) {
+  rp_op_scope scope;
+  RP_TRY(mx_type_ok("mxfp4_scores", out_type));
+  if (n_users < 0 || nnz < 0 || n_users > INT32_MAX - 1 || nnz > INT32_MAX) RP_FAIL(RPHIP_EINVAL, "mxfp4_scores: %lld users, %lld entries", (long long)n_users, (long long)nnz);
+  RP_TRY(rp_mx_check("mxfp4_scores", rows, cols, codes_dev, ld_codes, scales_dev, ld_scales));
+  if (exclude_history && rows != cols) RP_FAIL(RPHIP_EINVAL, "mxfp4_scores: exclude_history needs a square matrix, got %lld x %lld", (long long)rows, (long long)cols);
+  if (n_users == 0 || cols == 0) return RPHIP_OK;
+  if (!indptr_dev || !out_dev || (nnz > 0 && !indices_dev)) RP_FAIL(RPHIP_EINVAL, "mxfp4_scores: NULL argument");
+  if ((uintptr_t)out_dev % rp_type_bytes(out_type)) RP_FAIL(RPHIP_EINVAL, "mxfp4_scores: out is not aligned to its elements");
+  if (ld_out < cols) RP_FAIL(RPHIP_EINVAL, "mxfp4_scores: ld_out %lld < cols %lld", (long long)ld_out, (long long)cols);
+  RP_TRY(scope.enter(ctx));
+  const int nb = (int)rp_cdiv(cols, RP_MX), tiles = (int)rp_cdiv(nb, 64);
+  return rp_by_type(out_type, [&](auto tag) -> int {
+    using T = typename decltype(tag)::T;
+    for (int64_t u0 = 0; u0 < n_users; u0 += 65535) {
+      const dim3 grid(tiles, (unsigned)std::min<int64_t>(65535, n_users - u0));
+      if (weights_dev)
+        k_mx_scores<T, true><<<grid, 64, 0, (hipStream_t)stream>>>(indptr_dev, indices_dev, weights_dev, nnz, (int)rows, (int)cols, nb, codes_dev, ld_codes, scales_dev,
+                                                                   ld_scales, exclude_history, item_keep_dev, (T*)out_dev, ld_out, u0);
+      else
+        k_mx_scores<T, false><<<grid, 64, 0, (hipStream_t)stream>>>(indptr_dev, indices_dev, nullptr, nnz, (int)rows, (int)cols, nb, codes_dev, ld_codes, scales_dev,
+                                                                    ld_scales, exclude_history, item_keep_dev, (T*)out_dev, ld_out, u0);
+      RP_LAUNCHED();
+    }
+    return RPHIP_OK;
+  });
+}
