@@ -3,6 +3,7 @@
 #include "rp_ops.h"
 
 #include <algorithm>
+#include <type_traits>
 
 int rp_mx_check(const char* who, int64_t rows, int64_t cols, const uint8_t* codes, int64_t ld_codes, const uint8_t* scales, int64_t ld_scales) {
   const int64_t nb = rp_cdiv(cols, RP_MX);
@@ -185,25 +186,30 @@ extern "C" int rphip_mxfp4_dequantize(rphip_ctx* ctx, void* stream, int64_t rows
 }
 
 // ---- scores of histories -----------------------------------------------------------------------------------------------------------
-// out[u, :] = sum over the entries e of user u of w_e * W[idx_e, :], in f32, in the history's order: the rows of a history are
-// contiguous, their blocks run along the output, so a lane owns one block of 32 columns (16 code bytes, one scale) of every row and
-// keeps its 32 sums in registers.  One wave per (user, 2048 columns).
+// out[u, :] = sum over the entries e of user u of w_e * W[idx_e, :], in f32: the rows of a history are contiguous and their blocks run along
+// the output, so a lane owns one block of 32 columns (16 code bytes, one scale) of every row and keeps its 32 sums in registers: per
+// element half a conversion and one add.  A workgroup takes (user, 2048 columns); its waves take groups of four entries in turn and
+// add their sums up in wave order (the result does not depend on the launch).  Four rows are in flight while four are added.
+// Workgroups run through all users of a column tile before the next one: the rows' pieces of one tile (1 KB each) stay in the caches.
 constexpr int MXS_COLS = 64 * RP_MX;
-template <class T, bool WEIGHTED>
-__global__ __launch_bounds__(64) void k_mx_scores(const int32_t* __restrict__ indptr, const int32_t* __restrict__ indices, const float* __restrict__ weights, int64_t nnz,
-                                                  int rows, int cols, int nb, const uint8_t* __restrict__ codes, int64_t ldc, const uint8_t* __restrict__ scales,
-                                                  int64_t lds, int exclude, const uint8_t* __restrict__ keep, T* __restrict__ out, int64_t ldo, int64_t user0) {
+template <class T, bool WEIGHTED, int WAVES>
+__global__ __launch_bounds__(64 * WAVES) void k_mx_scores(const int32_t* __restrict__ indptr, const int32_t* __restrict__ indices, const float* __restrict__ weights,
+                                                          int64_t nnz, int rows, int cols, int nb, const uint8_t* __restrict__ codes, int64_t ldc,
+                                                          const uint8_t* __restrict__ scales, int64_t lds, int exclude, const uint8_t* __restrict__ keep,
+                                                          T* __restrict__ out, int64_t ldo, int64_t user0) {
   __shared__ uint32_t drop[64];  // bit c of word l: column 32 l + c of the tile gets -inf
-  const int lane = threadIdx.x;
-  const int64_t u = user0 + blockIdx.y;
-  const int b = blockIdx.x * 64 + lane;  // this lane's block of columns
-  const int c0 = blockIdx.x * MXS_COLS;
-  const bool mine = b < nb;
-  drop[lane] = 0;
+  __shared__ float sums[WAVES > 1 ? WAVES * 32 * 64 : 1];
+  const int lane = threadIdx.x & 63, wave = WAVES > 1 ? __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) : 0;
+  const int64_t u = user0 + blockIdx.x;
+  const int c0 = blockIdx.y * MXS_COLS;
+  const int b = min(blockIdx.y * 64 + lane, nb - 1);  // this lane's block of columns (lanes beyond the row repeat the last one)
+  if (wave == 0) drop[lane] = 0;
   __syncthreads();
   float acc[32];
 #pragma unroll
   for (int i = 0; i < 32; ++i) acc[i] = 0.0f;
+  const uint8_t* cbase = codes + (int64_t)b * 16;
+  const uint8_t* sbase = scales + b;
   const int64_t e1 = min((int64_t)indptr[u + 1], nnz);
   for (int64_t e0 = max((int64_t)indptr[u], (int64_t)0); e0 < e1; e0 += 64) {
     const int n = (int)min((int64_t)64, e1 - e0);
@@ -213,51 +219,111 @@ __global__ __launch_bounds__(64) void k_mx_scores(const int32_t* __restrict__ in
       idx = indices[e0 + lane];
       if ((unsigned)idx >= (unsigned)rows) idx = -1;
       if (WEIGHTED) wgt = weights[e0 + lane];
-      if (exclude && idx >= c0 && idx < c0 + MXS_COLS) atomicOr(&drop[(idx - c0) >> 5], 1u << (idx & 31));
+      if (exclude && wave == 0 && idx >= c0 && idx < c0 + MXS_COLS) atomicOr(&drop[(idx - c0) >> 5], 1u << (idx & 31));
     }
-    for (int k = 0; k < n; ++k) {
-      const int row = __builtin_amdgcn_readlane(idx, k);
-      if (row < 0) continue;
-      uint4 w = make_uint4(0, 0, 0, 0);
-      uint32_t byte = 0;
-      if (mine) {
-        w = *(const uint4*)(codes + (int64_t)row * ldc + (int64_t)b * 16);
-        byte = scales[(int64_t)row * lds + b];
-      }
-      const float s = rp_mx_scale(byte);
-      const float f = WEIGHTED ? __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(wgt), k)) : 1.0f;
-      float v[32];
-      rp_mx_unpack8(w.x, s, v);
-      rp_mx_unpack8(w.y, s, v + 8);
-      rp_mx_unpack8(w.z, s, v + 16);
-      rp_mx_unpack8(w.w, s, v + 24);
+    // entries that count move to the front, in order
+    const unsigned long long good = __ballot(idx >= 0);
+    const int m = (int)__popcll(good);
+    if (m < n) {
+      const int dst = idx >= 0 ? (int)__popcll(good & ((1ull << lane) - 1ull)) : 63;
+      const int keep_idx = __builtin_amdgcn_ds_permute(dst * 4, idx);
+      const int keep_w = __builtin_amdgcn_ds_permute(dst * 4, __float_as_int(wgt));
+      idx = keep_idx;
+      wgt = __int_as_float(keep_w);
+    }
+    uint4 w[2][4];
+    uint32_t sc[2][4];
+    auto fetch = [&](auto tag, int k) __attribute__((always_inline)) {  // rows k .. k + 3 (past the end: the last one again)
+      constexpr int S = decltype(tag)::value;
 #pragma unroll
-      for (int i = 0; i < 32; ++i) acc[i] = WEIGHTED ? fmaf(f, v[i], acc[i]) : acc[i] + v[i];
+      for (int i = 0; i < 4; ++i) {
+        const int64_t row = __builtin_amdgcn_readlane(idx, min(k + i, m - 1));
+        w[S][i] = *(const uint4*)(cbase + row * ldc);
+        sc[S][i] = sbase[row * lds];
+      }
+    };
+    auto add = [&](auto tag, int k) __attribute__((always_inline)) {
+      constexpr int S = decltype(tag)::value;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        if (k + i >= m) break;
+        const float s = rp_mx_scale(sc[S][i]);
+        const float f = WEIGHTED ? __int_as_float(__builtin_amdgcn_readlane(__float_as_int(wgt), k + i)) : 1.0f;
+        const uint32_t q[4] = {w[S][i].x, w[S][i].y, w[S][i].z, w[S][i].w};
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+          float v[8];
+          rp_mx_unpack8(q[g], s, v);
+#pragma unroll
+          for (int j = 0; j < 8; ++j) acc[g * 8 + j] = WEIGHTED ? fmaf(f, v[j], acc[g * 8 + j]) : acc[g * 8 + j] + v[j];
+        }
+      }
+    };
+    constexpr int STEP = 4 * WAVES;
+    int k = wave * 4;
+    if (k < m) {
+      fetch(std::integral_constant<int, 0>{}, k);
+      for (; k < m; k += 2 * STEP) {
+        fetch(std::integral_constant<int, 1>{}, k + STEP);
+        add(std::integral_constant<int, 0>{}, k);
+        fetch(std::integral_constant<int, 0>{}, k + 2 * STEP);
+        add(std::integral_constant<int, 1>{}, k + STEP);
+      }
     }
   }
-  __syncthreads();
-  if (!mine) return;
-  uint32_t m = drop[lane];
+  const bool mine = blockIdx.y * 64 + lane < nb;
   const int c = b * RP_MX;
   const int left = min(RP_MX, cols - c);
-  if (keep)
-    for (int i = 0; i < left; ++i) m |= keep[c + i] ? 0u : 1u << i;
   T* p = out + u * ldo + c;
+  if constexpr (WAVES > 1) {
+    // a lane of wave w ends with the columns [w * PC, (w + 1) * PC) of its block
+    constexpr int PC = 32 / WAVES;
 #pragma unroll
-  for (int i = 0; i < 32; ++i)
-    if ((m >> i) & 1) acc[i] = -INFINITY;
-  if (left == RP_MX) {
+    for (int i = 0; i < 32; ++i) sums[(wave * 32 + i) * 64 + lane] = acc[i];
+    __syncthreads();
+    if (!mine) return;
+    const uint32_t gone = drop[lane];
+    float v[PC];
 #pragma unroll
-    for (int g = 0; g < 4; ++g) {
-      rp_vec<T, 8> t;
+    for (int i = 0; i < PC; ++i) {
+      const int col = wave * PC + i;
+      v[i] = 0.0f;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) t.v[i] = rp_from_f32<T>(acc[g * 8 + i]);
-      rp_store_vec<T, 8>(p + g * 8, t);
+      for (int o = 0; o < WAVES; ++o) v[i] += sums[(o * 32 + col) * 64 + lane];
+      if (((gone >> col) & 1) || (keep && col < left && !keep[c + col])) v[i] = -INFINITY;
+    }
+    if (left == RP_MX) {
+      rp_vec<T, PC> t;
+#pragma unroll
+      for (int i = 0; i < PC; ++i) t.v[i] = rp_from_f32<T>(v[i]);
+      rp_store_vec<T, PC>(p + wave * PC, t);
+    } else {
+#pragma unroll
+      for (int i = 0; i < PC; ++i)
+        if (wave * PC + i < left) p[wave * PC + i] = rp_from_f32<T>(v[i]);
     }
   } else {
+    __syncthreads();
+    if (!mine) return;
+    uint32_t gone = drop[lane];
+    if (keep)
+      for (int i = 0; i < left; ++i) gone |= keep[c + i] ? 0u : 1u << i;
 #pragma unroll
     for (int i = 0; i < 32; ++i)
-      if (i < left) p[i] = rp_from_f32<T>(acc[i]);
+      if ((gone >> i) & 1) acc[i] = -INFINITY;
+    if (left == RP_MX) {
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        rp_vec<T, 8> t;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) t.v[i] = rp_from_f32<T>(acc[g * 8 + i]);
+        rp_store_vec<T, 8>(p + g * 8, t);
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < 32; ++i)
+        if (i < left) p[i] = rp_from_f32<T>(acc[i]);
+    }
   }
 }
 
@@ -274,19 +340,30 @@ extern "C" int rphip_mxfp4_scores(rphip_ctx* ctx, void* stream, int64_t n_users,
   if ((uintptr_t)out_dev % rp_type_bytes(out_type)) RP_FAIL(RPHIP_EINVAL, "mxfp4_scores: out is not aligned to its elements");
   if (ld_out < cols) RP_FAIL(RPHIP_EINVAL, "mxfp4_scores: ld_out %lld < cols %lld", (long long)ld_out, (long long)cols);
   RP_TRY(scope.enter(ctx));
-  const int nb = (int)rp_cdiv(cols, RP_MX), tiles = (int)rp_cdiv(nb, 64);
+  const int nb = (int)rp_cdiv(cols, RP_MX);
+  const int64_t tiles = rp_cdiv(nb, 64);
+  if (tiles > 65535) RP_FAIL(RPHIP_ELIMIT, "mxfp4_scores: at most %d columns", 65535 * MXS_COLS);
   return rp_by_type(out_type, [&](auto tag) -> int {
     using T = typename decltype(tag)::T;
-    for (int64_t u0 = 0; u0 < n_users; u0 += 65535) {
-      const dim3 grid(tiles, (unsigned)std::min<int64_t>(65535, n_users - u0));
-      if (weights_dev)
-        k_mx_scores<T, true><<<grid, 64, 0, (hipStream_t)stream>>>(indptr_dev, indices_dev, weights_dev, nnz, (int)rows, (int)cols, nb, codes_dev, ld_codes, scales_dev,
-                                                                   ld_scales, exclude_history, item_keep_dev, (T*)out_dev, ld_out, u0);
-      else
-        k_mx_scores<T, false><<<grid, 64, 0, (hipStream_t)stream>>>(indptr_dev, indices_dev, nullptr, nnz, (int)rows, (int)cols, nb, codes_dev, ld_codes, scales_dev,
-                                                                    ld_scales, exclude_history, item_keep_dev, (T*)out_dev, ld_out, u0);
-      RP_LAUNCHED();
-    }
-    return RPHIP_OK;
+    const hipStream_t st = (hipStream_t)stream;
+    auto go = [&](auto weighted, auto waves) -> int {
+      constexpr int WV = decltype(waves)::value;
+      constexpr int64_t strip = (int64_t)1 << 22;  // (users of a launch: below 2^32 threads)
+      for (int64_t u0 = 0; u0 < n_users; u0 += strip) {
+        const dim3 grid((unsigned)std::min(strip, n_users - u0), (unsigned)tiles);
+        k_mx_scores<T, decltype(weighted)::value, WV><<<grid, 64 * WV, 0, st>>>(indptr_dev, indices_dev, weights_dev, nnz, (int)rows, (int)cols, nb, codes_dev, ld_codes,
+                                                                            scales_dev, ld_scales, exclude_history, item_keep_dev, (T*)out_dev, ld_out, u0);
+        RP_LAUNCHED();
+      }
+      return RPHIP_OK;
+    };
+    using std::integral_constant;
+    const int64_t groups = n_users * tiles;
+    auto by_waves = [&](auto weighted) -> int {
+      if (groups <= 4 * ctx->n_cu) return go(weighted, integral_constant<int, 8>{});
+      if (groups <= 32 * ctx->n_cu) return go(weighted, integral_constant<int, 4>{});
+      return go(weighted, integral_constant<int, 1>{});
+    };
+    return weights_dev ? by_waves(std::true_type{}) : by_waves(std::false_type{});
   });
 }

@@ -8,6 +8,7 @@
 #include "rp_ops.h"
 
 #include <algorithm>
+#include <type_traits>
 
 namespace {
 
@@ -17,7 +18,12 @@ typedef int i32x8 __attribute__((ext_vector_type(8)));
 
 constexpr int KC = 128;  // K of a chunk: four MX blocks
 
-// ---- A as planes of bf16: [row][chunk][plane][128], zero beyond K --------------------------------------------------------------------
+// ---- the operands' workspace forms ---------------------------------------------------------------------------------------------------
+// A fragment is what the 64 lanes of a wave hand to one matrix instruction: lane (row = l & 15, g = l >> 4) holds 16 bytes.  Chunk c of a
+// row is its MX blocks 4 c .. 4 c + 3; lane group g takes block 4 c + g.  Inside a chunk K runs in the order (step s, g, 8 elements) for the
+// bf16 instruction and (g, 32 elements) for the 4-bit one - the same for both operands, which is all a product asks - so a lane's 16
+// code bytes are one MX block with one scale in either kernel.
+
 // by truncation: the high part never overflows, each remainder is exact
 template <int P>
 __device__ __forceinline__ void cut_planes(float x, uint16_t (&h)[P]) {
@@ -37,36 +43,60 @@ __device__ __forceinline__ void cut_planes(float x, uint16_t (&h)[P]) {
   }
 }
 
+// A -> planes [16-row block][chunk][plane][step 4][lane 64][8 bf16], zero beyond K and M: fragments are contiguous KB.  One thread
+// per (block, chunk, lane): it reads one MX block's worth of its row and writes a piece of 4 P fragments.
 template <class T, int P>
-__global__ __launch_bounds__(256) void k_mxg_planes(const T* __restrict__ a, int64_t lda, int M, int K, int nc, uint16_t* __restrict__ out) {
-  const int64_t unit = (int64_t)blockIdx.x * 256 + threadIdx.x;  // eight elements
-  const int upr = nc * (KC / 8);
-  const int64_t m = unit / upr;
-  if (m >= M) return;
-  const int q = (int)(unit - m * upr), k = q * 8;
-  const T* p = a + m * lda + k;
-  float v[8];
-  if (k + 8 <= K) {
-    const rp_vec<T, 8> t = rp_load_vec<T, 8>(p);
+__global__ __launch_bounds__(256) void k_mxg_planes(const T* __restrict__ a, int64_t lda, int M, int K, int nc, int64_t units, uint16_t* __restrict__ out) {
+  const int64_t unit = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (unit >= units) return;
+  const int lane = threadIdx.x & 63;
+  const int64_t frag = unit >> 6, mb = frag / nc;
+  const int c = (int)(frag - mb * nc);
+  const int64_t m = mb * 16 + (lane & 15);
+  const int k0 = c * KC + (lane >> 4) * 32;
+  uint4* o = (uint4*)(out + frag * (P * 4 * 512)) + lane;
+  const T* p = a + m * lda + k0;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = rp_to_f32(t.v[i]);
-  } else {
+  for (int s = 0; s < 4; ++s) {
+    float v[8];
+    if (m < M && k0 + s * 8 + 8 <= K) {
+      const rp_vec<T, 8> t = rp_load_vec<T, 8>(p + s * 8);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = k + i < K ? rp_to_f32(p[i]) : 0.0f;
+      for (int i = 0; i < 8; ++i) v[i] = rp_to_f32(t.v[i]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] = m < M && k0 + s * 8 + i < K ? rp_to_f32(p[s * 8 + i]) : 0.0f;
+    }
+    uint16_t h[8][P];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) cut_planes<P>(v[i], h[i]);
+#pragma unroll
+    for (int pl = 0; pl < P; ++pl) {
+      uint4 w;
+      w.x = h[0][pl] | (uint32_t)h[1][pl] << 16;
+      w.y = h[2][pl] | (uint32_t)h[3][pl] << 16;
+      w.z = h[4][pl] | (uint32_t)h[5][pl] << 16;
+      w.w = h[6][pl] | (uint32_t)h[7][pl] << 16;
+      o[(pl * 4 + s) * 64] = w;
+    }
   }
-  uint16_t h[8][P];
+}
+
+// Scales -> [16-row block][four chunks][lane 64] words: byte cc = the scale of the lane's block of chunk 4 q + cc.  Blocks beyond the
+// row get 0 (2^-127): whatever their codes hold, the product underflows to nothing.  Rows beyond the matrix repeat the last one.
+__global__ __launch_bounds__(256) void k_mxg_scales(const uint8_t* __restrict__ s, int64_t lds, int rows, int nb, int nq, int64_t units, uint32_t* __restrict__ out) {
+  const int64_t unit = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (unit >= units) return;
+  const int lane = threadIdx.x & 63;
+  const int64_t f = unit >> 6, rb = f / nq;
+  const int q = (int)(f - rb * nq);
+  const int64_t r = min(rb * 16 + (lane & 15), (int64_t)rows - 1);
+  const int b = q * 16 + (lane >> 4);
+  uint32_t w = 0;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) cut_planes<P>(v[i], h[i]);
-  uint16_t* o = out + (m * nc + q / (KC / 8)) * (P * KC) + (q % (KC / 8)) * 8;
-#pragma unroll
-  for (int pl = 0; pl < P; ++pl) {
-    uint4 w;
-    w.x = h[0][pl] | (uint32_t)h[1][pl] << 16;
-    w.y = h[2][pl] | (uint32_t)h[3][pl] << 16;
-    w.z = h[4][pl] | (uint32_t)h[5][pl] << 16;
-    w.w = h[6][pl] | (uint32_t)h[7][pl] << 16;
-    *(uint4*)(o + pl * KC) = w;
-  }
+  for (int cc = 0; cc < 4; ++cc)
+    if (b + cc * 4 < nb) w |= (uint32_t)s[r * lds + b + cc * 4] << (8 * cc);
+  out[unit] = w;
 }
 
 // eight codes (a dword) to eight bf16
@@ -78,133 +108,248 @@ __device__ __forceinline__ bf16x8 codes_bf16(uint32_t w, float s) {
 }
 
 struct gemm_args {
-  int M, N, nb, nc;          // nb: blocks of a row of W (and of an MXFP4 A), nc: chunks
-  const uint16_t* planes;    // 16-bit form of A
-  const uint8_t* a_codes; int64_t lda; const uint8_t* a_scales; int64_t ldas;  // MXFP4 A
-  const uint8_t* w; int64_t ldw; const uint8_t* ws; int64_t ldws;
+  int M, N, nb, nc, nq;      // nb: blocks of a row of W (and of an MXFP4 A); nc: chunks; nq: groups of four chunks
+  const uint8_t* planes;     // 16-bit form of A
+  const uint8_t* a_codes; int64_t lda; const uint32_t* a_scales;  // MXFP4 A (scales in the workspace form)
+  const uint8_t* w; int64_t ldw; const uint32_t* w_scales;
   void* c; int64_t ldc;
   float* part;               // split K: partial sums [split][M][N]
   int split;
+  int gx, gy, blocked;       // tiles, and whether the grid runs in blocks of 4 x 8
 };
 
-// Tile BM x BN, WM x WN waves.  The lane (l & 15, l >> 4) = (row, g) of a fragment holds block 4 c + g of its row; K runs in the order
-// (step s, g, 8 elements) inside a chunk - the same for both operands, which is all a product asks - so a lane's 16 code bytes are
-// one MX block with one scale.
-template <class OT, int P, int BM, int BN, int WM, int WN>
-__global__ __launch_bounds__(WM * WN * 64) void k_mxg_bf16(gemm_args g) {
-  constexpr int TM = BM / WM / 16, TN = BN / WN / 16, THREADS = WM * WN * 64;
-  __shared__ uint4 tile[BM * 16];  // one plane of a chunk: row r's 16-byte piece j at j ^ (r & 15)
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int fr = lane & 15, fg = lane >> 4;
-  const int m0 = blockIdx.y * BM, n0 = blockIdx.x * BN;
-  const int wm = (wave / WN) * TM * 16, wn = (wave % WN) * TN * 16;
-  f32x4 acc[TM][TN];
+// Workgroups go to the 8 XCDs round-robin and an XCD runs 32 of them at a time; those 32 become a block of 4 tile rows x 8 tile columns,
+// so that an XCD's L2 serves 12 operand panels for 32 tiles.  Grids of fewer than 256 such tiles, or of less than four rows, go row by
+// row: blocks would leave XCDs idle.
+__device__ __forceinline__ bool tile_of(const gemm_args& g, int& tm, int& tn) {
+  if (!g.blocked) {
+    tm = (int)blockIdx.x / g.gx;
+    tn = (int)blockIdx.x % g.gx;
+    return true;
+  }
+  const unsigned L = blockIdx.x, x = L & 7u, s8 = L >> 3, beta = s8 >> 5, pp = s8 & 31u;
+  const unsigned nbc = ((unsigned)g.gx + 7) / 8, gb = beta * 8u + x, row = gb / nbc, col = gb - row * nbc;
+  tm = (int)(row * 4 + pp / 8);
+  tn = (int)(col * 8 + pp % 8);
+  return tm < g.gy && tn < g.gx;
+}
+
+__device__ __forceinline__ void dma16(const uint8_t* from, uint8_t* to) {
+  __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)from, (__attribute__((address_space(3))) void*)to, 16, 0, 0);
+}
+
+template <int N>
+__device__ __forceinline__ void wait_loads_and_meet() {
+  asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
+  __builtin_amdgcn_s_barrier();  // bare: the fence of __syncthreads() would wait for every load in flight
+  asm volatile("" ::: "memory");
+}
+
+// D = W fragment x A fragment: a lane holds four neighbouring columns n of one row m.
+template <class OT, int TM, int TN>
+__device__ __forceinline__ void store_tile(const gemm_args& g, const f32x4 (&acc)[TM][TN], int m0, int n0, int lane) {
+  const int z = blockIdx.y;
 #pragma unroll
-  for (int i = 0; i < TM; ++i)
-#pragma unroll
-    for (int j = 0; j < TN; ++j) acc[i][j] = f32x4{0, 0, 0, 0};
-  const int c_begin = (int)((int64_t)g.nc * blockIdx.z / g.split), c_end = (int)((int64_t)g.nc * (blockIdx.z + 1) / g.split);
-  for (int c = c_begin; c < c_end; ++c) {
-    uint4 wq[TN];
-    float wsc[TN];
-    const int b = c * 4 + fg;
+  for (int i = 0; i < TM; ++i) {
+    const int m = m0 + i * 16 + (lane & 15);
+    if (m >= g.M) continue;
 #pragma unroll
     for (int j = 0; j < TN; ++j) {
-      const int n = min(n0 + wn + j * 16 + fr, g.N - 1);
-      wq[j] = make_uint4(0, 0, 0, 0);
-      uint32_t byte = 127;
-      if (b < g.nb) {
-        wq[j] = *(const uint4*)(g.w + (int64_t)n * g.ldw + (int64_t)b * 16);
-        byte = g.ws[(int64_t)n * g.ldws + b];
-      }
-      wsc[j] = rp_mx_scale(byte);
-    }
-    for (int p = 0; p < P; ++p) {
-      __syncthreads();
-      for (int q = threadIdx.x; q < BM * 16; q += THREADS) {
-        const int r = q >> 4, j = q & 15, m = min(m0 + r, g.M - 1);
-        tile[r * 16 + (j ^ (r & 15))] = *(const uint4*)(g.planes + (((int64_t)m * g.nc + c) * P + p) * KC + j * 8);
-      }
-      __syncthreads();
+      const int n = n0 + j * 16 + (lane >> 4) * 4;
+      if (g.split > 1) {
+        float* o = g.part + ((int64_t)z * g.M + m) * g.N + n;
+        if (n + 4 <= g.N) {
+          rp_vec<float, 4> t = {{acc[i][j][0], acc[i][j][1], acc[i][j][2], acc[i][j][3]}};
+          rp_store_vec<float, 4>(o, t);
+        } else {
 #pragma unroll
-      for (int s = 0; s < 4; ++s) {
-        bf16x8 wf[TN];
+          for (int e = 0; e < 4; ++e)
+            if (n + e < g.N) o[e] = acc[i][j][e];
+        }
+      } else {
+        OT* o = (OT*)g.c + (int64_t)m * g.ldc + n;
+        if (n + 4 <= g.N) {
+          rp_vec<OT, 4> t;
 #pragma unroll
-        for (int j = 0; j < TN; ++j) wf[j] = codes_bf16(s == 0 ? wq[j].x : s == 1 ? wq[j].y : s == 2 ? wq[j].z : wq[j].w, wsc[j]);
+          for (int e = 0; e < 4; ++e) t.v[e] = rp_from_f32<OT>(acc[i][j][e]);
+          rp_store_vec<OT, 4>(o, t);
+        } else {
 #pragma unroll
-        for (int i = 0; i < TM; ++i) {
-          const int r = wm + i * 16 + fr;
-          const bf16x8 af = __builtin_bit_cast(bf16x8, tile[r * 16 + ((fg * 4 + s) ^ (r & 15))]);
-#pragma unroll
-          for (int j = 0; j < TN; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(af, wf[j], acc[i][j], 0, 0, 0);
+          for (int e = 0; e < 4; ++e)
+            if (n + e < g.N) o[e] = rp_from_f32<OT>(acc[i][j][e]);
         }
       }
     }
   }
-#pragma unroll
-  for (int i = 0; i < TM; ++i)
-#pragma unroll
-    for (int j = 0; j < TN; ++j)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int m = m0 + wm + i * 16 + fg * 4 + e, n = n0 + wn + j * 16 + fr;
-        if (m >= g.M || n >= g.N) continue;
-        if (g.split > 1) g.part[((int64_t)blockIdx.z * g.M + m) * g.N + n] = acc[i][j][e];
-        else ((OT*)g.c)[(int64_t)m * g.ldc + n] = rp_from_f32<OT>(acc[i][j][e]);
-      }
 }
 
-template <class OT, int BM, int BN, int WM, int WN>
-__global__ __launch_bounds__(WM * WN * 64) void k_mxg_fp4(gemm_args g) {
-  constexpr int TM = BM / WM / 16, TN = BN / WN / 16;
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int fr = lane & 15, fg = lane >> 4;
-  const int m0 = blockIdx.y * BM, n0 = blockIdx.x * BN;
-  const int wm = (wave / WN) * TM * 16, wn = (wave % WN) * TN * 16;
+// 16-bit form.  Tile BM x BN, WM x WN waves, a ring of RING stages of A in LDS, each the half of a plane of a chunk (two of its four
+// steps), filled by LDS-DMA RING - 1 stages ahead; W goes from memory to registers one chunk ahead and is converted there, once per
+// plane and wave: 4 conversions per 8 codes against TM matrix instructions that use them.
+template <class OT, int P, int BM, int BN, int WM, int WN, int RING>
+__global__ __launch_bounds__(WM * WN * 64) void k_mxg_bf16(gemm_args g) {
+  constexpr int WAVES = WM * WN, TM = BM / WM / 16, TN = BN / WN / 16, STAGE = BM * 128, D = BM / 8 / WAVES;  // D: KB a wave requests per stage
+  static_assert(D * WAVES * 8 == BM, "every wave requests the same number of fragments");
+  extern __shared__ __attribute__((aligned(1024))) uint8_t ring[];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  int tm, tn;
+  if (!tile_of(g, tm, tn)) return;
+  const int m0 = tm * BM, wm = (wave / WN) * TM, wn = tn * (BN / 16) + (wave % WN) * TN;  // (wm, wn in fragments)
   f32x4 acc[TM][TN];
 #pragma unroll
   for (int i = 0; i < TM; ++i)
 #pragma unroll
     for (int j = 0; j < TN; ++j) acc[i][j] = f32x4{0, 0, 0, 0};
-  const int c_begin = (int)((int64_t)g.nc * blockIdx.z / g.split), c_end = (int)((int64_t)g.nc * (blockIdx.z + 1) / g.split);
-  for (int c = c_begin; c < c_end; ++c) {
-    const int b = c * 4 + fg;
-    uint4 aq[TM], wq[TN];
-    int as[TM], wsc[TN];
+  const int z = blockIdx.y;
+  const int c0 = (int)((int64_t)g.nc * z / g.split), c1 = (int)((int64_t)g.nc * (z + 1) / g.split);
+  const int t0 = c0 * P * 2, t1 = c1 * P * 2;
+  // A: fragment pairs (2 KB) of a stage, wave's share
+  const int mblocks = (g.M + 15) / 16;
+  const uint8_t* asrc[D];
 #pragma unroll
-    for (int i = 0; i < TM; ++i) {
-      const int m = min(m0 + wm + i * 16 + fr, g.M - 1);
-      aq[i] = make_uint4(0, 0, 0, 0);
-      as[i] = 127;
-      if (b < g.nb) aq[i] = *(const uint4*)(g.a_codes + (int64_t)m * g.lda + (int64_t)b * 16), as[i] = g.a_scales[(int64_t)m * g.ldas + b];
-    }
-#pragma unroll
-    for (int j = 0; j < TN; ++j) {
-      const int n = min(n0 + wn + j * 16 + fr, g.N - 1);
-      wq[j] = make_uint4(0, 0, 0, 0);
-      wsc[j] = 127;
-      if (b < g.nb) wq[j] = *(const uint4*)(g.w + (int64_t)n * g.ldw + (int64_t)b * 16), wsc[j] = g.ws[(int64_t)n * g.ldws + b];
-    }
-#pragma unroll
-    for (int i = 0; i < TM; ++i)
-#pragma unroll
-      for (int j = 0; j < TN; ++j) {
-        const i32x8 af = {(int)aq[i].x, (int)aq[i].y, (int)aq[i].z, (int)aq[i].w, 0, 0, 0, 0};
-        const i32x8 wf = {(int)wq[j].x, (int)wq[j].y, (int)wq[j].z, (int)wq[j].w, 0, 0, 0, 0};
-        acc[i][j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(af, wf, acc[i][j], 4, 4, 0, as[i], 0, wsc[j]);
-      }
+  for (int d = 0; d < D; ++d) {
+    const int f = wave * D + d, mb = min(m0 / 16 + (f >> 1), mblocks - 1);
+    asrc[d] = g.planes + ((int64_t)mb * g.nc * P) * 4096 + (f & 1) * 1024 + lane * 16;
   }
+  auto request = [&](int t) __attribute__((always_inline)) {
+    const int tt = min(t, t1 - 1);  // (a request past the end repeats the last one: the counted waits stay uniform)
+    uint8_t* to = ring + (t - t0) % RING * STAGE + wave * D * 1024;
+#pragma unroll
+    for (int d = 0; d < D; ++d) dma16(asrc[d] + (int64_t)tt * 2048, to + d * 1024);
+  };
+  // W
+  const uint8_t* wsrc[TN];
+  const uint32_t* wssrc[TN];
+  const int nblocks = (g.N + 15) / 16;
+#pragma unroll
+  for (int j = 0; j < TN; ++j) {
+    const int nbk = min(wn + j, nblocks - 1), n = min(nbk * 16 + (lane & 15), g.N - 1);
+    wsrc[j] = g.w + (int64_t)n * g.ldw;
+    wssrc[j] = g.w_scales + (int64_t)nbk * g.nq * 64 + lane;
+  }
+  uint4 wq[TN], wnext[TN];
+  uint32_t sc[TN], scnext[TN];
+  auto load_w = [&](int c) __attribute__((always_inline)) {
+    const int cc = min(c, g.nc - 1), b = min(cc * 4 + (lane >> 4), g.nb - 1);  // (a block beyond the row: A is zero there)
+#pragma unroll
+    for (int j = 0; j < TN; ++j) wnext[j] = *(const uint4*)(wsrc[j] + (int64_t)b * 16);
+#pragma unroll
+    for (int j = 0; j < TN; ++j) scnext[j] = wssrc[j][(cc >> 2) * 64];
+  };
+  if (t0 < t1) {
+    load_w(c0);
+#pragma unroll
+    for (int r = 0; r < RING - 1; ++r) request(t0 + r);
+    int t = t0;
+    for (int c = c0; c < c1; ++c) {
+#pragma unroll
+      for (int j = 0; j < TN; ++j) wq[j] = wnext[j], sc[j] = ((scnext[j] >> (8 * (c & 3))) & 255u) << 23;
+      load_w(c + 1);
+#pragma unroll 1
+      for (int p = 0; p < P; ++p) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h, ++t) {
+          wait_loads_and_meet<(RING - 2) * D>();
+          request(t + RING - 1);
+          const uint8_t* st = ring + (t - t0) % RING * STAGE + lane * 16;
+#pragma unroll
+          for (int s = 0; s < 2; ++s) {
+            bf16x8 wf[TN];
+#pragma unroll
+            for (int j = 0; j < TN; ++j) wf[j] = codes_bf16(h == 0 ? (s == 0 ? wq[j].x : wq[j].y) : (s == 0 ? wq[j].z : wq[j].w), __uint_as_float(sc[j]));
+#pragma unroll
+            for (int i = 0; i < TM; ++i) {
+              const bf16x8 af = *(const bf16x8*)(st + ((wm + i) * 2 + s) * 1024);
+#pragma unroll
+              for (int j = 0; j < TN; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(wf[j], af, acc[i][j], 0, 0, 0);
+            }
+          }
+        }
+      }
+    }
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // (the trailing requests write LDS)
+  }
+  store_tile<OT, TM, TN>(g, acc, m0 + wm * 16, wn * 16, lane);
+}
+
+// 4-bit form: codes of both operands through the ring (a stage is a chunk of both), scales in registers, four chunks to a word.
+template <class OT, int BM, int BN, int WM, int WN, int RING>
+__global__ __launch_bounds__(WM * WN * 64) void k_mxg_fp4(gemm_args g) {
+  constexpr int WAVES = WM * WN, TM = BM / WM / 16, TN = BN / WN / 16, STAGE = (BM + BN) * 64, D = (BM + BN) / 16 / WAVES;
+  static_assert(D * WAVES * 16 == BM + BN, "every wave requests the same number of fragments");
+  extern __shared__ __attribute__((aligned(1024))) uint8_t ring[];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  int tm, tn;
+  if (!tile_of(g, tm, tn)) return;
+  const int wm = (wave / WN) * TM, wn = (wave % WN) * TN;  // (in fragments of the tile)
+  f32x4 acc[TM][TN];
 #pragma unroll
   for (int i = 0; i < TM; ++i)
 #pragma unroll
-    for (int j = 0; j < TN; ++j)
+    for (int j = 0; j < TN; ++j) acc[i][j] = f32x4{0, 0, 0, 0};
+  const int z = blockIdx.y;
+  const int q0 = (int)((int64_t)g.nq * z / g.split), q1 = (int)((int64_t)g.nq * (z + 1) / g.split);
+  const int c0 = q0 * 4, c1 = min(q1 * 4, g.nc);
+  const uint8_t* src[D];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int m = m0 + wm + i * 16 + fg * 4 + e, n = n0 + wn + j * 16 + fr;
-        if (m >= g.M || n >= g.N) continue;
-        if (g.split > 1) g.part[((int64_t)blockIdx.z * g.M + m) * g.N + n] = acc[i][j][e];
-        else ((OT*)g.c)[(int64_t)m * g.ldc + n] = rp_from_f32<OT>(acc[i][j][e]);
-      }
+  for (int d = 0; d < D; ++d) {
+    const int f = wave * D + d;
+    src[d] = f < BM / 16 ? g.a_codes + (int64_t)min(tm * BM + f * 16 + (lane & 15), g.M - 1) * g.lda
+                         : g.w + (int64_t)min(tn * BN + (f - BM / 16) * 16 + (lane & 15), g.N - 1) * g.ldw;
+  }
+  auto request = [&](int c) __attribute__((always_inline)) {
+    const int b = min(min(c, c1 - 1) * 4 + (lane >> 4), g.nb - 1);  // (a block beyond the row: its scale is 2^-127 on both sides)
+    uint8_t* to = ring + (c - c0) % RING * STAGE + wave * D * 1024;
+#pragma unroll
+    for (int d = 0; d < D; ++d) dma16(src[d] + (int64_t)b * 16, to + d * 1024);
+  };
+  const int mblocks = (g.M + 15) / 16, nblocks = (g.N + 15) / 16;
+  const uint32_t* ssrc[TM + TN];
+#pragma unroll
+  for (int i = 0; i < TM; ++i) ssrc[i] = g.a_scales + (int64_t)min(tm * (BM / 16) + wm + i, mblocks - 1) * g.nq * 64 + lane;
+#pragma unroll
+  for (int j = 0; j < TN; ++j) ssrc[TM + j] = g.w_scales + (int64_t)min(tn * (BN / 16) + wn + j, nblocks - 1) * g.nq * 64 + lane;
+  uint32_t sc[TM + TN], scnext[TM + TN];
+  auto load_scales = [&](int q) __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < TM + TN; ++i) scnext[i] = ssrc[i][min(q, g.nq - 1) * 64];
+  };
+  if (c0 < c1) {
+    load_scales(q0);
+#pragma unroll
+    for (int r = 0; r < RING - 1; ++r) request(c0 + r);
+    for (int q = q0; q < q1; ++q) {
+#pragma unroll
+      for (int i = 0; i < TM + TN; ++i) sc[i] = scnext[i];
+      load_scales(q + 1);
+      auto chunk = [&](auto tag, int c) __attribute__((always_inline)) {
+        constexpr int CC = decltype(tag)::value;
+        wait_loads_and_meet<(RING - 2) * D>();
+        request(c + RING - 1);
+        const uint8_t* st = ring + (c - c0) % RING * STAGE + lane * 16;
+        i32x8 wf[TN];
+#pragma unroll
+        for (int j = 0; j < TN; ++j) {
+          const uint4 v = *(const uint4*)(st + (BM / 16 + wn + j) * 1024);
+          wf[j] = i32x8{(int)v.x, (int)v.y, (int)v.z, (int)v.w, 0, 0, 0, 0};
+        }
+#pragma unroll
+        for (int i = 0; i < TM; ++i) {
+          const uint4 v = *(const uint4*)(st + (wm + i) * 1024);
+          const i32x8 af = {(int)v.x, (int)v.y, (int)v.z, (int)v.w, 0, 0, 0, 0};
+#pragma unroll
+          for (int j = 0; j < TN; ++j) acc[i][j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(wf[j], af, acc[i][j], 4, 4, CC, (int)sc[TM + j], CC, (int)sc[i]);
+        }
+      };
+      const int c = q * 4;
+      chunk(std::integral_constant<int, 0>{}, c);
+      if (c + 1 < c1) chunk(std::integral_constant<int, 1>{}, c + 1);
+      if (c + 2 < c1) chunk(std::integral_constant<int, 2>{}, c + 2);
+      if (c + 3 < c1) chunk(std::integral_constant<int, 3>{}, c + 3);
+    }
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // (the trailing requests write LDS)
+  }
+  store_tile<OT, TM, TN>(g, acc, tm * BM + wm * 16, tn * BN + wn * 16, lane);
 }
 
 // split K: the parts in order, one rounding
@@ -218,33 +363,53 @@ __global__ __launch_bounds__(256) void k_mxg_join(const float* __restrict__ part
 }
 
 struct plan {
-  int planes = 0, split = 1;
+  int planes = 0, split = 1, nc = 0, nq = 0;
   int bm = 16, bn = 64;
-  int64_t plane_bytes = 0, part_bytes = 0;
-  int nc = 0;
+  int64_t plane_bytes = 0, a_scale_bytes = 0, w_scale_bytes = 0, part_bytes = 0;
+  int64_t total() const { return plane_bytes + a_scale_bytes + w_scale_bytes + part_bytes; }
 };
 
 plan make_plan(int n_cu, int64_t M, int64_t N, int64_t K, int32_t a_type) {
   plan p;
   p.planes = a_type == RPHIP_BF16 ? 1 : a_type == RPHIP_F16 ? 2 : a_type == RPHIP_F32 ? 3 : 0;
   p.nc = (int)rp_cdiv(K, KC);
-  p.bm = M <= 16 ? 16 : M <= 256 ? 64 : 128;
-  p.bn = p.bm == 128 ? 128 : 64;
-  const int64_t tiles = rp_cdiv(M, p.bm) * rp_cdiv(N, p.bn);
-  p.split = (int)std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(2 * n_cu / std::max<int64_t>(tiles, 1), p.nc / 4), 32));
-  p.plane_bytes = (M * p.nc * p.planes * KC * 2 + 255) & ~(int64_t)255;
+  p.nq = (int)rp_cdiv(p.nc, 4);
+  auto tiles = [&](int bm, int bn) { return rp_cdiv(M, bm) * rp_cdiv(N, bn); };
+  if (M <= 16) p.bm = p.planes ? 16 : 32, p.bn = p.planes ? 64 : 32;
+  else if (tiles(256, 256) >= n_cu) p.bm = 256, p.bn = 256;
+  else if (tiles(128, 128) >= n_cu) p.bm = 128, p.bn = 128;
+  else p.bm = 64, p.bn = 64;
+  const int64_t n = std::max<int64_t>(tiles(p.bm, p.bn), 1), depth = p.planes ? p.nc / 2 : p.nq;
+  p.split = (int)std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(2 * n_cu / n, depth), 16));
+  auto room = [](int64_t b) { return (b + 255) & ~(int64_t)255; };
+  p.plane_bytes = room(rp_cdiv(M, 16) * p.nc * p.planes * 4096);
+  p.a_scale_bytes = p.planes ? 0 : room(rp_cdiv(M, 16) * p.nq * 256);
+  p.w_scale_bytes = room(rp_cdiv(N, 16) * p.nq * 256);
   p.part_bytes = p.split > 1 ? M * N * 4 * p.split : 0;
   return p;
 }
 
-template <class OT, int BM, int BN, int WM, int WN>
-void launch_tiles(const gemm_args& g, int planes, hipStream_t st) {
-  const dim3 grid((unsigned)rp_cdiv(g.N, BN), (unsigned)rp_cdiv(g.M, BM), (unsigned)g.split);
-  const int threads = WM * WN * 64;
-  if (planes == 0) k_mxg_fp4<OT, BM, BN, WM, WN><<<grid, threads, 0, st>>>(g);
-  else if (planes == 1) k_mxg_bf16<OT, 1, BM, BN, WM, WN><<<grid, threads, 0, st>>>(g);
-  else if (planes == 2) k_mxg_bf16<OT, 2, BM, BN, WM, WN><<<grid, threads, 0, st>>>(g);
-  else k_mxg_bf16<OT, 3, BM, BN, WM, WN><<<grid, threads, 0, st>>>(g);
+template <int BM, int BN, class Kernel>
+int launch_tiles(Kernel kernel, gemm_args g, int threads, int lds, hipStream_t st) {
+  g.gx = (int)rp_cdiv(g.N, BN), g.gy = (int)rp_cdiv(g.M, BM);
+  g.blocked = g.gy >= 4 && (int64_t)g.gx * g.gy >= 256;
+  const int64_t blocks = rp_cdiv(g.gx, 8) * rp_cdiv(g.gy, 4), tiles = g.blocked ? rp_cdiv(blocks, 8) * 8 * 32 : (int64_t)g.gx * g.gy;
+  if (tiles * threads >= ((int64_t)1 << 32)) RP_FAIL(RPHIP_ELIMIT, "mxfp4_gemm_nt: %d x %d is more than a launch takes", g.M, g.N);
+  if (lds > 64 * 1024) RP_HIP(hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, lds));
+  kernel<<<dim3((unsigned)tiles, (unsigned)g.split), threads, lds, st>>>(g);
+  RP_LAUNCHED();
+  return RPHIP_OK;
+}
+template <class OT, int BM, int BN, int WM, int WN, int RING>
+int launch_fp4(const gemm_args& g, hipStream_t st) {
+  return launch_tiles<BM, BN>(k_mxg_fp4<OT, BM, BN, WM, WN, RING>, g, WM * WN * 64, RING * (BM + BN) * 64, st);
+}
+template <class OT, int BM, int BN, int WM, int WN, int RING>
+int launch_bf16(const gemm_args& g, int planes, hipStream_t st) {
+  constexpr int threads = WM * WN * 64, lds = RING * BM * 128;
+  if (planes == 1) return launch_tiles<BM, BN>(k_mxg_bf16<OT, 1, BM, BN, WM, WN, RING>, g, threads, lds, st);
+  if (planes == 2) return launch_tiles<BM, BN>(k_mxg_bf16<OT, 2, BM, BN, WM, WN, RING>, g, threads, lds, st);
+  return launch_tiles<BM, BN>(k_mxg_bf16<OT, 3, BM, BN, WM, WN, RING>, g, threads, lds, st);
 }
 
 int check_sizes(const char* who, int64_t M, int64_t N, int64_t K) {
@@ -261,7 +426,7 @@ extern "C" int rphip_mxfp4_gemm_nt_workspace(rphip_ctx* ctx, int64_t M, int64_t 
   RP_TRY(check_sizes("mxfp4_gemm_nt_workspace", M, N, K));
   if (a_type < RPHIP_F32 || a_type > RPHIP_MXFP4) RP_FAIL(RPHIP_EINVAL, "mxfp4_gemm_nt_workspace: element type %d", a_type);
   const plan p = make_plan(ctx->n_cu, M, N, K, a_type);
-  *bytes_out = p.plane_bytes + p.part_bytes;
+  *bytes_out = p.total();
   return RPHIP_OK;
 }
 
@@ -280,33 +445,54 @@ extern "C" int rphip_mxfp4_gemm_nt(rphip_ctx* ctx, void* stream, int64_t M, int6
   if (ldc < N || (uintptr_t)C_dev % rp_type_bytes(c_type)) RP_FAIL(RPHIP_EINVAL, "mxfp4_gemm_nt: ldc < N, or C is not aligned to its elements");
   RP_TRY(scope.enter(ctx));
   const plan p = make_plan(ctx->n_cu, M, N, K, a_type);
-  if (workspace_bytes < p.plane_bytes + p.part_bytes || (p.plane_bytes + p.part_bytes > 0 && !workspace_dev) || ((uintptr_t)workspace_dev & 255))
-    RP_FAIL(RPHIP_EINVAL, "mxfp4_gemm_nt: a workspace of %lld bytes, aligned to 256, is needed (rphip_mxfp4_gemm_nt_workspace)", (long long)(p.plane_bytes + p.part_bytes));
+  if (workspace_bytes < p.total() || (p.total() > 0 && !workspace_dev) || ((uintptr_t)workspace_dev & 255))
+    RP_FAIL(RPHIP_EINVAL, "mxfp4_gemm_nt: a workspace of %lld bytes, aligned to 256, is needed (rphip_mxfp4_gemm_nt_workspace)", (long long)p.total());
   const hipStream_t st = (hipStream_t)stream;
+  char* ws = (char*)workspace_dev;
   gemm_args g = {};
-  g.M = (int)M, g.N = (int)N, g.nb = (int)rp_cdiv(K, RP_MX), g.nc = p.nc;
-  g.planes = (const uint16_t*)workspace_dev;
-  g.a_codes = (const uint8_t*)A_dev, g.lda = lda, g.a_scales = a_scales_dev, g.ldas = ld_a_scales;
-  g.w = w_codes_dev, g.ldw = ld_w, g.ws = w_scales_dev, g.ldws = ld_w_scales;
-  g.c = C_dev, g.ldc = ldc, g.part = (float*)((char*)workspace_dev + p.plane_bytes), g.split = p.split;
-  if (p.planes && p.nc) {
-    const int64_t strip = std::max<int64_t>(1, ((int64_t)1 << 31) / ((int64_t)p.nc * (KC / 8)));  // rows of a launch of below 2^32 threads
-    for (int64_t m0 = 0; m0 < M; m0 += strip) {
+  g.M = (int)M, g.N = (int)N, g.nb = (int)rp_cdiv(K, RP_MX), g.nc = p.nc, g.nq = p.nq;
+  g.planes = (const uint8_t*)ws;
+  g.a_codes = (const uint8_t*)A_dev, g.lda = lda, g.a_scales = (const uint32_t*)(ws + p.plane_bytes);
+  g.w = w_codes_dev, g.ldw = ld_w, g.w_scales = (const uint32_t*)(ws + p.plane_bytes + p.a_scale_bytes);
+  g.c = C_dev, g.ldc = ldc, g.part = (float*)(ws + p.plane_bytes + p.a_scale_bytes + p.w_scale_bytes), g.split = p.split;
+  if (p.nc) {
+    // (below 2^32 threads a launch: M <= 2^20 and N <= 2^28 rows in strips of row blocks)
+    auto scales = [&](const uint8_t* s, int64_t lds, int64_t rows, uint32_t* o) -> int {
+      const int64_t strip = std::max<int64_t>(1, ((int64_t)1 << 25) / p.nq) * 16;
+      for (int64_t r0 = 0; r0 < rows; r0 += strip) {
+        const int64_t n = std::min(strip, rows - r0), units = rp_cdiv(n, 16) * p.nq * 64;
+        k_mxg_scales<<<(unsigned)rp_cdiv(units, 256), 256, 0, st>>>(s + r0 * lds, lds, (int)n, g.nb, p.nq, units, o + r0 / 16 * p.nq * 64);
+        RP_LAUNCHED();
+      }
+      return RPHIP_OK;
+    };
+    RP_TRY(scales(w_scales_dev, ld_w_scales, N, (uint32_t*)g.w_scales));
+    if (!p.planes) RP_TRY(scales(a_scales_dev, ld_a_scales, M, (uint32_t*)g.a_scales));
+    const int64_t strip = std::max<int64_t>(1, ((int64_t)1 << 25) / p.nc) * 16;
+    for (int64_t m0 = 0; p.planes && m0 < M; m0 += strip) {
       const int m = (int)std::min(strip, M - m0);
-      const unsigned grid = (unsigned)rp_cdiv((int64_t)m * p.nc * (KC / 8), 256);
-      uint16_t* o = (uint16_t*)workspace_dev + m0 * p.nc * p.planes * KC;
-      if (a_type == RPHIP_BF16) k_mxg_planes<__bf16, 1><<<grid, 256, 0, st>>>((const __bf16*)A_dev + m0 * lda, lda, m, (int)K, p.nc, o);
-      else if (a_type == RPHIP_F16) k_mxg_planes<_Float16, 2><<<grid, 256, 0, st>>>((const _Float16*)A_dev + m0 * lda, lda, m, (int)K, p.nc, o);
-      else k_mxg_planes<float, 3><<<grid, 256, 0, st>>>((const float*)A_dev + m0 * lda, lda, m, (int)K, p.nc, o);
+      const int64_t units = rp_cdiv(m, 16) * p.nc * 64;
+      const unsigned grid = (unsigned)rp_cdiv(units, 256);
+      uint16_t* o = (uint16_t*)(ws + m0 / 16 * p.nc * p.planes * 4096);
+      if (a_type == RPHIP_BF16) k_mxg_planes<__bf16, 1><<<grid, 256, 0, st>>>((const __bf16*)A_dev + m0 * lda, lda, m, (int)K, p.nc, units, o);
+      else if (a_type == RPHIP_F16) k_mxg_planes<_Float16, 2><<<grid, 256, 0, st>>>((const _Float16*)A_dev + m0 * lda, lda, m, (int)K, p.nc, units, o);
+      else k_mxg_planes<float, 3><<<grid, 256, 0, st>>>((const float*)A_dev + m0 * lda, lda, m, (int)K, p.nc, units, o);
       RP_LAUNCHED();
     }
   }
   return rp_by_type(c_type, [&](auto tag) -> int {
     using OT = typename decltype(tag)::T;
-    if (p.bm == 16) launch_tiles<OT, 16, 64, 1, 4>(g, p.planes, st);
-    else if (p.bm == 64) launch_tiles<OT, 64, 64, 2, 2>(g, p.planes, st);
-    else launch_tiles<OT, 128, 128, 2, 2>(g, p.planes, st);
-    RP_LAUNCHED();
+    if (p.planes == 0) {
+      if (p.bm == 32) RP_TRY((launch_fp4<OT, 32, 32, 1, 2, 4>(g, st)));
+      else if (p.bm == 64) RP_TRY((launch_fp4<OT, 64, 64, 2, 2, 4>(g, st)));
+      else if (p.bm == 128) RP_TRY((launch_fp4<OT, 128, 128, 2, 2, 4>(g, st)));
+      else RP_TRY((launch_fp4<OT, 256, 256, 2, 4, 4>(g, st)));
+    } else {
+      if (p.bm == 16) RP_TRY((launch_bf16<OT, 16, 64, 1, 2, 4>(g, p.planes, st)));
+      else if (p.bm == 64) RP_TRY((launch_bf16<OT, 64, 64, 2, 2, 4>(g, p.planes, st)));
+      else if (p.bm == 128) RP_TRY((launch_bf16<OT, 128, 128, 2, 2, 4>(g, p.planes, st)));
+      else RP_TRY((launch_bf16<OT, 256, 256, 2, 4, 4>(g, p.planes, st)));
+    }
     if (p.split > 1) {
       k_mxg_join<OT><<<(unsigned)rp_cdiv(M * N, 256), 256, 0, st>>>(g.part, p.split, g.M, g.N, (OT*)C_dev, ldc);
       RP_LAUNCHED();
