@@ -7,14 +7,22 @@
 #include "rp_ops.h"
 
 #include <algorithm>
+#include <type_traits>
+
+#include <float.h>
 
 namespace {
 
 constexpr int RPS_SHORT = 1024;      // longest prefix the list form ranks completely
 constexpr int SL_CAP = 4096;         // candidates collected in LDS
 constexpr int SL_THREADS = 1024;
-constexpr int SB_BINS = 4096;        // mass bins of the whole-row form: 64 per e-fold, the last one takes what lies below e^-64
-constexpr float SB_PER_E = 64.0f;
+constexpr int SB_BINS = 2048;        // mass bins of the whole-row form: 32 per e-fold, the last one takes what lies below e^-64
+constexpr double SB_PER_E = 32.0;
+constexpr int SB_CAP = 2048;         // entries of a list collected ahead
+constexpr int RC_FOUND = 512;        // ... of a workgroup's own part of them, in LDS
+constexpr int SR_THREADS = 256;      // threads of a workgroup that takes a slice of a row
+constexpr int64_t STRIP = 1024;      // rows whose workspace exists at a time (whole-row form: 58 KB each)
+constexpr int64_t STRIP_LISTS = 4096;  // (short prefixes: at most 8 KB each)
 
 struct sample_args {
   int64_t rows, ld, ld_ids, ld_u;
@@ -68,35 +76,83 @@ __device__ __forceinline__ float score_of(uint32_t key) { return __uint_as_float
 // log of a mass relative to the best score; equal scores give 0 (+inf among them)
 __device__ __forceinline__ double z_of(float x, float best, double inv_t_num) { return x == best ? 0.0 : ((double)x - (double)best) / inv_t_num; }
 
-__device__ __forceinline__ double shfl_up_f64(double v, int d) { return __hiloint2double(__shfl_up(__double2hiint(v), d), __shfl_up(__double2loint(v), d)); }
-__device__ __forceinline__ double shfl_f64(double v, int src) { return __hiloint2double(__shfl(__double2hiint(v), src), __shfl(__double2loint(v), src)); }
-__device__ __forceinline__ unsigned long long shfl_xor_u64(unsigned long long v, int m) {
-  const uint32_t lo = (uint32_t)__shfl_xor((int)(uint32_t)v, m), hi = (uint32_t)__shfl_xor((int)(uint32_t)(v >> 32), m);
-  return ((unsigned long long)hi << 32) | lo;
+// ---- exchanges inside a wave: in the vector unit where it can (data-parallel moves, lane swaps), no LDS round trips -----------------
+template <int CTRL, int ROWS = 0xf>
+__device__ __forceinline__ uint32_t dpp(uint32_t v) {  // lanes without a source get 0
+  return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, ROWS, 0xf, true);
 }
-__device__ __forceinline__ double wave_scan_f64(double v, int lane) {  // inclusive
-#pragma unroll
-  for (int d = 1; d < 64; d <<= 1) {
-    const double t = shfl_up_f64(v, d);
-    if (lane >= d) v += t;
-  }
+template <int CTRL, int ROWS = 0xf>
+__device__ __forceinline__ double dpp_f64(double v) {
+  return __hiloint2double((int)dpp<CTRL, ROWS>((uint32_t)__double2hiint(v)), (int)dpp<CTRL, ROWS>((uint32_t)__double2loint(v)));
+}
+template <int CTRL, int ROWS = 0xf>
+__device__ __forceinline__ unsigned long long dpp_u64(unsigned long long v) {
+  return ((unsigned long long)dpp<CTRL, ROWS>((uint32_t)(v >> 32)) << 32) | dpp<CTRL, ROWS>((uint32_t)v);
+}
+__device__ __forceinline__ double wave_scan_f64(double v) {  // inclusive
+  v += dpp_f64<0x111>(v);       // row_shr:1, 2, 4, 8
+  v += dpp_f64<0x112>(v);
+  v += dpp_f64<0x114>(v);
+  v += dpp_f64<0x118>(v);
+  v += dpp_f64<0x142, 0xa>(v);  // row_bcast:15, 31
+  v += dpp_f64<0x143, 0xc>(v);
   return v;
+}
+__device__ __forceinline__ unsigned long long wave_scan_u64(unsigned long long v) {
+  v += dpp_u64<0x111>(v);
+  v += dpp_u64<0x112>(v);
+  v += dpp_u64<0x114>(v);
+  v += dpp_u64<0x118>(v);
+  v += dpp_u64<0x142, 0xa>(v);
+  v += dpp_u64<0x143, 0xc>(v);
+  return v;
+}
+__device__ __forceinline__ uint32_t lane_u32(uint32_t v, int src) { return (uint32_t)__builtin_amdgcn_readlane((int)v, src); }  // src: the same in every lane
+__device__ __forceinline__ double lane_f64(double v, int src) {
+  return __hiloint2double((int)lane_u32((uint32_t)__double2hiint(v), src), (int)lane_u32((uint32_t)__double2loint(v), src));
+}
+__device__ __forceinline__ unsigned long long lane_u64(unsigned long long v, int src) {
+  return ((unsigned long long)lane_u32((uint32_t)(v >> 32), src) << 32) | lane_u32((uint32_t)v, src);
+}
+typedef unsigned int u32x2 __attribute__((ext_vector_type(2)));
+template <int M>
+__device__ __forceinline__ uint32_t xor_lane(uint32_t v, int lane) {
+  if constexpr (M == 1) return dpp<0xb1>(v);                 // quad_perm [1,0,3,2]
+  else if constexpr (M == 2) return dpp<0x4e>(v);            // quad_perm [2,3,0,1]
+  else if constexpr (M == 4) return dpp<0x1b>(dpp<0x141>(v));  // half mirror (xor 7), then quad_perm [3,2,1,0] (xor 3)
+  else if constexpr (M == 8) return dpp<0x128>(v);           // row_ror:8
+  else if constexpr (M == 16) {
+    const u32x2 r = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+    return lane & 16 ? r.x : r.y;
+  } else {
+    const u32x2 r = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+    return lane & 32 ? r.x : r.y;
+  }
 }
 
 // bitonic sort of 64 * PER entries, descending; entry lane * PER + i: steps shorter than PER stay in the lane's registers
+template <int PER, int LS>
+__device__ __forceinline__ void sort_step(unsigned long long (&e)[PER], int lane, int size) {
+  const bool first = ((lane & LS) == 0) == (((lane * PER) & size) == 0);  // this lane keeps the larger one (size > PER here)
+#pragma unroll
+  for (int i = 0; i < PER; ++i) {
+    const unsigned long long o = ((unsigned long long)xor_lane<LS>((uint32_t)(e[i] >> 32), lane) << 32) | xor_lane<LS>((uint32_t)e[i], lane);
+    e[i] = first == (e[i] > o) ? e[i] : o;
+  }
+}
 template <int PER>
 __device__ __forceinline__ void wave_sort(unsigned long long (&e)[PER], int lane) {
 #pragma unroll 1
   for (int size = 2; size <= 64 * PER; size <<= 1) {
 #pragma unroll 1
-    for (int step = size >> 1; step >= PER; step >>= 1) {
-      const int ls = step / PER;
-      const bool low = (lane & ls) == 0;
-#pragma unroll
-      for (int i = 0; i < PER; ++i) {
-        const unsigned long long o = shfl_xor_u64(e[i], ls);
-        const bool desc = ((lane * PER + i) & size) == 0;
-        e[i] = (low == desc) == (e[i] > o) ? e[i] : o;
+    for (int ls = size / (2 * PER); ls > 0; ls >>= 1) {
+      switch (ls) {
+        case 1: sort_step<PER, 1>(e, lane, size); break;
+        case 2: sort_step<PER, 2>(e, lane, size); break;
+        case 4: sort_step<PER, 4>(e, lane, size); break;
+        case 8: sort_step<PER, 8>(e, lane, size); break;
+        case 16: sort_step<PER, 16>(e, lane, size); break;
+        default: sort_step<PER, 32>(e, lane, size); break;
       }
     }
 #pragma unroll
@@ -115,117 +171,182 @@ __device__ __forceinline__ void wave_sort(unsigned long long (&e)[PER], int lane
   }
 }
 
-// One wave finishes a row from its leading candidates, ranked: entry lane * PER + i = key << 32 | ~index (0: none), all of the first
-// s.k ranks present.  Masses are float64 relative to the best candidate; when everything that carries mass has been drawn the rest is
-// taken relative to the best one left (a low temperature underflows: the definition does not).
+// a row's scores by 16 bytes: f(first index, scores, how many) for the pieces tid, tid + n, ... of [begin, end); four loads in flight
+template <class T>
+constexpr int PIECE = 16 / (int)sizeof(T);
+template <class T, class F>
+__device__ __forceinline__ void scan_row(const T* p, int begin, int end, int tid, int n, F&& f) {
+  constexpr int E = PIECE<T>;
+  const int64_t step = (int64_t)n * E;
+  int64_t j = begin + (int64_t)tid * E;
+  for (; j + 3 * step + E <= end; j += 4 * step) {
+    rp_vec<T, E> v[4];
+#pragma unroll
+    for (int q = 0; q < 4; ++q) v[q] = rp_load_vec<T, E>(p + j + q * step);
+#pragma unroll
+    for (int q = 0; q < 4; ++q) f((int)(j + q * step), v[q], E);
+  }
+  for (; j < end; j += step) {
+    rp_vec<T, E> v;
+    const int m = (int)min((int64_t)E, end - j);
+    if (m == E) v = rp_load_vec<T, E>(p + j);
+    else {
+#pragma unroll
+      for (int i = 0; i < E; ++i) v.v[i] = i < m ? p[j + i] : rp_from_f32<T>(-INFINITY);
+    }
+    f((int)j, v, m);
+  }
+}
+
+// 2^y for -1000 <= y <= 0: Taylor series of exp to the 11th power on [-ln2 / 2, ln2 / 2] (remainder < 2^-47 relative)
+__device__ __forceinline__ double exp2_le0(double y) {
+  const double n = rint(y), f = (y - n) * 0.69314718055994530942;
+  double q = 1.0 / 39916800.0;
+  q = fma(q, f, 1.0 / 3628800.0);
+  q = fma(q, f, 1.0 / 362880.0);
+  q = fma(q, f, 1.0 / 40320.0);
+  q = fma(q, f, 1.0 / 5040.0);
+  q = fma(q, f, 1.0 / 720.0);
+  q = fma(q, f, 1.0 / 120.0);
+  q = fma(q, f, 1.0 / 24.0);
+  q = fma(q, f, 1.0 / 6.0);
+  q = fma(q, f, 0.5);
+  q = fma(q, f, 1.0);
+  q = fma(q, f, 1.0);
+  return ldexp(q, (int)n);
+}
+
+// One wave finishes a row from its leading candidates: sorted[] (in LDS, this wave's own) holds them ranked, key << 32 | ~index, 0 where there
+// is none, all of the first s.k ranks among them.  Register i of lane l holds rank 64 i + l, its mass in float64 relative to the best
+// candidate, and the cumulative mass inside the register; a draw looks for the register and then asks all lanes at once, and only the
+// register that lost a candidate is summed again.  When what is left has next to no mass (a low temperature: the masses underflow, the
+// definition does not) it is taken relative to the best one left.
 template <int PER>
-__device__ void finish_row(const sample_args& a, int64_t r, const row_set& s, const unsigned long long (&e)[PER], int lane) {
+__device__ void finish_row(const sample_args& a, int64_t r, const row_set& s, const unsigned long long* sorted, int lane) {
+  float x[PER];
   int have = 0;
 #pragma unroll
-  for (int i = 0; i < PER; ++i) have += e[i] != 0 && lane * PER + i < s.k ? 1 : 0;
-#pragma unroll
-  for (int d = 1; d < 64; d <<= 1) have += __shfl_xor(have, d);
-  const float best = score_of((uint32_t)__shfl((int)(uint32_t)(e[0] >> 32), 0));
-  const double t = (double)s.temperature;
-  double m[PER];
-  int kept = have;
-  if (s.temperature > 0.0f) {
-    double own = 0.0;
-#pragma unroll
-    for (int i = 0; i < PER; ++i) {
-      m[i] = lane * PER + i < have ? exp(z_of(score_of((uint32_t)(e[i] >> 32)), best, t)) : 0.0;
-      own += m[i];
-    }
-    const double incl = wave_scan_f64(own, lane);
-    const double total = shfl_f64(incl, 63);
-    double c = incl - own;
-    const double border = (double)s.top_p * total;
-    int n = 0;  // leading ranks kept: those with less than top_p of the mass before them and at least min_p of the best one's mass
-#pragma unroll
-    for (int i = 0; i < PER; ++i) {
-      const int rank = lane * PER + i;
-      if (rank < have && (s.top_p >= 1.0f || rank == 0 || c < border) && m[i] >= (double)s.min_p) ++n;
-      c += m[i];
-    }
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) n += __shfl_xor(n, d);
-    kept = n;
+  for (int i = 0; i < PER; ++i) {
+    const uint32_t key = (uint32_t)(sorted[i * 64 + lane] >> 32);
+    x[i] = score_of(key);
+    have += (int)__popcll(__ballot(key != 0 && i * 64 + lane < s.k));
   }
-  const int n_out = min(a.draws, kept);
-  uint32_t gone = 0;  // bit i: rank lane * PER + i has been drawn
+  const bool greedy = s.temperature == 0.0f;
+  const double c = greedy ? 0.0 : 1.4426950408889634074 / (double)s.temperature;
+  float from = __uint_as_float(lane_u32(__float_as_uint(x[0]), 0));  // what the masses are relative to
+  auto mass_of = [&](float v) __attribute__((always_inline)) { return v == from ? 1.0 : exp2_le0(fmax(((double)v - (double)from) * c, -1000.0)); };
+  double m[PER], cum[PER], sum[PER];
+  int kept = have;
+  if (!greedy) {
+    double total = 0.0;
 #pragma unroll
-  for (int i = 0; i < PER; ++i)
-    if (lane * PER + i >= kept) gone |= 1u << i;
-  float from = best;  // what the masses are relative to
-  for (int d = 0; d < n_out; ++d) {
-    int rank;
-    double p = 1.0;
-    if (s.temperature > 0.0f) {
-      double own = 0.0, incl, total;
-      for (;;) {
-        own = 0.0;
+    for (int i = 0; i < PER; ++i) {
+      m[i] = i * 64 + lane < have ? mass_of(x[i]) : 0.0;
+      cum[i] = wave_scan_f64(m[i]);
+      sum[i] = lane_f64(cum[i], 63);
+      total += sum[i];
+    }
+    // leading ranks kept: those with less than top_p of the mass before them and at least min_p of the best one's mass
+    const double border = (double)s.top_p * total;
+    double before = 0.0;
+    kept = 0;
 #pragma unroll
-        for (int i = 0; i < PER; ++i)
-          if (!((gone >> i) & 1)) own += m[i];
-        incl = wave_scan_f64(own, lane);
-        total = shfl_f64(incl, 63);
-        if (total >= 1e-200) break;
-        // the best rank left becomes the reference (it gets mass 1)
-        float top = -INFINITY;
-#pragma unroll
-        for (int i = PER - 1; i >= 0; --i)
-          if (!((gone >> i) & 1)) top = score_of((uint32_t)(e[i] >> 32));
-        const unsigned long long who = __ballot(gone != (PER == 32 ? 0xffffffffu : (1u << PER) - 1u));
-        from = __uint_as_float((uint32_t)__shfl((int)__float_as_uint(top), (int)__ffsll((long long)who) - 1));
-#pragma unroll
-        for (int i = 0; i < PER; ++i)
-          if (!((gone >> i) & 1)) m[i] = exp(z_of(score_of((uint32_t)(e[i] >> 32)), from, t));
-      }
-      float uu = a.u[r * a.ld_u + d];
-      uu = uu > 0.0f ? fminf(uu, 0x1.fffffep-1f) : 0.0f;
-      const double want = (double)uu * total;
-      // the lane whose ranks pass the border; the last one with mass left if rounding lets none pass
-      unsigned long long cand = __ballot(incl > want && own > 0.0);
-      if (!cand) cand = 1ull << (63 - __clzll((long long)__ballot(own > 0.0)));
-      const int who = (int)__ffsll((long long)cand) - 1;
-      double c = incl - own, got = 0.0;
-      int at = 0;
-      bool passed = false;
+    for (int i = 0; i < PER; ++i) {
+      const int rank = i * 64 + lane;
+      kept += (int)__popcll(__ballot(rank < have && (s.top_p >= 1.0f || rank == 0 || before + (cum[i] - m[i]) < border) && m[i] >= (double)s.min_p));
+      before += sum[i];
+    }
+    if (kept < have) {
 #pragma unroll
       for (int i = 0; i < PER; ++i) {
-        if ((gone >> i) & 1) continue;
-        c += m[i];
-        if (!passed && m[i] > 0.0) at = i, got = m[i], passed = c > want;
+        if (i * 64 + lane >= kept) m[i] = 0.0;
+        cum[i] = wave_scan_f64(m[i]);
+        sum[i] = lane_f64(cum[i], 63);
       }
-      rank = __shfl(lane * PER + at, who);
-      p = shfl_f64(got, who) / total;
-    } else {
-      rank = d;
-    }
-    if (rank / PER == lane) {
-      const int i = rank % PER;
-      gone |= 1u << i;
-      unsigned long long v = 0;
-#pragma unroll
-      for (int j = 0; j < PER; ++j) v = j == i ? e[j] : v;
-      const int32_t at = (int32_t)~(uint32_t)v;
-      a.idx[r * a.draws + d] = a.ids ? a.ids[r * a.ld_ids + at] : at;
-      a.prob[r * a.draws + d] = (float)p;
     }
   }
-  for (int d = n_out + lane; d < a.draws; d += 64) {
-    a.idx[r * a.draws + d] = -1;
-    a.prob[r * a.draws + d] = 0.0f;
+  const int n_out = min(a.draws, kept);
+  uint32_t gone = 0;  // bit i: rank 64 i + lane has been drawn
+  for (int d0 = 0; d0 < a.draws; d0 += 64) {  // lane l keeps draw d0 + l
+    const int nd = min(64, n_out - d0);
+    float u = d0 + lane < n_out ? a.u[r * a.ld_u + d0 + lane] : 0.0f;
+    u = u > 0.0f ? fminf(u, 0x1.fffffep-1f) : 0.0f;
+    int rank = d0 + lane;
+    double part = 1.0, whole = 1.0;
+    for (int d = 0; !greedy && d < nd; ++d) {
+      double total = 0.0;
+#pragma unroll
+      for (int i = 0; i < PER; ++i) total += sum[i];
+      if (total < 1e-200) {  // (kept candidates are left)
+        bool looking = true;
+#pragma unroll
+        for (int i = 0; i < PER; ++i) {
+          const unsigned long long left = __ballot(i * 64 + lane < kept && !((gone >> i) & 1));
+          if (looking && left) {
+            from = __uint_as_float(lane_u32(__float_as_uint(x[i]), (int)__ffsll((long long)left) - 1));
+            looking = false;
+          }
+        }
+        total = 0.0;
+#pragma unroll
+        for (int i = 0; i < PER; ++i) {
+          m[i] = i * 64 + lane < kept && !((gone >> i) & 1) ? mass_of(x[i]) : 0.0;
+          cum[i] = wave_scan_f64(m[i]);
+          sum[i] = lane_f64(cum[i], 63);
+          total += sum[i];
+        }
+      }
+      const double want = (double)__uint_as_float(lane_u32(__float_as_uint(u), d)) * total;
+      // the register, then the first lane in it; the last candidate with mass if rounding lets none pass
+      double before = 0.0;
+      int at = -1;
+#pragma unroll
+      for (int i = 0; i < PER; ++i) {
+        if (at >= 0) continue;
+        if (before + sum[i] > want) {  // (the last register with mass at the latest: there before + sum = total, by the same adds, and u < 1)
+          const unsigned long long pass = __ballot(before + cum[i] > want && m[i] > 0.0);
+          const int who = pass ? (int)__ffsll((long long)pass) - 1 : 63 - (int)__clzll((long long)__ballot(m[i] > 0.0));
+          const double got = lane_f64(m[i], who);
+          at = i * 64 + who;
+          if (lane == d) rank = at, part = got, whole = total;
+          if (lane == who) m[i] = 0.0, gone |= 1u << i;
+          cum[i] = wave_scan_f64(m[i]);
+          sum[i] = lane_f64(cum[i], 63);
+        }
+        before += sum[i];
+      }
+    }
+    if (d0 + lane < a.draws) {
+      const bool drawn = d0 + lane < n_out;
+      int32_t item = -1;
+      if (drawn) {
+        const int32_t at = (int32_t) ~(uint32_t)sorted[rank];
+        item = a.ids ? a.ids[r * a.ld_ids + at] : at;
+      }
+      a.idx[r * a.draws + d0 + lane] = item;
+      a.prob[r * a.draws + d0 + lane] = drawn ? (float)(part / whole) : 0.0f;
+    }
   }
   if (lane == 0 && a.nnz) a.nnz[r] = n_out;
+}
+
+// sort in registers, ranks to this wave's LDS
+template <int PER>
+__device__ __forceinline__ void rank_row(unsigned long long (&e)[PER], unsigned long long* sorted, int lane) {
+  wave_sort<PER>(e, lane);
+#pragma unroll
+  for (int i = 0; i < PER; ++i) sorted[lane * PER + i] = e[i];
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");  // (one wave: its LDS accesses stay in order)
+  __builtin_amdgcn_wave_barrier();
 }
 
 // ---- rows that one wave holds ------------------------------------------------------------------------------------------------------
 // One wave per row: up to 64 * PER scores in registers, sorted there.
 template <class T, int PER>
 __global__ __launch_bounds__(256) void k_sample_wave(sample_args a) {
-  const int lane = threadIdx.x & 63;
-  const int64_t r = a.row0 + (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+  __shared__ unsigned long long sorted[4][64 * PER];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int64_t r = a.row0 + (int64_t)blockIdx.x * 4 + wave;
   if (r >= a.rows) return;
   const row_set s = rs_load(a, r);
   const T* p = (const T*)a.scores + r * a.ld;
@@ -236,8 +357,8 @@ __global__ __launch_bounds__(256) void k_sample_wave(sample_args a) {
     const uint32_t k = j < s.len ? key_of(rp_to_f32(p[j])) : 0u;
     e[i] = k ? ((unsigned long long)k << 32) | (uint32_t)~j : 0ull;
   }
-  wave_sort<PER>(e, lane);
-  finish_row<PER>(a, r, s, e, lane);
+  rank_row<PER>(e, sorted[wave], lane);
+  finish_row<PER>(a, r, s, sorted[wave], lane);
 }
 
 // ---- block helpers -------------------------------------------------------------------------------------------------------------------
@@ -255,10 +376,9 @@ __device__ __forceinline__ uint32_t block_max_u32(uint32_t v, uint32_t* red) {
 }
 template <int THREADS>
 __device__ __forceinline__ unsigned long long block_sum_u64(unsigned long long v, unsigned long long* red) {
-#pragma unroll
-  for (int d = 1; d < 64; d <<= 1) v += shfl_xor_u64(v, d);
+  v = wave_scan_u64(v);
   __syncthreads();
-  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
+  if ((threadIdx.x & 63) == 63) red[threadIdx.x >> 6] = v;
   __syncthreads();
   v = 0;
 #pragma unroll
@@ -266,18 +386,65 @@ __device__ __forceinline__ unsigned long long block_sum_u64(unsigned long long v
   return v;
 }
 
-// bitonic sort of n (a power of two <= SL_CAP) entries in LDS, descending
-__device__ void block_sort(unsigned long long* e, int n) {
-  for (int size = 2; size <= n; size <<= 1)
-    for (int step = size >> 1; step > 0; step >>= 1) {
+// bitonic sort of n (a power of two, 64 .. SL_CAP) entries in LDS, descending: steps of 64 and more through LDS, the shorter ones in the
+// registers of a wave that takes 64 entries at a time (15 barriers for 1024 entries instead of 55)
+template <int LS>
+__device__ __forceinline__ void sort_lanes(unsigned long long& e, int lane, bool desc) {
+  const unsigned long long o = ((unsigned long long)xor_lane<LS>((uint32_t)(e >> 32), lane) << 32) | xor_lane<LS>((uint32_t)e, lane);
+  e = (((lane & LS) == 0) == desc) == (e > o) ? e : o;
+}
+__device__ __forceinline__ void block_sort(unsigned long long* e, int n) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  __syncthreads();
+  for (int i = wave * 64 + lane; i < n; i += SL_THREADS) {
+    unsigned long long v = e[i];
+    sort_lanes<1>(v, lane, (i & 2) == 0);
+    sort_lanes<2>(v, lane, (i & 4) == 0);
+    sort_lanes<1>(v, lane, (i & 4) == 0);
+    sort_lanes<4>(v, lane, (i & 8) == 0);
+    sort_lanes<2>(v, lane, (i & 8) == 0);
+    sort_lanes<1>(v, lane, (i & 8) == 0);
+    sort_lanes<8>(v, lane, (i & 16) == 0);
+    sort_lanes<4>(v, lane, (i & 16) == 0);
+    sort_lanes<2>(v, lane, (i & 16) == 0);
+    sort_lanes<1>(v, lane, (i & 16) == 0);
+    sort_lanes<16>(v, lane, (i & 32) == 0);
+    sort_lanes<8>(v, lane, (i & 32) == 0);
+    sort_lanes<4>(v, lane, (i & 32) == 0);
+    sort_lanes<2>(v, lane, (i & 32) == 0);
+    sort_lanes<1>(v, lane, (i & 32) == 0);
+    const bool desc = (i & 64) == 0;
+    sort_lanes<32>(v, lane, desc);
+    sort_lanes<16>(v, lane, desc);
+    sort_lanes<8>(v, lane, desc);
+    sort_lanes<4>(v, lane, desc);
+    sort_lanes<2>(v, lane, desc);
+    sort_lanes<1>(v, lane, desc);
+    e[i] = v;
+  }
+  for (int size = 128; size <= n; size <<= 1) {
+    for (int step = size >> 1; step >= 64; step >>= 1) {
       __syncthreads();
       for (int q = threadIdx.x; q < n / 2; q += SL_THREADS) {
-        const int i = (q / step) * 2 * step + q % step, j = i + step;
+        const int i = (q & ~(step - 1)) * 2 + (q & (step - 1)), j = i + step;
         const unsigned long long x = e[i], y = e[j];
         const bool desc = (i & size) == 0;
         if (desc ? x < y : x > y) e[i] = y, e[j] = x;
       }
     }
+    __syncthreads();
+    for (int i = wave * 64 + lane; i < n; i += SL_THREADS) {
+      unsigned long long v = e[i];
+      const bool desc = (i & size) == 0;
+      sort_lanes<32>(v, lane, desc);
+      sort_lanes<16>(v, lane, desc);
+      sort_lanes<8>(v, lane, desc);
+      sort_lanes<4>(v, lane, desc);
+      sort_lanes<2>(v, lane, desc);
+      sort_lanes<1>(v, lane, desc);
+      e[i] = v;
+    }
+  }
   __syncthreads();
 }
 
@@ -289,7 +456,7 @@ struct sel_shared {
   uint32_t digit, before;
 };
 template <class T>
-__device__ uint32_t select_key(const T* p, int len, int n, sel_shared& sh, int* equal) {
+__device__ __forceinline__ uint32_t select_key(const T* p, int len, int n, sel_shared& sh, int* equal) {
   uint32_t prefix = 0, left = (uint32_t)n;
   for (int shift = 24; shift >= 0; shift -= 8) {
     __syncthreads();
@@ -322,55 +489,118 @@ __device__ uint32_t select_key(const T* p, int len, int n, sel_shared& sh, int* 
 // k <= 1024: one workgroup per row finds a score that at least k candidates reach, collects those candidates, ranks them.
 // The threshold: every thread takes the best of two groups of the row's scores; if k of those 2048 group maxima reach a value, k
 // candidates do.  For rows in no particular order few more than k candidates reach the k-th largest group maximum (1.1 k at k = 200,
-// 1.4 k at 1000).  Rows that break this - thousands of equal scores - take the radix descent.
-template <class T>
-__global__ __launch_bounds__(SL_THREADS) void k_sample_topk(sample_args a) {
+// 1.4 k at 1000).  Rows that break this - thousands of equal scores - take the radix descent.  CACHED: the row stays in registers between
+// the two passes over it (up to TK_CACHE pieces of 16 bytes a thread).
+constexpr int TK_CACHE = 8;
+template <class T, bool CACHED>
+__global__ __launch_bounds__(SL_THREADS, 8) void k_sample_topk(sample_args a, unsigned long long* __restrict__ lists, int32_t* __restrict__ counts, int cap) {
+  constexpr int E = PIECE<T>;
   __shared__ unsigned long long list[SL_CAP];
-  __shared__ uint32_t red[SL_THREADS / 64];
+  __shared__ uint32_t red[2][SL_THREADS / 64], tally[3][3];
   __shared__ uint32_t n_list, cnt;
   __shared__ sel_shared sel;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int64_t r = a.row0 + blockIdx.x;
   const row_set s = rs_load(a, r);
   const T* p = (const T*)a.scores + r * a.ld;
-  uint32_t g0 = 0, g1 = 0;
-  {
-    int j = threadIdx.x;
-    for (; j + SL_THREADS < s.len; j += 2 * SL_THREADS) {
-      g0 = max(g0, key_of(rp_to_f32(p[j])));
-      g1 = max(g1, key_of(rp_to_f32(p[j + SL_THREADS])));
-    }
-    if (j < s.len) g0 = max(g0, key_of(rp_to_f32(p[j])));
-  }
-  // the largest prefix of key bits that at least k group maxima reach; 1 (every candidate) if fewer than k groups have one
-  uint32_t floor_key = 0;
-  for (int bit = 31; bit >= 0; --bit) {
-    const uint32_t t = floor_key | (1u << bit);
-    __syncthreads();
-    if (threadIdx.x == 0) cnt = 0;
-    __syncthreads();
-    const uint32_t c = (uint32_t)__popcll(__ballot(g0 >= t)) + (uint32_t)__popcll(__ballot(g1 >= t));
-    if (lane == 0 && c) atomicAdd(&cnt, c);
-    __syncthreads();
-    const uint32_t n = cnt;
-    if (n >= (uint32_t)s.k) {
-      floor_key = t;
-      if (n <= (uint32_t)s.k + (uint32_t)s.k / 4) break;
-    }
-  }
-  if (floor_key == 0) floor_key = 1;
-  __syncthreads();
   if (threadIdx.x == 0) n_list = 0;
-  __syncthreads();
-  for (int j0 = wave * 64; j0 < s.len; j0 += SL_THREADS) {
-    const int j = j0 + lane;
-    const uint32_t k = j < s.len ? key_of(rp_to_f32(p[j])) : 0u;
-    const unsigned long long hit = __ballot(k >= floor_key);
-    if (hit == 0) continue;
-    uint32_t at = 0;
-    if (lane == 0) at = atomicAdd(&n_list, (uint32_t)__popcll(hit));
-    at = (uint32_t)__shfl((int)at, 0) + (uint32_t)__popcll(hit & ((1ull << lane) - 1ull));
-    if (k >= floor_key && at < SL_CAP) list[at] = ((unsigned long long)k << 32) | (uint32_t)~j;
+  rp_vec<T, E> held[CACHED ? TK_CACHE : 1];
+  float f0 = -INFINITY, f1 = -INFINITY;
+  auto maxima = [&](const rp_vec<T, E>& v) __attribute__((always_inline)) {  // (as numbers: the maximum leaves NaN out)
+#pragma unroll
+    for (int i = 0; i < E / 2; ++i) {
+      f0 = fmaxf(f0, rp_to_f32(v.v[i]));
+      f1 = fmaxf(f1, rp_to_f32(v.v[i + E / 2]));
+    }
+  };
+  if constexpr (CACHED) {
+#pragma unroll
+    for (int q = 0; q < TK_CACHE; ++q) {
+      const int j = (q * SL_THREADS + (int)threadIdx.x) * E;
+      if (j + E <= s.len) held[q] = rp_load_vec<T, E>(p + j);
+      else {
+#pragma unroll
+        for (int i = 0; i < E; ++i) held[q].v[i] = j + i < s.len ? p[j + i] : rp_from_f32<T>(-INFINITY);
+      }
+    }
+#pragma unroll
+    for (int q = 0; q < TK_CACHE; ++q) maxima(held[q]);
+  } else {
+    scan_row<T>(p, 0, s.len, threadIdx.x, SL_THREADS, [&](int, const rp_vec<T, E>& v, int) __attribute__((always_inline)) { maxima(v); });
+  }
+  const uint32_t g0 = key_of(f0), g1 = key_of(f1);
+  // a value that at least k group maxima reach, and hardly more: four-way search between the least and the largest of them.  lo is always
+  // reached by k (at 0 by all 2048), hi never.
+  uint32_t lo, hi;
+  {
+    uint32_t v_hi = max(g0, g1), v_lo = ~min(g0, g1);
+    v_hi = max(v_hi, xor_lane<1>(v_hi, lane)), v_lo = max(v_lo, xor_lane<1>(v_lo, lane));
+    v_hi = max(v_hi, xor_lane<2>(v_hi, lane)), v_lo = max(v_lo, xor_lane<2>(v_lo, lane));
+    v_hi = max(v_hi, xor_lane<4>(v_hi, lane)), v_lo = max(v_lo, xor_lane<4>(v_lo, lane));
+    v_hi = max(v_hi, xor_lane<8>(v_hi, lane)), v_lo = max(v_lo, xor_lane<8>(v_lo, lane));
+    v_hi = max(v_hi, xor_lane<16>(v_hi, lane)), v_lo = max(v_lo, xor_lane<16>(v_lo, lane));
+    v_hi = max(v_hi, xor_lane<32>(v_hi, lane)), v_lo = max(v_lo, xor_lane<32>(v_lo, lane));
+    if (lane == 0) red[0][wave] = v_hi, red[1][wave] = v_lo;
+    if (threadIdx.x < 9) tally[threadIdx.x / 3][threadIdx.x % 3] = 0;
+    __syncthreads();
+    hi = 0, lo = 0;
+#pragma unroll
+    for (int w = 0; w < SL_THREADS / 64; ++w) hi = max(hi, red[0][w]), lo = max(lo, red[1][w]);
+    lo = ~lo;
+    hi += hi != 0xffffffffu;
+  }
+  const uint32_t k = (uint32_t)s.k, enough = k + k / 4;
+  for (int it = 0; hi - lo > 1; it = it == 2 ? 0 : it + 1) {
+    const uint32_t q = max((hi - lo) / 4, 1u);
+    const uint32_t t1 = lo + q, t2 = min(t1 + q, hi), t3 = min(t2 + q, hi);
+    const uint32_t c1 = (uint32_t)__popcll(__ballot(g0 >= t1)) + (uint32_t)__popcll(__ballot(g1 >= t1));
+    const uint32_t c2 = (uint32_t)__popcll(__ballot(g0 >= t2)) + (uint32_t)__popcll(__ballot(g1 >= t2));
+    const uint32_t c3 = (uint32_t)__popcll(__ballot(g0 >= t3)) + (uint32_t)__popcll(__ballot(g1 >= t3));
+    if (lane == 0) {
+      if (c1) atomicAdd(&tally[it][0], c1);
+      if (c2) atomicAdd(&tally[it][1], c2);
+      if (c3) atomicAdd(&tally[it][2], c3);
+    }
+    __syncthreads();  // (one barrier a step: the tallies of three steps take turns, the one of the step before is cleared here)
+    const uint32_t n1 = tally[it][0], n2 = tally[it][1], n3 = tally[it][2];
+    if (threadIdx.x < 3) tally[it == 0 ? 2 : it - 1][threadIdx.x] = 0;
+    uint32_t at;
+    if (n3 >= k) lo = t3, at = n3;
+    else if (n2 >= k) lo = t2, hi = t3, at = n2;
+    else if (n1 >= k) lo = t1, hi = t2, at = n1;
+    else hi = t1, at = 0xffffffffu;
+    if (at <= enough) break;
+  }
+  const float least = lo > 0x00800000u ? score_of(lo) : -FLT_MAX;  // (every candidate: neither -inf nor NaN passes)
+  auto take = [&](int j, const rp_vec<T, E>& v) __attribute__((always_inline)) {
+    float top = rp_to_f32(v.v[0]);
+#pragma unroll
+    for (int i = 1; i < E; ++i) top = fmaxf(top, rp_to_f32(v.v[i]));
+    if (!(top >= least)) return;
+#pragma unroll
+    for (int i = 0; i < E; ++i) {
+      const float x = rp_to_f32(v.v[i]);
+      if (x >= least) {
+        const uint32_t at = atomicAdd(&n_list, 1u);
+        if (at < SL_CAP) list[at] = ((unsigned long long)key_of(x) << 32) | (uint32_t) ~(j + i);
+      }
+    }
+  };
+  if constexpr (CACHED) {
+    unsigned long long hits = 0;  // bit q E + i; the few that pass are read again
+#pragma unroll
+    for (int q = 0; q < TK_CACHE; ++q)
+#pragma unroll
+      for (int i = 0; i < E; ++i) hits |= rp_to_f32(held[q].v[i]) >= least ? 1ull << (q * E + i) : 0ull;
+    while (hits) {
+      const int bit = (int)__ffsll((long long)hits) - 1;
+      hits &= hits - 1;
+      const int j = (bit / E * SL_THREADS + (int)threadIdx.x) * E + bit % E;
+      const uint32_t at = atomicAdd(&n_list, 1u);
+      if (at < SL_CAP) list[at] = ((unsigned long long)key_of(rp_to_f32(p[j])) << 32) | (uint32_t)~j;
+    }
+  } else {
+    scan_row<T>(p, 0, s.len, threadIdx.x, SL_THREADS, [&](int j, const rp_vec<T, E>& v, int) __attribute__((always_inline)) { take(j, v); });
   }
   __syncthreads();
   int n = (int)n_list;
@@ -382,75 +612,87 @@ __global__ __launch_bounds__(SL_THREADS) void k_sample_topk(sample_args a) {
     __syncthreads();
     for (int j0 = 0; j0 < s.len; j0 += SL_THREADS) {  // in index order: the first `equal` ties are taken
       const int j = j0 + threadIdx.x;
-      const uint32_t k = j < s.len ? key_of(rp_to_f32(p[j])) : 0u;
-      const unsigned long long tie = __ballot(k == kk);
+      const uint32_t key = j < s.len ? key_of(rp_to_f32(p[j])) : 0u;
+      const unsigned long long tie = __ballot(key == kk);
       __syncthreads();
-      if (lane == 0) red[wave] = (uint32_t)__popcll(tie);
+      if (lane == 0) red[0][wave] = (uint32_t)__popcll(tie);
       __syncthreads();
       uint32_t before = cnt, all = 0;
       for (int w = 0; w < SL_THREADS / 64; ++w) {
-        before += w < wave ? red[w] : 0u;
-        all += red[w];
+        before += w < wave ? red[0][w] : 0u;
+        all += red[0][w];
       }
-      const bool take = k > kk || (k == kk && before + (uint32_t)__popcll(tie & ((1ull << lane) - 1ull)) < (uint32_t)equal);
-      if (take) list[atomicAdd(&n_list, 1u)] = ((unsigned long long)k << 32) | (uint32_t)~j;  // (s.k <= 1024 entries in all)
+      const bool in = key > kk || (key == kk && before + (uint32_t)__popcll(tie & ((1ull << lane) - 1ull)) < (uint32_t)equal);
+      if (in) list[atomicAdd(&n_list, 1u)] = ((unsigned long long)key << 32) | (uint32_t)~j;  // (s.k <= 1024 entries in all)
       __syncthreads();
       if (threadIdx.x == 0) cnt += all;
     }
     __syncthreads();
     n = (int)n_list;
   }
-  if (n > RPS_SHORT) {
-    int n2 = 2 * RPS_SHORT;
+  if (n > cap) {  // more than one wave ranks (ties, or an order the groups did not expect): the best `cap`, s.k of them count
+    int n2 = 512;
     while (n2 < n) n2 <<= 1;
     for (int i = n + threadIdx.x; i < n2; i += SL_THREADS) list[i] = 0;
     block_sort(list, n2);
-    n = RPS_SHORT;  // (s.k of them count)
+    n = cap;
   }
-  if (wave != 0) return;
-  if (n <= 256) {
-    unsigned long long e[4];
+  if ((int)threadIdx.x < n) lists[(int64_t)blockIdx.x * cap + threadIdx.x] = list[threadIdx.x];
+  if (threadIdx.x == 0) counts[blockIdx.x] = n;
+}
+
+// ... and one wave per row ranks them and draws (its 90 - 170 registers would halve the selection's workgroups per CU)
+template <int PER>
+__device__ __forceinline__ void rank_list(const unsigned long long* __restrict__ list, int n, unsigned long long* sorted, int lane) {
+  unsigned long long e[PER];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) e[i] = lane * 4 + i < n ? list[lane * 4 + i] : 0ull;
-    wave_sort<4>(e, lane);
-    finish_row<4>(a, r, s, e, lane);
-  } else {
-    unsigned long long e[16];
-#pragma unroll
-    for (int i = 0; i < 16; ++i) e[i] = lane * 16 + i < n ? list[lane * 16 + i] : 0ull;
-    wave_sort<16>(e, lane);
-    finish_row<16>(a, r, s, e, lane);
-  }
+  for (int i = 0; i < PER; ++i) e[i] = i * 64 + lane < n ? list[i * 64 + lane] : 0ull;
+  rank_row<PER>(e, sorted, lane);
+}
+// (CAP: the lists' length; KEEP >= k: what the draws look at)
+template <int CAP, int KEEP>
+__global__ __launch_bounds__(64) void k_sample_lists(sample_args a, const unsigned long long* __restrict__ lists, const int32_t* __restrict__ counts) {
+  __shared__ unsigned long long sorted[CAP];
+  const int lane = threadIdx.x;
+  const int64_t r = a.row0 + blockIdx.x;
+  const int n = counts[blockIdx.x];
+  const row_set s = rs_load(a, r);
+  const unsigned long long* list = lists + (int64_t)blockIdx.x * CAP;
+  if (CAP > KEEP && n <= KEEP) rank_list<KEEP / 64>(list, n, sorted, lane);
+  else rank_list<CAP / 64>(list, n, sorted, lane);
+  finish_row<KEEP / 64>(a, r, s, sorted, lane);
 }
 
 // ---- whole rows, any prefix, one draw ------------------------------------------------------------------------------------------------
-// 2^(z log2 e) for z <= 0 in fixed point: Taylor to the 11th power on [-1/2, 1/2] (remainder < 2^-47 relative), 0 below 2^-shift.
-__device__ __forceinline__ double exp_le0(double z) {
-  const double t = fmax(z * 1.4426950408889634074, -1000.0);
-  const double n = rint(t), f = (t - n) * 0.69314718055994530942;
-  double q = 1.0 / 39916800.0;
-  q = fma(q, f, 1.0 / 3628800.0);
-  q = fma(q, f, 1.0 / 362880.0);
-  q = fma(q, f, 1.0 / 40320.0);
-  q = fma(q, f, 1.0 / 5040.0);
-  q = fma(q, f, 1.0 / 720.0);
-  q = fma(q, f, 1.0 / 120.0);
-  q = fma(q, f, 1.0 / 24.0);
-  q = fma(q, f, 1.0 / 6.0);
-  q = fma(q, f, 0.5);
-  q = fma(q, f, 1.0);
-  q = fma(q, f, 1.0);
-  return ldexp(q, (int)n);
-}
-
+// masses of a row's candidates relative to its best score
 struct row_mass {
   float best;
-  double t;      // temperature
+  double c;      // log2(e) / temperature
   double scale;  // 2^shift
   bool greedy;
-  __device__ __forceinline__ double z(float x) const { return x == best ? 0.0 : greedy ? -1000.0 : ((double)x - (double)best) / t; }
-  __device__ __forceinline__ int bin(double z) const { return (int)fmin(-z * (double)SB_PER_E, (double)(SB_BINS - 1)); }
-  __device__ __forceinline__ unsigned long long mass(double z) const { return z <= -690.0 ? 0ull : (unsigned long long)rint(exp_le0(z) * scale); }
+  // base-2 logarithm of the mass: 0 for the best score (+inf among them)
+  __device__ __forceinline__ double log2_of(float x) const { return x == best ? 0.0 : greedy ? -1000.0 : fmax(((double)x - (double)best) * c, -1000.0); }
+  __device__ __forceinline__ int bin(double y) const { return (int)fmin(y * (-SB_PER_E * 0.69314718055994530942), (double)(SB_BINS - 1)); }
+  __device__ __forceinline__ unsigned long long mass(double y) const { return (unsigned long long)rint(exp2_le0(y) * scale); }
+};
+__device__ __forceinline__ row_mass rm_make(uint32_t best, const row_set& s, int shift) {
+  row_mass rm;
+  rm.best = score_of(best);
+  rm.greedy = s.temperature == 0.0f;
+  rm.c = rm.greedy ? 1.0 : 1.4426950408889634074 / (double)s.temperature;
+  rm.scale = ldexp(1.0, shift);
+  return rm;
+}
+
+// a row's part of the workspace
+struct row_ws {
+  unsigned long long hist_m[SB_BINS];  // masses per bin
+  unsigned long long above, count;     // mass of the candidates with at least min_p of the best one's mass; candidates
+  unsigned long long list[2][SB_CAP];  // candidates of bin b1 (where top-p ends) and of the bins b2 (where the draw can fall)
+  uint32_t hist_c[SB_BINS];            // candidates per bin
+  uint32_t n_list[2];
+  int32_t b1, b2_lo, b2_hi;            // b1 < 0: top-p does not cut; b2_hi < b2_lo: nothing was collected
+  uint32_t best[64];                   // per slice
 };
 
 struct seek_shared {
@@ -463,74 +705,88 @@ struct seek_shared {
   uint32_t hist_c[256];
 };
 
-// First candidate in rank order with (by_count: rank + 1 >= target; otherwise: cumulative mass up to and with it >= target).  hist_m /
-// hist_c: the row's masses and counts per bin.  Returns its index (-1: none) and, in *incl / *own, the cumulative mass with it and its own.
+// Cumulative masses (and counts) over the bins, thread t owning the bins [t PB, (t + 1) PB): before[] are the sums in front of them.
+template <int THREADS>
+__device__ __forceinline__ unsigned long long scan_bins(const unsigned long long (&v)[SB_BINS / THREADS], unsigned long long (&before)[SB_BINS / THREADS],
+                                                        unsigned long long* red) {
+  unsigned long long own = 0;
+#pragma unroll
+  for (int i = 0; i < SB_BINS / THREADS; ++i) own += v[i];
+  const unsigned long long incl = wave_scan_u64(own);
+  const int wave = threadIdx.x >> 6;
+  __syncthreads();
+  if ((threadIdx.x & 63) == 63) red[wave] = incl;
+  __syncthreads();
+  unsigned long long run = incl - own, total = 0;
+#pragma unroll
+  for (int w = 0; w < THREADS / 64; ++w) {
+    run += w < wave ? red[w] : 0ull;
+    total += red[w];
+  }
+#pragma unroll
+  for (int i = 0; i < SB_BINS / THREADS; ++i) {
+    before[i] = run;
+    run += v[i];
+  }
+  return total;
+}
+
+__device__ __forceinline__ unsigned long long border_of(float top_p, unsigned long long total) { return max((unsigned long long)ceil((double)top_p * (double)total), 1ull); }
+__device__ __forceinline__ unsigned long long want_of(float u, unsigned long long kept) {
+  u = u > 0.0f ? fminf(u, 0x1.fffffep-1f) : 0.0f;
+  return min((unsigned long long)floor((double)u * (double)kept) + 1ull, kept);
+}
+
+// First candidate in rank order with (by_count: rank + 1 >= target; otherwise: cumulative mass up to and with it >= target).
+// list / n_list: the candidates of the bins lo .. hi, if they were collected ahead (n_list <= SB_CAP).  Returns its index (-1: none) and,
+// in *incl / *own, the cumulative mass with it and its own.
 template <class T>
-__device__ int seek(const T* p, int len, const row_mass& rm, const unsigned long long* hist_m, const uint32_t* hist_c, bool by_count, unsigned long long target,
-                    seek_shared& sh, unsigned long long* incl, unsigned long long* own) {
+__device__ __forceinline__ int seek(const T* p, int len, const row_mass& rm, const row_ws& ws, bool by_count, unsigned long long target, seek_shared& sh, const unsigned long long* ahead,
+                    int n_ahead, int lo, int hi, unsigned long long* incl, unsigned long long* own) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  // the bin: thread t owns the bins [4 t, 4 t + 4)
   constexpr int PB = SB_BINS / SL_THREADS;
-  unsigned long long c[PB], m[PB], sc = 0, sm = 0;
+  unsigned long long m[PB], c[PB], bm[PB], bc[PB];
 #pragma unroll
   for (int i = 0; i < PB; ++i) {
-    m[i] = hist_m[threadIdx.x * PB + i];
-    c[i] = hist_c ? hist_c[threadIdx.x * PB + i] : 0u;
-    sc += c[i];
-    sm += m[i];
+    m[i] = ws.hist_m[threadIdx.x * PB + i];
+    c[i] = by_count ? ws.hist_c[threadIdx.x * PB + i] : 0u;
+    bc[i] = 0;
   }
-  unsigned long long ic = sc, im = sm;
-#pragma unroll
-  for (int d = 1; d < 64; d <<= 1) {
-    const uint32_t a0 = __shfl_up((uint32_t)ic, d), a1 = __shfl_up((uint32_t)(ic >> 32), d), b0 = __shfl_up((uint32_t)im, d), b1 = __shfl_up((uint32_t)(im >> 32), d);
-    if (lane >= d) {
-      ic += ((unsigned long long)a1 << 32) | a0;
-      im += ((unsigned long long)b1 << 32) | b0;
-    }
-  }
-  __syncthreads();
-  if (lane == 63) sh.red64[wave] = by_count ? ic : im;
   if (threadIdx.x == 0) sh.bin = SB_BINS, sh.n_list = 0, sh.found = 0xffffffffu;
-  __syncthreads();
-  unsigned long long run = (by_count ? ic - sc : im - sm);
-  for (int w = 0; w < wave; ++w) run += sh.red64[w];
-  // masses before the bin are wanted for both kinds of target
-  unsigned long long run_m = im - sm;
-  __syncthreads();
-  if (lane == 63) sh.red64[wave] = im;
-  __syncthreads();
-  for (int w = 0; w < wave; ++w) run_m += sh.red64[w];
+  scan_bins<SL_THREADS>(m, bm, sh.red64);
+  if (by_count) scan_bins<SL_THREADS>(c, bc, sh.red64);
 #pragma unroll
   for (int i = 0; i < PB; ++i) {
-    const unsigned long long step = by_count ? c[i] : m[i];
-    if (run < target && run + step >= target) {
-      sh.bin = threadIdx.x * PB + i;
-      sh.before32 = (uint32_t)(by_count ? run : 0);
-      sh.before64 = run_m;
-    }
-    run += step;
-    run_m += m[i];
+    const unsigned long long run = by_count ? bc[i] : bm[i], step = by_count ? c[i] : m[i];
+    if (run < target && run + step >= target) sh.bin = threadIdx.x * PB + i;
   }
+  __syncthreads();
+  const bool have = n_ahead >= 0 && (int)sh.bin >= lo && (int)sh.bin <= hi;  // (never by count)
+#pragma unroll
+  for (int i = 0; i < PB; ++i)
+    if ((int)threadIdx.x * PB + i == (have ? lo : (int)sh.bin)) sh.before64 = bm[i], sh.before32 = (uint32_t)bc[i];
   __syncthreads();
   const int b = (int)sh.bin;
   if (b >= SB_BINS) return -1;
   unsigned long long mass_before = sh.before64;
   unsigned long long count_before = sh.before32;
-  // collect the bin
-  for (int j0 = wave * 64; j0 < len; j0 += SL_THREADS) {
-    const int j = j0 + lane;
-    const float x = j < len ? rp_to_f32(p[j]) : 0.0f;
-    const uint32_t k = j < len ? key_of(x) : 0u;
-    const bool in = k != 0 && rm.bin(rm.z(score_of(k))) == b;
-    const unsigned long long hit = __ballot(in);
-    if (hit == 0) continue;
-    uint32_t at = 0;
-    if (lane == 0) at = atomicAdd(&sh.n_list, (uint32_t)__popcll(hit));
-    at = (uint32_t)__shfl((int)at, 0) + (uint32_t)__popcll(hit & ((1ull << lane) - 1ull));
-    if (in && at < SL_CAP) sh.list[at] = ((unsigned long long)k << 32) | (uint32_t)~j;
+  int n = n_ahead;
+  if (have) {
+    for (int i = threadIdx.x; i < n; i += SL_THREADS) sh.list[i] = ahead[i];
+  } else {  // collect the bin
+    scan_row<T>(p, 0, len, threadIdx.x, SL_THREADS, [&](int j, const rp_vec<T, PIECE<T>>& v, int) __attribute__((always_inline)) {
+#pragma unroll
+      for (int i = 0; i < PIECE<T>; ++i) {
+        const uint32_t k = key_of(rp_to_f32(v.v[i]));
+        if (k != 0 && rm.bin(rm.log2_of(score_of(k))) == b) {
+          const uint32_t at = atomicAdd(&sh.n_list, 1u);
+          if (at < SL_CAP) sh.list[at] = ((unsigned long long)k << 32) | (uint32_t) ~(j + i);
+        }
+      }
+    });
+    __syncthreads();
+    n = (int)sh.n_list;
   }
-  __syncthreads();
-  const int n = (int)sh.n_list;
   if (n <= SL_CAP) {
     int n2 = 64;
     while (n2 < n) n2 <<= 1;
@@ -539,13 +795,8 @@ __device__ int seek(const T* p, int len, const row_mass& rm, const unsigned long
     // cumulative sums along the sorted list: 1024 entries at a time
     for (int i0 = 0; i0 < n; i0 += SL_THREADS) {
       const int i = i0 + threadIdx.x;
-      const unsigned long long mine = i < n ? rm.mass(rm.z(score_of((uint32_t)(sh.list[i] >> 32)))) : 0ull;
-      unsigned long long s = mine;
-#pragma unroll
-      for (int d = 1; d < 64; d <<= 1) {
-        const uint32_t b0 = __shfl_up((uint32_t)s, d), b1 = __shfl_up((uint32_t)(s >> 32), d);
-        if (lane >= d) s += ((unsigned long long)b1 << 32) | b0;
-      }
+      const unsigned long long mine = i < n ? rm.mass(rm.log2_of(score_of((uint32_t)(sh.list[i] >> 32)))) : 0ull;
+      const unsigned long long s = wave_scan_u64(mine);
       __syncthreads();
       if (lane == 63) sh.red64[wave] = s;
       __syncthreads();
@@ -581,7 +832,7 @@ __device__ int seek(const T* p, int len, const row_mass& rm, const unsigned long
     for (int j = threadIdx.x; j < len; j += SL_THREADS) {
       const uint32_t k = key_of(rp_to_f32(p[j]));
       if (k == 0 || (shift != 24 && (k >> (shift + 8)) != (prefix >> (shift + 8)))) continue;
-      const double z = rm.z(score_of(k));
+      const double z = rm.log2_of(score_of(k));
       if (rm.bin(z) != b) continue;
       atomicAdd(&sh.hist_c[(k >> shift) & 255], 1u);
       const unsigned long long mm = rm.mass(z);
@@ -605,7 +856,7 @@ __device__ int seek(const T* p, int len, const row_mass& rm, const unsigned long
     count_before = sh.before32;
     mass_before = sh.before64;
   }
-  const unsigned long long each = rm.mass(rm.z(score_of(prefix)));
+  const unsigned long long each = rm.mass(rm.log2_of(score_of(prefix)));
   // the ordinal among the equal scores
   const unsigned long long nth = by_count ? target - count_before : each ? (target - mass_before + each - 1) / each : 1ull;
   *incl = mass_before + nth * each;
@@ -634,20 +885,177 @@ __device__ int seek(const T* p, int len, const row_mass& rm, const unsigned long
   return (int)sh.found;
 }
 
-// One workgroup per row: best score, masses and counts per bin, then three seeks - the k-th candidate (only if k cuts), the end of the
-// top-p prefix, the draw.
+// The whole-row form runs in four launches, the first three with a row's slices spread over workgroups:
+//   best     the slices' best scores; clears the row's workspace
+//   hist     masses and counts per bin (fixed point: the order of the atomics does not matter)
+//   collect  the candidates of the bin where top-p ends and of the bins where the draw can fall (known up to one bin's mass)
+//   draw     one workgroup: the exact end of the kept prefix, then the draw
+// Read three times, from memory once where it fits the caches.
+__device__ __forceinline__ void slice_of(int len, int slices, int s, int& begin, int& end) {
+  const int64_t pieces = ((int64_t)len + 7) / 8;
+  begin = (int)(pieces * s / slices * 8);
+  end = (int)min(pieces * (s + 1) / slices * 8, (int64_t)len);
+}
+
 template <class T>
-__global__ __launch_bounds__(SL_THREADS) void k_sample_row(sample_args a, int shift) {
+__global__ __launch_bounds__(SR_THREADS) void k_row_best(sample_args a, row_ws* __restrict__ wss) {
+  __shared__ uint32_t red[SR_THREADS / 64];
+  const int slices = gridDim.y, sl = blockIdx.y;
+  const int64_t r = a.row0 + blockIdx.x;
+  row_ws& ws = wss[blockIdx.x];
+  for (int i = sl * SR_THREADS + threadIdx.x; i < SB_BINS; i += slices * SR_THREADS) ws.hist_m[i] = 0, ws.hist_c[i] = 0;
+  if (sl == 0 && threadIdx.x == 0) ws.above = 0, ws.count = 0, ws.n_list[0] = 0, ws.n_list[1] = 0;
+  const row_set s = rs_load(a, r);
+  int begin, end;
+  slice_of(s.len, slices, sl, begin, end);
+  uint32_t best = 0;
+  scan_row<T>((const T*)a.scores + r * a.ld, begin, end, threadIdx.x, SR_THREADS, [&](int, const rp_vec<T, PIECE<T>>& v, int) __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < PIECE<T>; ++i) best = max(best, key_of(rp_to_f32(v.v[i])));
+  });
+  best = block_max_u32<SR_THREADS>(best, red);
+  if (threadIdx.x == 0) ws.best[sl] = best;
+}
+
+__device__ __forceinline__ uint32_t best_of(const row_ws& ws, int slices) {
+  uint32_t best = 0;
+  for (int i = 0; i < slices; ++i) best = max(best, ws.best[i]);
+  return best;
+}
+
+template <class T, bool COUNT>
+__global__ __launch_bounds__(SR_THREADS) void k_row_hist(sample_args a, row_ws* __restrict__ wss, int shift) {
   __shared__ unsigned long long hist_m[SB_BINS];
-  __shared__ uint32_t hist_c[SB_BINS];
+  __shared__ uint32_t hist_c[COUNT ? SB_BINS : 1];
+  __shared__ unsigned long long red[SR_THREADS / 64];
+  const int slices = gridDim.y, sl = blockIdx.y;
+  const int64_t r = a.row0 + blockIdx.x;
+  row_ws& ws = wss[blockIdx.x];
+  const row_set s = rs_load(a, r);
+  const uint32_t best = best_of(ws, slices);
+  if (best == 0) return;
+  const row_mass rm = rm_make(best, s, shift);
+  for (int i = threadIdx.x; i < SB_BINS; i += SR_THREADS) {
+    hist_m[i] = 0;
+    if (COUNT) hist_c[i] = 0;
+  }
+  __syncthreads();
+  int begin, end;
+  slice_of(s.len, slices, sl, begin, end);
+  unsigned long long above = 0, count = 0;
+  const double least = (double)s.min_p;
+  scan_row<T>((const T*)a.scores + r * a.ld, begin, end, threadIdx.x, SR_THREADS, [&](int, const rp_vec<T, PIECE<T>>& v, int) __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < PIECE<T>; ++i) {
+      const uint32_t k = key_of(rp_to_f32(v.v[i]));
+      if (k == 0) continue;
+      const double y = rm.log2_of(score_of(k));
+      const double e = exp2_le0(y);
+      const unsigned long long m = (unsigned long long)rint(e * rm.scale);
+      const int b = rm.bin(y);
+      if (m) atomicAdd(&hist_m[b], m);
+      if (COUNT) {
+        atomicAdd(&hist_c[b], 1u);
+        ++count;
+      }
+      if (e >= least) above += m;
+    }
+  });
+  above = block_sum_u64<SR_THREADS>(above, red);
+  if (COUNT) count = block_sum_u64<SR_THREADS>(count, red);
+  __syncthreads();
+  for (int i = threadIdx.x; i < SB_BINS; i += SR_THREADS) {
+    if (hist_m[i]) atomicAdd(&ws.hist_m[i], hist_m[i]);
+    if (COUNT && hist_c[i]) atomicAdd(&ws.hist_c[i], hist_c[i]);
+  }
+  if (threadIdx.x == 0) {
+    if (above) atomicAdd(&ws.above, above);
+    if (COUNT && count) atomicAdd(&ws.count, count);
+  }
+}
+
+template <class T, bool COUNT>
+__global__ __launch_bounds__(SR_THREADS) void k_row_collect(sample_args a, row_ws* __restrict__ wss, int slices, int shift) {
+  __shared__ unsigned long long red[SR_THREADS / 64];
+  __shared__ unsigned long long range[2];
+  __shared__ int bins[3];
+  __shared__ unsigned long long found[2][RC_FOUND];
+  __shared__ uint32_t n_found[2], at_found[2];
+  const int sl = blockIdx.y;
+  const int64_t r = a.row0 + blockIdx.x;
+  row_ws& ws = wss[blockIdx.x];
+  const row_set s = rs_load(a, r);
+  const uint32_t best = best_of(ws, slices);
+  if (best == 0) return;
+  const row_mass rm = rm_make(best, s, shift);
+  if (threadIdx.x == 0) bins[0] = -1, bins[1] = 0, bins[2] = -1, n_found[0] = 0, n_found[1] = 0;
+  // where top-p ends, and between which masses the draw falls
+  constexpr int PB = SB_BINS / SR_THREADS;
+  unsigned long long m[PB], before[PB];
+#pragma unroll
+  for (int i = 0; i < PB; ++i) m[i] = ws.hist_m[threadIdx.x * PB + i];
+  const unsigned long long total = scan_bins<SR_THREADS>(m, before, red);
+  const bool known = !rm.greedy && !(COUNT && (unsigned long long)s.k < ws.count);  // (otherwise the total itself is not known yet)
+  if (known) {
+    const unsigned long long border = border_of(s.top_p, total);
+    const bool cuts = s.top_p < 1.0f && border < total;
+    if (threadIdx.x == 0) range[0] = range[1] = total;
+    __syncthreads();
+    if (cuts) {
+#pragma unroll
+      for (int i = 0; i < PB; ++i)
+        if (before[i] < border && before[i] + m[i] >= border) bins[0] = threadIdx.x * PB + i, range[0] = border, range[1] = before[i] + m[i];
+    }
+    __syncthreads();
+    const unsigned long long most = max(ws.above, (unsigned long long)rm.scale);
+    const float u = a.u[r * a.ld_u];
+    const unsigned long long w0 = want_of(u, min(range[0], most)), w1 = want_of(u, min(range[1], most));
+#pragma unroll
+    for (int i = 0; i < PB; ++i) {
+      if (before[i] < w0 && before[i] + m[i] >= w0) bins[1] = threadIdx.x * PB + i;
+      if (before[i] < w1 && before[i] + m[i] >= w1) bins[2] = threadIdx.x * PB + i;
+    }
+  }
+  __syncthreads();
+  const int b1 = bins[0], lo = bins[1], hi = bins[2];
+  if (sl == 0 && threadIdx.x == 0) ws.b1 = b1, ws.b2_lo = lo, ws.b2_hi = hi;
+  if (b1 < 0 && hi < lo) return;
+  int begin, end;
+  slice_of(s.len, gridDim.y, sl, begin, end);
+  scan_row<T>((const T*)a.scores + r * a.ld, begin, end, threadIdx.x, SR_THREADS, [&](int j, const rp_vec<T, PIECE<T>>& v, int) __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < PIECE<T>; ++i) {
+      const uint32_t k = key_of(rp_to_f32(v.v[i]));
+      if (k == 0) continue;
+      const int b = rm.bin(rm.log2_of(score_of(k)));
+      const unsigned long long entry = ((unsigned long long)k << 32) | (uint32_t) ~(j + i);
+      auto put = [&](int which) __attribute__((always_inline)) {
+        uint32_t at = atomicAdd(&n_found[which], 1u);
+        if (at < RC_FOUND) found[which][at] = entry;
+        else if ((at = atomicAdd(&ws.n_list[which], 1u)) < SB_CAP) ws.list[which][at] = entry;
+      };
+      if (b == b1) put(0);
+      if (b >= lo && b <= hi) put(1);
+    }
+  });
+  // (one reservation per workgroup: thousands of atomics on one address would be the launch)
+  __syncthreads();
+  if (threadIdx.x < 2) at_found[threadIdx.x] = atomicAdd(&ws.n_list[threadIdx.x], min(n_found[threadIdx.x], (uint32_t)RC_FOUND));
+  __syncthreads();
+#pragma unroll
+  for (int which = 0; which < 2; ++which)
+    for (uint32_t i = threadIdx.x; i < min(n_found[which], (uint32_t)RC_FOUND); i += SR_THREADS)
+      if (at_found[which] + i < SB_CAP) ws.list[which][at_found[which] + i] = found[which][i];
+}
+
+template <class T, bool COUNT>
+__global__ __launch_bounds__(SL_THREADS) void k_row_draw(sample_args a, const row_ws* __restrict__ wss, int slices, int shift) {
   __shared__ seek_shared sh;
   const int64_t r = a.row0 + blockIdx.x;
+  const row_ws& ws = wss[blockIdx.x];
   const row_set s = rs_load(a, r);
   const T* p = (const T*)a.scores + r * a.ld;
-  for (int i = threadIdx.x; i < SB_BINS; i += SL_THREADS) hist_m[i] = 0, hist_c[i] = 0;
-  uint32_t best = 0;
-  for (int j = threadIdx.x; j < s.len; j += SL_THREADS) best = max(best, key_of(rp_to_f32(p[j])));
-  best = block_max_u32<SL_THREADS>(best, sh.red32);
+  const uint32_t best = best_of(ws, slices);
   if (best == 0) {  // nothing to draw from
     if (threadIdx.x == 0) {
       a.idx[r] = -1;
@@ -656,46 +1064,27 @@ __global__ __launch_bounds__(SL_THREADS) void k_sample_row(sample_args a, int sh
     }
     return;
   }
-  row_mass rm;
-  rm.best = score_of(best);
-  rm.greedy = s.temperature == 0.0f;
-  rm.t = rm.greedy ? 1.0 : (double)s.temperature;
-  rm.scale = ldexp(1.0, shift);
-  unsigned long long above = 0, count = 0;  // mass of the candidates with at least min_p of the best one's mass
-  for (int j = threadIdx.x; j < s.len; j += SL_THREADS) {
-    const uint32_t k = key_of(rp_to_f32(p[j]));
-    if (k == 0) continue;
-    const double z = rm.z(score_of(k));
-    const unsigned long long m = rm.mass(z);
-    const int b = rm.bin(z);
-    if (m) atomicAdd(&hist_m[b], m);
-    atomicAdd(&hist_c[b], 1u);
-    ++count;
-    if (s.min_p <= 0.0f || exp_le0(z) >= (double)s.min_p) above += m;
-  }
-  above = block_sum_u64<SL_THREADS>(above, sh.red64);
-  count = block_sum_u64<SL_THREADS>(count, sh.red64);
-  unsigned long long incl = 0, own = 0;
-  unsigned long long total = 0;
-  for (int i = threadIdx.x; i < SB_BINS; i += SL_THREADS) total += hist_m[i];
+  const row_mass rm = rm_make(best, s, shift);
+  const int n1 = ws.b1 >= 0 && ws.n_list[0] <= SB_CAP ? (int)ws.n_list[0] : -1;
+  const int n2 = ws.b2_hi >= ws.b2_lo && ws.n_list[1] <= SB_CAP ? (int)ws.n_list[1] : -1;
+  unsigned long long incl = 0, own = 0, total = 0;
+  for (int i = threadIdx.x; i < SB_BINS; i += SL_THREADS) total += ws.hist_m[i];
   total = block_sum_u64<SL_THREADS>(total, sh.red64);
-  if ((unsigned long long)s.k < count) {
-    seek<T>(p, s.len, rm, hist_m, hist_c, true, (unsigned long long)s.k, sh, &incl, &own);
+  if (COUNT && (unsigned long long)s.k < ws.count) {
+    seek<T>(p, s.len, rm, ws, true, (unsigned long long)s.k, sh, nullptr, -1, 0, -1, &incl, &own);
     total = incl;
   }
   unsigned long long kept = total;
   if (s.top_p < 1.0f && !rm.greedy) {
-    const unsigned long long border = max((unsigned long long)ceil((double)s.top_p * (double)total), 1ull);
+    const unsigned long long border = border_of(s.top_p, total);
     if (border < kept) {
-      seek<T>(p, s.len, rm, hist_m, hist_c, false, border, sh, &incl, &own);
+      seek<T>(p, s.len, rm, ws, false, border, sh, ws.list[0], n1, ws.b1, ws.b1, &incl, &own);
       kept = incl;
     }
   }
-  if (!rm.greedy) kept = min(kept, max(above, (unsigned long long)rm.scale));
-  float u = a.u[r * a.ld_u];
-  u = u > 0.0f ? fminf(u, 0x1.fffffep-1f) : 0.0f;
-  const unsigned long long want = rm.greedy ? 1ull : min((unsigned long long)floor((double)u * (double)kept) + 1ull, kept);
-  const int at = seek<T>(p, s.len, rm, hist_m, hist_c, false, want, sh, &incl, &own);
+  if (!rm.greedy) kept = min(kept, max(ws.above, (unsigned long long)rm.scale));
+  const unsigned long long want = rm.greedy ? 1ull : want_of(a.u[r * a.ld_u], kept);
+  const int at = seek<T>(p, s.len, rm, ws, false, want, sh, ws.list[1], n2, ws.b2_lo, ws.b2_hi, &incl, &own);
   if (threadIdx.x == 0) {
     a.idx[r] = at < 0 ? -1 : a.ids ? a.ids[r * a.ld_ids + at] : at;
     a.prob[r] = at < 0 ? 0.0f : rm.greedy ? 1.0f : (float)((double)own / (double)kept);
@@ -703,14 +1092,28 @@ __global__ __launch_bounds__(SL_THREADS) void k_sample_row(sample_args a, int sh
   }
 }
 
+// which form a call takes, and its workspace
+enum sample_form { FORM_WAVE4, FORM_WAVE16, FORM_LISTS, FORM_ROWS };
+sample_form form_of(int64_t width, int64_t k) { return width <= 256 ? FORM_WAVE4 : width <= RPS_SHORT ? FORM_WAVE16 : k <= RPS_SHORT ? FORM_LISTS : FORM_ROWS; }
+// entries of a row's list: the selection hands over 1.1 to 1.4 times k candidates
+int list_of(int64_t k) { return k <= 128 ? 256 : k <= 384 ? 512 : 1024; }
+int64_t workspace_of(int64_t rows, int64_t width, int64_t k) {
+  switch (form_of(width, k)) {
+    case FORM_LISTS: return std::min(rows, STRIP_LISTS) * (list_of(k) * 8 + 4);
+    case FORM_ROWS: return std::min(rows, STRIP) * (int64_t)sizeof(row_ws);
+    default: return 0;
+  }
+}
+int64_t reach_of(int64_t width, int32_t top_k) { return top_k > 0 ? std::min<int64_t>(top_k, width) : width; }
+
 bool bad_fraction(float v) { return !(v >= 0.0f && v <= 1.0f); }
 
 }  // namespace
 
 extern "C" int rphip_sample_workspace(rphip_ctx* ctx, int64_t rows, int64_t width, int32_t draws, int32_t top_k, int64_t* bytes_out) {
   if (!ctx || !bytes_out) RP_FAIL(RPHIP_EINVAL, "sample_workspace: NULL argument");
-  (void)rows, (void)width, (void)draws, (void)top_k;
-  *bytes_out = 0;
+  if (rows < 0 || width < 0 || draws < 1 || top_k < 0) RP_FAIL(RPHIP_EINVAL, "sample_workspace: %lld rows of %lld, draws = %d, top_k = %d", (long long)rows, (long long)width, draws, top_k);
+  *bytes_out = workspace_of(rows, width, reach_of(width, top_k));
   return RPHIP_OK;
 }
 
@@ -727,14 +1130,16 @@ extern "C" int rphip_sample(rphip_ctx* ctx, void* stream, int64_t rows, int64_t 
   if (bad_fraction(params->top_p) || bad_fraction(params->min_p)) RP_FAIL(RPHIP_EINVAL, "sample: top_p %g, min_p %g: 0 .. 1 expected", params->top_p, params->min_p);
   if (params->top_k < 0) RP_FAIL(RPHIP_EINVAL, "sample: top_k = %d", params->top_k);
   if (params->top_k_dev && params->top_k == 0) RP_FAIL(RPHIP_EINVAL, "sample: top_k per row needs top_k as their bound");
-  const int64_t k = params->top_k > 0 ? std::min<int64_t>(params->top_k, width) : width;
+  const int64_t k = reach_of(width, params->top_k);
   if (draws > 1 && k > RPS_SHORT)
     RP_FAIL(RPHIP_ELIMIT, "sample: %d draws without replacement need top_k (or the width) <= %d, got %lld", draws, RPS_SHORT, (long long)k);
   if (rows == 0) return RPHIP_OK;
   if (!idx_dev || !prob_dev || !u_dev || (width > 0 && !scores_dev)) RP_FAIL(RPHIP_EINVAL, "sample: NULL argument");
   if ((uintptr_t)scores_dev % rp_type_bytes(type)) RP_FAIL(RPHIP_EINVAL, "sample: scores are not aligned to their elements");
   RP_TRY(scope.enter(ctx));
-  (void)workspace_dev, (void)workspace_bytes;
+  const int64_t need = workspace_of(rows, width, k);
+  if (workspace_bytes < need || (need > 0 && !workspace_dev) || ((uintptr_t)workspace_dev & 255))
+    RP_FAIL(RPHIP_EINVAL, "sample: a workspace of %lld bytes, aligned to 256, is needed (rphip_sample_workspace)", (long long)need);
   sample_args a = {rows, ld, ld_ids, ld_u, (int)width, draws, scores_dev, lengths_dev, ids_dev, u_dev, params->temperature, params->top_p, params->min_p, params->top_k,
                    params->temperature_dev, params->top_p_dev, params->min_p_dev, params->top_k_dev, idx_dev, prob_dev, nnz_dev, 0};
   int bits = 0;
@@ -743,15 +1148,53 @@ extern "C" int rphip_sample(rphip_ctx* ctx, void* stream, int64_t rows, int64_t 
   return rp_by_type(type, [&](auto tag) -> int {
     using T = typename decltype(tag)::T;
     const hipStream_t st = (hipStream_t)stream;
-    constexpr int64_t STRIP = 1 << 20;  // rows of a launch
-    for (a.row0 = 0; a.row0 < rows; a.row0 += STRIP) {
-      const unsigned n = (unsigned)std::min<int64_t>(STRIP, rows - a.row0);
-      if (width <= 256) k_sample_wave<T, 4><<<(n + 3) / 4, 256, 0, st>>>(a);
-      else if (width <= RPS_SHORT) k_sample_wave<T, 16><<<(n + 3) / 4, 256, 0, st>>>(a);
-      else if (k <= RPS_SHORT) k_sample_topk<T><<<n, SL_THREADS, 0, st>>>(a);
-      else k_sample_row<T><<<n, SL_THREADS, 0, st>>>(a, shift);
-      RP_LAUNCHED();
+    switch (form_of(width, k)) {
+      case FORM_WAVE4:
+      case FORM_WAVE16:
+        for (a.row0 = 0; a.row0 < rows; a.row0 += 1 << 20) {
+          const unsigned n = (unsigned)std::min<int64_t>(1 << 20, rows - a.row0);
+          if (width <= 256) k_sample_wave<T, 4><<<(n + 3) / 4, 256, 0, st>>>(a);
+          else k_sample_wave<T, 16><<<(n + 3) / 4, 256, 0, st>>>(a);
+          RP_LAUNCHED();
+        }
+        return RPHIP_OK;
+      case FORM_LISTS:
+        for (a.row0 = 0; a.row0 < rows; a.row0 += STRIP_LISTS) {
+          const unsigned n = (unsigned)std::min(STRIP_LISTS, rows - a.row0);
+          const int cap = list_of(k);
+          unsigned long long* lists = (unsigned long long*)workspace_dev;
+          int32_t* counts = (int32_t*)(lists + std::min(rows, STRIP_LISTS) * cap);
+          if (width <= TK_CACHE * SL_THREADS * PIECE<T>) k_sample_topk<T, true><<<n, SL_THREADS, 0, st>>>(a, lists, counts, cap);
+          else k_sample_topk<T, false><<<n, SL_THREADS, 0, st>>>(a, lists, counts, cap);
+          RP_LAUNCHED();
+          if (cap == 256) k_sample_lists<256, 256><<<n, 64, 0, st>>>(a, lists, counts);
+          else if (k <= 256) k_sample_lists<512, 256><<<n, 64, 0, st>>>(a, lists, counts);
+          else if (cap == 512) k_sample_lists<512, 512><<<n, 64, 0, st>>>(a, lists, counts);
+          else k_sample_lists<1024, 1024><<<n, 64, 0, st>>>(a, lists, counts);
+          RP_LAUNCHED();
+        }
+        return RPHIP_OK;
+      default: {
+        // slices of a row: about eight workgroups per CU in all, of no fewer than 1024 scores
+        const int slices = (int)std::max<int64_t>(1, std::min<int64_t>({8 * (int64_t)ctx->n_cu / std::min<int64_t>(rows, STRIP), width / 1024, 64}));
+        auto go = [&](auto by_count) -> int {
+          constexpr bool COUNT = decltype(by_count)::value;
+          for (a.row0 = 0; a.row0 < rows; a.row0 += STRIP) {
+            const unsigned n = (unsigned)std::min<int64_t>(STRIP, rows - a.row0);
+            row_ws* ws = (row_ws*)workspace_dev;
+            k_row_best<T><<<dim3(n, slices), SR_THREADS, 0, st>>>(a, ws);
+            RP_LAUNCHED();
+            k_row_hist<T, COUNT><<<dim3(n, slices), SR_THREADS, 0, st>>>(a, ws, shift);
+            RP_LAUNCHED();
+            k_row_collect<T, COUNT><<<dim3(n, slices), SR_THREADS, 0, st>>>(a, ws, slices, shift);
+            RP_LAUNCHED();
+            k_row_draw<T, COUNT><<<n, SL_THREADS, 0, st>>>(a, ws, slices, shift);
+            RP_LAUNCHED();
+          }
+          return RPHIP_OK;
+        };
+        return params->top_k > 0 ? go(std::true_type{}) : go(std::false_type{});
+      }
     }
-    return RPHIP_OK;
   });
 }
