@@ -352,6 +352,86 @@ __global__ __launch_bounds__(WM * WN * 64) void k_mxg_fp4(gemm_args g) {
   store_tile<OT, TM, TN>(g, acc, tm * BM + wm * 16, tn * BN + wn * 16, lane);
 }
 
+// ---- few rows of A -------------------------------------------------------------------------------------------------------------------
+// M <= 4: every element of W is wanted M times, so its bytes are the time, and the vector unit keeps up: half a conversion and M
+// multiply-adds in float32 per element (no planes, no workspace).  A wave takes GV_ROWS rows of W at once, a lane every 64th MX block of
+// them: 1 KB contiguous per row and step; A's block is read and converted once for the GV_ROWS rows.
+constexpr int GV_ROWS = 4;
+template <class T, class OT, int M>
+__global__ __launch_bounds__(256) void k_mxg_rows(const T* __restrict__ a, int64_t lda, int m_real, int N, int K, int nb, const uint8_t* __restrict__ w, int64_t ldw,
+                                                  const uint8_t* __restrict__ ws, int64_t ldws, OT* __restrict__ c, int64_t ldc) {
+  const int lane = threadIdx.x & 63;
+  const int64_t n0 = ((int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6)) * GV_ROWS;
+  if (n0 >= N) return;
+  const uint8_t* wr[GV_ROWS];
+  const uint8_t* sr[GV_ROWS];
+#pragma unroll
+  for (int r = 0; r < GV_ROWS; ++r) {
+    const int64_t n = min(n0 + r, (int64_t)N - 1);
+    wr[r] = w + n * ldw;
+    sr[r] = ws + n * ldws;
+  }
+  const T* ar[M];
+#pragma unroll
+  for (int m = 0; m < M; ++m) ar[m] = a + (int64_t)min(m, m_real - 1) * lda;
+  float acc[GV_ROWS][M];
+#pragma unroll
+  for (int r = 0; r < GV_ROWS; ++r)
+#pragma unroll
+    for (int m = 0; m < M; ++m) acc[r][m] = 0.0f;
+  uint4 q[GV_ROWS], qn[GV_ROWS];
+  uint32_t s[GV_ROWS], sn[GV_ROWS];
+  auto fetch = [&](int b) __attribute__((always_inline)) {
+    const int bb = min(b, nb - 1);
+#pragma unroll
+    for (int r = 0; r < GV_ROWS; ++r) {
+      qn[r] = *(const uint4*)(wr[r] + (int64_t)bb * 16);
+      sn[r] = sr[r][bb];
+    }
+  };
+  if (lane < nb) fetch(lane);
+  for (int b = lane; b < nb; b += 64) {
+#pragma unroll
+    for (int r = 0; r < GV_ROWS; ++r) q[r] = qn[r], s[r] = sn[r];
+    fetch(b + 64);
+    const int k = b * RP_MX;
+    const bool whole = k + RP_MX <= K;
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      float v[M][8];
+#pragma unroll
+      for (int m = 0; m < M; ++m) {
+        if (whole) {
+          const rp_vec<T, 8> t = rp_load_vec<T, 8>(ar[m] + k + g * 8);
+#pragma unroll
+          for (int i = 0; i < 8; ++i) v[m][i] = rp_to_f32(t.v[i]);
+        } else {
+#pragma unroll
+          for (int i = 0; i < 8; ++i) v[m][i] = k + g * 8 + i < K ? rp_to_f32(ar[m][k + g * 8 + i]) : 0.0f;
+        }
+      }
+#pragma unroll
+      for (int r = 0; r < GV_ROWS; ++r) {
+        float x[8];
+        rp_mx_unpack8(g == 0 ? q[r].x : g == 1 ? q[r].y : g == 2 ? q[r].z : q[r].w, rp_mx_scale(s[r]), x);
+#pragma unroll
+        for (int m = 0; m < M; ++m)
+#pragma unroll
+          for (int i = 0; i < 8; ++i) acc[r][m] = fmaf(v[m][i], x[i], acc[r][m]);
+      }
+    }
+  }
+#pragma unroll
+  for (int r = 0; r < GV_ROWS; ++r)
+#pragma unroll
+    for (int m = 0; m < M; ++m) {
+      float t = acc[r][m];
+#pragma unroll
+      for (int d = 32; d > 0; d >>= 1) t += __shfl_xor(t, d);
+      if (lane == 0 && n0 + r < N && m < m_real) c[(int64_t)m * ldc + n0 + r] = rp_from_f32<OT>(t);
+    }
+}
+
 // split K: the parts in order, one rounding
 template <class OT>
 __global__ __launch_bounds__(256) void k_mxg_join(const float* __restrict__ part, int split, int M, int N, OT* __restrict__ c, int64_t ldc) {
@@ -364,6 +444,7 @@ __global__ __launch_bounds__(256) void k_mxg_join(const float* __restrict__ part
 
 struct plan {
   int planes = 0, split = 1, nc = 0, nq = 0;
+  bool rows = false;  // few rows of A: k_mxg_rows
   int bm = 16, bn = 64;
   int64_t plane_bytes = 0, a_scale_bytes = 0, w_scale_bytes = 0, part_bytes = 0;
   int64_t total() const { return plane_bytes + a_scale_bytes + w_scale_bytes + part_bytes; }
@@ -375,6 +456,8 @@ plan make_plan(int n_cu, int64_t M, int64_t N, int64_t K, int32_t a_type) {
   p.nc = (int)rp_cdiv(K, KC);
   p.nq = (int)rp_cdiv(p.nc, 4);
   auto tiles = [&](int bm, int bn) { return rp_cdiv(M, bm) * rp_cdiv(N, bn); };
+  p.rows = p.planes != 0 && M <= 4;
+  if (p.rows) return p;
   if (M <= 16) p.bm = p.planes ? 16 : 32, p.bn = p.planes ? 64 : 32;
   else if (tiles(256, 256) >= n_cu) p.bm = 256, p.bn = 256;
   else if (tiles(128, 128) >= n_cu) p.bm = 128, p.bn = 128;
@@ -455,6 +538,20 @@ extern "C" int rphip_mxfp4_gemm_nt(rphip_ctx* ctx, void* stream, int64_t M, int6
   g.a_codes = (const uint8_t*)A_dev, g.lda = lda, g.a_scales = (const uint32_t*)(ws + p.plane_bytes);
   g.w = w_codes_dev, g.ldw = ld_w, g.w_scales = (const uint32_t*)(ws + p.plane_bytes + p.a_scale_bytes);
   g.c = C_dev, g.ldc = ldc, g.part = (float*)(ws + p.plane_bytes + p.a_scale_bytes + p.w_scale_bytes), g.split = p.split;
+  if (p.rows)
+    return rp_by_type(a_type, [&](auto at) -> int {
+      return rp_by_type(c_type, [&](auto ct) -> int {
+        using T = typename decltype(at)::T;
+        using OT = typename decltype(ct)::T;
+        const unsigned grid = (unsigned)rp_cdiv(N, 4 * GV_ROWS);
+        auto go = [&](auto kernel) { kernel<<<grid, 256, 0, st>>>((const T*)A_dev, lda, (int)M, (int)N, (int)K, g.nb, w_codes_dev, ld_w, w_scales_dev, ld_w_scales, (OT*)C_dev, ldc); };
+        if (M == 1) go(k_mxg_rows<T, OT, 1>);
+        else if (M == 2) go(k_mxg_rows<T, OT, 2>);
+        else go(k_mxg_rows<T, OT, 4>);
+        RP_LAUNCHED();
+        return RPHIP_OK;
+      });
+    });
   if (p.nc) {
     // (below 2^32 threads a launch: M <= 2^20 and N <= 2^28 rows in strips of row blocks)
     auto scales = [&](const uint8_t* s, int64_t lds, int64_t rows, uint32_t* o) -> int {
