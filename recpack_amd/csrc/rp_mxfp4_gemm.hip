@@ -15,6 +15,7 @@ namespace {
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef int i32x8 __attribute__((ext_vector_type(8)));
+typedef int i32x4 __attribute__((ext_vector_type(4)));
 
 constexpr int KC = 128;  // K of a chunk: four MX blocks
 
@@ -43,51 +44,41 @@ __device__ __forceinline__ void cut_planes(float x, uint16_t (&h)[P]) {
   }
 }
 
-// A -> planes [16-row block][chunk][plane][step 4][lane 64][8 bf16], zero beyond K and M: fragments are contiguous KB.  One thread
-// per (block, chunk, lane): it reads one MX block's worth of its row and writes a piece of 4 P fragments.
+// A -> planes [16-row block][chunk][plane][step 4][lane 64][8 bf16], zero beyond K and M: fragments are contiguous KB.  One wave per
+// (block, chunk, step), the four steps of a chunk in one workgroup: together they read whole lines.
 template <class T, int P>
-__global__ __launch_bounds__(256) void k_mxg_planes(const T* __restrict__ a, int64_t lda, int M, int K, int nc, int64_t units, uint16_t* __restrict__ out) {
-  const int64_t unit = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (unit >= units) return;
-  const int lane = threadIdx.x & 63;
-  const int64_t frag = unit >> 6, mb = frag / nc;
-  const int c = (int)(frag - mb * nc);
-  const int64_t m = mb * 16 + (lane & 15);
-  const int k0 = c * KC + (lane >> 4) * 32;
-  uint4* o = (uint4*)(out + frag * (P * 4 * 512)) + lane;
-  const T* p = a + m * lda + k0;
+__device__ __forceinline__ void cut_fragment(const T* __restrict__ a, int64_t lda, int M, int K, int nc, int64_t frag, int s, int lane, uint16_t* __restrict__ out) {
+  const int64_t mb = frag / nc, m = mb * 16 + (lane & 15);
+  const int c = (int)(frag - mb * nc), k = c * KC + (lane >> 4) * 32 + s * 8;
+  const T* p = a + m * lda + k;
+  float v[8];
+  if (m < M && k + 8 <= K) {
+    const rp_vec<T, 8> t = rp_load_vec<T, 8>(p);
 #pragma unroll
-  for (int s = 0; s < 4; ++s) {
-    float v[8];
-    if (m < M && k0 + s * 8 + 8 <= K) {
-      const rp_vec<T, 8> t = rp_load_vec<T, 8>(p + s * 8);
+    for (int i = 0; i < 8; ++i) v[i] = rp_to_f32(t.v[i]);
+  } else {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) v[i] = rp_to_f32(t.v[i]);
-    } else {
+    for (int i = 0; i < 8; ++i) v[i] = m < M && k + i < K ? rp_to_f32(p[i]) : 0.0f;
+  }
+  uint16_t h[8][P];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) v[i] = m < M && k0 + s * 8 + i < K ? rp_to_f32(p[s * 8 + i]) : 0.0f;
-    }
-    uint16_t h[8][P];
+  for (int i = 0; i < 8; ++i) cut_planes<P>(v[i], h[i]);
+  uint4* o = (uint4*)(out + (frag * P * 4 + s) * 512) + lane;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) cut_planes<P>(v[i], h[i]);
-#pragma unroll
-    for (int pl = 0; pl < P; ++pl) {
-      uint4 w;
-      w.x = h[0][pl] | (uint32_t)h[1][pl] << 16;
-      w.y = h[2][pl] | (uint32_t)h[3][pl] << 16;
-      w.z = h[4][pl] | (uint32_t)h[5][pl] << 16;
-      w.w = h[6][pl] | (uint32_t)h[7][pl] << 16;
-      o[(pl * 4 + s) * 64] = w;
-    }
+  for (int pl = 0; pl < P; ++pl) {
+    uint4 w;
+    w.x = h[0][pl] | (uint32_t)h[1][pl] << 16;
+    w.y = h[2][pl] | (uint32_t)h[3][pl] << 16;
+    w.z = h[4][pl] | (uint32_t)h[5][pl] << 16;
+    w.w = h[6][pl] | (uint32_t)h[7][pl] << 16;
+    o[pl * 4 * 64] = w;
   }
 }
 
 // Scales -> [16-row block][four chunks][lane 64] words: byte cc = the scale of the lane's block of chunk 4 q + cc.  Blocks beyond the
 // row get 0 (2^-127): whatever their codes hold, the product underflows to nothing.  Rows beyond the matrix repeat the last one.
-__global__ __launch_bounds__(256) void k_mxg_scales(const uint8_t* __restrict__ s, int64_t lds, int rows, int nb, int nq, int64_t units, uint32_t* __restrict__ out) {
-  const int64_t unit = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (unit >= units) return;
-  const int lane = threadIdx.x & 63;
+__device__ __forceinline__ void pack_scales(const uint8_t* __restrict__ s, int64_t lds, int rows, int nb, int nq, int64_t unit, uint32_t* __restrict__ out) {
+  const int lane = (int)(unit & 63);
   const int64_t f = unit >> 6, rb = f / nq;
   const int q = (int)(f - rb * nq);
   const int64_t r = min(rb * 16 + (lane & 15), (int64_t)rows - 1);
@@ -97,6 +88,24 @@ __global__ __launch_bounds__(256) void k_mxg_scales(const uint8_t* __restrict__ 
   for (int cc = 0; cc < 4; ++cc)
     if (b + cc * 4 < nb) w |= (uint32_t)s[r * lds + b + cc * 4] << (8 * cc);
   out[unit] = w;
+}
+
+// One launch for all of them: workgroups [0, wg_w) pack W's scales, the others cut A (P > 0) or pack A's scales.
+template <class T, int P>
+__global__ __launch_bounds__(256) void k_mxg_prepare(const uint8_t* __restrict__ ws, int64_t ldws, int N, int nb, int nq, int64_t w_units, uint32_t* __restrict__ w_out,
+                                                     unsigned wg_w, const T* __restrict__ a, int64_t lda, int M, int K, int nc, int64_t a_units, void* __restrict__ a_out) {
+  if (blockIdx.x < wg_w) {
+    const int64_t unit = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (unit < w_units) pack_scales(ws, ldws, N, nb, nq, unit, w_out);
+    return;
+  }
+  const int64_t wg = blockIdx.x - wg_w;
+  if constexpr (P > 0) {
+    if (wg < a_units) cut_fragment<T, P>(a, lda, M, K, nc, wg, threadIdx.x >> 6, threadIdx.x & 63, (uint16_t*)a_out);
+  } else {
+    const int64_t unit = wg * 256 + threadIdx.x;
+    if (unit < a_units) pack_scales(a, lda, M, nb, nq, unit, (uint32_t*)a_out);
+  }
 }
 
 // eight codes (a dword) to eight bf16
@@ -140,7 +149,7 @@ __device__ __forceinline__ void dma16(const uint8_t* from, uint8_t* to) {
 
 template <int N>
 __device__ __forceinline__ void wait_loads_and_meet() {
-  asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
+  asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(N) : "memory");  // (my reads of the stage about to be refilled have landed)
   __builtin_amdgcn_s_barrier();  // bare: the fence of __syncthreads() would wait for every load in flight
   asm volatile("" ::: "memory");
 }
@@ -183,18 +192,26 @@ __device__ __forceinline__ void store_tile(const gemm_args& g, const f32x4 (&acc
   }
 }
 
-// 16-bit form.  Tile BM x BN, WM x WN waves, a ring of RING stages of A in LDS, each the half of a plane of a chunk (two of its four
-// steps), filled by LDS-DMA RING - 1 stages ahead; W goes from memory to registers one chunk ahead and is converted there, once per
-// plane and wave: 4 conversions per 8 codes against TM matrix instructions that use them.
-template <class OT, int P, int BM, int BN, int WM, int WN, int RING>
+// Everything a loop reads comes through LDS: a load into registers beside LDS-DMA requests makes the compiler wait for all of them.
+// Fragments' rows and blocks past the matrices repeat the last ones: their sums are not stored, or meet zeros of A (bf16) or scales of
+// 2^-127 (4-bit).
+
+// 16-bit form.  Tile BM x BN, WM x WN waves.  A in a ring of three stages, each the half of a plane of a chunk (two of its four steps),
+// requested two stages ahead; W's codes and scales in two slots, a chunk ahead, converted in registers once per plane and wave (4 conversions
+// per 8 codes against TM matrix instructions that use them).
+template <class OT, int P, int BM, int BN, int WM, int WN>
 __global__ __launch_bounds__(WM * WN * 64) void k_mxg_bf16(gemm_args g) {
-  constexpr int WAVES = WM * WN, TM = BM / WM / 16, TN = BN / WN / 16, STAGE = BM * 128, D = BM / 8 / WAVES;  // D: KB a wave requests per stage
-  static_assert(D * WAVES * 8 == BM, "every wave requests the same number of fragments");
+  constexpr int WAVES = WM * WN, TM = BM / WM / 16, TN = BN / WN / 16, RING = 3;
+  constexpr int STAGE = BM * 128, D = BM / 8 / WAVES;                // A: bytes of a stage, KB a wave requests of it
+  constexpr int WCODES = BN * 64, DW = BN / 16 / WAVES;              // W: bytes of a slot, KB a wave requests of it
+  constexpr int WSCALES = BN * 16, SLANES = BN / WAVES;              // scales: bytes of a slot, lanes of a wave's request
+  constexpr int WOFF = RING * STAGE, SOFF = WOFF + 2 * WCODES, X = DW + 1;
+  static_assert(D * WAVES * 8 == BM && DW * WAVES * 16 == BN && SLANES <= 64, "every wave requests the same number of pieces");
   extern __shared__ __attribute__((aligned(1024))) uint8_t ring[];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   int tm, tn;
   if (!tile_of(g, tm, tn)) return;
-  const int m0 = tm * BM, wm = (wave / WN) * TM, wn = tn * (BN / 16) + (wave % WN) * TN;  // (wm, wn in fragments)
+  const int m0 = tm * BM, wm = (wave / WN) * TM, wn = (wave % WN) * TN;  // (wm, wn in fragments of the tile)
   f32x4 acc[TM][TN];
 #pragma unroll
   for (int i = 0; i < TM; ++i)
@@ -203,80 +220,83 @@ __global__ __launch_bounds__(WM * WN * 64) void k_mxg_bf16(gemm_args g) {
   const int z = blockIdx.y;
   const int c0 = (int)((int64_t)g.nc * z / g.split), c1 = (int)((int64_t)g.nc * (z + 1) / g.split);
   const int t0 = c0 * P * 2, t1 = c1 * P * 2;
-  // A: fragment pairs (2 KB) of a stage, wave's share
-  const int mblocks = (g.M + 15) / 16;
+  const int mblocks = (g.M + 15) / 16, nblocks = (g.N + 15) / 16;
   const uint8_t* asrc[D];
 #pragma unroll
   for (int d = 0; d < D; ++d) {
     const int f = wave * D + d, mb = min(m0 / 16 + (f >> 1), mblocks - 1);
     asrc[d] = g.planes + ((int64_t)mb * g.nc * P) * 4096 + (f & 1) * 1024 + lane * 16;
   }
-  auto request = [&](int t) __attribute__((always_inline)) {
-    const int tt = min(t, t1 - 1);  // (a request past the end repeats the last one: the counted waits stay uniform)
-    uint8_t* to = ring + (t - t0) % RING * STAGE + wave * D * 1024;
+  auto request_a = [&](int t, int stage) __attribute__((always_inline)) {
+    const int tt = min(t, t1 - 1);  // (past the end: the last one again, the counted waits stay uniform)
+    uint8_t* to = ring + stage * STAGE + wave * D * 1024;
 #pragma unroll
     for (int d = 0; d < D; ++d) dma16(asrc[d] + (int64_t)tt * 2048, to + d * 1024);
   };
-  // W
-  const uint8_t* wsrc[TN];
-  const uint32_t* wssrc[TN];
-  const int nblocks = (g.N + 15) / 16;
+  const uint8_t* wsrc[DW];
 #pragma unroll
-  for (int j = 0; j < TN; ++j) {
-    const int nbk = min(wn + j, nblocks - 1), n = min(nbk * 16 + (lane & 15), g.N - 1);
-    wsrc[j] = g.w + (int64_t)n * g.ldw;
-    wssrc[j] = g.w_scales + (int64_t)nbk * g.nq * 64 + lane;
-  }
-  uint4 wq[TN], wnext[TN];
-  uint32_t sc[TN], scnext[TN];
-  auto load_w = [&](int c) __attribute__((always_inline)) {
-    const int cc = min(c, g.nc - 1), b = min(cc * 4 + (lane >> 4), g.nb - 1);  // (a block beyond the row: A is zero there)
+  for (int d = 0; d < DW; ++d) wsrc[d] = g.w + (int64_t)min(tn * BN + (wave * DW + d) * 16 + (lane & 15), g.N - 1) * g.ldw;
+  const uint8_t* ssrc = (const uint8_t*)g.w_scales + (int64_t)min(tn * (BN / 16) + (wave * SLANES + lane) / 16, nblocks - 1) * g.nq * 256 + (lane & 15) * 16;
+  auto request_w = [&](int c) __attribute__((always_inline)) {
+    const int cc = min(c, c1 - 1), b = min(cc * 4 + (lane >> 4), g.nb - 1);
 #pragma unroll
-    for (int j = 0; j < TN; ++j) wnext[j] = *(const uint4*)(wsrc[j] + (int64_t)b * 16);
-#pragma unroll
-    for (int j = 0; j < TN; ++j) scnext[j] = wssrc[j][(cc >> 2) * 64];
+    for (int d = 0; d < DW; ++d) dma16(wsrc[d] + (int64_t)b * 16, ring + WOFF + (c & 1) * WCODES + (wave * DW + d) * 1024);
+    if (SLANES == 64 || lane < SLANES) dma16(ssrc + (int64_t)(cc >> 2) * 256, ring + SOFF + (c & 1) * WSCALES + wave * SLANES * 16);
   };
   if (t0 < t1) {
-    load_w(c0);
-#pragma unroll
-    for (int r = 0; r < RING - 1; ++r) request(t0 + r);
-    int t = t0;
+    request_w(c0);
+    request_a(t0, 0);
+    request_a(t0 + 1, 1);
+    int t = t0, stage = 0;
+    i32x4 wq[TN];
+    uint32_t sc[TN];
     for (int c = c0; c < c1; ++c) {
+#pragma unroll(P < 3 ? P : 1)
+      for (int pl = 0; pl < P; ++pl)
 #pragma unroll
-      for (int j = 0; j < TN; ++j) wq[j] = wnext[j], sc[j] = ((scnext[j] >> (8 * (c & 3))) & 255u) << 23;
-      load_w(c + 1);
-#pragma unroll 1
-      for (int p = 0; p < P; ++p) {
+      for (int h = 0; h < 2; ++h, ++t) {
+        const int s4 = pl * 2 + h;
+        // newer than this stage: the next one, and the W requests if the step before made some
+        if (s4 == 1) wait_loads_and_meet<D + X>();
+        else wait_loads_and_meet<D>();
+        if (s4 == 0) request_w(c + 1);
+        request_a(t + 2, stage == 0 ? 2 : stage - 1);
+        if (s4 == 0) {
 #pragma unroll
-        for (int h = 0; h < 2; ++h, ++t) {
-          wait_loads_and_meet<(RING - 2) * D>();
-          request(t + RING - 1);
-          const uint8_t* st = ring + (t - t0) % RING * STAGE + lane * 16;
-#pragma unroll
-          for (int s = 0; s < 2; ++s) {
-            bf16x8 wf[TN];
-#pragma unroll
-            for (int j = 0; j < TN; ++j) wf[j] = codes_bf16(h == 0 ? (s == 0 ? wq[j].x : wq[j].y) : (s == 0 ? wq[j].z : wq[j].w), __uint_as_float(sc[j]));
-#pragma unroll
-            for (int i = 0; i < TM; ++i) {
-              const bf16x8 af = *(const bf16x8*)(st + ((wm + i) * 2 + s) * 1024);
-#pragma unroll
-              for (int j = 0; j < TN; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(wf[j], af, acc[i][j], 0, 0, 0);
-            }
+          for (int j = 0; j < TN; ++j) {
+            wq[j] = *(const i32x4*)(ring + WOFF + (c & 1) * WCODES + (wn + j) * 1024 + lane * 16);
+            sc[j] = ((*(const uint32_t*)(ring + SOFF + (c & 1) * WSCALES + (wn + j) * 256 + lane * 4) >> (8 * (c & 3))) & 255u) << 23;
           }
         }
+        const uint8_t* st = ring + stage * STAGE + lane * 16;
+#pragma unroll
+        for (int s = 0; s < 2; ++s) {
+          bf16x8 wf[TN];
+#pragma unroll
+          for (int j = 0; j < TN; ++j) wf[j] = codes_bf16((uint32_t)wq[j][h * 2 + s], __uint_as_float(sc[j]));
+#pragma unroll
+          for (int i = 0; i < TM; ++i) {
+            const bf16x8 af = *(const bf16x8*)(st + ((wm + i) * 2 + s) * 1024);
+#pragma unroll
+            for (int j = 0; j < TN; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(wf[j], af, acc[i][j], 0, 0, 0);
+          }
+        }
+        stage = stage == 2 ? 0 : stage + 1;
       }
     }
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // (the trailing requests write LDS)
   }
-  store_tile<OT, TM, TN>(g, acc, m0 + wm * 16, wn * 16, lane);
+  store_tile<OT, TM, TN>(g, acc, m0 + wm * 16, tn * BN + wn * 16, lane);
 }
 
-// 4-bit form: codes of both operands through the ring (a stage is a chunk of both), scales in registers, four chunks to a word.
-template <class OT, int BM, int BN, int WM, int WN, int RING>
+// 4-bit form: codes of both operands in a ring of four stages (a stage is a chunk of both), requested three ahead; scales of four chunks in
+// two slots.
+template <class OT, int BM, int BN, int WM, int WN>
 __global__ __launch_bounds__(WM * WN * 64) void k_mxg_fp4(gemm_args g) {
-  constexpr int WAVES = WM * WN, TM = BM / WM / 16, TN = BN / WN / 16, STAGE = (BM + BN) * 64, D = (BM + BN) / 16 / WAVES;
-  static_assert(D * WAVES * 16 == BM + BN, "every wave requests the same number of fragments");
+  constexpr int WAVES = WM * WN, TM = BM / WM / 16, TN = BN / WN / 16, RING = 4;
+  constexpr int STAGE = (BM + BN) * 64, D = (BM + BN) / 16 / WAVES;
+  constexpr int SCALES = (BM + BN) * 16, SLANES = (BM + BN) / WAVES, SOFF = RING * STAGE;
+  static_assert(D * WAVES * 16 == BM + BN && SLANES <= 64, "every wave requests the same number of pieces");
   extern __shared__ __attribute__((aligned(1024))) uint8_t ring[];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   int tm, tn;
@@ -290,6 +310,7 @@ __global__ __launch_bounds__(WM * WN * 64) void k_mxg_fp4(gemm_args g) {
   const int z = blockIdx.y;
   const int q0 = (int)((int64_t)g.nq * z / g.split), q1 = (int)((int64_t)g.nq * (z + 1) / g.split);
   const int c0 = q0 * 4, c1 = min(q1 * 4, g.nc);
+  const int mblocks = (g.M + 15) / 16, nblocks = (g.N + 15) / 16;
   const uint8_t* src[D];
 #pragma unroll
   for (int d = 0; d < D; ++d) {
@@ -298,47 +319,48 @@ __global__ __launch_bounds__(WM * WN * 64) void k_mxg_fp4(gemm_args g) {
                          : g.w + (int64_t)min(tn * BN + (f - BM / 16) * 16 + (lane & 15), g.N - 1) * g.ldw;
   }
   auto request = [&](int c) __attribute__((always_inline)) {
-    const int b = min(min(c, c1 - 1) * 4 + (lane >> 4), g.nb - 1);  // (a block beyond the row: its scale is 2^-127 on both sides)
-    uint8_t* to = ring + (c - c0) % RING * STAGE + wave * D * 1024;
+    const int b = min(min(c, c1 - 1) * 4 + (lane >> 4), g.nb - 1);
+    uint8_t* to = ring + (c & 3) * STAGE + wave * D * 1024;
 #pragma unroll
     for (int d = 0; d < D; ++d) dma16(src[d] + (int64_t)b * 16, to + d * 1024);
   };
-  const int mblocks = (g.M + 15) / 16, nblocks = (g.N + 15) / 16;
-  const uint32_t* ssrc[TM + TN];
-#pragma unroll
-  for (int i = 0; i < TM; ++i) ssrc[i] = g.a_scales + (int64_t)min(tm * (BM / 16) + wm + i, mblocks - 1) * g.nq * 64 + lane;
-#pragma unroll
-  for (int j = 0; j < TN; ++j) ssrc[TM + j] = g.w_scales + (int64_t)min(tn * (BN / 16) + wn + j, nblocks - 1) * g.nq * 64 + lane;
-  uint32_t sc[TM + TN], scnext[TM + TN];
-  auto load_scales = [&](int q) __attribute__((always_inline)) {
-#pragma unroll
-    for (int i = 0; i < TM + TN; ++i) scnext[i] = ssrc[i][min(q, g.nq - 1) * 64];
+  const int sf = (wave * SLANES + lane) / 16;  // the fragment whose scales this lane requests
+  const uint8_t* ssrc = (sf < BM / 16 ? (const uint8_t*)g.a_scales + (int64_t)min(tm * (BM / 16) + sf, mblocks - 1) * g.nq * 256
+                                      : (const uint8_t*)g.w_scales + (int64_t)min(tn * (BN / 16) + sf - BM / 16, nblocks - 1) * g.nq * 256) + (lane & 15) * 16;
+  auto request_scales = [&](int q) __attribute__((always_inline)) {
+    if (SLANES == 64 || lane < SLANES) dma16(ssrc + (int64_t)min(q, q1 - 1) * 256, ring + SOFF + (q & 1) * SCALES + wave * SLANES * 16);
   };
   if (c0 < c1) {
-    load_scales(q0);
+    request_scales(q0);
 #pragma unroll
     for (int r = 0; r < RING - 1; ++r) request(c0 + r);
+    int sc[TM + TN];
     for (int q = q0; q < q1; ++q) {
-#pragma unroll
-      for (int i = 0; i < TM + TN; ++i) sc[i] = scnext[i];
-      load_scales(q + 1);
       auto chunk = [&](auto tag, int c) __attribute__((always_inline)) {
         constexpr int CC = decltype(tag)::value;
         wait_loads_and_meet<(RING - 2) * D>();
+        if (CC == 0) request_scales(q + 1);
         request(c + RING - 1);
-        const uint8_t* st = ring + (c - c0) % RING * STAGE + lane * 16;
+        if (CC == 0) {
+          const uint8_t* ss = ring + SOFF + (q & 1) * SCALES + lane * 4;
+#pragma unroll
+          for (int i = 0; i < TM; ++i) sc[i] = *(const int*)(ss + (wm + i) * 256);
+#pragma unroll
+          for (int j = 0; j < TN; ++j) sc[TM + j] = *(const int*)(ss + (BM / 16 + wn + j) * 256);
+        }
+        const uint8_t* st = ring + (c & 3) * STAGE + lane * 16;
         i32x8 wf[TN];
 #pragma unroll
         for (int j = 0; j < TN; ++j) {
-          const uint4 v = *(const uint4*)(st + (BM / 16 + wn + j) * 1024);
-          wf[j] = i32x8{(int)v.x, (int)v.y, (int)v.z, (int)v.w, 0, 0, 0, 0};
+          const i32x4 v = *(const i32x4*)(st + (BM / 16 + wn + j) * 1024);
+          wf[j] = i32x8{v.x, v.y, v.z, v.w, 0, 0, 0, 0};
         }
 #pragma unroll
         for (int i = 0; i < TM; ++i) {
-          const uint4 v = *(const uint4*)(st + (wm + i) * 1024);
-          const i32x8 af = {(int)v.x, (int)v.y, (int)v.z, (int)v.w, 0, 0, 0, 0};
+          const i32x4 v = *(const i32x4*)(st + (wm + i) * 1024);
+          const i32x8 af = {v.x, v.y, v.z, v.w, 0, 0, 0, 0};
 #pragma unroll
-          for (int j = 0; j < TN; ++j) acc[i][j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(wf[j], af, acc[i][j], 4, 4, CC, (int)sc[TM + j], CC, (int)sc[i]);
+          for (int j = 0; j < TN; ++j) acc[i][j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(wf[j], af, acc[i][j], 4, 4, CC, sc[TM + j], CC, sc[i]);
         }
       };
       const int c = q * 4;
@@ -463,7 +485,9 @@ plan make_plan(int n_cu, int64_t M, int64_t N, int64_t K, int32_t a_type) {
   else if (tiles(128, 128) >= n_cu) p.bm = 128, p.bn = 128;
   else p.bm = 64, p.bn = 64;
   const int64_t n = std::max<int64_t>(tiles(p.bm, p.bn), 1), depth = p.planes ? p.nc / 2 : p.nq;
-  p.split = (int)std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(2 * n_cu / n, depth), 16));
+  // workgroups that a CU holds at once: small tiles wait for memory together
+  const int per_cu = p.bm >= 256 ? 1 : p.bm == 128 ? 2 : p.bm == 64 ? 4 : 8;
+  p.split = (int)std::max<int64_t>(1, std::min<int64_t>({per_cu * (int64_t)n_cu / n, depth, 16}));
   auto room = [](int64_t b) { return (b + 255) & ~(int64_t)255; };
   p.plane_bytes = room(rp_cdiv(M, 16) * p.nc * p.planes * 4096);
   p.a_scale_bytes = p.planes ? 0 : room(rp_cdiv(M, 16) * p.nq * 256);
@@ -483,16 +507,16 @@ int launch_tiles(Kernel kernel, gemm_args g, int threads, int lds, hipStream_t s
   RP_LAUNCHED();
   return RPHIP_OK;
 }
-template <class OT, int BM, int BN, int WM, int WN, int RING>
+template <class OT, int BM, int BN, int WM, int WN>
 int launch_fp4(const gemm_args& g, hipStream_t st) {
-  return launch_tiles<BM, BN>(k_mxg_fp4<OT, BM, BN, WM, WN, RING>, g, WM * WN * 64, RING * (BM + BN) * 64, st);
+  return launch_tiles<BM, BN>(k_mxg_fp4<OT, BM, BN, WM, WN>, g, WM * WN * 64, 4 * (BM + BN) * 64 + 2 * (BM + BN) * 16, st);
 }
-template <class OT, int BM, int BN, int WM, int WN, int RING>
+template <class OT, int BM, int BN, int WM, int WN>
 int launch_bf16(const gemm_args& g, int planes, hipStream_t st) {
-  constexpr int threads = WM * WN * 64, lds = RING * BM * 128;
-  if (planes == 1) return launch_tiles<BM, BN>(k_mxg_bf16<OT, 1, BM, BN, WM, WN, RING>, g, threads, lds, st);
-  if (planes == 2) return launch_tiles<BM, BN>(k_mxg_bf16<OT, 2, BM, BN, WM, WN, RING>, g, threads, lds, st);
-  return launch_tiles<BM, BN>(k_mxg_bf16<OT, 3, BM, BN, WM, WN, RING>, g, threads, lds, st);
+  constexpr int threads = WM * WN * 64, lds = 3 * BM * 128 + 2 * BN * 64 + 2 * BN * 16;
+  if (planes == 1) return launch_tiles<BM, BN>(k_mxg_bf16<OT, 1, BM, BN, WM, WN>, g, threads, lds, st);
+  if (planes == 2) return launch_tiles<BM, BN>(k_mxg_bf16<OT, 2, BM, BN, WM, WN>, g, threads, lds, st);
+  return launch_tiles<BM, BN>(k_mxg_bf16<OT, 3, BM, BN, WM, WN>, g, threads, lds, st);
 }
 
 int check_sizes(const char* who, int64_t M, int64_t N, int64_t K) {
@@ -553,42 +577,33 @@ extern "C" int rphip_mxfp4_gemm_nt(rphip_ctx* ctx, void* stream, int64_t M, int6
       });
     });
   if (p.nc) {
-    // (below 2^32 threads a launch: M <= 2^20 and N <= 2^28 rows in strips of row blocks)
-    auto scales = [&](const uint8_t* s, int64_t lds, int64_t rows, uint32_t* o) -> int {
-      const int64_t strip = std::max<int64_t>(1, ((int64_t)1 << 25) / p.nq) * 16;
-      for (int64_t r0 = 0; r0 < rows; r0 += strip) {
-        const int64_t n = std::min(strip, rows - r0), units = rp_cdiv(n, 16) * p.nq * 64;
-        k_mxg_scales<<<(unsigned)rp_cdiv(units, 256), 256, 0, st>>>(s + r0 * lds, lds, (int)n, g.nb, p.nq, units, o + r0 / 16 * p.nq * 64);
-        RP_LAUNCHED();
-      }
-      return RPHIP_OK;
+    const int64_t w_units = rp_cdiv(N, 16) * p.nq * 64, wg_w = rp_cdiv(w_units, 256);
+    const int64_t a_units = p.planes ? rp_cdiv(M, 16) * p.nc : rp_cdiv(M, 16) * p.nq * 64, wg_a = p.planes ? a_units : rp_cdiv(a_units, 256);
+    if ((wg_w + wg_a) * 256 >= ((int64_t)1 << 32))
+      RP_FAIL(RPHIP_ELIMIT, "mxfp4_gemm_nt: %lld x %lld x %lld: more 16-row blocks than one launch prepares (split M or N)", (long long)M, (long long)N, (long long)K);
+    auto go = [&](auto kernel, auto type, const void* a, int64_t ld, void* o) {
+      using T = decltype(type);
+      kernel<<<(unsigned)(wg_w + wg_a), 256, 0, st>>>(w_scales_dev, ld_w_scales, (int)N, g.nb, p.nq, w_units, (uint32_t*)g.w_scales, (unsigned)wg_w, (const T*)a, ld, (int)M,
+                                                     (int)K, p.nc, a_units, o);
     };
-    RP_TRY(scales(w_scales_dev, ld_w_scales, N, (uint32_t*)g.w_scales));
-    if (!p.planes) RP_TRY(scales(a_scales_dev, ld_a_scales, M, (uint32_t*)g.a_scales));
-    const int64_t strip = std::max<int64_t>(1, ((int64_t)1 << 25) / p.nc) * 16;
-    for (int64_t m0 = 0; p.planes && m0 < M; m0 += strip) {
-      const int m = (int)std::min(strip, M - m0);
-      const int64_t units = rp_cdiv(m, 16) * p.nc * 64;
-      const unsigned grid = (unsigned)rp_cdiv(units, 256);
-      uint16_t* o = (uint16_t*)(ws + m0 / 16 * p.nc * p.planes * 4096);
-      if (a_type == RPHIP_BF16) k_mxg_planes<__bf16, 1><<<grid, 256, 0, st>>>((const __bf16*)A_dev + m0 * lda, lda, m, (int)K, p.nc, units, o);
-      else if (a_type == RPHIP_F16) k_mxg_planes<_Float16, 2><<<grid, 256, 0, st>>>((const _Float16*)A_dev + m0 * lda, lda, m, (int)K, p.nc, units, o);
-      else k_mxg_planes<float, 3><<<grid, 256, 0, st>>>((const float*)A_dev + m0 * lda, lda, m, (int)K, p.nc, units, o);
-      RP_LAUNCHED();
-    }
+    if (a_type == RPHIP_BF16) go(k_mxg_prepare<__bf16, 1>, __bf16{}, A_dev, lda, (void*)g.planes);
+    else if (a_type == RPHIP_F16) go(k_mxg_prepare<_Float16, 2>, _Float16{}, A_dev, lda, (void*)g.planes);
+    else if (a_type == RPHIP_F32) go(k_mxg_prepare<float, 3>, 0.0f, A_dev, lda, (void*)g.planes);
+    else go(k_mxg_prepare<uint8_t, 0>, uint8_t{0}, a_scales_dev, ld_a_scales, (void*)g.a_scales);
+    RP_LAUNCHED();
   }
   return rp_by_type(c_type, [&](auto tag) -> int {
     using OT = typename decltype(tag)::T;
     if (p.planes == 0) {
-      if (p.bm == 32) RP_TRY((launch_fp4<OT, 32, 32, 1, 2, 4>(g, st)));
-      else if (p.bm == 64) RP_TRY((launch_fp4<OT, 64, 64, 2, 2, 4>(g, st)));
-      else if (p.bm == 128) RP_TRY((launch_fp4<OT, 128, 128, 2, 2, 4>(g, st)));
-      else RP_TRY((launch_fp4<OT, 256, 256, 2, 4, 4>(g, st)));
+      if (p.bm == 32) RP_TRY((launch_fp4<OT, 32, 32, 1, 2>(g, st)));
+      else if (p.bm == 64) RP_TRY((launch_fp4<OT, 64, 64, 2, 2>(g, st)));
+      else if (p.bm == 128) RP_TRY((launch_fp4<OT, 128, 128, 2, 2>(g, st)));
+      else RP_TRY((launch_fp4<OT, 256, 256, 2, 4>(g, st)));
     } else {
-      if (p.bm == 16) RP_TRY((launch_bf16<OT, 16, 64, 1, 2, 4>(g, p.planes, st)));
-      else if (p.bm == 64) RP_TRY((launch_bf16<OT, 64, 64, 2, 2, 4>(g, p.planes, st)));
-      else if (p.bm == 128) RP_TRY((launch_bf16<OT, 128, 128, 2, 2, 4>(g, p.planes, st)));
-      else RP_TRY((launch_bf16<OT, 256, 256, 2, 4, 4>(g, p.planes, st)));
+      if (p.bm == 16) RP_TRY((launch_bf16<OT, 16, 64, 1, 2>(g, p.planes, st)));
+      else if (p.bm == 64) RP_TRY((launch_bf16<OT, 64, 64, 2, 2>(g, p.planes, st)));
+      else if (p.bm == 128) RP_TRY((launch_bf16<OT, 128, 128, 2, 2>(g, p.planes, st)));
+      else RP_TRY((launch_bf16<OT, 256, 256, 2, 4>(g, p.planes, st)));
     }
     if (p.split > 1) {
       k_mxg_join<OT><<<(unsigned)rp_cdiv(M * N, 256), 256, 0, st>>>(g.part, p.split, g.M, g.N, (OT*)C_dev, ldc);
