@@ -289,14 +289,14 @@ __global__ __launch_bounds__(WM * WN * 64) void k_mxg_bf16(gemm_args g) {
   store_tile<OT, TM, TN>(g, acc, m0 + wm * 16, tn * BN + wn * 16, lane);
 }
 
-// 4-bit form: codes of both operands in a ring of four stages (a stage is a chunk of both), requested three ahead; scales of four chunks in
-// two slots.
+// 4-bit form: codes of both operands in two slots, a stage (two chunks of both) ahead; scales in two slots of four chunks.  A piece is
+// eight rows of 128 bytes: 64 bytes a row and chunk fetched every cache line twice (1.16 -> 0.98 ms at 4096 x 20000 x 20000).
 template <class OT, int BM, int BN, int WM, int WN>
 __global__ __launch_bounds__(WM * WN * 64) void k_mxg_fp4(gemm_args g) {
-  constexpr int WAVES = WM * WN, TM = BM / WM / 16, TN = BN / WN / 16, RING = 4;
-  constexpr int STAGE = (BM + BN) * 64, D = (BM + BN) / 16 / WAVES;
-  constexpr int SCALES = (BM + BN) * 16, SLANES = (BM + BN) / WAVES, SOFF = RING * STAGE;
-  static_assert(D * WAVES * 16 == BM + BN && SLANES <= 64, "every wave requests the same number of pieces");
+  constexpr int WAVES = WM * WN, TM = BM / WM / 16, TN = BN / WN / 16;
+  constexpr int STAGE = (BM + BN) * 128, D = (BM + BN) / 8 / WAVES;
+  constexpr int SCALES = (BM + BN) * 16, SLANES = (BM + BN) / WAVES, SOFF = 2 * STAGE;
+  static_assert(D * WAVES * 8 == BM + BN && SLANES <= 64, "every wave requests the same number of pieces");
   extern __shared__ __attribute__((aligned(1024))) uint8_t ring[];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   int tm, tn;
@@ -309,18 +309,19 @@ __global__ __launch_bounds__(WM * WN * 64) void k_mxg_fp4(gemm_args g) {
     for (int j = 0; j < TN; ++j) acc[i][j] = f32x4{0, 0, 0, 0};
   const int z = blockIdx.y;
   const int q0 = (int)((int64_t)g.nq * z / g.split), q1 = (int)((int64_t)g.nq * (z + 1) / g.split);
-  const int c0 = q0 * 4, c1 = min(q1 * 4, g.nc);
+  const int s0 = q0 * 2, s1 = min(q1 * 2, (g.nc + 1) / 2);  // stages: two chunks
   const int mblocks = (g.M + 15) / 16, nblocks = (g.N + 15) / 16;
+  // a piece: 8 rows x 128 bytes; row r's block j of the stage lies at j ^ (r & 7)
+  const int pr = lane >> 3, pj = (lane & 7) ^ pr;
   const uint8_t* src[D];
 #pragma unroll
   for (int d = 0; d < D; ++d) {
     const int f = wave * D + d;
-    src[d] = f < BM / 16 ? g.a_codes + (int64_t)min(tm * BM + f * 16 + (lane & 15), g.M - 1) * g.lda
-                         : g.w + (int64_t)min(tn * BN + (f - BM / 16) * 16 + (lane & 15), g.N - 1) * g.ldw;
+    src[d] = f < BM / 8 ? g.a_codes + (int64_t)min(tm * BM + f * 8 + pr, g.M - 1) * g.lda : g.w + (int64_t)min(tn * BN + (f - BM / 8) * 8 + pr, g.N - 1) * g.ldw;
   }
-  auto request = [&](int c) __attribute__((always_inline)) {
-    const int b = min(min(c, c1 - 1) * 4 + (lane >> 4), g.nb - 1);
-    uint8_t* to = ring + (c & 3) * STAGE + wave * D * 1024;
+  auto request = [&](int s) __attribute__((always_inline)) {
+    const int b = min(min(s, s1 - 1) * 8 + pj, g.nb - 1);
+    uint8_t* to = ring + (s & 1) * STAGE + wave * D * 1024;
 #pragma unroll
     for (int d = 0; d < D; ++d) dma16(src[d] + (int64_t)b * 16, to + d * 1024);
   };
@@ -330,44 +331,48 @@ __global__ __launch_bounds__(WM * WN * 64) void k_mxg_fp4(gemm_args g) {
   auto request_scales = [&](int q) __attribute__((always_inline)) {
     if (SLANES == 64 || lane < SLANES) dma16(ssrc + (int64_t)min(q, q1 - 1) * 256, ring + SOFF + (q & 1) * SCALES + wave * SLANES * 16);
   };
-  if (c0 < c1) {
+  if (s0 < s1) {
     request_scales(q0);
-#pragma unroll
-    for (int r = 0; r < RING - 1; ++r) request(c0 + r);
+    request(s0);
     int sc[TM + TN];
+    const int fr = lane & 15, fg = lane >> 4;
+    const uint8_t* rd = ring + fr * 128;
     for (int q = q0; q < q1; ++q) {
-      auto chunk = [&](auto tag, int c) __attribute__((always_inline)) {
-        constexpr int CC = decltype(tag)::value;
-        wait_loads_and_meet<(RING - 2) * D>();
-        if (CC == 0) request_scales(q + 1);
-        request(c + RING - 1);
-        if (CC == 0) {
+      auto stage = [&](auto tag, int s) __attribute__((always_inline)) {
+        constexpr int H = decltype(tag)::value;
+        wait_loads_and_meet<0>();
+        if (H == 0) request_scales(q + 1);
+        request(s + 1);
+        if (H == 0) {
           const uint8_t* ss = ring + SOFF + (q & 1) * SCALES + lane * 4;
 #pragma unroll
           for (int i = 0; i < TM; ++i) sc[i] = *(const int*)(ss + (wm + i) * 256);
 #pragma unroll
           for (int j = 0; j < TN; ++j) sc[TM + j] = *(const int*)(ss + (BM / 16 + wn + j) * 256);
         }
-        const uint8_t* st = ring + (c & 3) * STAGE + lane * 16;
-        i32x8 wf[TN];
 #pragma unroll
-        for (int j = 0; j < TN; ++j) {
-          const i32x4 v = *(const i32x4*)(st + (BM / 16 + wn + j) * 1024);
-          wf[j] = i32x8{v.x, v.y, v.z, v.w, 0, 0, 0, 0};
-        }
+        for (int p = 0; p < 2; ++p) {
+          const uint8_t* st = rd + H * STAGE + (((p * 4 + fg) ^ (fr & 7)) * 16);
+          i32x8 wf[TN];
 #pragma unroll
-        for (int i = 0; i < TM; ++i) {
-          const i32x4 v = *(const i32x4*)(st + (wm + i) * 1024);
-          const i32x8 af = {v.x, v.y, v.z, v.w, 0, 0, 0, 0};
+          for (int j = 0; j < TN; ++j) {
+            const i32x4 v = *(const i32x4*)(st + (BM / 16 + wn + j) * 2048);
+            wf[j] = i32x8{v.x, v.y, v.z, v.w, 0, 0, 0, 0};
+          }
 #pragma unroll
-          for (int j = 0; j < TN; ++j) acc[i][j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(wf[j], af, acc[i][j], 4, 4, CC, sc[TM + j], CC, sc[i]);
+          for (int i = 0; i < TM; ++i) {
+            const i32x4 v = *(const i32x4*)(st + (wm + i) * 2048);
+            const i32x8 af = {v.x, v.y, v.z, v.w, 0, 0, 0, 0};
+#pragma unroll
+            for (int j = 0; j < TN; ++j) {
+              if (p == 0) acc[i][j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(wf[j], af, acc[i][j], 4, 4, H * 2, sc[TM + j], H * 2, sc[i]);
+              else acc[i][j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(wf[j], af, acc[i][j], 4, 4, H * 2 + 1, sc[TM + j], H * 2 + 1, sc[i]);
+            }
+          }
         }
       };
-      const int c = q * 4;
-      chunk(std::integral_constant<int, 0>{}, c);
-      if (c + 1 < c1) chunk(std::integral_constant<int, 1>{}, c + 1);
-      if (c + 2 < c1) chunk(std::integral_constant<int, 2>{}, c + 2);
-      if (c + 3 < c1) chunk(std::integral_constant<int, 3>{}, c + 3);
+      stage(std::integral_constant<int, 0>{}, q * 2);
+      if (q * 2 + 1 < s1) stage(std::integral_constant<int, 1>{}, q * 2 + 1);
     }
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // (the trailing requests write LDS)
   }
@@ -377,14 +382,16 @@ __global__ __launch_bounds__(WM * WN * 64) void k_mxg_fp4(gemm_args g) {
 // ---- few rows of A -------------------------------------------------------------------------------------------------------------------
 // M <= 4: every element of W is wanted M times, so its bytes are the time, and the vector unit keeps up: half a conversion and M
 // multiply-adds in float32 per element (no planes, no workspace).  A wave takes GV_ROWS rows of W at once, a lane every 64th MX block of
-// them: 1 KB contiguous per row and step; A's block is read and converted once for the GV_ROWS rows.
+// them: 1 KB contiguous per row and step.  The four waves of a workgroup share A's 2048 elements of a step in LDS as float32, in
+// the order [16 bytes of a block][block]: a lane reads its block without bank conflicts (from memory, 64 - 128 bytes apart, these reads
+// took longer than W: 80 us instead of 48 at 1 x 20000 x 20000 in f32).
 constexpr int GV_ROWS = 4;
 template <class T, class OT, int M>
 __global__ __launch_bounds__(256) void k_mxg_rows(const T* __restrict__ a, int64_t lda, int m_real, int N, int K, int nb, const uint8_t* __restrict__ w, int64_t ldw,
                                                   const uint8_t* __restrict__ ws, int64_t ldws, OT* __restrict__ c, int64_t ldc) {
+  __shared__ f32x4 sa[M][8 * 64];
   const int lane = threadIdx.x & 63;
   const int64_t n0 = ((int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6)) * GV_ROWS;
-  if (n0 >= N) return;
   const uint8_t* wr[GV_ROWS];
   const uint8_t* sr[GV_ROWS];
 #pragma unroll
@@ -393,9 +400,6 @@ __global__ __launch_bounds__(256) void k_mxg_rows(const T* __restrict__ a, int64
     wr[r] = w + n * ldw;
     sr[r] = ws + n * ldws;
   }
-  const T* ar[M];
-#pragma unroll
-  for (int m = 0; m < M; ++m) ar[m] = a + (int64_t)min(m, m_real - 1) * lda;
   float acc[GV_ROWS][M];
 #pragma unroll
   for (int r = 0; r < GV_ROWS; ++r)
@@ -404,34 +408,46 @@ __global__ __launch_bounds__(256) void k_mxg_rows(const T* __restrict__ a, int64
   uint4 q[GV_ROWS], qn[GV_ROWS];
   uint32_t s[GV_ROWS], sn[GV_ROWS];
   auto fetch = [&](int b) __attribute__((always_inline)) {
-    const int bb = min(b, nb - 1);
+    const int bb = min(b, nb - 1);  // (a block beyond the row: A is zero there)
 #pragma unroll
     for (int r = 0; r < GV_ROWS; ++r) {
       qn[r] = *(const uint4*)(wr[r] + (int64_t)bb * 16);
       sn[r] = sr[r][bb];
     }
   };
-  if (lane < nb) fetch(lane);
-  for (int b = lane; b < nb; b += 64) {
+  rp_vec<T, 8> an[M];  // this thread's eight elements of the next step
+  auto fetch_a = [&](int b0) __attribute__((always_inline)) {
+    const int64_t k = (int64_t)b0 * RP_MX + threadIdx.x * 8;
+#pragma unroll
+    for (int m = 0; m < M; ++m) {
+      const T* p = a + (int64_t)min(m, m_real - 1) * lda + k;
+      if (k + 8 <= K) an[m] = rp_load_vec<T, 8>(p);
+      else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) an[m].v[i] = k + i < K ? p[i] : (T)0.0f;
+      }
+    }
+  };
+  fetch(lane);
+  fetch_a(0);
+  for (int b0 = 0; b0 < nb; b0 += 64) {
+    __syncthreads();
+    const int at = (threadIdx.x & 3) * 2 * 64 + (threadIdx.x >> 2);
+#pragma unroll
+    for (int m = 0; m < M; ++m) {
+      sa[m][at] = f32x4{rp_to_f32(an[m].v[0]), rp_to_f32(an[m].v[1]), rp_to_f32(an[m].v[2]), rp_to_f32(an[m].v[3])};
+      sa[m][at + 64] = f32x4{rp_to_f32(an[m].v[4]), rp_to_f32(an[m].v[5]), rp_to_f32(an[m].v[6]), rp_to_f32(an[m].v[7])};
+    }
+    __syncthreads();
 #pragma unroll
     for (int r = 0; r < GV_ROWS; ++r) q[r] = qn[r], s[r] = sn[r];
-    fetch(b + 64);
-    const int k = b * RP_MX;
-    const bool whole = k + RP_MX <= K;
+    fetch(b0 + 64 + lane);
+    fetch_a(b0 + 64);
 #pragma unroll
     for (int g = 0; g < 4; ++g) {
-      float v[M][8];
+      f32x4 v[M][2];
 #pragma unroll
-      for (int m = 0; m < M; ++m) {
-        if (whole) {
-          const rp_vec<T, 8> t = rp_load_vec<T, 8>(ar[m] + k + g * 8);
-#pragma unroll
-          for (int i = 0; i < 8; ++i) v[m][i] = rp_to_f32(t.v[i]);
-        } else {
-#pragma unroll
-          for (int i = 0; i < 8; ++i) v[m][i] = k + g * 8 + i < K ? rp_to_f32(ar[m][k + g * 8 + i]) : 0.0f;
-        }
-      }
+      for (int m = 0; m < M; ++m) v[m][0] = sa[m][g * 128 + lane], v[m][1] = sa[m][g * 128 + 64 + lane];
 #pragma unroll
       for (int r = 0; r < GV_ROWS; ++r) {
         float x[8];
@@ -439,7 +455,7 @@ __global__ __launch_bounds__(256) void k_mxg_rows(const T* __restrict__ a, int64
 #pragma unroll
         for (int m = 0; m < M; ++m)
 #pragma unroll
-          for (int i = 0; i < 8; ++i) acc[r][m] = fmaf(v[m][i], x[i], acc[r][m]);
+          for (int i = 0; i < 8; ++i) acc[r][m] = fmaf(v[m][i >> 2][i & 3], x[i], acc[r][m]);
       }
     }
   }
@@ -472,22 +488,42 @@ struct plan {
   int64_t total() const { return plane_bytes + a_scale_bytes + w_scale_bytes + part_bytes; }
 };
 
+// Which tile, and into how many parts K is split: by rounds of workgroups over the CUs.  Measured on W of 20000 x 20000 unless said.
 plan make_plan(int n_cu, int64_t M, int64_t N, int64_t K, int32_t a_type) {
   plan p;
   p.planes = a_type == RPHIP_BF16 ? 1 : a_type == RPHIP_F16 ? 2 : a_type == RPHIP_F32 ? 3 : 0;
   p.nc = (int)rp_cdiv(K, KC);
   p.nq = (int)rp_cdiv(p.nc, 4);
-  auto tiles = [&](int bm, int bn) { return rp_cdiv(M, bm) * rp_cdiv(N, bn); };
-  p.rows = p.planes != 0 && M <= 4;
+  // the vector unit's form: f32 105 us against 120 at M = 4, 16 bits 63 against 91 at M = 2 (but 110 at 4)
+  p.rows = p.planes != 0 && M <= (p.planes == 3 ? 4 : 2) && K > 0;
   if (p.rows) return p;
-  if (M <= 16) p.bm = p.planes ? 16 : 32, p.bn = p.planes ? 64 : 32;
-  else if (tiles(256, 256) >= n_cu) p.bm = 256, p.bn = 256;
-  else if (tiles(128, 128) >= n_cu) p.bm = 128, p.bn = 128;
-  else p.bm = 64, p.bn = 64;
-  const int64_t n = std::max<int64_t>(tiles(p.bm, p.bn), 1), depth = p.planes ? p.nc / 2 : p.nq;
-  // workgroups that a CU holds at once: small tiles wait for memory together
-  const int per_cu = p.bm >= 256 ? 1 : p.bm == 128 ? 2 : p.bm == 64 ? 4 : 8;
-  p.split = (int)std::max<int64_t>(1, std::min<int64_t>({per_cu * (int64_t)n_cu / n, depth, 16}));
+  auto tiles = [&](int bm, int bn) { return std::max<int64_t>(rp_cdiv(M, bm) * rp_cdiv(N, bn), 1); };
+  auto rounds = [&](int bm, int bn, int per_cu) { return rp_cdiv(tiles(bm, bn), per_cu * n_cu); };
+  if (p.planes) {
+    const int64_t steps = (int64_t)p.nc * p.planes * 2;
+    int per_cu = 1;  // workgroups a CU should see when K is split: small tiles wait for memory together
+    if (M <= 16) {
+      p.bm = 16, p.bn = 64, per_cu = 5;
+    } else if (M > 128 && tiles(128, 256) >= n_cu) {
+      // a 128 x 256 tile takes 0.57 of a 256 x 256 one (527 and 302 us a round); three planes do not fit the larger one's registers
+      p.bn = 256;
+      p.bm = p.planes == 3 || rounds(128, 256, 1) * 57 < rounds(256, 256, 1) * 100 ? 128 : 256;
+    } else if (M > 64 && tiles(128, 128) * steps >= 40000) {
+      p.bm = 128, p.bn = 128, per_cu = 5;  // (M = 128: 157 us in eight parts, 199 with 64 x 64 tiles; 1000 x 3000 x 3000: 39 against 36)
+    } else {
+      p.bm = 64, p.bn = 64, per_cu = 4;
+    }
+    const int64_t n = tiles(p.bm, p.bn);
+    // (a part of fewer than 24 steps costs more to join than it saves: 500 x 2000 x 2000 in f16 24 us whole, 28 in four parts)
+    p.split = (int)std::max<int64_t>(1, std::min<int64_t>({(per_cu * (int64_t)n_cu + n / 2) / n, steps / 24, 16}));
+  } else {
+    // a round of 64 x 64 tiles (four a CU), 128 x 128 (two), 256 x 256 (one) takes 34, 45, 58 us at K = 8000
+    const int64_t t64 = rounds(64, 64, 4) * 58, t128 = rounds(128, 128, 2) * 76, t256 = rounds(256, 256, 1) * 100;
+    p.bm = M <= 32 ? 32 : t64 <= t128 && t64 <= t256 ? 64 : t128 <= t256 ? 128 : 256;
+    p.bn = p.bm;
+    const int64_t n = tiles(p.bm, p.bn);
+    p.split = (int)std::max<int64_t>(1, std::min<int64_t>({(n_cu + n / 2) / n, p.nq / 8, 16}));
+  }
   auto room = [](int64_t b) { return (b + 255) & ~(int64_t)255; };
   p.plane_bytes = room(rp_cdiv(M, 16) * p.nc * p.planes * 4096);
   p.a_scale_bytes = p.planes ? 0 : room(rp_cdiv(M, 16) * p.nq * 256);
@@ -509,7 +545,7 @@ int launch_tiles(Kernel kernel, gemm_args g, int threads, int lds, hipStream_t s
 }
 template <class OT, int BM, int BN, int WM, int WN>
 int launch_fp4(const gemm_args& g, hipStream_t st) {
-  return launch_tiles<BM, BN>(k_mxg_fp4<OT, BM, BN, WM, WN>, g, WM * WN * 64, 4 * (BM + BN) * 64 + 2 * (BM + BN) * 16, st);
+  return launch_tiles<BM, BN>(k_mxg_fp4<OT, BM, BN, WM, WN>, g, WM * WN * 64, 2 * (BM + BN) * 128 + 2 * (BM + BN) * 16, st);
 }
 template <class OT, int BM, int BN, int WM, int WN>
 int launch_bf16(const gemm_args& g, int planes, hipStream_t st) {
@@ -602,7 +638,8 @@ extern "C" int rphip_mxfp4_gemm_nt(rphip_ctx* ctx, void* stream, int64_t M, int6
     } else {
       if (p.bm == 16) RP_TRY((launch_bf16<OT, 16, 64, 1, 2>(g, p.planes, st)));
       else if (p.bm == 64) RP_TRY((launch_bf16<OT, 64, 64, 2, 2>(g, p.planes, st)));
-      else if (p.bm == 128) RP_TRY((launch_bf16<OT, 128, 128, 2, 2>(g, p.planes, st)));
+      else if (p.bm == 128 && p.bn == 128) RP_TRY((launch_bf16<OT, 128, 128, 2, 2>(g, p.planes, st)));
+      else if (p.bm == 128) RP_TRY((launch_bf16<OT, 128, 256, 2, 4>(g, p.planes, st)));
       else RP_TRY((launch_bf16<OT, 256, 256, 2, 4>(g, p.planes, st)));
     }
     if (p.split > 1) {

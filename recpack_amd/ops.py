@@ -106,7 +106,10 @@ def mxfp4_quantize(ctx, x: torch.Tensor, transpose: bool = False, out: MXFP4 | N
     rows, cols = (x.shape[1], x.shape[0]) if transpose else x.shape
     blocks = -(-cols // BLOCK)
     if out is None:
-        out = MXFP4(torch.empty(rows, blocks * 16, dtype=torch.uint8, device=x.device), torch.empty(rows, blocks, dtype=torch.uint8, device=x.device), cols)
+        # (rows of more than a cache line start at one: the products read them by lines)
+        width = blocks * 16
+        codes = torch.empty(rows, -(-width // 128) * 128 if width > 128 else width, dtype=torch.uint8, device=x.device)
+        out = MXFP4(codes[:, :width], torch.empty(rows, blocks, dtype=torch.uint8, device=x.device), cols)
     elif out.shape != (rows, cols):
         raise ValueError(f"out: {(rows, cols)} expected, got {out.shape}")
     _on(ctx, codes=out.codes, scales=out.scales)

@@ -453,3 +453,37 @@ def test_sample_strides_and_empty(ctx, ops):
         assert idx.shape == (0, 2) and nnz.shape == (0,)
     idx, prob, nnz = ops.sample(ctx, torch.zeros(3, 0, device="cuda"), torch.zeros(3, 2, device="cuda"))
     assert (idx == -1).all() and (prob == 0).all() and (nnz == 0).all()
+
+
+# ---- products in every tile shape: large enough for the plans that fill the card ------------------------------------------------------------
+
+def values_gpu(ops, ctx, m):
+    """float64 values on the GPU, by the format (the codes' table and 2^(s - 127))."""
+    lut = torch.from_numpy(np.concatenate([GRID, -GRID])).cuda()
+    c = torch.stack((m.codes & 15, m.codes >> 4), -1).view(m.shape[0], -1).long()
+    return (lut[c] * torch.exp2(m.scales.double() - 127).repeat_interleave(32, 1))[:, :m.cols]
+
+
+@pytest.mark.parametrize("dtype,m,n,k", [
+    (torch.bfloat16, 1100, 8010, 200), (torch.float16, 1100, 8010, 330), (torch.float32, 1100, 8010, 130),  # 128 x 256 tiles
+    (torch.bfloat16, 2050, 8200, 257), (torch.float16, 2050, 8200, 90),                                     # 256 x 256
+    (torch.bfloat16, 130, 20001, 8100), (torch.float32, 200, 9001, 4000),                                   # 128 x 128, K in parts
+    (torch.bfloat16, 33, 3001, 6000), (torch.float16, 64, 999, 9000), (torch.float32, 9, 2000, 5001), (torch.float32, 4, 5003, 7001),
+    ("mxfp4", 4000, 4200, 300), ("mxfp4", 600, 3001, 1000), ("mxfp4", 200, 1999, 5000), ("mxfp4", 20, 700, 9000)])
+def test_product_large(ctx, ops, dtype, m, n, k):
+    g = torch.Generator(device="cuda").manual_seed(m + n + k)
+    a = torch.randn(m, k, device="cuda", generator=g)
+    w = random_mxfp4(ops, n, k, 3)
+    if dtype == "mxfp4":
+        a = ops.mxfp4_quantize(ctx, a)
+        A, terms, out_type = values_gpu(ops, ctx, a), k, torch.float32
+    else:
+        a = a.to(dtype)
+        A, terms, out_type = a.double(), k * {torch.float32: 3, torch.float16: 2, torch.bfloat16: 1}[dtype], dtype
+    W = values_gpu(ops, ctx, w)
+    got = ops.mxfp4_gemm_nt(ctx, a, w)
+    want = A @ W.t()
+    bound = 8 * math.sqrt(terms) * 2.0 ** -23 * (A.abs() @ W.abs().t()) + torch.finfo(out_type).eps / 2 * want.abs() + torch.finfo(out_type).tiny
+    assert got.dtype == out_type
+    assert ((got.double() - want).abs() <= bound).all()
+    assert torch.equal(got, ops.mxfp4_gemm_nt(ctx, a, w))  # no part of K is added in another order
