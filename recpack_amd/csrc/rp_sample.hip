@@ -16,8 +16,8 @@ namespace {
 constexpr int RPS_SHORT = 1024;      // longest prefix the list form ranks completely
 constexpr int SL_CAP = 4096;         // candidates collected in LDS
 constexpr int SL_THREADS = 1024;
-constexpr int SB_BINS = 2048;        // mass bins of the whole-row form: 32 per e-fold, the last one takes what lies below e^-64
-constexpr double SB_PER_E = 32.0;
+constexpr int SB_BINS = 4096;        // mass bins of the whole-row form: 128 per e-fold, the last one takes what lies below e^-32
+constexpr double SB_PER_E = 128.0;
 constexpr int SB_CAP = 2048;         // entries of a list collected ahead
 constexpr int RC_FOUND = 512;        // ... of a workgroup's own part of them, in LDS
 constexpr int SR_THREADS = 256;      // threads of a workgroup that takes a slice of a row
@@ -128,6 +128,15 @@ __device__ __forceinline__ uint32_t xor_lane(uint32_t v, int lane) {
     const u32x2 r = __builtin_amdgcn_permlane32_swap(v, v, false, false);
     return lane & 32 ? r.x : r.y;
   }
+}
+
+__device__ __forceinline__ uint32_t wave_max_u32(uint32_t v, int lane) {
+  v = max(v, xor_lane<1>(v, lane));
+  v = max(v, xor_lane<2>(v, lane));
+  v = max(v, xor_lane<4>(v, lane));
+  v = max(v, xor_lane<8>(v, lane));
+  v = max(v, xor_lane<16>(v, lane));
+  return lane_u32(max(v, xor_lane<32>(v, lane)), 0);
 }
 
 // bitonic sort of 64 * PER entries, descending; entry lane * PER + i: steps shorter than PER stay in the lane's registers
@@ -265,6 +274,9 @@ __device__ void finish_row(const sample_args& a, int64_t r, const row_set& s, co
       }
     }
   }
+  double floor_of[PER];
+#pragma unroll
+  for (int i = 0; i < PER; ++i) floor_of[i] = greedy ? 0.0 : sum[i] * 0.015625;
   const int n_out = min(a.draws, kept);
   uint32_t gone = 0;  // bit i: rank 64 i + lane has been drawn
   for (int d0 = 0; d0 < a.draws; d0 += 64) {  // lane l keeps draw d0 + l
@@ -293,6 +305,7 @@ __device__ void finish_row(const sample_args& a, int64_t r, const row_set& s, co
           m[i] = i * 64 + lane < kept && !((gone >> i) & 1) ? mass_of(x[i]) : 0.0;
           cum[i] = wave_scan_f64(m[i]);
           sum[i] = lane_f64(cum[i], 63);
+          floor_of[i] = sum[i] * 0.015625;
           total += sum[i];
         }
       }
@@ -310,8 +323,15 @@ __device__ void finish_row(const sample_args& a, int64_t r, const row_set& s, co
           at = i * 64 + who;
           if (lane == d) rank = at, part = got, whole = total;
           if (lane == who) m[i] = 0.0, gone |= 1u << i;
-          cum[i] = wave_scan_f64(m[i]);
-          sum[i] = lane_f64(cum[i], 63);
+          // (what is left keeps a relative precision of 2^-46 as long as it is no less than 2^-6 of the last full sum)
+          if (sum[i] - got >= floor_of[i]) {
+            cum[i] -= lane >= who ? got : 0.0;
+            sum[i] = lane_f64(cum[i], 63);
+          } else {
+            cum[i] = wave_scan_f64(m[i]);
+            sum[i] = lane_f64(cum[i], 63);
+            floor_of[i] = sum[i] * 0.015625;
+          }
         }
         before += sum[i];
       }
@@ -489,14 +509,14 @@ __device__ __forceinline__ uint32_t select_key(const T* p, int len, int n, sel_s
 // k <= 1024: one workgroup per row finds a score that at least k candidates reach, collects those candidates, ranks them.
 // The threshold: every thread takes the best of two groups of the row's scores; if k of those 2048 group maxima reach a value, k
 // candidates do.  For rows in no particular order few more than k candidates reach the k-th largest group maximum (1.1 k at k = 200,
-// 1.4 k at 1000).  Rows that break this - thousands of equal scores - take the radix descent.  CACHED: the row stays in registers between
-// the two passes over it (up to TK_CACHE pieces of 16 bytes a thread).
-constexpr int TK_CACHE = 8;
-template <class T, bool CACHED>
+// 1.4 k at 1000).  Rows that break this - thousands of equal scores - take the radix descent.  A thread keeps the best score of each of its
+// HELD pieces of 16 bytes and reads again only those that reach the threshold (HELD = 0: any width, the whole row is read twice).
+constexpr int TK_HELD = 8;
+template <class T, int HELD>
 __global__ __launch_bounds__(SL_THREADS, 8) void k_sample_topk(sample_args a, unsigned long long* __restrict__ lists, int32_t* __restrict__ counts, int cap) {
   constexpr int E = PIECE<T>;
   __shared__ unsigned long long list[SL_CAP];
-  __shared__ uint32_t red[2][SL_THREADS / 64], tally[3][3];
+  __shared__ uint32_t red[2][SL_THREADS / 64], hist[256], pick[2];
   __shared__ uint32_t n_list, cnt;
   __shared__ sel_shared sel;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
@@ -504,103 +524,127 @@ __global__ __launch_bounds__(SL_THREADS, 8) void k_sample_topk(sample_args a, un
   const row_set s = rs_load(a, r);
   const T* p = (const T*)a.scores + r * a.ld;
   if (threadIdx.x == 0) n_list = 0;
-  rp_vec<T, E> held[CACHED ? TK_CACHE : 1];
-  float f0 = -INFINITY, f1 = -INFINITY;
-  auto maxima = [&](const rp_vec<T, E>& v) __attribute__((always_inline)) {  // (as numbers: the maximum leaves NaN out)
+  float f0 = -INFINITY, f1 = -INFINITY, tops[HELD > 0 ? HELD : 1];
+  auto maxima = [&](const rp_vec<T, E>& v) __attribute__((always_inline)) -> float {  // (as numbers: the maximum leaves NaN out)
+    float x = -INFINITY, y = -INFINITY;
 #pragma unroll
     for (int i = 0; i < E / 2; ++i) {
-      f0 = fmaxf(f0, rp_to_f32(v.v[i]));
-      f1 = fmaxf(f1, rp_to_f32(v.v[i + E / 2]));
+      x = fmaxf(x, rp_to_f32(v.v[i]));
+      y = fmaxf(y, rp_to_f32(v.v[i + E / 2]));
     }
+    f0 = fmaxf(f0, x);
+    f1 = fmaxf(f1, y);
+    return fmaxf(x, y);
   };
-  if constexpr (CACHED) {
+  if constexpr (HELD > 0) {
 #pragma unroll
-    for (int q = 0; q < TK_CACHE; ++q) {
-      const int j = (q * SL_THREADS + (int)threadIdx.x) * E;
-      if (j + E <= s.len) held[q] = rp_load_vec<T, E>(p + j);
-      else {
+    for (int q0 = 0; q0 < HELD; q0 += 4) {  // (four loads in flight: sixteen waves of two workgroups do the rest)
+      rp_vec<T, E> v[4];
 #pragma unroll
-        for (int i = 0; i < E; ++i) held[q].v[i] = j + i < s.len ? p[j + i] : rp_from_f32<T>(-INFINITY);
+      for (int q = 0; q < 4; ++q) {
+        const int j = ((q0 + q) * SL_THREADS + (int)threadIdx.x) * E;
+        if (j + E <= s.len) v[q] = rp_load_vec<T, E>(p + j);
+        else {
+#pragma unroll
+          for (int i = 0; i < E; ++i) v[q].v[i] = j + i < s.len ? p[j + i] : rp_from_f32<T>(-INFINITY);
+        }
       }
-    }
 #pragma unroll
-    for (int q = 0; q < TK_CACHE; ++q) maxima(held[q]);
+      for (int q = 0; q < 4; ++q) tops[q0 + q] = maxima(v[q]);
+      __builtin_amdgcn_sched_barrier(0);
+    }
   } else {
     scan_row<T>(p, 0, s.len, threadIdx.x, SL_THREADS, [&](int, const rp_vec<T, E>& v, int) __attribute__((always_inline)) { maxima(v); });
   }
   const uint32_t g0 = key_of(f0), g1 = key_of(f1);
-  // a value that at least k group maxima reach, and hardly more: four-way search between the least and the largest of them.  lo is always
-  // reached by k (at 0 by all 2048), hi never.
+  // a value that at least k group maxima reach, and hardly more: a histogram of 256 steps between the least and the largest of them, then
+  // of the step where the k-th lies, until few enough reach its lower end.  All 2048 reach lo, `above` of them reach hi.
   uint32_t lo, hi;
   {
     uint32_t v_hi = max(g0, g1), v_lo = ~min(g0, g1);
-    v_hi = max(v_hi, xor_lane<1>(v_hi, lane)), v_lo = max(v_lo, xor_lane<1>(v_lo, lane));
-    v_hi = max(v_hi, xor_lane<2>(v_hi, lane)), v_lo = max(v_lo, xor_lane<2>(v_lo, lane));
-    v_hi = max(v_hi, xor_lane<4>(v_hi, lane)), v_lo = max(v_lo, xor_lane<4>(v_lo, lane));
-    v_hi = max(v_hi, xor_lane<8>(v_hi, lane)), v_lo = max(v_lo, xor_lane<8>(v_lo, lane));
-    v_hi = max(v_hi, xor_lane<16>(v_hi, lane)), v_lo = max(v_lo, xor_lane<16>(v_lo, lane));
-    v_hi = max(v_hi, xor_lane<32>(v_hi, lane)), v_lo = max(v_lo, xor_lane<32>(v_lo, lane));
+    v_hi = wave_max_u32(v_hi, lane), v_lo = wave_max_u32(v_lo, lane);
     if (lane == 0) red[0][wave] = v_hi, red[1][wave] = v_lo;
-    if (threadIdx.x < 9) tally[threadIdx.x / 3][threadIdx.x % 3] = 0;
+    if (threadIdx.x < 256) hist[threadIdx.x] = 0;
     __syncthreads();
     hi = 0, lo = 0;
 #pragma unroll
     for (int w = 0; w < SL_THREADS / 64; ++w) hi = max(hi, red[0][w]), lo = max(lo, red[1][w]);
     lo = ~lo;
-    hi += hi != 0xffffffffu;
   }
   const uint32_t k = (uint32_t)s.k, enough = k + k / 4;
-  for (int it = 0; hi - lo > 1; it = it == 2 ? 0 : it + 1) {
-    const uint32_t q = max((hi - lo) / 4, 1u);
-    const uint32_t t1 = lo + q, t2 = min(t1 + q, hi), t3 = min(t2 + q, hi);
-    const uint32_t c1 = (uint32_t)__popcll(__ballot(g0 >= t1)) + (uint32_t)__popcll(__ballot(g1 >= t1));
-    const uint32_t c2 = (uint32_t)__popcll(__ballot(g0 >= t2)) + (uint32_t)__popcll(__ballot(g1 >= t2));
-    const uint32_t c3 = (uint32_t)__popcll(__ballot(g0 >= t3)) + (uint32_t)__popcll(__ballot(g1 >= t3));
-    if (lane == 0) {
-      if (c1) atomicAdd(&tally[it][0], c1);
-      if (c2) atomicAdd(&tally[it][1], c2);
-      if (c3) atomicAdd(&tally[it][2], c3);
+  uint32_t above = 0, steps = 256;  // group maxima beyond the range [lo, lo + (steps << shift))
+  for (int shift = max(24 - (int)__clz(hi - lo + 1), 0); hi > lo;) {
+    const uint32_t b0 = (g0 - lo) >> shift, b1 = (g1 - lo) >> shift;
+    if (g0 >= lo && b0 < steps) atomicAdd(&hist[b0], 1u);
+    if (g1 >= lo && b1 < steps) atomicAdd(&hist[b1], 1u);
+    __syncthreads();
+    if (wave == 0) {  // lane l: the bins 255 - 4 l downwards
+      uint32_t h[4], own = 0;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) h[i] = hist[255 - 4 * lane - i], own += h[i], hist[255 - 4 * lane - i] = 0;
+      uint32_t incl = own;
+      incl += dpp<0x111>(incl);
+      incl += dpp<0x112>(incl);
+      incl += dpp<0x114>(incl);
+      incl += dpp<0x118>(incl);
+      incl += dpp<0x142, 0xa>(incl);
+      incl += dpp<0x143, 0xc>(incl);
+      uint32_t run = above + incl - own;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        if (run < k && run + h[i] >= k) pick[0] = 255 - 4 * lane - i, pick[1] = run;
+        run += h[i];
+      }
     }
-    __syncthreads();  // (one barrier a step: the tallies of three steps take turns, the one of the step before is cleared here)
-    const uint32_t n1 = tally[it][0], n2 = tally[it][1], n3 = tally[it][2];
-    if (threadIdx.x < 3) tally[it == 0 ? 2 : it - 1][threadIdx.x] = 0;
-    uint32_t at;
-    if (n3 >= k) lo = t3, at = n3;
-    else if (n2 >= k) lo = t2, hi = t3, at = n2;
-    else if (n1 >= k) lo = t1, hi = t2, at = n1;
-    else hi = t1, at = 0xffffffffu;
-    if (at <= enough) break;
+    __syncthreads();
+    const uint32_t bin = pick[0];
+    above = pick[1];
+    lo += bin << shift;
+    if (shift == 0) break;
+    const uint32_t reach = (uint32_t)__popcll(__ballot(g0 >= lo)) + (uint32_t)__popcll(__ballot(g1 >= lo));
+    if (lane == 0) red[0][wave] = reach;
+    __syncthreads();
+    uint32_t n = 0;
+#pragma unroll
+    for (int w = 0; w < SL_THREADS / 64; ++w) n += red[0][w];
+    if (n <= enough) break;
+    steps = shift >= 8 ? 256u : 1u << shift;
+    shift = max(shift - 8, 0);
   }
   const float least = lo > 0x00800000u ? score_of(lo) : -FLT_MAX;  // (every candidate: neither -inf nor NaN passes)
-  auto take = [&](int j, const rp_vec<T, E>& v) __attribute__((always_inline)) {
-    float top = rp_to_f32(v.v[0]);
-#pragma unroll
-    for (int i = 1; i < E; ++i) top = fmaxf(top, rp_to_f32(v.v[i]));
-    if (!(top >= least)) return;
+  auto take = [&](int j, const rp_vec<T, E>& v, int m) __attribute__((always_inline)) {
 #pragma unroll
     for (int i = 0; i < E; ++i) {
       const float x = rp_to_f32(v.v[i]);
-      if (x >= least) {
+      if (i < m && x >= least) {
         const uint32_t at = atomicAdd(&n_list, 1u);
         if (at < SL_CAP) list[at] = ((unsigned long long)key_of(x) << 32) | (uint32_t) ~(j + i);
       }
     }
   };
-  if constexpr (CACHED) {
-    unsigned long long hits = 0;  // bit q E + i; the few that pass are read again
+  if constexpr (HELD > 0) {  // the few pieces that hold one are read again
+    uint32_t hits = 0;
 #pragma unroll
-    for (int q = 0; q < TK_CACHE; ++q)
-#pragma unroll
-      for (int i = 0; i < E; ++i) hits |= rp_to_f32(held[q].v[i]) >= least ? 1ull << (q * E + i) : 0ull;
+    for (int q = 0; q < HELD; ++q) hits |= tops[q] >= least ? 1u << q : 0u;
     while (hits) {
-      const int bit = (int)__ffsll((long long)hits) - 1;
+      const int j = (((int)__ffs((int)hits) - 1) * SL_THREADS + (int)threadIdx.x) * E;
       hits &= hits - 1;
-      const int j = (bit / E * SL_THREADS + (int)threadIdx.x) * E + bit % E;
-      const uint32_t at = atomicAdd(&n_list, 1u);
-      if (at < SL_CAP) list[at] = ((unsigned long long)key_of(rp_to_f32(p[j])) << 32) | (uint32_t)~j;
+      rp_vec<T, E> v;
+      const int m = min(E, s.len - j);
+      if (m == E) v = rp_load_vec<T, E>(p + j);
+      else {
+#pragma unroll
+        for (int i = 0; i < E; ++i) v.v[i] = i < m ? p[j + i] : (T)0.0f;
+      }
+      take(j, v, m);
     }
   } else {
-    scan_row<T>(p, 0, s.len, threadIdx.x, SL_THREADS, [&](int j, const rp_vec<T, E>& v, int) __attribute__((always_inline)) { take(j, v); });
+    scan_row<T>(p, 0, s.len, threadIdx.x, SL_THREADS, [&](int j, const rp_vec<T, E>& v, int m) __attribute__((always_inline)) {
+      float top = rp_to_f32(v.v[0]);
+#pragma unroll
+      for (int i = 1; i < E; ++i) top = fmaxf(top, rp_to_f32(v.v[i]));
+      if (top >= least) take(j, v, m);
+    });
   }
   __syncthreads();
   int n = (int)n_list;
@@ -738,42 +782,36 @@ __device__ __forceinline__ unsigned long long want_of(float u, unsigned long lon
 }
 
 // First candidate in rank order with (by_count: rank + 1 >= target; otherwise: cumulative mass up to and with it >= target).
-// list / n_list: the candidates of the bins lo .. hi, if they were collected ahead (n_list <= SB_CAP).  Returns its index (-1: none) and,
-// in *incl / *own, the cumulative mass with it and its own.
+// m / bm: this thread's bins and the masses before them, c / bc: the same in counts (by_count only).  ahead / n_ahead: the candidates of
+// the bins lo .. hi, if they were collected (n_ahead >= 0).  Returns its index (-1: none) and, in *incl / *own, the cumulative mass with it
+// and its own.
+constexpr int SEEK_PB = SB_BINS / SL_THREADS;
 template <class T>
-__device__ __forceinline__ int seek(const T* p, int len, const row_mass& rm, const row_ws& ws, bool by_count, unsigned long long target, seek_shared& sh, const unsigned long long* ahead,
-                    int n_ahead, int lo, int hi, unsigned long long* incl, unsigned long long* own) {
+__device__ __forceinline__ int seek(const T* p, int len, const row_mass& rm, const unsigned long long (&m)[SEEK_PB], const unsigned long long (&bm)[SEEK_PB],
+                                    const unsigned long long (&c)[SEEK_PB], const unsigned long long (&bc)[SEEK_PB], bool by_count, unsigned long long target,
+                                    seek_shared& sh, const unsigned long long* ahead, int n_ahead, int lo, int hi, unsigned long long* incl, unsigned long long* own) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  constexpr int PB = SB_BINS / SL_THREADS;
-  unsigned long long m[PB], c[PB], bm[PB], bc[PB];
-#pragma unroll
-  for (int i = 0; i < PB; ++i) {
-    m[i] = ws.hist_m[threadIdx.x * PB + i];
-    c[i] = by_count ? ws.hist_c[threadIdx.x * PB + i] : 0u;
-    bc[i] = 0;
-  }
   if (threadIdx.x == 0) sh.bin = SB_BINS, sh.n_list = 0, sh.found = 0xffffffffu;
-  scan_bins<SL_THREADS>(m, bm, sh.red64);
-  if (by_count) scan_bins<SL_THREADS>(c, bc, sh.red64);
+  __syncthreads();
 #pragma unroll
-  for (int i = 0; i < PB; ++i) {
+  for (int i = 0; i < SEEK_PB; ++i) {
     const unsigned long long run = by_count ? bc[i] : bm[i], step = by_count ? c[i] : m[i];
-    if (run < target && run + step >= target) sh.bin = threadIdx.x * PB + i;
+    if (run < target && run + step >= target) sh.bin = threadIdx.x * SEEK_PB + i;
   }
   __syncthreads();
   const bool have = n_ahead >= 0 && (int)sh.bin >= lo && (int)sh.bin <= hi;  // (never by count)
 #pragma unroll
-  for (int i = 0; i < PB; ++i)
-    if ((int)threadIdx.x * PB + i == (have ? lo : (int)sh.bin)) sh.before64 = bm[i], sh.before32 = (uint32_t)bc[i];
+  for (int i = 0; i < SEEK_PB; ++i)
+    if ((int)threadIdx.x * SEEK_PB + i == (have ? lo : (int)sh.bin)) sh.before64 = bm[i], sh.before32 = (uint32_t)bc[i];
   __syncthreads();
   const int b = (int)sh.bin;
   if (b >= SB_BINS) return -1;
   unsigned long long mass_before = sh.before64;
   unsigned long long count_before = sh.before32;
   int n = n_ahead;
-  if (have) {
+  if (have && n > 256) {
     for (int i = threadIdx.x; i < n; i += SL_THREADS) sh.list[i] = ahead[i];
-  } else {  // collect the bin
+  } else if (!have) {  // collect the bin
     scan_row<T>(p, 0, len, threadIdx.x, SL_THREADS, [&](int j, const rp_vec<T, PIECE<T>>& v, int) __attribute__((always_inline)) {
 #pragma unroll
       for (int i = 0; i < PIECE<T>; ++i) {
@@ -786,6 +824,37 @@ __device__ __forceinline__ int seek(const T* p, int len, const row_mass& rm, con
     });
     __syncthreads();
     n = (int)sh.n_list;
+  }
+  if (n <= 256) {  // one wave ranks them and adds up
+    if (wave == 0) {
+      unsigned long long e[4];
+      const unsigned long long* from = have ? ahead : sh.list;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) e[i] = i * 64 + lane < n ? from[i * 64 + lane] : 0ull;
+      rank_row<4>(e, sh.list, lane);
+      unsigned long long run = mass_before;
+      bool looking = true;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int rank = i * 64 + lane;
+        const unsigned long long mine = rank < n ? rm.mass(rm.log2_of(score_of((uint32_t)(sh.list[rank] >> 32)))) : 0ull;
+        const unsigned long long cum = run + wave_scan_u64(mine);
+        const unsigned long long pass = __ballot(rank < n && (by_count ? count_before + rank + 1 == target : cum >= target));
+        if (looking && pass) {
+          const int who = (int)__ffsll((long long)pass) - 1;
+          looking = false;
+          if (lane == who) sh.found = (uint32_t)rank, sh.before64 = cum, sh.mass64 = mine;
+        }
+        run = lane_u64(cum, 63);
+      }
+    }
+    __syncthreads();
+    const uint32_t f = sh.found;
+    const unsigned long long got = f == 0xffffffffu ? 0ull : sh.list[f];
+    *incl = sh.before64;
+    *own = sh.mass64;
+    __syncthreads();
+    return f == 0xffffffffu ? -1 : (int)~(uint32_t)got;
   }
   if (n <= SL_CAP) {
     int n2 = 64;
@@ -917,10 +986,10 @@ __global__ __launch_bounds__(SR_THREADS) void k_row_best(sample_args a, row_ws* 
   if (threadIdx.x == 0) ws.best[sl] = best;
 }
 
+// (one load a lane: a loop over the slices is a chain of as many scalar loads, 10 us of a launch)
 __device__ __forceinline__ uint32_t best_of(const row_ws& ws, int slices) {
-  uint32_t best = 0;
-  for (int i = 0; i < slices; ++i) best = max(best, ws.best[i]);
-  return best;
+  const int lane = threadIdx.x & 63;
+  return wave_max_u32(lane < slices ? ws.best[lane] : 0u, lane);
 }
 
 template <class T, bool COUNT>
@@ -1067,24 +1136,30 @@ __global__ __launch_bounds__(SL_THREADS) void k_row_draw(sample_args a, const ro
   const row_mass rm = rm_make(best, s, shift);
   const int n1 = ws.b1 >= 0 && ws.n_list[0] <= SB_CAP ? (int)ws.n_list[0] : -1;
   const int n2 = ws.b2_hi >= ws.b2_lo && ws.n_list[1] <= SB_CAP ? (int)ws.n_list[1] : -1;
-  unsigned long long incl = 0, own = 0, total = 0;
-  for (int i = threadIdx.x; i < SB_BINS; i += SL_THREADS) total += ws.hist_m[i];
-  total = block_sum_u64<SL_THREADS>(total, sh.red64);
+  unsigned long long incl = 0, own = 0, m[SEEK_PB], bm[SEEK_PB], c[SEEK_PB], bc[SEEK_PB];
+#pragma unroll
+  for (int i = 0; i < SEEK_PB; ++i) {
+    m[i] = ws.hist_m[threadIdx.x * SEEK_PB + i];
+    c[i] = COUNT ? ws.hist_c[threadIdx.x * SEEK_PB + i] : 0u;
+    bc[i] = 0;
+  }
+  unsigned long long total = scan_bins<SL_THREADS>(m, bm, sh.red64);
   if (COUNT && (unsigned long long)s.k < ws.count) {
-    seek<T>(p, s.len, rm, ws, true, (unsigned long long)s.k, sh, nullptr, -1, 0, -1, &incl, &own);
+    scan_bins<SL_THREADS>(c, bc, sh.red64);
+    seek<T>(p, s.len, rm, m, bm, c, bc, true, (unsigned long long)s.k, sh, nullptr, -1, 0, -1, &incl, &own);
     total = incl;
   }
   unsigned long long kept = total;
   if (s.top_p < 1.0f && !rm.greedy) {
     const unsigned long long border = border_of(s.top_p, total);
     if (border < kept) {
-      seek<T>(p, s.len, rm, ws, false, border, sh, ws.list[0], n1, ws.b1, ws.b1, &incl, &own);
+      seek<T>(p, s.len, rm, m, bm, c, bc, false, border, sh, ws.list[0], n1, ws.b1, ws.b1, &incl, &own);
       kept = incl;
     }
   }
   if (!rm.greedy) kept = min(kept, max(ws.above, (unsigned long long)rm.scale));
   const unsigned long long want = rm.greedy ? 1ull : want_of(a.u[r * a.ld_u], kept);
-  const int at = seek<T>(p, s.len, rm, ws, false, want, sh, ws.list[1], n2, ws.b2_lo, ws.b2_hi, &incl, &own);
+  const int at = seek<T>(p, s.len, rm, m, bm, c, bc, false, want, sh, ws.list[1], n2, ws.b2_lo, ws.b2_hi, &incl, &own);
   if (threadIdx.x == 0) {
     a.idx[r] = at < 0 ? -1 : a.ids ? a.ids[r * a.ld_ids + at] : at;
     a.prob[r] = at < 0 ? 0.0f : rm.greedy ? 1.0f : (float)((double)own / (double)kept);
@@ -1164,8 +1239,9 @@ extern "C" int rphip_sample(rphip_ctx* ctx, void* stream, int64_t rows, int64_t 
           const int cap = list_of(k);
           unsigned long long* lists = (unsigned long long*)workspace_dev;
           int32_t* counts = (int32_t*)(lists + std::min(rows, STRIP_LISTS) * cap);
-          if (width <= TK_CACHE * SL_THREADS * PIECE<T>) k_sample_topk<T, true><<<n, SL_THREADS, 0, st>>>(a, lists, counts, cap);
-          else k_sample_topk<T, false><<<n, SL_THREADS, 0, st>>>(a, lists, counts, cap);
+          constexpr int64_t piece = SL_THREADS * PIECE<T>;
+          if (width <= TK_HELD * piece) k_sample_topk<T, TK_HELD><<<n, SL_THREADS, 0, st>>>(a, lists, counts, cap);
+          else k_sample_topk<T, 0><<<n, SL_THREADS, 0, st>>>(a, lists, counts, cap);
           RP_LAUNCHED();
           if (cap == 256) k_sample_lists<256, 256><<<n, 64, 0, st>>>(a, lists, counts);
           else if (k <= 256) k_sample_lists<512, 256><<<n, 64, 0, st>>>(a, lists, counts);
