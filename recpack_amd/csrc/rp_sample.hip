@@ -1117,9 +1117,44 @@ __global__ __launch_bounds__(SR_THREADS) void k_row_collect(sample_args a, row_w
       if (at_found[which] + i < SB_CAP) ws.list[which][at_found[which] + i] = found[which][i];
 }
 
+// A list of at most 256 candidates, ranked by one wave: sorted[] and the cumulative masses behind `before`, and each one's own.
+struct ranked_list {
+  unsigned long long sorted[256], cum[256], own[256];
+};
+__device__ __forceinline__ void rank_masses(unsigned long long (&e)[4], int n, unsigned long long before, const row_mass& rm, ranked_list& out, int lane) {
+  rank_row<4>(e, out.sorted, lane);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int rank = i * 64 + lane;
+    const unsigned long long mine = rank < n ? rm.mass(rm.log2_of(score_of((uint32_t)(out.sorted[rank] >> 32)))) : 0ull;
+    const unsigned long long cum = before + wave_scan_u64(mine);
+    out.cum[rank] = cum;
+    out.own[rank] = mine;
+    before = lane_u64(cum, 63);
+  }
+}
+// the first rank whose cumulative mass reaches the target (n if none); any whole wave
+__device__ __forceinline__ int rank_reaching(const ranked_list& l, int n, unsigned long long target, int lane) {
+  int at = n;
+#pragma unroll
+  for (int i = 3; i >= 0; --i) {
+    const unsigned long long pass = __ballot(i * 64 + lane < n && l.cum[i * 64 + lane] >= target);
+    if (pass) at = i * 64 + (int)__ffsll((long long)pass) - 1;
+  }
+  return at;
+}
+
 template <class T, bool COUNT>
 __global__ __launch_bounds__(SL_THREADS) void k_row_draw(sample_args a, const row_ws* __restrict__ wss, int slices, int shift) {
-  __shared__ seek_shared sh;
+  __shared__ union {
+    seek_shared seek;
+    struct {
+      ranked_list list[2];
+      unsigned long long before[2], kept;
+    } two;
+  } sh;
+  __shared__ unsigned long long red64[SL_THREADS / 64];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int64_t r = a.row0 + blockIdx.x;
   const row_ws& ws = wss[blockIdx.x];
   const row_set s = rs_load(a, r);
@@ -1134,8 +1169,14 @@ __global__ __launch_bounds__(SL_THREADS) void k_row_draw(sample_args a, const ro
     return;
   }
   const row_mass rm = rm_make(best, s, shift);
-  const int n1 = ws.b1 >= 0 && ws.n_list[0] <= SB_CAP ? (int)ws.n_list[0] : -1;
-  const int n2 = ws.b2_hi >= ws.b2_lo && ws.n_list[1] <= SB_CAP ? (int)ws.n_list[1] : -1;
+  const int b1 = ws.b1, b2_lo = ws.b2_lo, b2_hi = ws.b2_hi;
+  const int n1 = b1 >= 0 && ws.n_list[0] <= SB_CAP ? (int)ws.n_list[0] : -1;
+  const int n2 = b2_hi >= b2_lo && ws.n_list[1] <= SB_CAP ? (int)ws.n_list[1] : -1;
+  unsigned long long e[4];
+  if (wave < 2) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) e[i] = i * 64 + lane < (wave == 0 ? n1 : n2) ? ws.list[wave][i * 64 + lane] : 0ull;
+  }
   unsigned long long incl = 0, own = 0, m[SEEK_PB], bm[SEEK_PB], c[SEEK_PB], bc[SEEK_PB];
 #pragma unroll
   for (int i = 0; i < SEEK_PB; ++i) {
@@ -1143,23 +1184,55 @@ __global__ __launch_bounds__(SL_THREADS) void k_row_draw(sample_args a, const ro
     c[i] = COUNT ? ws.hist_c[threadIdx.x * SEEK_PB + i] : 0u;
     bc[i] = 0;
   }
-  unsigned long long total = scan_bins<SL_THREADS>(m, bm, sh.red64);
-  if (COUNT && (unsigned long long)s.k < ws.count) {
-    scan_bins<SL_THREADS>(c, bc, sh.red64);
-    seek<T>(p, s.len, rm, m, bm, c, bc, true, (unsigned long long)s.k, sh, nullptr, -1, 0, -1, &incl, &own);
+  unsigned long long total = scan_bins<SL_THREADS>(m, bm, red64);
+  const unsigned long long most = max(ws.above, (unsigned long long)rm.scale);
+  const bool cut_by_count = COUNT && (unsigned long long)s.k < ws.count;
+  // the common case - both lists are there and short: a wave each, side by side
+  if (!cut_by_count && !rm.greedy && (b1 < 0 || (n1 >= 1 && n1 <= 256)) && n2 >= 1 && n2 <= 256) {
+#pragma unroll
+    for (int i = 0; i < SEEK_PB; ++i) {
+      if ((int)threadIdx.x * SEEK_PB + i == b1) sh.two.before[0] = bm[i];
+      if ((int)threadIdx.x * SEEK_PB + i == b2_lo) sh.two.before[1] = bm[i];
+    }
+    __syncthreads();
+    if (wave == 0) {
+      unsigned long long kept = total;
+      if (b1 >= 0) {
+        rank_masses(e, n1, sh.two.before[0], rm, sh.two.list[0], lane);
+        kept = sh.two.list[0].cum[min(rank_reaching(sh.two.list[0], n1, border_of(s.top_p, total), lane), n1 - 1)];
+      }
+      if (lane == 0) sh.two.kept = min(kept, most);
+    } else if (wave == 1) {
+      rank_masses(e, n2, sh.two.before[1], rm, sh.two.list[1], lane);
+    }
+    __syncthreads();
+    if (wave != 1) return;
+    const unsigned long long kept = sh.two.kept;
+    const int rank = min(rank_reaching(sh.two.list[1], n2, want_of(a.u[r * a.ld_u], kept), lane), n2 - 1);
+    if (lane == 0) {
+      const int at = (int)~(uint32_t)sh.two.list[1].sorted[rank];
+      a.idx[r] = a.ids ? a.ids[r * a.ld_ids + at] : at;
+      a.prob[r] = (float)((double)sh.two.list[1].own[rank] / (double)kept);
+      if (a.nnz) a.nnz[r] = 1;
+    }
+    return;
+  }
+  if (cut_by_count) {
+    scan_bins<SL_THREADS>(c, bc, red64);
+    seek<T>(p, s.len, rm, m, bm, c, bc, true, (unsigned long long)s.k, sh.seek, nullptr, -1, 0, -1, &incl, &own);
     total = incl;
   }
   unsigned long long kept = total;
   if (s.top_p < 1.0f && !rm.greedy) {
     const unsigned long long border = border_of(s.top_p, total);
     if (border < kept) {
-      seek<T>(p, s.len, rm, m, bm, c, bc, false, border, sh, ws.list[0], n1, ws.b1, ws.b1, &incl, &own);
+      seek<T>(p, s.len, rm, m, bm, c, bc, false, border, sh.seek, ws.list[0], n1, b1, b1, &incl, &own);
       kept = incl;
     }
   }
-  if (!rm.greedy) kept = min(kept, max(ws.above, (unsigned long long)rm.scale));
+  if (!rm.greedy) kept = min(kept, most);
   const unsigned long long want = rm.greedy ? 1ull : want_of(a.u[r * a.ld_u], kept);
-  const int at = seek<T>(p, s.len, rm, m, bm, c, bc, false, want, sh, ws.list[1], n2, ws.b2_lo, ws.b2_hi, &incl, &own);
+  const int at = seek<T>(p, s.len, rm, m, bm, c, bc, false, want, sh.seek, ws.list[1], n2, b2_lo, b2_hi, &incl, &own);
   if (threadIdx.x == 0) {
     a.idx[r] = at < 0 ? -1 : a.ids ? a.ids[r * a.ld_ids + at] : at;
     a.prob[r] = at < 0 ? 0.0f : rm.greedy ? 1.0f : (float)((double)own / (double)kept);
