@@ -186,14 +186,163 @@ extern "C" int rphip_mxfp4_dequantize(rphip_ctx* ctx, void* stream, int64_t rows
 }
 
 // ---- scores of histories -----------------------------------------------------------------------------------------------------------
-// out[u, :] = sum over the entries e of user u of w_e * W[idx_e, :], in f32: the rows of a history are contiguous and their blocks run along
-// the output, so a lane owns one block of 32 columns (16 code bytes, one scale) of every row and keeps its 32 sums in registers: per
-// element half a conversion and one add.  A workgroup takes (user, 2048 columns); its waves take groups of four entries in turn and
-// add their sums up in wave order (the result does not depend on the launch).  Four rows are in flight while four are added.
-// Workgroups run through all users of a column tile before the next one: the rows' pieces of one tile (1 KB each) stay in the caches.
+// out[u, :] = sum over the entries e of user u of w_e * W[idx_e, :], in f32.  The rows of a history are contiguous and their blocks run along
+// the output.  A workgroup takes (user, 2048 columns); its waves take groups of four entries in turn and add their sums up in wave order
+// (the result does not depend on the launch).  Workgroups run through all users of a column tile before the next one: the rows' pieces
+// of one tile (1 KB each) stay in the caches.
 constexpr int MXS_COLS = 64 * RP_MX;
-template <class T, bool WEIGHTED, int WAVES>
-__global__ __launch_bounds__(64 * WAVES) void k_mx_scores(const int32_t* __restrict__ indptr, const int32_t* __restrict__ indices, const float* __restrict__ weights,
+
+// what both forms share: the entries of a chunk of 64, those that count moved to the front, in order; the history's own columns
+struct mxs_chunk {
+  int idx, m;
+  float wgt;
+};
+template <bool WEIGHTED>
+__device__ __forceinline__ mxs_chunk mxs_entries(const int32_t* __restrict__ indices, const float* __restrict__ weights, int64_t e0, int64_t e1, int rows, bool mark, int c0,
+                                                 uint32_t* drop, int lane) {
+  mxs_chunk k = {-1, 0, 0.0f};
+  const int n = (int)min((int64_t)64, e1 - e0);
+  if (lane < n) {
+    k.idx = indices[e0 + lane];
+    if ((unsigned)k.idx >= (unsigned)rows) k.idx = -1;
+    if (WEIGHTED) k.wgt = weights[e0 + lane];
+    if (mark && k.idx >= c0 && k.idx < c0 + MXS_COLS) atomicOr(&drop[(k.idx - c0) >> 5], 1u << (k.idx & 31));
+  }
+  const unsigned long long good = __ballot(k.idx >= 0);
+  k.m = (int)__popcll(good);
+  if (k.m < n) {
+    const int dst = k.idx >= 0 ? (int)__popcll(good & ((1ull << lane) - 1ull)) : 63;
+    k.idx = __builtin_amdgcn_ds_permute(dst * 4, k.idx);
+    if (WEIGHTED) k.wgt = __int_as_float(__builtin_amdgcn_ds_permute(dst * 4, __float_as_int(k.wgt)));
+  }
+  return k;
+}
+
+// Binary histories on the matrix pipe.  v_mfma_scale_f32_16x16x128 sums over K = 4 groups of 32, each with its own scale: the groups are four
+// history rows, the 16 columns of its right operand 16 MX blocks of them as they lie in memory (lane (block, row): 16 bytes and a
+// scale), its left operand a one per output row that picks one element of the 32.  Two such selections turn four rows' blocks into
+// 16 x 32 sums without a conversion: 64 elements a cycle and SIMD against 5 - 7 converted and added in the vector unit.  The selection
+// is laid out so that a lane ends with 8 neighbouring columns of its block.
+typedef int mxs_i32x8 __attribute__((ext_vector_type(8)));
+typedef int mxs_i32x4 __attribute__((ext_vector_type(4)));
+constexpr int MXS_GROUPS = MXS_COLS / 512;  // fragments of 16 blocks
+template <class T, int WAVES>
+__global__ __launch_bounds__(64 * WAVES) void k_mx_scores_sum(const int32_t* __restrict__ indptr, const int32_t* __restrict__ indices, int64_t nnz, int rows, int cols, int nb,
+                                                              const uint8_t* __restrict__ codes, int64_t ldc, const uint8_t* __restrict__ scales, int64_t lds, int exclude,
+                                                              const uint8_t* __restrict__ keep, T* __restrict__ out, int64_t ldo, int64_t user0) {
+  __shared__ uint32_t drop[64];  // bit c of word l: column 32 l + c of the tile gets -inf
+  __shared__ rp_f32x4 sums[WAVES > 1 ? WAVES * MXS_GROUPS * 2 * 64 : 1];
+  const int lane = threadIdx.x & 63, wave = WAVES > 1 ? __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) : 0;
+  const int fr = lane & 15, fg = lane >> 4;
+  const int64_t u = user0 + blockIdx.x;
+  const int b0 = blockIdx.y * 64;
+  if (wave == 0) drop[lane] = 0;
+  __syncthreads();
+  // left operand: output row q (this lane's fr) of half h picks element (q >> 2) * 8 + h * 4 + (q & 3) of every group's 32; code of 1.0: 2
+  mxs_i32x8 pick[2];
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    const int j = (fr >> 2) * 8 + h * 4 + (fr & 3);
+#pragma unroll
+    for (int w = 0; w < 8; ++w) pick[h][w] = w == j / 8 ? 2 << (j % 8 * 4) : 0;
+  }
+  rp_f32x4 acc[MXS_GROUPS][2];
+#pragma unroll
+  for (int q = 0; q < MXS_GROUPS; ++q)
+#pragma unroll
+    for (int h = 0; h < 2; ++h) acc[q][h] = rp_f32x4{0, 0, 0, 0};
+  int64_t co[MXS_GROUPS];  // this lane's blocks (past the row: the last one; not stored)
+#pragma unroll
+  for (int q = 0; q < MXS_GROUPS; ++q) co[q] = min(b0 + q * 16 + fr, nb - 1);
+  const int64_t e1 = min((int64_t)indptr[u + 1], nnz);
+  for (int64_t e0 = max((int64_t)indptr[u], (int64_t)0); e0 < e1; e0 += 64) {
+    const mxs_chunk ch = mxs_entries<false>(indices, nullptr, e0, e1, rows, exclude && wave == 0, blockIdx.y * MXS_COLS, drop, lane);
+    mxs_i32x4 w[2][MXS_GROUPS];
+    int sc[2][MXS_GROUPS];
+    auto fetch = [&](auto tag, int k) __attribute__((always_inline)) {  // entries k .. k + 3, one a lane group; past the end: zeros
+      constexpr int S = decltype(tag)::value;
+      const int64_t row = __shfl(ch.idx, (k + fg) & 63);
+      const bool there = k + fg < ch.m;
+#pragma unroll
+      for (int q = 0; q < MXS_GROUPS; ++q) {
+        w[S][q] = mxs_i32x4{0, 0, 0, 0};
+        sc[S][q] = 0;
+        if (there) {
+          w[S][q] = *(const mxs_i32x4*)(codes + row * ldc + co[q] * 16);
+          sc[S][q] = scales[row * lds + co[q]];
+        }
+      }
+    };
+    auto add = [&](auto tag) __attribute__((always_inline)) {
+      constexpr int S = decltype(tag)::value;
+#pragma unroll
+      for (int q = 0; q < MXS_GROUPS; ++q) {
+        const mxs_i32x8 v = {w[S][q].x, w[S][q].y, w[S][q].z, w[S][q].w, 0, 0, 0, 0};
+#pragma unroll
+        for (int h = 0; h < 2; ++h) acc[q][h] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(pick[h], v, acc[q][h], 4, 4, 0, 127, 0, sc[S][q]);
+      }
+    };
+    constexpr int STEP = 4 * WAVES;
+    using set0 = std::integral_constant<int, 0>;
+    using set1 = std::integral_constant<int, 1>;
+    int k = wave * 4;
+    if (k < ch.m) {
+      fetch(set0{}, k);
+      for (; k < ch.m; k += 2 * STEP) {
+        fetch(set1{}, k + STEP);
+        add(set0{});
+        fetch(set0{}, k + 2 * STEP);
+        add(set1{});
+      }
+    }
+  }
+  // lane (fr, fg): columns 8 fg .. 8 fg + 7 of the blocks 16 q + fr
+  if (WAVES > 1) {
+#pragma unroll
+    for (int q = 0; q < MXS_GROUPS; ++q)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) sums[((wave * MXS_GROUPS + q) * 2 + h) * 64 + lane] = acc[q][h];
+  }
+  __syncthreads();
+#pragma unroll
+  for (int q = 0; q < MXS_GROUPS; ++q) {
+    if (WAVES > 1) {
+      if (q % WAVES != wave) continue;  // (the waves share the fragments out)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        acc[q][h] = sums[q * 2 * 64 + h * 64 + lane];
+#pragma unroll
+        for (int o = 1; o < WAVES; ++o) acc[q][h] += sums[((o * MXS_GROUPS + q) * 2 + h) * 64 + lane];
+      }
+    }
+    const int b = b0 + q * 16 + fr;
+    if (b >= nb) continue;
+    const int c = b * RP_MX + fg * 8, left = min(8, cols - c);
+    uint32_t gone = drop[q * 16 + fr] >> (fg * 8);
+    float v[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      v[i] = acc[q][i >> 2][i & 3];
+      if (((gone >> i) & 1) || (keep && i < left && !keep[c + i])) v[i] = -INFINITY;
+    }
+    T* p = out + u * ldo + c;
+    if (left == 8) {
+      rp_vec<T, 8> t;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) t.v[i] = rp_from_f32<T>(v[i]);
+      rp_store_vec<T, 8>(p, t);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (i < left) p[i] = rp_from_f32<T>(v[i]);
+    }
+  }
+}
+
+// Weighted histories in the vector unit: a lane owns one block of 32 columns of every row and keeps its 32 sums in registers, half a
+// conversion and one multiply-add per element; four rows in flight while four are added.
+template <class T, int WAVES>
+__global__ __launch_bounds__(64 * WAVES) void k_mx_scores_weighted(const int32_t* __restrict__ indptr, const int32_t* __restrict__ indices, const float* __restrict__ weights,
                                                           int64_t nnz, int rows, int cols, int nb, const uint8_t* __restrict__ codes, int64_t ldc,
                                                           const uint8_t* __restrict__ scales, int64_t lds, int exclude, const uint8_t* __restrict__ keep,
                                                           T* __restrict__ out, int64_t ldo, int64_t user0) {
@@ -212,25 +361,9 @@ __global__ __launch_bounds__(64 * WAVES) void k_mx_scores(const int32_t* __restr
   const uint8_t* sbase = scales + b;
   const int64_t e1 = min((int64_t)indptr[u + 1], nnz);
   for (int64_t e0 = max((int64_t)indptr[u], (int64_t)0); e0 < e1; e0 += 64) {
-    const int n = (int)min((int64_t)64, e1 - e0);
-    int idx = -1;
-    float wgt = 0.0f;
-    if (lane < n) {
-      idx = indices[e0 + lane];
-      if ((unsigned)idx >= (unsigned)rows) idx = -1;
-      if (WEIGHTED) wgt = weights[e0 + lane];
-      if (exclude && wave == 0 && idx >= c0 && idx < c0 + MXS_COLS) atomicOr(&drop[(idx - c0) >> 5], 1u << (idx & 31));
-    }
-    // entries that count move to the front, in order
-    const unsigned long long good = __ballot(idx >= 0);
-    const int m = (int)__popcll(good);
-    if (m < n) {
-      const int dst = idx >= 0 ? (int)__popcll(good & ((1ull << lane) - 1ull)) : 63;
-      const int keep_idx = __builtin_amdgcn_ds_permute(dst * 4, idx);
-      const int keep_w = __builtin_amdgcn_ds_permute(dst * 4, __float_as_int(wgt));
-      idx = keep_idx;
-      wgt = __int_as_float(keep_w);
-    }
+    const mxs_chunk ch = mxs_entries<true>(indices, weights, e0, e1, rows, exclude && wave == 0, c0, drop, lane);
+    const int idx = ch.idx, m = ch.m;
+    const float wgt = ch.wgt;
     uint4 w[2][4];
     uint32_t sc[2][4];
     auto fetch = [&](auto tag, int k) __attribute__((always_inline)) {  // rows k .. k + 3 (past the end: the last one again)
@@ -248,14 +381,14 @@ __global__ __launch_bounds__(64 * WAVES) void k_mx_scores(const int32_t* __restr
       for (int i = 0; i < 4; ++i) {
         if (k + i >= m) break;
         const float s = rp_mx_scale(sc[S][i]);
-        const float f = WEIGHTED ? __int_as_float(__builtin_amdgcn_readlane(__float_as_int(wgt), k + i)) : 1.0f;
+        const float f = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(wgt), k + i));
         const uint32_t q[4] = {w[S][i].x, w[S][i].y, w[S][i].z, w[S][i].w};
 #pragma unroll
         for (int g = 0; g < 4; ++g) {
           float v[8];
           rp_mx_unpack8(q[g], s, v);
 #pragma unroll
-          for (int j = 0; j < 8; ++j) acc[g * 8 + j] = WEIGHTED ? fmaf(f, v[j], acc[g * 8 + j]) : acc[g * 8 + j] + v[j];
+          for (int j = 0; j < 8; ++j) acc[g * 8 + j] = fmaf(f, v[j], acc[g * 8 + j]);
         }
       }
     };
@@ -346,24 +479,26 @@ extern "C" int rphip_mxfp4_scores(rphip_ctx* ctx, void* stream, int64_t n_users,
   return rp_by_type(out_type, [&](auto tag) -> int {
     using T = typename decltype(tag)::T;
     const hipStream_t st = (hipStream_t)stream;
-    auto go = [&](auto weighted, auto waves) -> int {
+    constexpr int64_t strip = (int64_t)1 << 22;  // (users of a launch: below 2^32 threads)
+    auto go = [&](auto waves) -> int {
       constexpr int WV = decltype(waves)::value;
-      constexpr int64_t strip = (int64_t)1 << 22;  // (users of a launch: below 2^32 threads)
       for (int64_t u0 = 0; u0 < n_users; u0 += strip) {
         const dim3 grid((unsigned)std::min(strip, n_users - u0), (unsigned)tiles);
-        k_mx_scores<T, decltype(weighted)::value, WV><<<grid, 64 * WV, 0, st>>>(indptr_dev, indices_dev, weights_dev, nnz, (int)rows, (int)cols, nb, codes_dev, ld_codes,
-                                                                            scales_dev, ld_scales, exclude_history, item_keep_dev, (T*)out_dev, ld_out, u0);
+        if (weights_dev)
+          k_mx_scores_weighted<T, WV><<<grid, 64 * WV, 0, st>>>(indptr_dev, indices_dev, weights_dev, nnz, (int)rows, (int)cols, nb, codes_dev, ld_codes, scales_dev, ld_scales,
+                                                                exclude_history, item_keep_dev, (T*)out_dev, ld_out, u0);
+        else
+          k_mx_scores_sum<T, WV><<<grid, 64 * WV, 0, st>>>(indptr_dev, indices_dev, nnz, (int)rows, (int)cols, nb, codes_dev, ld_codes, scales_dev, ld_scales, exclude_history,
+                                                           item_keep_dev, (T*)out_dev, ld_out, u0);
         RP_LAUNCHED();
       }
       return RPHIP_OK;
     };
+    // few (user, tile) pairs: more waves to each
     using std::integral_constant;
     const int64_t groups = n_users * tiles;
-    auto by_waves = [&](auto weighted) -> int {
-      if (groups <= 4 * ctx->n_cu) return go(weighted, integral_constant<int, 8>{});
-      if (groups <= 32 * ctx->n_cu) return go(weighted, integral_constant<int, 4>{});
-      return go(weighted, integral_constant<int, 1>{});
-    };
-    return weights_dev ? by_waves(std::true_type{}) : by_waves(std::false_type{});
+    if (groups <= 4 * ctx->n_cu) return go(integral_constant<int, 8>{});
+    if (groups <= 32 * ctx->n_cu) return go(integral_constant<int, 4>{});
+    return go(integral_constant<int, 1>{});
   });
 }

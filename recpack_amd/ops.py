@@ -105,13 +105,13 @@ class MXFP4:
 
     @classmethod
     def empty(cls, rows: int, cols: int, device) -> "MXFP4":
-        """Room for a matrix.  (Rows of more than a cache line start at one: the products read them by lines.)"""
+        """Room for a matrix.  (The rows of one beyond a MB start at cache lines: the products read them by lines.)"""
         blocks = -(-cols // BLOCK)
         width = blocks * 16
-        line = -(-width // 128) * 128
-        codes = torch.empty((rows, line if width > 128 else width), dtype=torch.uint8, device=device)
+        line = -(-width // 128) * 128 if rows * width > 1 << 20 else width
+        codes = torch.empty((rows, line), dtype=torch.uint8, device=device)
         m = cls.__new__(cls)
-        m.codes, m.cols = codes[:, :width] if width > 128 and line != width else codes, cols
+        m.codes, m.cols = codes[:, :width] if line != width else codes, cols
         m.scales = torch.empty((rows, blocks), dtype=torch.uint8, device=device)
         return m
 
