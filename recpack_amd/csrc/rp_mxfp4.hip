@@ -188,9 +188,23 @@ extern "C" int rphip_mxfp4_dequantize(rphip_ctx* ctx, void* stream, int64_t rows
 // ---- scores of histories -----------------------------------------------------------------------------------------------------------
 // out[u, :] = sum over the entries e of user u of w_e * W[idx_e, :], in f32.  The rows of a history are contiguous and their blocks run along
 // the output.  A workgroup takes (user, 2048 columns); its waves take groups of four entries in turn and add their sums up in wave order
-// (the result does not depend on the launch).  Workgroups run through all users of a column tile before the next one: the rows' pieces
-// of one tile (1 KB each) stay in the caches.
+// (the result does not depend on the launch).
 constexpr int MXS_COLS = 64 * RP_MX;
+
+// Which user and column tile.  Workgroups go to the 8 XCDs round-robin: while eight tiles are left each XCD takes one of them for all
+// users, so that its L2 meets every history's pieces (1 KB) of the popular rows; the remaining tiles go through the XCDs together.
+__device__ __forceinline__ void mxs_task(unsigned users, int tiles, unsigned& user, int& tile) {
+  const unsigned L = blockIdx.x, full = (unsigned)tiles / 8 * 8;
+  if (L < full * users) {
+    const unsigned s = L >> 3;
+    tile = (int)(s / users * 8 + (L & 7));
+    user = s % users;
+  } else {
+    const unsigned s = L - full * users;
+    tile = (int)(full + s / users);
+    user = s % users;
+  }
+}
 
 // what both forms share: the entries of a chunk of 64, those that count moved to the front, in order; the history's own columns
 struct mxs_chunk {
@@ -229,13 +243,16 @@ constexpr int MXS_GROUPS = MXS_COLS / 512;  // fragments of 16 blocks
 template <class T, int WAVES>
 __global__ __launch_bounds__(64 * WAVES) void k_mx_scores_sum(const int32_t* __restrict__ indptr, const int32_t* __restrict__ indices, int64_t nnz, int rows, int cols, int nb,
                                                               const uint8_t* __restrict__ codes, int64_t ldc, const uint8_t* __restrict__ scales, int64_t lds, int exclude,
-                                                              const uint8_t* __restrict__ keep, T* __restrict__ out, int64_t ldo, int64_t user0) {
+                                                              const uint8_t* __restrict__ keep, T* __restrict__ out, int64_t ldo, int64_t user0, unsigned users, int tiles) {
   __shared__ uint32_t drop[64];  // bit c of word l: column 32 l + c of the tile gets -inf
   __shared__ rp_f32x4 sums[WAVES > 1 ? WAVES * MXS_GROUPS * 2 * 64 : 1];
   const int lane = threadIdx.x & 63, wave = WAVES > 1 ? __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) : 0;
   const int fr = lane & 15, fg = lane >> 4;
-  const int64_t u = user0 + blockIdx.x;
-  const int b0 = blockIdx.y * 64;
+  unsigned user;
+  int tile;
+  mxs_task(users, tiles, user, tile);
+  const int64_t u = user0 + user;
+  const int b0 = tile * 64;
   if (wave == 0) drop[lane] = 0;
   __syncthreads();
   // left operand: output row q (this lane's fr) of half h picks element (q >> 2) * 8 + h * 4 + (q & 3) of every group's 32; code of 1.0: 2
@@ -256,7 +273,7 @@ __global__ __launch_bounds__(64 * WAVES) void k_mx_scores_sum(const int32_t* __r
   for (int q = 0; q < MXS_GROUPS; ++q) co[q] = min(b0 + q * 16 + fr, nb - 1);
   const int64_t e1 = min((int64_t)indptr[u + 1], nnz);
   for (int64_t e0 = max((int64_t)indptr[u], (int64_t)0); e0 < e1; e0 += 64) {
-    const mxs_chunk ch = mxs_entries<false>(indices, nullptr, e0, e1, rows, exclude && wave == 0, blockIdx.y * MXS_COLS, drop, lane);
+    const mxs_chunk ch = mxs_entries<false>(indices, nullptr, e0, e1, rows, exclude && wave == 0, tile * MXS_COLS, drop, lane);
     mxs_i32x4 w[2][MXS_GROUPS];
     int sc[2][MXS_GROUPS];
     auto fetch = [&](auto tag, int k) __attribute__((always_inline)) {  // entries k .. k + 3, one a lane group; past the end: zeros
@@ -345,13 +362,16 @@ template <class T, int WAVES>
 __global__ __launch_bounds__(64 * WAVES) void k_mx_scores_weighted(const int32_t* __restrict__ indptr, const int32_t* __restrict__ indices, const float* __restrict__ weights,
                                                           int64_t nnz, int rows, int cols, int nb, const uint8_t* __restrict__ codes, int64_t ldc,
                                                           const uint8_t* __restrict__ scales, int64_t lds, int exclude, const uint8_t* __restrict__ keep,
-                                                          T* __restrict__ out, int64_t ldo, int64_t user0) {
+                                                          T* __restrict__ out, int64_t ldo, int64_t user0, unsigned users, int tiles) {
   __shared__ uint32_t drop[64];  // bit c of word l: column 32 l + c of the tile gets -inf
   __shared__ float sums[WAVES > 1 ? WAVES * 32 * 64 : 1];
   const int lane = threadIdx.x & 63, wave = WAVES > 1 ? __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) : 0;
-  const int64_t u = user0 + blockIdx.x;
-  const int c0 = blockIdx.y * MXS_COLS;
-  const int b = min(blockIdx.y * 64 + lane, nb - 1);  // this lane's block of columns (lanes beyond the row repeat the last one)
+  unsigned user;
+  int tile;
+  mxs_task(users, tiles, user, tile);
+  const int64_t u = user0 + user;
+  const int c0 = tile * MXS_COLS;
+  const int b = min(tile * 64 + lane, nb - 1);  // this lane's block of columns (lanes beyond the row repeat the last one)
   if (wave == 0) drop[lane] = 0;
   __syncthreads();
   float acc[32];
@@ -404,7 +424,7 @@ __global__ __launch_bounds__(64 * WAVES) void k_mx_scores_weighted(const int32_t
       }
     }
   }
-  const bool mine = blockIdx.y * 64 + lane < nb;
+  const bool mine = tile * 64 + lane < nb;
   const int c = b * RP_MX;
   const int left = min(RP_MX, cols - c);
   T* p = out + u * ldo + c;
@@ -479,17 +499,18 @@ extern "C" int rphip_mxfp4_scores(rphip_ctx* ctx, void* stream, int64_t n_users,
   return rp_by_type(out_type, [&](auto tag) -> int {
     using T = typename decltype(tag)::T;
     const hipStream_t st = (hipStream_t)stream;
-    constexpr int64_t strip = (int64_t)1 << 22;  // (users of a launch: below 2^32 threads)
+    const int64_t strip = std::max<int64_t>(1, ((int64_t)1 << 22) / tiles);  // (users of a launch: below 2^32 threads)
     auto go = [&](auto waves) -> int {
       constexpr int WV = decltype(waves)::value;
       for (int64_t u0 = 0; u0 < n_users; u0 += strip) {
-        const dim3 grid((unsigned)std::min(strip, n_users - u0), (unsigned)tiles);
+        const unsigned users = (unsigned)std::min(strip, n_users - u0);
+        const unsigned grid = users * (unsigned)tiles;
         if (weights_dev)
           k_mx_scores_weighted<T, WV><<<grid, 64 * WV, 0, st>>>(indptr_dev, indices_dev, weights_dev, nnz, (int)rows, (int)cols, nb, codes_dev, ld_codes, scales_dev, ld_scales,
-                                                                exclude_history, item_keep_dev, (T*)out_dev, ld_out, u0);
+                                                                exclude_history, item_keep_dev, (T*)out_dev, ld_out, u0, users, (int)tiles);
         else
           k_mx_scores_sum<T, WV><<<grid, 64 * WV, 0, st>>>(indptr_dev, indices_dev, nnz, (int)rows, (int)cols, nb, codes_dev, ld_codes, scales_dev, ld_scales, exclude_history,
-                                                           item_keep_dev, (T*)out_dev, ld_out, u0);
+                                                           item_keep_dev, (T*)out_dev, ld_out, u0, users, (int)tiles);
         RP_LAUNCHED();
       }
       return RPHIP_OK;
