@@ -95,6 +95,35 @@ def to_binary_csr(X) -> sp.csr_matrix:
     return M
 
 
+def item_mask(X, exclude_items, select_items):
+    """The items that may be recommended, as a boolean mask (None: all): ExcludeItems / SelectItems with their argument checks
+    (recpack/postprocessing/filters.py:58-101)."""
+    n_items = X.shape[1]
+    keep = None
+    for items, select in ((exclude_items, False), (select_items, True)):
+        if items is None:
+            continue
+        items = np.asarray(items)
+        if len(items) == 0 or np.amax(items) > n_items:  # filters.py:69-70, 91-92
+            raise ValueError(f"{X.shape} and {items.shape}")
+        m = np.zeros(n_items, dtype=bool) if select else np.ones(n_items, dtype=bool)
+        m[items] = select
+        keep = m if keep is None else (keep & m)
+    return keep
+
+
+def draw_uniforms(u, seed, users: int, n: int) -> np.ndarray:
+    """The uniforms of predict_sample: given ([users, n]), or from numpy's generator with ``seed``."""
+    if n < 1:
+        raise ValueError(f"n = {n}: at least one item has to be drawn")
+    if u is None:
+        return np.random.default_rng(seed).random((users, n), dtype=np.float32)
+    u = np.ascontiguousarray(u, dtype=np.float32)
+    if u.shape != (users, n):
+        raise ValueError(f"u has shape {u.shape}, expected {(users, n)}")
+    return u
+
+
 class Algorithm(*_AlgorithmBases):
     """recpack/algorithms/base.py:33-217 (the public protocol below mirrors the reference verbatim - module docstring)."""
 
@@ -219,6 +248,10 @@ class ItemSimilarityMatrixAlgorithm(Algorithm):
         ctx = get_context()
         return ctx, _lib.DeviceCSR.from_host(ctx, X.indptr, X.indices, X.shape)
 
+    def _upload_histories(self, X):
+        """The prediction input on the device, as predict multiplies it."""
+        return self._upload(self._transform_predict_input(X))
+
     def _predict(self, X: sp.csr_matrix) -> sp.csr_matrix:
         ctx, dX = self._upload(X)
         try:
@@ -237,16 +270,7 @@ class ItemSimilarityMatrixAlgorithm(Algorithm):
         self._check_fit_complete()
         X = self._transform_predict_input(X)
         n_items = X.shape[1]
-        keep = None
-        for items, select in ((exclude_items, False), (select_items, True)):
-            if items is None:
-                continue
-            items = np.asarray(items)
-            if len(items) == 0 or np.amax(items) > n_items:  # filters.py:69-70, 91-92
-                raise ValueError(f"{X.shape} and {items.shape}")
-            m = np.zeros(n_items, dtype=bool) if select else np.ones(n_items, dtype=bool)
-            m[items] = select
-            keep = m if keep is None else (keep & m)
+        keep = item_mask(X, exclude_items, select_items)
         ctx, dX = self._upload(X)
         try:
             idx, val, nnz = _lib.predict_topk(ctx, self._model, dX, min(int(K), max(1, n_items)), exclude_history, item_keep=keep)
@@ -256,6 +280,42 @@ class ItemSimilarityMatrixAlgorithm(Algorithm):
         indptr = np.zeros(X.shape[0] + 1, dtype=np.int64)
         np.cumsum(nnz, out=indptr[1:])
         return sp.csr_matrix((val[mask].astype(np.float64), idx[mask], indptr), shape=X.shape)
+
+    def predict_sample(self, X, n: int = 1, K: int = 100, temperature: float = 1.0, top_p: float = 1.0, min_p: float = 0.0, exclude_history: bool = False, exclude_items=None,
+                       select_items=None, u=None, seed=None):
+        """``n`` items per user DRAWN from the ``K`` best scores (K <= 1024) instead of the best ones: a stochastic policy, with the
+        probability of every draw - what off-policy evaluation of logged recommendations needs.  Extension (the reference always
+        recommends the best scores).
+
+        An item's chance is proportional to exp(score / temperature) among the K best, cut to the shortest prefix with ``top_p`` of the
+        mass and to items with at least ``min_p`` of the best one's; drawn items are not drawn again.  Temperature 0: the best n.  ``u``:
+        uniforms [users, n], or drawn with ``seed``.  The filters are those of :meth:`predict_topk`.  Returns (items int32 [users, n] in
+        drawn order, -1 where a user has no more candidates; probabilities float32 [users, n])."""
+        import torch
+
+        from recpack_amd import ops
+
+        self._check_fit_complete()
+        ctx, dX = self._upload_histories(X)
+        try:
+            users, n_items = dX.shape
+            K = min(int(K), max(1, n_items))
+            if not 1 <= K <= ops.SLATE_MAX:
+                raise ValueError(f"predict_sample draws from the K best scores, 1 <= K <= {ops.SLATE_MAX}, got {K}")
+            keep = item_mask(dX, exclude_items, select_items)
+            u = draw_uniforms(u, seed, users, n)
+            device = f"cuda:{ctx.device}"
+            idx = torch.empty((users, K), dtype=torch.int32, device=device)
+            val = torch.empty((users, K), dtype=torch.float32, device=device)
+            nnz = torch.empty(users, dtype=torch.int32, device=device)
+            keep_t = None if keep is None else torch.from_numpy(keep.astype(np.uint8)).to(device)
+            with torch.cuda.device(ctx.device):
+                _lib.predict_topk_dev(ctx, self._model, dX, K, idx, val, nnz, exclude_history, item_keep_t=keep_t)
+                ctx.sync()  # (written on the context's stream, read on torch's)
+                items, probs, _ = ops.sample(ctx, val, torch.from_numpy(u).to(device), temperature=temperature, top_p=top_p, min_p=min_p, lengths=nnz, ids=idx)
+                return items.cpu().numpy(), probs.cpu().numpy()
+        finally:
+            dX.close()
 
     def _check_fit_complete(self):
         super()._check_fit_complete()
@@ -371,6 +431,15 @@ class EASE(ItemSimilarityMatrixAlgorithm):
         if self.density:
             self._prune()
         self._empty_rows_ = self._model.empty_rows()
+
+    def compress(self, profiles: bool = False) -> "CompressedEASE":  # noqa: F821
+        """This fitted model in 4 bits per similarity (:class:`recpack_amd.CompressedEASE`); this one stays as it is."""
+        from recpack_amd.compressed import CompressedEASE
+
+        self._check_fit_complete()
+        c = CompressedEASE(self.l2, self.alpha, self.density, profiles)
+        c._compress(self._model)
+        return c
 
     def _prune(self):
         """ease.py:97-109: keep the ``int(density * n * n)`` largest |B_ij| (np.prod for the removed np.product), on the

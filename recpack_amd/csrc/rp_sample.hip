@@ -1241,8 +1241,8 @@ __global__ __launch_bounds__(SL_THREADS) void k_row_draw(sample_args a, const ro
 }
 
 // which form a call takes, and its workspace
-enum sample_form { FORM_WAVE4, FORM_WAVE16, FORM_LISTS, FORM_ROWS };
-sample_form form_of(int64_t width, int64_t k) { return width <= 256 ? FORM_WAVE4 : width <= RPS_SHORT ? FORM_WAVE16 : k <= RPS_SHORT ? FORM_LISTS : FORM_ROWS; }
+enum sample_form { FORM_WAVE, FORM_LISTS, FORM_ROWS };
+sample_form form_of(int64_t width, int64_t k) { return width <= RPS_SHORT ? FORM_WAVE : k <= RPS_SHORT ? FORM_LISTS : FORM_ROWS; }
 // entries of a row's list: the selection hands over 1.1 to 1.4 times k candidates
 int list_of(int64_t k) { return k <= 128 ? 256 : k <= 384 ? 512 : 1024; }
 int64_t workspace_of(int64_t rows, int64_t width, int64_t k) {
@@ -1297,11 +1297,12 @@ extern "C" int rphip_sample(rphip_ctx* ctx, void* stream, int64_t rows, int64_t 
     using T = typename decltype(tag)::T;
     const hipStream_t st = (hipStream_t)stream;
     switch (form_of(width, k)) {
-      case FORM_WAVE4:
-      case FORM_WAVE16:
+      case FORM_WAVE:
         for (a.row0 = 0; a.row0 < rows; a.row0 += 1 << 20) {
           const unsigned n = (unsigned)std::min<int64_t>(1 << 20, rows - a.row0);
-          if (width <= 256) k_sample_wave<T, 4><<<(n + 3) / 4, 256, 0, st>>>(a);
+          if (width <= 64) k_sample_wave<T, 1><<<(n + 3) / 4, 256, 0, st>>>(a);
+          else if (width <= 256) k_sample_wave<T, 4><<<(n + 3) / 4, 256, 0, st>>>(a);
+          else if (width <= 512) k_sample_wave<T, 8><<<(n + 3) / 4, 256, 0, st>>>(a);
           else k_sample_wave<T, 16><<<(n + 3) / 4, 256, 0, st>>>(a);
           RP_LAUNCHED();
         }

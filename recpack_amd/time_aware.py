@@ -236,6 +236,10 @@ class TARSItemKNN(TopKItemSimilarityMatrixAlgorithm):
         ctx = get_context()
         return ctx, W, _lib.DeviceCSR.from_host_valued(ctx, W)
 
+    def _upload_histories(self, X):
+        ctx, _, dW = self._valued_upload(self._transform_predict_input(X))
+        return ctx, dW
+
     def _predict(self, X) -> sp.csr_matrix:
         ctx, W, dW = self._valued_upload(X)
         try:
