@@ -22,7 +22,6 @@ constexpr int SB_CAP = 2048;         // entries of a list collected ahead
 constexpr int RC_FOUND = 512;        // ... of a workgroup's own part of them, in LDS
 constexpr int SR_THREADS = 256;      // threads of a workgroup that takes a slice of a row
 constexpr int64_t STRIP = 1024;      // rows whose workspace exists at a time (whole-row form: 58 KB each)
-constexpr int64_t STRIP_LISTS = 4096;  // (short prefixes: at most 8 KB each)
 
 struct sample_args {
   int64_t rows, ld, ld_ids, ld_u;
@@ -207,140 +206,141 @@ __device__ __forceinline__ void scan_row(const T* p, int begin, int end, int tid
   }
 }
 
-// 2^y for -1000 <= y <= 0: Taylor series of exp to the 11th power on [-ln2 / 2, ln2 / 2] (remainder < 2^-47 relative)
+// 2^y for -1000 <= y <= 0: Taylor series of exp to the 11th power on [-ln2 / 2, ln2 / 2] (remainder < 2^-47 relative).  The coefficients are
+// kept in scalar registers: as vector constants, ahead of a loop, they take 22 of the 64 registers that eight waves per SIMD leave.
+__device__ __forceinline__ double in_scalar(double c) {
+  asm("" : "+s"(c));
+  return c;
+}
 __device__ __forceinline__ double exp2_le0(double y) {
-  const double n = rint(y), f = (y - n) * 0.69314718055994530942;
-  double q = 1.0 / 39916800.0;
-  q = fma(q, f, 1.0 / 3628800.0);
-  q = fma(q, f, 1.0 / 362880.0);
-  q = fma(q, f, 1.0 / 40320.0);
-  q = fma(q, f, 1.0 / 5040.0);
-  q = fma(q, f, 1.0 / 720.0);
-  q = fma(q, f, 1.0 / 120.0);
-  q = fma(q, f, 1.0 / 24.0);
-  q = fma(q, f, 1.0 / 6.0);
+  const double n = rint(y), f = (y - n) * in_scalar(0.69314718055994530942);
+  double q = fma(f, in_scalar(1.0 / 39916800.0), in_scalar(1.0 / 3628800.0));
+  q = fma(q, f, in_scalar(1.0 / 362880.0));
+  q = fma(q, f, in_scalar(1.0 / 40320.0));
+  q = fma(q, f, in_scalar(1.0 / 5040.0));
+  q = fma(q, f, in_scalar(1.0 / 720.0));
+  q = fma(q, f, in_scalar(1.0 / 120.0));
+  q = fma(q, f, in_scalar(1.0 / 24.0));
+  q = fma(q, f, in_scalar(1.0 / 6.0));
   q = fma(q, f, 0.5);
   q = fma(q, f, 1.0);
   q = fma(q, f, 1.0);
   return ldexp(q, (int)n);
 }
 
-// One wave finishes a row from its leading candidates: sorted[] (in LDS, this wave's own) holds them ranked, key << 32 | ~index, 0 where there
-// is none, all of the first s.k ranks among them.  Register i of lane l holds rank 64 i + l, its mass in float64 relative to the best
-// candidate, and the cumulative mass inside the register; a draw looks for the register and then asks all lanes at once, and only the
-// register that lost a candidate is summed again.  When what is left has next to no mass (a low temperature: the masses underflow, the
-// definition does not) it is taken relative to the best one left.
+// One wave finishes a row from its leading candidates: sorted[] (in LDS) holds 64 * PER of them ranked, key << 32 | ~index, key 0 where there
+// is none, all of the first s.k ranks among them.  Lane l has the ranks l PER .. l PER + PER - 1: their masses in float64 relative to the best
+// candidate, and the masses up to and with each of them; NaN instead where there is nothing to draw.  A draw asks all lanes for the first
+// one that the uniform falls into and takes that mass off those behind it: a chain of a dozen dependent instructions, whatever PER is.  What is left is summed
+// again when it has come down to 2^-6 of the last full sum (so that it keeps a relative precision of 2^-46), and when it has next to no mass
+// (a low temperature: the masses underflow, the definition does not) taken relative to the best one left.
 template <int PER>
-__device__ void finish_row(const sample_args& a, int64_t r, const row_set& s, const unsigned long long* sorted, int lane) {
-  float x[PER];
+__device__ __forceinline__ void finish_row(const sample_args& a, int64_t r, const row_set& s, const unsigned long long* sorted, int lane) {
+  const bool greedy = s.temperature == 0.0f;
+  const double c = greedy ? 0.0 : 1.4426950408889634074 / (double)s.temperature;
+  auto score_at = [&](int rank) __attribute__((always_inline)) { return score_of((uint32_t)(sorted[rank] >> 32)); };
+  float from = score_at(0);  // what the masses are relative to
+  auto mass_of = [&](float v) __attribute__((always_inline)) { return v == from ? 1.0 : exp2_le0(fmax(((double)v - (double)from) * c, -1000.0)); };
+  double m[PER], upto[PER], total = 0.0;
+  uint32_t out = 0;  // bit i: this lane's i-th rank is not kept, or drawn
+  auto add_up = [&]() __attribute__((always_inline)) {
+    double own = 0.0;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      own += (out >> i) & 1 ? 0.0 : m[i];
+      upto[i] = own;
+    }
+    const double all = wave_scan_f64(own);
+    total = lane_f64(all, 63);
+#pragma unroll
+    for (int i = 0; i < PER; ++i) upto[i] += all - own;
+  };
   int have = 0;
 #pragma unroll
   for (int i = 0; i < PER; ++i) {
-    const uint32_t key = (uint32_t)(sorted[i * 64 + lane] >> 32);
-    x[i] = score_of(key);
-    have += (int)__popcll(__ballot(key != 0 && i * 64 + lane < s.k));
+    const int rank = lane * PER + i;
+    const uint32_t key = (uint32_t)(sorted[rank] >> 32);
+    const bool candidate = key != 0 && rank < s.k;
+    have += (int)__popcll(__ballot(candidate));
+    m[i] = candidate && !greedy ? mass_of(score_of(key)) : 0.0;
   }
-  const bool greedy = s.temperature == 0.0f;
-  const double c = greedy ? 0.0 : 1.4426950408889634074 / (double)s.temperature;
-  float from = __uint_as_float(lane_u32(__float_as_uint(x[0]), 0));  // what the masses are relative to
-  auto mass_of = [&](float v) __attribute__((always_inline)) { return v == from ? 1.0 : exp2_le0(fmax(((double)v - (double)from) * c, -1000.0)); };
-  double m[PER], cum[PER], sum[PER];
   int kept = have;
   if (!greedy) {
-    double total = 0.0;
-#pragma unroll
-    for (int i = 0; i < PER; ++i) {
-      m[i] = i * 64 + lane < have ? mass_of(x[i]) : 0.0;
-      cum[i] = wave_scan_f64(m[i]);
-      sum[i] = lane_f64(cum[i], 63);
-      total += sum[i];
-    }
+    add_up();
     // leading ranks kept: those with less than top_p of the mass before them and at least min_p of the best one's mass
     const double border = (double)s.top_p * total;
-    double before = 0.0;
     kept = 0;
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
-      const int rank = i * 64 + lane;
-      kept += (int)__popcll(__ballot(rank < have && (s.top_p >= 1.0f || rank == 0 || before + (cum[i] - m[i]) < border) && m[i] >= (double)s.min_p));
-      before += sum[i];
-    }
-    if (kept < have) {
-#pragma unroll
-      for (int i = 0; i < PER; ++i) {
-        if (i * 64 + lane >= kept) m[i] = 0.0;
-        cum[i] = wave_scan_f64(m[i]);
-        sum[i] = lane_f64(cum[i], 63);
-      }
+      const int rank = lane * PER + i;
+      kept += (int)__popcll(__ballot(rank < have && (s.top_p >= 1.0f || rank == 0 || upto[i] - m[i] < border) && m[i] >= (double)s.min_p));
     }
   }
-  double floor_of[PER];
+  const int own_kept = min(max(kept - lane * PER, 0), PER);
+  out = ~((1u << own_kept) - 1u);
+  auto hide = [&]() __attribute__((always_inline)) {
 #pragma unroll
-  for (int i = 0; i < PER; ++i) floor_of[i] = greedy ? 0.0 : sum[i] * 0.015625;
+    for (int i = 0; i < PER; ++i) upto[i] = (out >> i) & 1 ? (double)NAN : upto[i];
+  };
+  double floor_of = 0.0;
+  if (!greedy) {
+    if (kept < have) add_up();
+    floor_of = total * 0.015625;
+    hide();
+  }
   const int n_out = min(a.draws, kept);
-  uint32_t gone = 0;  // bit i: rank 64 i + lane has been drawn
   for (int d0 = 0; d0 < a.draws; d0 += 64) {  // lane l keeps draw d0 + l
     const int nd = min(64, n_out - d0);
     float u = d0 + lane < n_out ? a.u[r * a.ld_u + d0 + lane] : 0.0f;
     u = u > 0.0f ? fminf(u, 0x1.fffffep-1f) : 0.0f;
-    int rank = d0 + lane;
+    int pick = d0 + lane;
     double part = 1.0, whole = 1.0;
     for (int d = 0; !greedy && d < nd; ++d) {
-      double total = 0.0;
+      if (total < floor_of) {
+        add_up();
+        if (total < 1e-200) {  // (kept candidates are left)
+          const uint32_t in = ~out & ((1u << PER) - 1u);
+          const int who = (int)__ffsll((long long)__ballot(in != 0)) - 1;
+          from = score_at(who * PER + (int)lane_u32((uint32_t)__ffs((int)in) - 1u, who));
 #pragma unroll
-      for (int i = 0; i < PER; ++i) total += sum[i];
-      if (total < 1e-200) {  // (kept candidates are left)
-        bool looking = true;
-#pragma unroll
-        for (int i = 0; i < PER; ++i) {
-          const unsigned long long left = __ballot(i * 64 + lane < kept && !((gone >> i) & 1));
-          if (looking && left) {
-            from = __uint_as_float(lane_u32(__float_as_uint(x[i]), (int)__ffsll((long long)left) - 1));
-            looking = false;
-          }
+          for (int i = 0; i < PER; ++i) m[i] = (in >> i) & 1 ? mass_of(score_at(lane * PER + i)) : 0.0;
+          add_up();
         }
-        total = 0.0;
-#pragma unroll
-        for (int i = 0; i < PER; ++i) {
-          m[i] = i * 64 + lane < kept && !((gone >> i) & 1) ? mass_of(x[i]) : 0.0;
-          cum[i] = wave_scan_f64(m[i]);
-          sum[i] = lane_f64(cum[i], 63);
-          floor_of[i] = sum[i] * 0.015625;
-          total += sum[i];
-        }
+        floor_of = total * 0.015625;
+        hide();
       }
       const double want = (double)__uint_as_float(lane_u32(__float_as_uint(u), d)) * total;
-      // the register, then the first lane in it; the last candidate with mass if rounding lets none pass
-      double before = 0.0;
       int at = -1;
+      double own = 0.0;
 #pragma unroll
-      for (int i = 0; i < PER; ++i) {
-        if (at >= 0) continue;
-        if (before + sum[i] > want) {  // (the last register with mass at the latest: there before + sum = total, by the same adds, and u < 1)
-          const unsigned long long pass = __ballot(before + cum[i] > want && m[i] > 0.0);
-          const int who = pass ? (int)__ffsll((long long)pass) - 1 : 63 - (int)__clzll((long long)__ballot(m[i] > 0.0));
-          const double got = lane_f64(m[i], who);
-          at = i * 64 + who;
-          if (lane == d) rank = at, part = got, whole = total;
-          if (lane == who) m[i] = 0.0, gone |= 1u << i;
-          // (what is left keeps a relative precision of 2^-46 as long as it is no less than 2^-6 of the last full sum)
-          if (sum[i] - got >= floor_of[i]) {
-            cum[i] -= lane >= who ? got : 0.0;
-            sum[i] = lane_f64(cum[i], 63);
-          } else {
-            cum[i] = wave_scan_f64(m[i]);
-            sum[i] = lane_f64(cum[i], 63);
-            floor_of[i] = sum[i] * 0.015625;
-          }
-        }
-        before += sum[i];
+      for (int i = PER - 1; i >= 0; --i) {
+        const bool here = upto[i] > want;
+        at = here ? i : at;
+        own = here ? m[i] : own;
       }
+      unsigned long long pass = __ballot(at >= 0);
+      if (pass == 0) {  // (u < 1: only if rounding lets none pass) the last one
+        const uint32_t in = ~out & ((1u << PER) - 1u);
+        at = 31 - (int)__clz((int)in);
+        pass = __ballot(in != 0);
+        pass = 1ull << (63 - (int)__clzll((long long)pass));
+#pragma unroll
+        for (int i = 0; i < PER; ++i) own = i == at ? m[i] : own;
+      }
+      const int who = (int)__ffsll((long long)pass) - 1;
+      const double got = lane_f64(own, who);
+      const int drawn = who * PER + (int)lane_u32((uint32_t)at, who), mine = drawn - lane * PER;
+      if (lane == d) pick = drawn, part = got, whole = total;
+      out |= (uint32_t)mine < (uint32_t)PER ? 1u << mine : 0u;
+#pragma unroll
+      for (int i = 0; i < PER; ++i) upto[i] -= i > mine ? got : i == mine ? (double)NAN : 0.0;
+      total -= got;
     }
     if (d0 + lane < a.draws) {
       const bool drawn = d0 + lane < n_out;
       int32_t item = -1;
       if (drawn) {
-        const int32_t at = (int32_t) ~(uint32_t)sorted[rank];
+        const int32_t at = (int32_t) ~(uint32_t)sorted[pick];
         item = a.ids ? a.ids[r * a.ld_ids + at] : at;
       }
       a.idx[r * a.draws + d0 + lane] = item;
@@ -413,33 +413,39 @@ __device__ __forceinline__ void sort_lanes(unsigned long long& e, int lane, bool
   const unsigned long long o = ((unsigned long long)xor_lane<LS>((uint32_t)(e >> 32), lane) << 32) | xor_lane<LS>((uint32_t)e, lane);
   e = (((lane & LS) == 0) == desc) == (e > o) ? e : o;
 }
+// ... of 64 entries, one to a lane, in the given direction
+__device__ __forceinline__ void merge_lanes(unsigned long long& v, int lane, bool desc) {
+  sort_lanes<32>(v, lane, desc);
+  sort_lanes<16>(v, lane, desc);
+  sort_lanes<8>(v, lane, desc);
+  sort_lanes<4>(v, lane, desc);
+  sort_lanes<2>(v, lane, desc);
+  sort_lanes<1>(v, lane, desc);
+}
+__device__ __forceinline__ void sort_run(unsigned long long& v, int lane, bool desc) {
+  sort_lanes<1>(v, lane, (lane & 2) == 0);
+  sort_lanes<2>(v, lane, (lane & 4) == 0);
+  sort_lanes<1>(v, lane, (lane & 4) == 0);
+  sort_lanes<4>(v, lane, (lane & 8) == 0);
+  sort_lanes<2>(v, lane, (lane & 8) == 0);
+  sort_lanes<1>(v, lane, (lane & 8) == 0);
+  sort_lanes<8>(v, lane, (lane & 16) == 0);
+  sort_lanes<4>(v, lane, (lane & 16) == 0);
+  sort_lanes<2>(v, lane, (lane & 16) == 0);
+  sort_lanes<1>(v, lane, (lane & 16) == 0);
+  sort_lanes<16>(v, lane, (lane & 32) == 0);
+  sort_lanes<8>(v, lane, (lane & 32) == 0);
+  sort_lanes<4>(v, lane, (lane & 32) == 0);
+  sort_lanes<2>(v, lane, (lane & 32) == 0);
+  sort_lanes<1>(v, lane, (lane & 32) == 0);
+  merge_lanes(v, lane, desc);
+}
 __device__ __forceinline__ void block_sort(unsigned long long* e, int n) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   __syncthreads();
   for (int i = wave * 64 + lane; i < n; i += SL_THREADS) {
     unsigned long long v = e[i];
-    sort_lanes<1>(v, lane, (i & 2) == 0);
-    sort_lanes<2>(v, lane, (i & 4) == 0);
-    sort_lanes<1>(v, lane, (i & 4) == 0);
-    sort_lanes<4>(v, lane, (i & 8) == 0);
-    sort_lanes<2>(v, lane, (i & 8) == 0);
-    sort_lanes<1>(v, lane, (i & 8) == 0);
-    sort_lanes<8>(v, lane, (i & 16) == 0);
-    sort_lanes<4>(v, lane, (i & 16) == 0);
-    sort_lanes<2>(v, lane, (i & 16) == 0);
-    sort_lanes<1>(v, lane, (i & 16) == 0);
-    sort_lanes<16>(v, lane, (i & 32) == 0);
-    sort_lanes<8>(v, lane, (i & 32) == 0);
-    sort_lanes<4>(v, lane, (i & 32) == 0);
-    sort_lanes<2>(v, lane, (i & 32) == 0);
-    sort_lanes<1>(v, lane, (i & 32) == 0);
-    const bool desc = (i & 64) == 0;
-    sort_lanes<32>(v, lane, desc);
-    sort_lanes<16>(v, lane, desc);
-    sort_lanes<8>(v, lane, desc);
-    sort_lanes<4>(v, lane, desc);
-    sort_lanes<2>(v, lane, desc);
-    sort_lanes<1>(v, lane, desc);
+    sort_run(v, lane, (i & 64) == 0);
     e[i] = v;
   }
   for (int size = 128; size <= n; size <<= 1) {
@@ -455,17 +461,206 @@ __device__ __forceinline__ void block_sort(unsigned long long* e, int n) {
     __syncthreads();
     for (int i = wave * 64 + lane; i < n; i += SL_THREADS) {
       unsigned long long v = e[i];
-      const bool desc = (i & size) == 0;
-      sort_lanes<32>(v, lane, desc);
-      sort_lanes<16>(v, lane, desc);
-      sort_lanes<8>(v, lane, desc);
-      sort_lanes<4>(v, lane, desc);
-      sort_lanes<2>(v, lane, desc);
-      sort_lanes<1>(v, lane, desc);
+      merge_lanes(v, lane, (i & size) == 0);
       e[i] = v;
     }
   }
   __syncthreads();
+}
+
+// ---- a workgroup to a row: runs of 64 candidates, one to a wave -------------------------------------------------------------------------
+// how many entries of a run of LEN (a power of two, ranked) are larger; three runs side by side, so that three reads are under way
+template <int LEN, int N>
+__device__ __forceinline__ int count_above(const unsigned long long* const (&run)[N], unsigned long long v) {
+  int c[N];
+#pragma unroll
+  for (int q = 0; q < N; ++q) c[q] = 0;
+#pragma unroll
+  for (int step = LEN / 2; step > 0; step >>= 1) {
+#pragma unroll
+    for (int q = 0; q < N; ++q) c[q] += run[q][c[q] + step - 1] > v ? step : 0;
+  }
+  int sum = 0;
+#pragma unroll
+  for (int q = 0; q < N; ++q) sum += c[q] + (run[q][c[q]] > v ? 1 : 0);
+  return sum;
+}
+
+// Ranks n <= 64 * runs entries of list[] (key << 32 | ~index; runs is 4, 8 or 16): every wave sorts 64 in its registers, then four runs at
+// a time are joined: an entry's place is its own plus, in each other run, the number of larger ones.  Every thread of the workgroup calls
+// it; list[] holds 128 * runs entries, the ranked ones start at the pointer that is returned (behind the last: entries with key 0).
+__device__ __forceinline__ const unsigned long long* rank_runs(unsigned long long* list, int n, int runs) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  unsigned long long* other = list + 64 * runs;
+  unsigned long long v = 0;
+  int rank = 0;
+  if (wave < runs) {
+    v = (int)threadIdx.x < n ? list[threadIdx.x] : (unsigned long long)threadIdx.x;  // (all different, so that places are, too)
+    sort_run(v, lane, true);
+    list[threadIdx.x] = v;
+  }
+  __syncthreads();
+  if (wave < runs) {
+    const unsigned long long* group = list + (wave & ~3) * 64;
+    const unsigned long long* const run[3] = {group + ((wave + 1) & 3) * 64, group + ((wave + 2) & 3) * 64, group + ((wave + 3) & 3) * 64};
+    rank = (wave & ~3) * 64 + lane + count_above<64>(run, v);
+    other[rank] = v;
+  }
+  __syncthreads();
+  if (runs == 4) return other;
+  if (wave < runs) {
+    const int mine = wave >> 2;
+    if (runs == 8) {
+      const unsigned long long* const run[1] = {other + (mine ^ 1) * 256};
+      rank += count_above<256>(run, v) - mine * 256;
+    } else {
+      const unsigned long long* const run[3] = {other + ((mine + 1) & 3) * 256, other + ((mine + 2) & 3) * 256, other + ((mine + 3) & 3) * 256};
+      rank += count_above<256>(run, v) - mine * 256;
+    }
+    list[rank] = v;
+  }
+  __syncthreads();
+  return list;
+}
+
+// The row's draws from its ranked candidates (rank_runs), as finish_row defines them: wave i has the masses of the ranks 64 i .. 64 i + 63 and
+// their cumulative sums inside the run, in LDS behind that; wave 0 draws, its lane i holding run i's sum: one look finds the run, a
+// second one the candidate in it, and only that run is summed again.
+struct group_shared {
+  double m[RPS_SHORT], cum[RPS_SHORT], sum[16];
+  int count[2][16];
+};
+__device__ __forceinline__ void finish_group(const sample_args& a, int64_t r, const row_set& s, const unsigned long long* sorted, int runs, group_shared& sh) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, rank = threadIdx.x;
+  const bool greedy = s.temperature == 0.0f;
+  const double c = greedy ? 0.0 : 1.4426950408889634074 / (double)s.temperature;
+  float from = score_of((uint32_t)(sorted[0] >> 32));  // what the masses are relative to
+  auto mass_of = [&](float v) __attribute__((always_inline)) { return v == from ? 1.0 : exp2_le0(fmax(((double)v - (double)from) * c, -1000.0)); };
+  double mine = 0.0, incl = 0.0;
+  bool candidate = false;
+  if (wave < runs) {
+    const uint32_t key = (uint32_t)(sorted[rank] >> 32);
+    candidate = key != 0 && rank < s.k;
+    if (!greedy) {
+      mine = candidate ? mass_of(score_of(key)) : 0.0;
+      incl = wave_scan_f64(mine);
+      if (lane == 63) sh.sum[wave] = incl;
+    }
+    const int n = (int)__popcll(__ballot(candidate));
+    if (lane == 0) sh.count[0][wave] = n;
+  }
+  __syncthreads();
+  int have = 0;
+  for (int w = 0; w < runs; ++w) have += sh.count[0][w];
+  int kept = have;
+  if (!greedy) {
+    double before = 0.0, total = 0.0;
+    for (int w = 0; w < runs; ++w) {
+      before += w < wave ? sh.sum[w] : 0.0;
+      total += sh.sum[w];
+    }
+    // leading ranks kept: those with less than top_p of the mass before them and at least min_p of the best one's mass
+    const double border = (double)s.top_p * total;
+    if (wave < runs) {
+      const int n = (int)__popcll(__ballot(candidate && (s.top_p >= 1.0f || rank == 0 || before + (incl - mine) < border) && mine >= (double)s.min_p));
+      if (lane == 0) sh.count[1][wave] = n;
+    }
+    __syncthreads();
+    kept = 0;
+    for (int w = 0; w < runs; ++w) kept += sh.count[1][w];
+    if (wave < runs) {
+      if (kept < have) {
+        if (rank >= kept) mine = 0.0;
+        incl = wave_scan_f64(mine);
+      }
+      sh.m[rank] = mine;
+      sh.cum[rank] = incl;
+      if (lane == 63) sh.sum[wave] = incl;
+    }
+    __syncthreads();
+  }
+  if (wave != 0) return;
+  // lane i: of run i (runs <= 16: in one row of lanes), and of the runs in front of it
+  double sum = !greedy && lane < runs ? sh.sum[lane] : 0.0, floor_of = sum * 0.015625, ahead = 0.0, total = 0.0, total_floor = 0.0;
+  auto add_up = [&]() __attribute__((always_inline)) {
+    double upto = sum;
+    upto += dpp_f64<0x111>(upto);
+    upto += dpp_f64<0x112>(upto);
+    upto += dpp_f64<0x114>(upto);
+    upto += dpp_f64<0x118>(upto);
+    ahead = upto - sum;
+    total = lane_f64(upto, 15);
+    total_floor = total * 0.015625;
+  };
+  if (!greedy) add_up();
+  const int n_out = min(a.draws, kept);
+  uint32_t gone = 0;  // bit i: rank 64 i + lane has been drawn
+  for (int d0 = 0; d0 < a.draws; d0 += 64) {  // lane l keeps draw d0 + l
+    const int nd = min(64, n_out - d0);
+    float u = d0 + lane < n_out ? a.u[r * a.ld_u + d0 + lane] : 0.0f;
+    u = u > 0.0f ? fminf(u, 0x1.fffffep-1f) : 0.0f;
+    int pick = d0 + lane;
+    double part = 1.0, whole = 1.0;
+    for (int d = 0; !greedy && d < nd; ++d) {
+      if (total < total_floor) {  // (precision: as for a run's sum below)
+        add_up();
+        if (total < 1e-200) {  // (kept candidates are left: relative to the best of them from here on)
+          int first = -1;
+          for (int i = runs - 1; i >= 0; --i) {
+            const unsigned long long left = __ballot(i * 64 + lane < kept && !((gone >> i) & 1));
+            first = left ? i * 64 + (int)__ffsll((long long)left) - 1 : first;
+          }
+          from = score_of((uint32_t)(sorted[first] >> 32));
+          for (int i = 0; i < runs; ++i) {
+            const int at = i * 64 + lane;
+            const double mass = at < kept && !((gone >> i) & 1) ? mass_of(score_of((uint32_t)(sorted[at] >> 32))) : 0.0;
+            const double in = wave_scan_f64(mass);
+            sh.m[at] = mass;
+            sh.cum[at] = in;
+            const double all = lane_f64(in, 63);
+            if (lane == i) sum = all, floor_of = all * 0.015625;
+          }
+          add_up();
+        }
+      }
+      const double want = (double)__uint_as_float(lane_u32(__float_as_uint(u), d)) * total;
+      // the run, then the first lane in it; the last ones with mass if rounding lets none pass (u < 1)
+      const unsigned long long some = __ballot(sum > 0.0), runs_pass = __ballot(ahead + sum > want) & some;
+      const int i = runs_pass ? (int)__ffsll((long long)runs_pass) - 1 : 63 - (int)__clzll((long long)some);
+      double m = sh.m[i * 64 + lane], cum = sh.cum[i * 64 + lane];
+      const unsigned long long with = __ballot(m > 0.0), pass = __ballot(lane_f64(ahead, i) + cum > want) & with;
+      const int who = pass ? (int)__ffsll((long long)pass) - 1 : 63 - (int)__clzll((long long)with);
+      const double got = lane_f64(m, who);
+      if (lane == d) pick = i * 64 + who, part = got, whole = total;
+      if (lane == who) m = 0.0, gone |= 1u << i, sh.m[i * 64 + who] = 0.0;
+      // (what is left keeps a relative precision of 2^-46 as long as it is no less than 2^-6 of the last full sum)
+      double left = lane_f64(cum, 63) - got;
+      if (left >= lane_f64(floor_of, i)) {
+        cum -= lane >= who ? got : 0.0;
+      } else {
+        cum = wave_scan_f64(m);
+        left = lane_f64(cum, 63);
+        if (lane == i) floor_of = left * 0.015625;
+      }
+      sh.cum[i * 64 + lane] = cum;
+      if (lane == i) sum = left;
+      ahead -= lane > i ? got : 0.0;
+      total -= got;
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");  // (one wave: its LDS accesses stay in order)
+      __builtin_amdgcn_wave_barrier();
+    }
+    if (d0 + lane < a.draws) {
+      const bool drawn = d0 + lane < n_out;
+      int32_t item = -1;
+      if (drawn) {
+        const int32_t at = (int32_t) ~(uint32_t)sorted[pick];
+        item = a.ids ? a.ids[r * a.ld_ids + at] : at;
+      }
+      a.idx[r * a.draws + d0 + lane] = item;
+      a.prob[r * a.draws + d0 + lane] = drawn ? (float)(part / whole) : 0.0f;
+    }
+  }
+  if (lane == 0 && a.nnz) a.nnz[r] = n_out;
 }
 
 // The exact form of "the n-th of the row in rank order" for any row (thousands of equal scores, adversarial orders): radix descent over
@@ -513,9 +708,15 @@ __device__ __forceinline__ uint32_t select_key(const T* p, int len, int n, sel_s
 // HELD pieces of 16 bytes and reads again only those that reach the threshold (HELD = 0: any width, the whole row is read twice).
 constexpr int TK_HELD = 8;
 template <class T, int HELD>
-__global__ __launch_bounds__(SL_THREADS, 8) void k_sample_topk(sample_args a, unsigned long long* __restrict__ lists, int32_t* __restrict__ counts, int cap) {
+__global__ __launch_bounds__(SL_THREADS, 8) void k_sample_topk(sample_args a) {
   constexpr int E = PIECE<T>;
-  __shared__ unsigned long long list[SL_CAP];
+  __shared__ union {
+    unsigned long long list[SL_CAP];
+    struct {
+      unsigned long long ranked[2 * RPS_SHORT];
+      group_shared group;
+    };
+  } sh;
   __shared__ uint32_t red[2][SL_THREADS / 64], hist[256], pick[2];
   __shared__ uint32_t n_list, cnt;
   __shared__ sel_shared sel;
@@ -618,7 +819,7 @@ __global__ __launch_bounds__(SL_THREADS, 8) void k_sample_topk(sample_args a, un
       const float x = rp_to_f32(v.v[i]);
       if (i < m && x >= least) {
         const uint32_t at = atomicAdd(&n_list, 1u);
-        if (at < SL_CAP) list[at] = ((unsigned long long)key_of(x) << 32) | (uint32_t) ~(j + i);
+        if (at < SL_CAP) sh.list[at] = ((unsigned long long)key_of(x) << 32) | (uint32_t) ~(j + i);
       }
     }
   };
@@ -667,44 +868,22 @@ __global__ __launch_bounds__(SL_THREADS, 8) void k_sample_topk(sample_args a, un
         all += red[0][w];
       }
       const bool in = key > kk || (key == kk && before + (uint32_t)__popcll(tie & ((1ull << lane) - 1ull)) < (uint32_t)equal);
-      if (in) list[atomicAdd(&n_list, 1u)] = ((unsigned long long)key << 32) | (uint32_t)~j;  // (s.k <= 1024 entries in all)
+      if (in) sh.list[atomicAdd(&n_list, 1u)] = ((unsigned long long)key << 32) | (uint32_t)~j;  // (s.k <= 1024 entries in all)
       __syncthreads();
       if (threadIdx.x == 0) cnt += all;
     }
     __syncthreads();
     n = (int)n_list;
   }
-  if (n > cap) {  // more than one wave ranks (ties, or an order the groups did not expect): the best `cap`, s.k of them count
-    int n2 = 512;
+  if (n > RPS_SHORT) {  // (ties, or an order the groups did not expect) the best of them, s.k count
+    int n2 = 2 * RPS_SHORT;
     while (n2 < n) n2 <<= 1;
-    for (int i = n + threadIdx.x; i < n2; i += SL_THREADS) list[i] = 0;
-    block_sort(list, n2);
-    n = cap;
+    for (int i = n + threadIdx.x; i < n2; i += SL_THREADS) sh.list[i] = 0;
+    block_sort(sh.list, n2);
+    n = RPS_SHORT;
   }
-  if ((int)threadIdx.x < n) lists[(int64_t)blockIdx.x * cap + threadIdx.x] = list[threadIdx.x];
-  if (threadIdx.x == 0) counts[blockIdx.x] = n;
-}
-
-// ... and one wave per row ranks them and draws (its 90 - 170 registers would halve the selection's workgroups per CU)
-template <int PER>
-__device__ __forceinline__ void rank_list(const unsigned long long* __restrict__ list, int n, unsigned long long* sorted, int lane) {
-  unsigned long long e[PER];
-#pragma unroll
-  for (int i = 0; i < PER; ++i) e[i] = i * 64 + lane < n ? list[i * 64 + lane] : 0ull;
-  rank_row<PER>(e, sorted, lane);
-}
-// (CAP: the lists' length; KEEP >= k: what the draws look at)
-template <int CAP, int KEEP>
-__global__ __launch_bounds__(64) void k_sample_lists(sample_args a, const unsigned long long* __restrict__ lists, const int32_t* __restrict__ counts) {
-  __shared__ unsigned long long sorted[CAP];
-  const int lane = threadIdx.x;
-  const int64_t r = a.row0 + blockIdx.x;
-  const int n = counts[blockIdx.x];
-  const row_set s = rs_load(a, r);
-  const unsigned long long* list = lists + (int64_t)blockIdx.x * CAP;
-  if (CAP > KEEP && n <= KEEP) rank_list<KEEP / 64>(list, n, sorted, lane);
-  else rank_list<CAP / 64>(list, n, sorted, lane);
-  finish_row<KEEP / 64>(a, r, s, sorted, lane);
+  const int runs = n <= 256 ? 4 : n <= 512 ? 8 : 16;
+  finish_group(a, r, s, rank_runs(sh.list, n, runs), runs, sh.group);
 }
 
 // ---- whole rows, any prefix, one draw ------------------------------------------------------------------------------------------------
@@ -1243,11 +1422,8 @@ __global__ __launch_bounds__(SL_THREADS) void k_row_draw(sample_args a, const ro
 // which form a call takes, and its workspace
 enum sample_form { FORM_WAVE, FORM_LISTS, FORM_ROWS };
 sample_form form_of(int64_t width, int64_t k) { return width <= RPS_SHORT ? FORM_WAVE : k <= RPS_SHORT ? FORM_LISTS : FORM_ROWS; }
-// entries of a row's list: the selection hands over 1.1 to 1.4 times k candidates
-int list_of(int64_t k) { return k <= 128 ? 256 : k <= 384 ? 512 : 1024; }
 int64_t workspace_of(int64_t rows, int64_t width, int64_t k) {
   switch (form_of(width, k)) {
-    case FORM_LISTS: return std::min(rows, STRIP_LISTS) * (list_of(k) * 8 + 4);
     case FORM_ROWS: return std::min(rows, STRIP) * (int64_t)sizeof(row_ws);
     default: return 0;
   }
@@ -1308,19 +1484,11 @@ extern "C" int rphip_sample(rphip_ctx* ctx, void* stream, int64_t rows, int64_t 
         }
         return RPHIP_OK;
       case FORM_LISTS:
-        for (a.row0 = 0; a.row0 < rows; a.row0 += STRIP_LISTS) {
-          const unsigned n = (unsigned)std::min(STRIP_LISTS, rows - a.row0);
-          const int cap = list_of(k);
-          unsigned long long* lists = (unsigned long long*)workspace_dev;
-          int32_t* counts = (int32_t*)(lists + std::min(rows, STRIP_LISTS) * cap);
+        for (a.row0 = 0; a.row0 < rows; a.row0 += 1 << 20) {
+          const unsigned n = (unsigned)std::min<int64_t>(1 << 20, rows - a.row0);
           constexpr int64_t piece = SL_THREADS * PIECE<T>;
-          if (width <= TK_HELD * piece) k_sample_topk<T, TK_HELD><<<n, SL_THREADS, 0, st>>>(a, lists, counts, cap);
-          else k_sample_topk<T, 0><<<n, SL_THREADS, 0, st>>>(a, lists, counts, cap);
-          RP_LAUNCHED();
-          if (cap == 256) k_sample_lists<256, 256><<<n, 64, 0, st>>>(a, lists, counts);
-          else if (k <= 256) k_sample_lists<512, 256><<<n, 64, 0, st>>>(a, lists, counts);
-          else if (cap == 512) k_sample_lists<512, 512><<<n, 64, 0, st>>>(a, lists, counts);
-          else k_sample_lists<1024, 1024><<<n, 64, 0, st>>>(a, lists, counts);
+          if (width <= TK_HELD * piece) k_sample_topk<T, TK_HELD><<<n, SL_THREADS, 0, st>>>(a);
+          else k_sample_topk<T, 0><<<n, SL_THREADS, 0, st>>>(a);
           RP_LAUNCHED();
         }
         return RPHIP_OK;
