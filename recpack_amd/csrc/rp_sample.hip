@@ -361,6 +361,104 @@ __device__ __forceinline__ void rank_row(unsigned long long (&e)[PER], unsigned 
 }
 
 // ---- rows that one wave holds ------------------------------------------------------------------------------------------------------
+// wave_sort for 32-bit entries: a step is one exchange and one instruction (the median with the largest or the smallest number)
+__device__ __forceinline__ uint32_t larger_if(uint32_t x, uint32_t y, uint32_t all_ones) { return max(min(x, y), min(max(x, y), all_ones)); }
+template <int PER>
+__device__ __forceinline__ void wave_sort_u32(uint32_t (&e)[PER], int lane) {
+#pragma unroll
+  for (int size = 2; size <= 64 * PER; size <<= 1) {
+    const uint32_t down = ((lane * PER) & size) == 0 ? ~0u : 0u;  // (size >= PER: of the whole lane)
+#pragma unroll
+    for (int ls = size / (2 * PER); ls > 0; ls >>= 1) {
+      const uint32_t keep = (lane & ls) == 0 ? down : ~down;
+#pragma unroll
+      for (int i = 0; i < PER; ++i) {
+        const uint32_t o = ls == 1    ? xor_lane<1>(e[i], lane)
+                           : ls == 2  ? xor_lane<2>(e[i], lane)
+                           : ls == 4  ? xor_lane<4>(e[i], lane)
+                           : ls == 8  ? xor_lane<8>(e[i], lane)
+                           : ls == 16 ? xor_lane<16>(e[i], lane)
+                                      : xor_lane<32>(e[i], lane);
+        e[i] = larger_if(e[i], o, keep);
+      }
+    }
+#pragma unroll
+    for (int step = PER >> 1; step > 0; step >>= 1) {
+      if (step >= size) continue;
+#pragma unroll
+      for (int i = 0; i < PER; ++i) {
+        if (i & step) continue;
+        const uint32_t keep = size >= PER ? down : (i & size) == 0 ? ~0u : 0u, x = e[i], y = e[i + step];
+        e[i] = larger_if(x, y, keep);
+        e[i + step] = larger_if(x, y, ~keep);
+      }
+    }
+  }
+}
+
+// Ranks a row's keys (lane l has the positions l, 64 + l, ..) into this wave's LDS: by their leading bits first, with the position in place of
+// the others - a third of the work of sorting 64-bit entries.  Scores that differ in the last 8 to 10 bits of 32 only may then stand the
+// wrong way round: two rounds of exchanges between neighbours put that right where it is rare, the full sort where it is not (16-bit
+// scores never need it).
+template <int PER>
+__device__ __forceinline__ void rank_keys(const uint32_t (&key)[PER], unsigned long long* sorted, int lane) {
+  constexpr uint32_t AT = 64 * PER - 1;
+  uint32_t* keys = (uint32_t*)sorted;
+  uint32_t p[PER];
+#pragma unroll
+  for (int i = 0; i < PER; ++i) {
+    const uint32_t at = i * 64 + lane;
+    keys[at] = key[i];
+    p[i] = (key[i] & ~AT) | (AT - at);
+  }
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");  // (one wave: its LDS accesses stay in order)
+  __builtin_amdgcn_wave_barrier();
+  wave_sort_u32<PER>(p, lane);
+  unsigned long long e[PER];
+#pragma unroll
+  for (int i = 0; i < PER; ++i) {
+    const uint32_t at = AT - (p[i] & AT);
+    e[i] = ((unsigned long long)keys[at] << 32) | (uint32_t)~at;
+  }
+  auto next = [&]() __attribute__((always_inline)) {
+    const unsigned long long v = __shfl(e[0], min(lane + 1, 63));
+    return lane < 63 ? v : 0ull;
+  };
+  auto wrong = [&]() __attribute__((always_inline)) {
+    bool w = e[PER - 1] < next();
+#pragma unroll
+    for (int i = 0; i + 1 < PER; ++i) w = w || e[i] < e[i + 1];
+    return __ballot(w) != 0;
+  };
+  if (wrong()) {
+#pragma unroll 1
+    for (int round = 0; round < (PER > 1 ? 2 : 0); ++round) {
+#pragma unroll
+      for (int odd = 0; odd < 2; ++odd) {
+        unsigned long long last = 0, first = 0;
+        if (odd) {
+          const unsigned long long behind = next(), ahead = __shfl(e[PER - 1], max(lane - 1, 0));
+          last = max(e[PER - 1], behind);
+          first = lane > 0 ? min(ahead, e[0]) : e[0];
+        }
+#pragma unroll
+        for (int i = odd; i + 1 < PER; i += 2) {
+          const unsigned long long x = e[i], y = e[i + 1];
+          e[i] = max(x, y), e[i + 1] = min(x, y);
+        }
+        if (odd) e[0] = first, e[PER - 1] = last;
+      }
+    }
+    if (wrong()) wave_sort<PER>(e, lane);
+  }
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+#pragma unroll
+  for (int i = 0; i < PER; ++i) sorted[lane * PER + i] = e[i];
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+}
+
 // One wave per row: up to 64 * PER scores in registers, sorted there.
 template <class T, int PER>
 __global__ __launch_bounds__(256) void k_sample_wave(sample_args a) {
@@ -370,14 +468,10 @@ __global__ __launch_bounds__(256) void k_sample_wave(sample_args a) {
   if (r >= a.rows) return;
   const row_set s = rs_load(a, r);
   const T* p = (const T*)a.scores + r * a.ld;
-  unsigned long long e[PER];
+  uint32_t key[PER];
 #pragma unroll
-  for (int i = 0; i < PER; ++i) {  // (any order will do: neighbouring lanes read neighbours)
-    const int j = i * 64 + lane;
-    const uint32_t k = j < s.len ? key_of(rp_to_f32(p[j])) : 0u;
-    e[i] = k ? ((unsigned long long)k << 32) | (uint32_t)~j : 0ull;
-  }
-  rank_row<PER>(e, sorted[wave], lane);
+  for (int i = 0; i < PER; ++i) key[i] = i * 64 + lane < s.len ? key_of(rp_to_f32(p[i * 64 + lane])) : 0u;
+  rank_keys<PER>(key, sorted[wave], lane);
   finish_row<PER>(a, r, s, sorted[wave], lane);
 }
 

@@ -424,6 +424,21 @@ def test_sample_ties_and_extremes(ctx, ops, width):
     check_sample(ctx, ops, x, torch.rand(rows, 1, generator=g), temperature=0.0)
 
 
+@pytest.mark.parametrize("width,top_k", [(2, 0), (5, 0), (64, 0), (65, 0), (200, 0), (256, 0), (257, 0), (500, 0), (513, 0), (1024, 0), (3000, 120), (3000, 400), (3000, 1000), (40000, 1000)])
+@pytest.mark.parametrize("apart", [1, 2, 64, 10 ** 6])
+def test_sample_close_scores(ctx, ops, width, top_k, apart):
+    """Scores that share their leading bits: some neighbours, some groups, all of them; equal ones among them."""
+    g = gen(width + apart)
+    step = torch.arange(width) // max(1, min(apart, width)) * 100.0  # groups of `apart` scores within some ulps of each other
+    x = (1000.0 + step).float()
+    x = (x.view(torch.int32) + torch.randint(0, 256, (6, width), generator=g, dtype=torch.int32)).view(torch.float32)
+    x = torch.stack([row[torch.randperm(width, generator=g)] for row in x])
+    x[1::2] *= -1
+    n = min(top_k or width, 64)
+    check_sample(ctx, ops, x, torch.zeros(6, n), temperature=0.0, top_k=top_k)
+    check_sample(ctx, ops, x, torch.rand(6, n, generator=g), temperature=0.05, top_k=top_k, top_p=0.9)
+
+
 def test_sample_far_below(ctx, ops):
     """Candidates far below the best one: by value in one coarse bin, drawn after the rest is gone."""
     x = torch.cat([torch.tensor([[50.0, 49.0]]), torch.randn(1, 30000, generator=gen(0)) - 400], 1)
