@@ -580,36 +580,43 @@ __device__ __forceinline__ int count_above(const unsigned long long* const (&run
   return sum;
 }
 
-// Ranks n <= 64 * runs entries of list[] (key << 32 | ~index; runs is 4, 8 or 16): every wave sorts 64 in its registers, then four runs at
-// a time are joined: an entry's place is its own plus, in each other run, the number of larger ones.  Every thread of the workgroup calls
-// it; list[] holds 128 * runs entries, the ranked ones start at the pointer that is returned (behind the last: entries with key 0).
+// Ranks 256 entries, one to a thread of four waves (t: 0 .. 255; all different): every wave sorts 64 in its registers, then the runs are joined:
+// an entry's place is its own plus, in each other run, the number of larger ones.  The ranked ones stand in to[]; list[] is overwritten.
+// Returns this thread's place.  Waves without entries (`on` false) call it for its barriers.
+__device__ __forceinline__ int rank_256(unsigned long long& v, unsigned long long* list, unsigned long long* to, int t, bool on) {
+  const int lane = t & 63, wave = t >> 6;
+  int rank = 0;
+  if (on) {
+    sort_run(v, lane, true);
+    list[t] = v;
+  }
+  __syncthreads();
+  if (on) {
+    const unsigned long long* const run[3] = {list + ((wave + 1) & 3) * 64, list + ((wave + 2) & 3) * 64, list + ((wave + 3) & 3) * 64};
+    rank = lane + count_above<64>(run, v);
+    to[rank] = v;
+  }
+  __syncthreads();
+  return rank;
+}
+
+// Ranks n <= 64 * runs entries of list[] (key << 32 | ~index; runs is 4, 8 or 16), 256 at a time and these joined in the same way.  Every thread
+// of the workgroup calls it; list[] holds 128 * runs entries, the ranked ones start at the pointer that is returned (behind the last:
+// entries with key 0).
 __device__ __forceinline__ const unsigned long long* rank_runs(unsigned long long* list, int n, int runs) {
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int wave = threadIdx.x >> 6, mine = wave >> 2;
   unsigned long long* other = list + 64 * runs;
   unsigned long long v = 0;
-  int rank = 0;
-  if (wave < runs) {
-    v = (int)threadIdx.x < n ? list[threadIdx.x] : (unsigned long long)threadIdx.x;  // (all different, so that places are, too)
-    sort_run(v, lane, true);
-    list[threadIdx.x] = v;
-  }
-  __syncthreads();
-  if (wave < runs) {
-    const unsigned long long* group = list + (wave & ~3) * 64;
-    const unsigned long long* const run[3] = {group + ((wave + 1) & 3) * 64, group + ((wave + 2) & 3) * 64, group + ((wave + 3) & 3) * 64};
-    rank = (wave & ~3) * 64 + lane + count_above<64>(run, v);
-    other[rank] = v;
-  }
-  __syncthreads();
+  if (wave < runs) v = (int)threadIdx.x < n ? list[threadIdx.x] : (unsigned long long)threadIdx.x;  // (all different, so that places are, too)
+  int rank = rank_256(v, list + mine * 256, other + mine * 256, threadIdx.x & 255, wave < runs);
   if (runs == 4) return other;
   if (wave < runs) {
-    const int mine = wave >> 2;
     if (runs == 8) {
       const unsigned long long* const run[1] = {other + (mine ^ 1) * 256};
-      rank += count_above<256>(run, v) - mine * 256;
+      rank += count_above<256>(run, v);
     } else {
       const unsigned long long* const run[3] = {other + ((mine + 1) & 3) * 256, other + ((mine + 2) & 3) * 256, other + ((mine + 3) & 3) * 256};
-      rank += count_above<256>(run, v) - mine * 256;
+      rank += count_above<256>(run, v);
     }
     list[rank] = v;
   }
@@ -1390,23 +1397,11 @@ __global__ __launch_bounds__(SR_THREADS) void k_row_collect(sample_args a, row_w
       if (at_found[which] + i < SB_CAP) ws.list[which][at_found[which] + i] = found[which][i];
 }
 
-// A list of at most 256 candidates, ranked by one wave: sorted[] and the cumulative masses behind `before`, and each one's own.
+// A list of at most 256 candidates, ranked by four waves: sorted[] and the cumulative masses with those in front of the list, and each one's own.
 struct ranked_list {
-  unsigned long long sorted[256], cum[256], own[256];
+  unsigned long long runs[256], sorted[256], cum[256], own[256], sum[4], before;
 };
-__device__ __forceinline__ void rank_masses(unsigned long long (&e)[4], int n, unsigned long long before, const row_mass& rm, ranked_list& out, int lane) {
-  rank_row<4>(e, out.sorted, lane);
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int rank = i * 64 + lane;
-    const unsigned long long mine = rank < n ? rm.mass(rm.log2_of(score_of((uint32_t)(out.sorted[rank] >> 32)))) : 0ull;
-    const unsigned long long cum = before + wave_scan_u64(mine);
-    out.cum[rank] = cum;
-    out.own[rank] = mine;
-    before = lane_u64(cum, 63);
-  }
-}
-// the first rank whose cumulative mass reaches the target (n if none); any whole wave
+// the first rank whose cumulative mass reaches the target (n if none); a whole wave
 __device__ __forceinline__ int rank_reaching(const ranked_list& l, int n, unsigned long long target, int lane) {
   int at = n;
 #pragma unroll
@@ -1421,10 +1416,7 @@ template <class T, bool COUNT>
 __global__ __launch_bounds__(SL_THREADS) void k_row_draw(sample_args a, const row_ws* __restrict__ wss, int slices, int shift) {
   __shared__ union {
     seek_shared seek;
-    struct {
-      ranked_list list[2];
-      unsigned long long before[2], kept;
-    } two;
+    ranked_list two[2];
   } sh;
   __shared__ unsigned long long red64[SL_THREADS / 64];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
@@ -1445,11 +1437,9 @@ __global__ __launch_bounds__(SL_THREADS) void k_row_draw(sample_args a, const ro
   const int b1 = ws.b1, b2_lo = ws.b2_lo, b2_hi = ws.b2_hi;
   const int n1 = b1 >= 0 && ws.n_list[0] <= SB_CAP ? (int)ws.n_list[0] : -1;
   const int n2 = b2_hi >= b2_lo && ws.n_list[1] <= SB_CAP ? (int)ws.n_list[1] : -1;
-  unsigned long long e[4];
-  if (wave < 2) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) e[i] = i * 64 + lane < (wave == 0 ? n1 : n2) ? ws.list[wave][i * 64 + lane] : 0ull;
-  }
+  const int which = wave >> 2, t = threadIdx.x & 255;  // (waves 0 - 3: the first list, 4 - 7: the second one)
+  unsigned long long e = t;
+  if (which < 2 && t < (which == 0 ? n1 : n2)) e = ws.list[which][t];
   unsigned long long incl = 0, own = 0, m[SEEK_PB], bm[SEEK_PB], c[SEEK_PB], bc[SEEK_PB];
 #pragma unroll
   for (int i = 0; i < SEEK_PB; ++i) {
@@ -1460,32 +1450,43 @@ __global__ __launch_bounds__(SL_THREADS) void k_row_draw(sample_args a, const ro
   unsigned long long total = scan_bins<SL_THREADS>(m, bm, red64);
   const unsigned long long most = max(ws.above, (unsigned long long)rm.scale);
   const bool cut_by_count = COUNT && (unsigned long long)s.k < ws.count;
-  // the common case - both lists are there and short: a wave each, side by side
+  // the common case - both lists are there and short: four waves each, side by side
   if (!cut_by_count && !rm.greedy && (b1 < 0 || (n1 >= 1 && n1 <= 256)) && n2 >= 1 && n2 <= 256) {
 #pragma unroll
     for (int i = 0; i < SEEK_PB; ++i) {
-      if ((int)threadIdx.x * SEEK_PB + i == b1) sh.two.before[0] = bm[i];
-      if ((int)threadIdx.x * SEEK_PB + i == b2_lo) sh.two.before[1] = bm[i];
+      if ((int)threadIdx.x * SEEK_PB + i == b1) sh.two[0].before = bm[i];
+      if ((int)threadIdx.x * SEEK_PB + i == b2_lo) sh.two[1].before = bm[i];
+    }
+    const bool on = which == 1 || (which == 0 && b1 >= 0);
+    ranked_list& mine = sh.two[which & 1];
+    const int rank = rank_256(e, mine.runs, mine.sorted, t, on);
+    unsigned long long own = 0, cum = 0;
+    if (on) {  // (this thread's entry, where it belongs)
+      own = rank < (which == 0 ? n1 : n2) ? rm.mass(rm.log2_of(score_of((uint32_t)(e >> 32)))) : 0ull;
+      mine.own[rank] = own;
     }
     __syncthreads();
-    if (wave == 0) {
-      unsigned long long kept = total;
-      if (b1 >= 0) {
-        rank_masses(e, n1, sh.two.before[0], rm, sh.two.list[0], lane);
-        kept = sh.two.list[0].cum[min(rank_reaching(sh.two.list[0], n1, border_of(s.top_p, total), lane), n1 - 1)];
-      }
-      if (lane == 0) sh.two.kept = min(kept, most);
-    } else if (wave == 1) {
-      rank_masses(e, n2, sh.two.before[1], rm, sh.two.list[1], lane);
+    if (on) {
+      cum = wave_scan_u64(mine.own[t]);
+      if (lane == 63) mine.sum[wave & 3] = cum;
     }
     __syncthreads();
-    if (wave != 1) return;
-    const unsigned long long kept = sh.two.kept;
-    const int rank = min(rank_reaching(sh.two.list[1], n2, want_of(a.u[r * a.ld_u], kept), lane), n2 - 1);
+    if (on) {
+      cum += mine.before;
+#pragma unroll
+      for (int w = 0; w < 3; ++w) cum += w < (wave & 3) ? mine.sum[w] : 0ull;
+      mine.cum[t] = cum;
+    }
+    __syncthreads();
+    if (wave != 0) return;
+    unsigned long long kept = total;
+    if (b1 >= 0) kept = sh.two[0].cum[min(rank_reaching(sh.two[0], n1, border_of(s.top_p, total), lane), n1 - 1)];
+    kept = min(kept, most);
+    const int at_rank = min(rank_reaching(sh.two[1], n2, want_of(a.u[r * a.ld_u], kept), lane), n2 - 1);
     if (lane == 0) {
-      const int at = (int)~(uint32_t)sh.two.list[1].sorted[rank];
+      const int at = (int)~(uint32_t)sh.two[1].sorted[at_rank];
       a.idx[r] = a.ids ? a.ids[r * a.ld_ids + at] : at;
-      a.prob[r] = (float)((double)sh.two.list[1].own[rank] / (double)kept);
+      a.prob[r] = (float)((double)sh.two[1].own[at_rank] / (double)kept);
       if (a.nnz) a.nnz[r] = 1;
     }
     return;
