@@ -304,6 +304,8 @@ class ItemSimilarityMatrixAlgorithm(Algorithm):
                 raise ValueError(f"predict_sample draws from the K best scores, 1 <= K <= {ops.SLATE_MAX}, got {K}")
             keep = item_mask(dX, exclude_items, select_items)
             u = draw_uniforms(u, seed, users, n)
+            if users == 0:
+                return np.full((0, n), -1, np.int32), np.zeros((0, n), np.float32)
             device = f"cuda:{ctx.device}"
             idx = torch.empty((users, K), dtype=torch.int32, device=device)
             val = torch.empty((users, K), dtype=torch.float32, device=device)

@@ -72,16 +72,26 @@ class CompressedEASE(Algorithm):
     def _matrices(self):
         """(rows, columns) on the device; an unpickled model is uploaded on its first use."""
         if getattr(self, "_rows", None) is None:
-            if getattr(self, "_host", None) is None:
+            host = getattr(self, "_host", None)
+            if host is not None:
+                self._columns = self._upload(host[1])
+                self._rows = self._upload(host[0])  # (the last one: it says that both are there, also to another thread)
+                self._host = None
+            elif getattr(self, "_rows", None) is None:
                 raise AttributeError("CompressedEASE is not fitted")
-            import torch
-
-            from recpack_amd import ops
-
-            device = f"cuda:{get_context().device}"
-            self._rows, self._columns = (None if m is None else ops.MXFP4(torch.from_numpy(m[0]).to(device), torch.from_numpy(m[1]).to(device), self.n_items_) for m in self._host)
-            self._host = None
         return self._rows, self._columns
+
+    def _upload(self, arrays):
+        import torch
+
+        from recpack_amd import ops
+
+        if arrays is None:
+            return None
+        m = ops.MXFP4.empty(arrays[0].shape[0], self.n_items_, f"cuda:{get_context().device}")
+        m.codes.copy_(torch.from_numpy(arrays[0]))
+        m.scales.copy_(torch.from_numpy(arrays[1]))
+        return m
 
     def _check_fit_complete(self):
         if getattr(self, "_rows", None) is None and getattr(self, "_host", None) is None:

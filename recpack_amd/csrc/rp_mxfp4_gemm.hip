@@ -408,11 +408,11 @@ __global__ __launch_bounds__(256) void k_mxg_rows(const T* __restrict__ a, int64
   uint4 q[GV_ROWS], qn[GV_ROWS];
   uint32_t s[GV_ROWS], sn[GV_ROWS];
   auto fetch = [&](int b) __attribute__((always_inline)) {
-    const int bb = min(b, nb - 1);  // (a block beyond the row: A is zero there)
+    const int bb = min(b, nb - 1);  // (a block beyond the row: A is zero there, the scale 2^-127: no infinity meets a zero)
 #pragma unroll
     for (int r = 0; r < GV_ROWS; ++r) {
       qn[r] = *(const uint4*)(wr[r] + (int64_t)bb * 16);
-      sn[r] = sr[r][bb];
+      sn[r] = b < nb ? sr[r][bb] : 0u;
     }
   };
   rp_vec<T, 8> an[M];  // this thread's eight elements of the next step

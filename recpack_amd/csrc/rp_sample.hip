@@ -1543,7 +1543,7 @@ extern "C" int rphip_sample(rphip_ctx* ctx, void* stream, int64_t rows, int64_t 
   if (!params) RP_FAIL(RPHIP_EINVAL, "sample: params is NULL");
   if (type != RPHIP_F32 && type != RPHIP_F16 && type != RPHIP_BF16) RP_FAIL(RPHIP_EINVAL, "sample: element type %d: RPHIP_F32, RPHIP_F16 or RPHIP_BF16 expected", type);
   if (rows < 0 || width < 0 || width > ((int64_t)1 << 30)) RP_FAIL(RPHIP_EINVAL, "sample: %lld rows of %lld scores", (long long)rows, (long long)width);
-  if (draws < 1) RP_FAIL(RPHIP_EINVAL, "sample: draws = %d", draws);
+  if (draws < 1 || draws > 1 << 30) RP_FAIL(RPHIP_EINVAL, "sample: draws = %d", draws);
   if (ld < width || (ids_dev && ld_ids < width) || ld_u < draws) RP_FAIL(RPHIP_EINVAL, "sample: a leading dimension is smaller than its rows");
   if (!(params->temperature >= 0.0f) || params->temperature > 3.4e38f) RP_FAIL(RPHIP_EINVAL, "sample: temperature %g: a finite number >= 0 expected", params->temperature);
   if (bad_fraction(params->top_p) || bad_fraction(params->min_p)) RP_FAIL(RPHIP_EINVAL, "sample: top_p %g, min_p %g: 0 .. 1 expected", params->top_p, params->min_p);

@@ -155,6 +155,20 @@ def test_predict_sample_of_every_algorithm(ease, data):
         knn.predict_sample(data, 2, exclude_items=[])
 
 
+def test_no_users(ease, small):
+    empty = sp.csr_matrix((0, 333))
+    assert small.predict_topk(empty, 5).shape == (0, 333)
+    assert tuple(small.scores(empty).shape) == (0, 333)
+    for algo in (small, ease):
+        items, probs = algo.predict_sample(empty, 3, K=10)
+        assert items.shape == probs.shape == (0, 3)
+    # users without a history, among others
+    X = sp.csr_matrix((np.ones(3), ([1, 1, 3], [0, 5, 7])), shape=(5, 333))
+    for algo in (small, ease):
+        items, probs = algo.predict_sample(X, 2, K=10, seed=1)
+        assert (items[[0, 2, 4]] == -1).all() and (probs[[0, 2, 4]] == 0).all() and (items[[1, 3]] >= 0).all()
+
+
 def test_pickle(small, data):
     other = pickle.loads(pickle.dumps(small))
     assert torch.equal(other.scores(data), small.scores(data))

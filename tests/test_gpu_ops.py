@@ -502,3 +502,111 @@ def test_product_large(ctx, ops, dtype, m, n, k):
     assert got.dtype == out_type
     assert ((got.double() - want).abs() <= bound).all()
     assert torch.equal(got, ops.mxfp4_gemm_nt(ctx, a, w))  # no part of K is added in another order
+
+
+# ---- what is left alone, what is huge ---------------------------------------------------------------------------------------------------------
+
+def framed(rows, cols, dtype, value=7):
+    """An output inside a larger buffer, and a check that the frame around it is as it was."""
+    big = torch.full((rows + 2, cols + 5), value, dtype=dtype, device="cuda")
+    out = big[1:-1, 3:-2]
+
+    def untouched():
+        frame = torch.ones_like(big, dtype=torch.bool)
+        frame[1:-1, 3:-2] = False
+        return bool((big[frame] == value).all())
+
+    return out, untouched
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_nothing_around_an_output_is_written(ctx, ops, dtype):
+    g = gen(4)
+    w = random_mxfp4(ops, 333, 333, 5)
+    for rows in (1, 3, 17, 70):
+        out, untouched = framed(rows, 333, dtype)
+        assert torch.equal(ops.mxfp4_gemm_nt(ctx, torch.randn(rows, 333, generator=g).cuda(), w, out=out).contiguous(), out) and untouched()
+        indptr = torch.arange(rows + 1, dtype=torch.int32).cuda() * 3
+        indices = torch.randint(0, 333, (rows * 3,), generator=g, dtype=torch.int32).cuda()
+        for weights in (None, torch.rand(rows * 3, generator=g).cuda()):
+            out, untouched = framed(rows, 333, dtype)
+            ops.mxfp4_scores(ctx, indptr, indices, w, weights=weights, out=out)
+            assert untouched() and not (out == 7).all()
+    out, untouched = framed(333, 333, dtype)
+    ops.mxfp4_dequantize(ctx, w, out=out)
+    assert untouched()
+    # the codes of a matrix inside a larger one
+    codes, scales = torch.full((12, 32 * 16), 9, dtype=torch.uint8, device="cuda"), torch.full((12, 32), 9, dtype=torch.uint8, device="cuda")
+    m = ops.MXFP4(codes[1:-1, 16:16 * 5], scales[1:-1, 2:6], 100)
+    x = torch.randn(10, 100, generator=g).to(dtype).cuda()
+    for transpose in (False, True):
+        codes.fill_(9), scales.fill_(9)
+        ops.mxfp4_quantize(ctx, x.t().contiguous() if transpose else x, transpose=transpose, out=m)
+        np.testing.assert_array_equal(values_of(m), quantised_reference(x.double().cpu().numpy())[2])
+        assert int((codes == 9).sum()) >= 12 * 32 * 16 - 10 * 64 and bool((codes[:, :16] == 9).all()) and bool((codes[:, 80:] == 9).all())
+        assert bool((codes[0] == 9).all()) and bool((codes[-1] == 9).all()) and bool((scales[:, 6:] == 9).all()) and bool((scales[0] == 9).all())
+
+
+@pytest.mark.parametrize("m,n,k", [(0, 5, 7), (5, 0, 7), (5, 7, 0), (1, 7, 0), (40, 70, 0)])
+def test_empty_products(ctx, ops, m, n, k):
+    w = ops.mxfp4_quantize(ctx, torch.ones(n, k, device="cuda"))
+    for a in (torch.ones(m, k, device="cuda"), ops.mxfp4_quantize(ctx, torch.ones(m, k, device="cuda"))):
+        got = ops.mxfp4_gemm_nt(ctx, a, w, out=torch.full((m, n), 3.0, device="cuda"))
+        assert got.shape == (m, n) and bool((got == 0).all())
+
+
+@pytest.mark.parametrize("m", [1, 4, 40])
+def test_product_of_the_largest_scale(ctx, ops, m):
+    """6 x 2^127 in a row's last block is no number of float32 (quantising makes no scale that large): the row's sums are not finite, the others'
+    are not touched.  Infinite in one pass over float32; with A in bf16 planes 1 = 1 + 0 + 0, and 0 times infinity is NaN."""
+    w = ops.mxfp4_quantize(ctx, torch.ones(6, 70, device="cuda"))
+    w.scales[2, 2], w.codes[2, 32] = 254, 0x07
+    got = ops.mxfp4_gemm_nt(ctx, torch.ones(m, 70, device="cuda"), w)
+    assert not bool(got[:, 2].isfinite().any()) and bool((got[:, [0, 1, 3, 4, 5]] == 70).all())
+    assert m > 4 or bool(got[:, 2].isinf().all())
+
+
+def test_offsets_past_32_bits(ctx, ops):
+    """Inputs and outputs of more than 2^32 bytes (2^31 elements): the last rows are those of the last rows alone."""
+    rows, cols = 70001, 33001
+    x = torch.empty(rows, cols, dtype=torch.float16, device="cuda").normal_(generator=torch.Generator(device="cuda").manual_seed(1))
+    last = x[-5:].clone()
+    q, ql = ops.mxfp4_quantize(ctx, x), ops.mxfp4_quantize(ctx, last)
+    assert torch.equal(q.codes[-5:], ql.codes) and torch.equal(q.scales[-5:], ql.scales)
+    t = ops.mxfp4_quantize(ctx, x, transpose=True)
+    part = ops.mxfp4_quantize(ctx, x[69984:].contiguous(), transpose=True)  # (a multiple of 32 rows in front)
+    assert torch.equal(t.codes[:, 69984 // 2:], part.codes) and torch.equal(t.scales[:, 69984 // 32:], part.scales)
+    back = ops.mxfp4_dequantize(ctx, q, dtype=torch.float16)
+    assert torch.equal(back[-5:], ops.mxfp4_dequantize(ctx, ql, dtype=torch.float16))
+    del t, part, back
+    u = torch.rand(rows, 4, device="cuda")
+    for k in (20, 0):
+        n = 4 if k else 1
+        got, want = ops.sample(ctx, x, u[:, :n], top_k=k), ops.sample(ctx, last, u[-5:, :n], top_k=k)
+        assert all(torch.equal(a[-5:], b) for a, b in zip(got, want))
+    indptr = torch.arange(rows + 1, dtype=torch.int32, device="cuda")
+    indices = torch.arange(rows, dtype=torch.int32, device="cuda")
+    out = ops.mxfp4_scores(ctx, indptr, indices, q, dtype=torch.float16)  # (every history is one row of the matrix)
+    assert torch.equal(out[-5:], ops.mxfp4_dequantize(ctx, ql, dtype=torch.float16))
+    del out
+    w = ops.mxfp4_quantize(ctx, torch.randn(40000, 96, device="cuda"))
+    a = torch.randn(60001, 96, device="cuda", dtype=torch.float16)
+    got = ops.mxfp4_gemm_nt(ctx, a, w)
+    assert got.numel() > 2 ** 31 and torch.equal(got[-3:], ops.mxfp4_gemm_nt(ctx, a[-300:], w)[-3:])
+
+
+def test_codes_past_4_gib(ctx, ops):
+    n = 100000
+    w = ops.MXFP4.empty(n, n, "cuda")
+    w.codes.random_(generator=torch.Generator(device="cuda").manual_seed(2))
+    w.scales.random_(120, 130, generator=torch.Generator(device="cuda").manual_seed(3))
+    at = torch.tensor([n - 1, 5, n - 2, 99998 - 1], dtype=torch.int32, device="cuda")
+    few = ops.MXFP4(w.codes[at.long()].contiguous(), w.scales[at.long()].contiguous(), n)
+    rows = ops.mxfp4_dequantize(ctx, few).double()
+    got = ops.mxfp4_scores(ctx, torch.tensor([0, 4, 5], dtype=torch.int32, device="cuda"), torch.cat([at, at[:1]]), w)
+    assert torch.equal(got[1].double(), rows[0])
+    assert bool(((got[0].double() - rows.sum(0)).abs() <= 4 * 2.0 ** -23 * rows.abs().sum(0)).all())
+    a = torch.randn(2, n, device="cuda")
+    want = a.double() @ rows.t()
+    got = ops.mxfp4_gemm_nt(ctx, a, w)[:, at.long()].double()
+    assert bool(((got - want).abs() <= 8 * math.sqrt(n) * 2.0 ** -23 * (a.double().abs() @ rows.abs().t())).all())

@@ -78,7 +78,7 @@ def sample(rows=2, width=10, scores=P, type=0, ld=10, lengths=None, ids=None, ld
 
 
 @pytest.mark.parametrize("change,message", [
-    (dict(params=False), "params"), (dict(type=3), "element type"), (dict(rows=-1), "rows of"), (dict(width=2 ** 30 + 1, ld=2 ** 31), "rows of"), (dict(draws=0), "draws"),
+    (dict(params=False), "params"), (dict(type=3), "element type"), (dict(rows=-1), "rows of"), (dict(width=2 ** 30 + 1, ld=2 ** 31), "rows of"), (dict(draws=0), "draws"), (dict(draws=2 ** 30 + 1, ldu=2 ** 31), "draws"),
     (dict(ld=9), "leading dimension"), (dict(ids=P, ld_ids=9), "leading dimension"), (dict(draws=2, ldu=1), "leading dimension"), (dict(temperature=-1.0), "temperature"),
     (dict(temperature=float("nan")), "temperature"), (dict(temperature=float("inf")), "temperature"), (dict(top_p=1.5), "top_p"), (dict(top_p=float("nan")), "top_p"),
     (dict(min_p=-0.1), "min_p"), (dict(top_k=-1), "top_k"), (dict(top_k_dev=P), "bound"), (dict(idx=None), "NULL argument"), (dict(u=None), "NULL argument"),
