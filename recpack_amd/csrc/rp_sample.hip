@@ -16,8 +16,8 @@ namespace {
 constexpr int RPS_SHORT = 1024;      // longest prefix the list form ranks completely
 constexpr int SL_CAP = 4096;         // candidates collected in LDS
 constexpr int SL_THREADS = 1024;
-constexpr int SB_BINS = 4096;        // mass bins of the whole-row form: 128 per e-fold, the last one takes what lies below e^-32
-constexpr double SB_PER_E = 128.0;
+constexpr int SB_BINS = 4096;        // mass bins of the whole-row form: 128 per factor of two, the last one takes what lies below 2^-32
+constexpr int SB_PER = 128;
 constexpr int SB_CAP = 2048;         // entries of a list collected ahead
 constexpr int RC_FOUND = 512;        // ... of a workgroup's own part of them, in LDS
 constexpr int SR_THREADS = 256;      // threads of a workgroup that takes a slice of a row
@@ -988,23 +988,40 @@ __global__ __launch_bounds__(SL_THREADS, 8) void k_sample_topk(sample_args a) {
 }
 
 // ---- whole rows, any prefix, one draw ------------------------------------------------------------------------------------------------
-// masses of a row's candidates relative to its best score
+// Masses of a row's candidates relative to its best score, by t = 128 log2(mass) (0 for the best score, +inf among them; -8000 where next to
+// nothing is left).  Its nearest whole number is the bin; 2^(t / 128) is a power of two from a table of 128, times a polynomial of degree 4
+// on +-ln2 / 256 (remainder < 2^-49 relative); as whole numbers of 2^-shift (shift <= 50: the add of 2^52 rounds).  Some 20 instructions; a
+// series of degree 11 and the conversion to 64 bits took 40 (512 rows of 100000: 99 us of 247).
 struct row_mass {
   float best;
-  double c;      // log2(e) / temperature
+  double c;      // 128 log2(e) / temperature
   double scale;  // 2^shift
   bool greedy;
-  // base-2 logarithm of the mass: 0 for the best score (+inf among them)
-  __device__ __forceinline__ double log2_of(float x) const { return x == best ? 0.0 : greedy ? -1000.0 : fmax(((double)x - (double)best) * c, -1000.0); }
-  __device__ __forceinline__ int bin(double y) const { return (int)fmin(y * (-SB_PER_E * 0.69314718055994530942), (double)(SB_BINS - 1)); }
-  __device__ __forceinline__ unsigned long long mass(double y) const { return (unsigned long long)rint(exp2_le0(y) * scale); }
+  const double* powers;  // 2^(j / 128), in LDS
+  __device__ __forceinline__ double t_of(float x) const { return x == best ? 0.0 : greedy ? -8000.0 : fmax(((double)x - (double)best) * c, -8000.0); }
+  __device__ __forceinline__ int bin(double t) const { return min(-(int)rint(t), SB_BINS - 1); }
+  __device__ __forceinline__ double part(double t) const {
+    constexpr double L = 0.69314718055994530942 / SB_PER;
+    const double n = rint(t), f = t - n;
+    const int i = (int)n;
+    double q = fma(f, in_scalar(L * L * L * L / 24.0), in_scalar(L * L * L / 6.0));
+    q = fma(q, f, in_scalar(L * L / 2.0));
+    q = fma(q, f, in_scalar(L));
+    q = fma(q, f, 1.0);
+    return ldexp(powers[i & (SB_PER - 1)], i >> 7) * q;
+  }
+  __device__ __forceinline__ unsigned long long whole(double part) const { return (unsigned long long)__double_as_longlong(fma(part, scale, 0x1p52)) ^ 0x4330000000000000ull; }
+  __device__ __forceinline__ unsigned long long mass(double t) const { return whole(part(t)); }
 };
-__device__ __forceinline__ row_mass rm_make(uint32_t best, const row_set& s, int shift) {
+// (every thread of the workgroup; a barrier has to follow; without `powers` for t and bins only)
+__device__ __forceinline__ row_mass rm_make(uint32_t best, const row_set& s, int shift, double* powers) {
+  if (powers && threadIdx.x < SB_PER) powers[threadIdx.x] = 2.0 * exp2_le0((double)threadIdx.x / SB_PER - 1.0);
   row_mass rm;
   rm.best = score_of(best);
   rm.greedy = s.temperature == 0.0f;
-  rm.c = rm.greedy ? 1.0 : 1.4426950408889634074 / (double)s.temperature;
+  rm.c = rm.greedy ? 1.0 : 1.4426950408889634074 * SB_PER / (double)s.temperature;
   rm.scale = ldexp(1.0, shift);
+  rm.powers = powers;
   return rm;
 }
 
@@ -1012,6 +1029,7 @@ __device__ __forceinline__ row_mass rm_make(uint32_t best, const row_set& s, int
 struct row_ws {
   unsigned long long hist_m[SB_BINS];  // masses per bin
   unsigned long long above, count;     // mass of the candidates with at least min_p of the best one's mass; candidates
+  unsigned long long total, before[2]; // all mass; the masses in front of the lists' bins
   unsigned long long list[2][SB_CAP];  // candidates of bin b1 (where top-p ends) and of the bins b2 (where the draw can fall)
   uint32_t hist_c[SB_BINS];            // candidates per bin
   uint32_t n_list[2];
@@ -1096,7 +1114,7 @@ __device__ __forceinline__ int seek(const T* p, int len, const row_mass& rm, con
 #pragma unroll
       for (int i = 0; i < PIECE<T>; ++i) {
         const uint32_t k = key_of(rp_to_f32(v.v[i]));
-        if (k != 0 && rm.bin(rm.log2_of(score_of(k))) == b) {
+        if (k != 0 && rm.bin(rm.t_of(score_of(k))) == b) {
           const uint32_t at = atomicAdd(&sh.n_list, 1u);
           if (at < SL_CAP) sh.list[at] = ((unsigned long long)k << 32) | (uint32_t) ~(j + i);
         }
@@ -1117,7 +1135,7 @@ __device__ __forceinline__ int seek(const T* p, int len, const row_mass& rm, con
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const int rank = i * 64 + lane;
-        const unsigned long long mine = rank < n ? rm.mass(rm.log2_of(score_of((uint32_t)(sh.list[rank] >> 32)))) : 0ull;
+        const unsigned long long mine = rank < n ? rm.mass(rm.t_of(score_of((uint32_t)(sh.list[rank] >> 32)))) : 0ull;
         const unsigned long long cum = run + wave_scan_u64(mine);
         const unsigned long long pass = __ballot(rank < n && (by_count ? count_before + rank + 1 == target : cum >= target));
         if (looking && pass) {
@@ -1144,7 +1162,7 @@ __device__ __forceinline__ int seek(const T* p, int len, const row_mass& rm, con
     // cumulative sums along the sorted list: 1024 entries at a time
     for (int i0 = 0; i0 < n; i0 += SL_THREADS) {
       const int i = i0 + threadIdx.x;
-      const unsigned long long mine = i < n ? rm.mass(rm.log2_of(score_of((uint32_t)(sh.list[i] >> 32)))) : 0ull;
+      const unsigned long long mine = i < n ? rm.mass(rm.t_of(score_of((uint32_t)(sh.list[i] >> 32)))) : 0ull;
       const unsigned long long s = wave_scan_u64(mine);
       __syncthreads();
       if (lane == 63) sh.red64[wave] = s;
@@ -1181,7 +1199,7 @@ __device__ __forceinline__ int seek(const T* p, int len, const row_mass& rm, con
     for (int j = threadIdx.x; j < len; j += SL_THREADS) {
       const uint32_t k = key_of(rp_to_f32(p[j]));
       if (k == 0 || (shift != 24 && (k >> (shift + 8)) != (prefix >> (shift + 8)))) continue;
-      const double z = rm.log2_of(score_of(k));
+      const double z = rm.t_of(score_of(k));
       if (rm.bin(z) != b) continue;
       atomicAdd(&sh.hist_c[(k >> shift) & 255], 1u);
       const unsigned long long mm = rm.mass(z);
@@ -1205,7 +1223,7 @@ __device__ __forceinline__ int seek(const T* p, int len, const row_mass& rm, con
     count_before = sh.before32;
     mass_before = sh.before64;
   }
-  const unsigned long long each = rm.mass(rm.log2_of(score_of(prefix)));
+  const unsigned long long each = rm.mass(rm.t_of(score_of(prefix)));
   // the ordinal among the equal scores
   const unsigned long long nth = by_count ? target - count_before : each ? (target - mass_before + each - 1) / each : 1ull;
   *incl = mass_before + nth * each;
@@ -1234,12 +1252,14 @@ __device__ __forceinline__ int seek(const T* p, int len, const row_mass& rm, con
   return (int)sh.found;
 }
 
-// The whole-row form runs in four launches, the first three with a row's slices spread over workgroups:
+// The whole-row form runs in four or five launches, three of them with a row's slices spread over workgroups:
 //   best     the slices' best scores; clears the row's workspace
 //   hist     masses and counts per bin (fixed point: the order of the atomics does not matter)
-//   collect  the candidates of the bin where top-p ends and of the bins where the draw can fall (known up to one bin's mass)
+//   bins     the bin where top-p ends and the bins where the draw can fall (known up to one bin's mass); few rows: inside collect
+//   collect  the candidates of these bins
 //   draw     one workgroup: the exact end of the kept prefix, then the draw
-// Read three times, from memory once where it fits the caches.
+// Read three times, from memory once where it fits the caches.  (The last slice of hist in the place of bins needs a fence in every
+// workgroup that writes its XCD's cache back: 16 us instead of 7 for one row, 350 instead of 80 for 512.)
 __device__ __forceinline__ void slice_of(int len, int slices, int s, int& begin, int& end) {
   const int64_t pieces = ((int64_t)len + 7) / 8;
   begin = (int)(pieces * s / slices * 8);
@@ -1274,6 +1294,7 @@ __device__ __forceinline__ uint32_t best_of(const row_ws& ws, int slices) {
 
 template <class T, bool COUNT>
 __global__ __launch_bounds__(SR_THREADS) void k_row_hist(sample_args a, row_ws* __restrict__ wss, int shift) {
+  __shared__ double powers[SB_PER];
   __shared__ unsigned long long hist_m[SB_BINS];
   __shared__ uint32_t hist_c[COUNT ? SB_BINS : 1];
   __shared__ unsigned long long red[SR_THREADS / 64];
@@ -1283,7 +1304,7 @@ __global__ __launch_bounds__(SR_THREADS) void k_row_hist(sample_args a, row_ws* 
   const row_set s = rs_load(a, r);
   const uint32_t best = best_of(ws, slices);
   if (best == 0) return;
-  const row_mass rm = rm_make(best, s, shift);
+  const row_mass rm = rm_make(best, s, shift, powers);
   for (int i = threadIdx.x; i < SB_BINS; i += SR_THREADS) {
     hist_m[i] = 0;
     if (COUNT) hist_c[i] = 0;
@@ -1298,10 +1319,9 @@ __global__ __launch_bounds__(SR_THREADS) void k_row_hist(sample_args a, row_ws* 
     for (int i = 0; i < PIECE<T>; ++i) {
       const uint32_t k = key_of(rp_to_f32(v.v[i]));
       if (k == 0) continue;
-      const double y = rm.log2_of(score_of(k));
-      const double e = exp2_le0(y);
-      const unsigned long long m = (unsigned long long)rint(e * rm.scale);
-      const int b = rm.bin(y);
+      const double t = rm.t_of(score_of(k)), e = rm.part(t);
+      const unsigned long long m = rm.whole(e);
+      const int b = rm.bin(t);
       if (m) atomicAdd(&hist_m[b], m);
       if (COUNT) {
         atomicAdd(&hist_c[b], 1u);
@@ -1323,28 +1343,22 @@ __global__ __launch_bounds__(SR_THREADS) void k_row_hist(sample_args a, row_ws* 
   }
 }
 
-template <class T, bool COUNT>
-__global__ __launch_bounds__(SR_THREADS) void k_row_collect(sample_args a, row_ws* __restrict__ wss, int slices, int shift) {
-  __shared__ unsigned long long red[SR_THREADS / 64];
-  __shared__ unsigned long long range[2];
+// where top-p ends, and between which masses the draw falls: every thread of the workgroup
+struct row_bins {
+  int b1, lo, hi;
+  unsigned long long total;
+};
+template <int THREADS, bool COUNT>
+__device__ __forceinline__ row_bins find_bins(const row_ws& ws, const row_set& s, float u, int shift, unsigned long long (&before)[SB_BINS / THREADS]) {
+  __shared__ unsigned long long red[THREADS / 64], range[2];
   __shared__ int bins[3];
-  __shared__ unsigned long long found[2][RC_FOUND];
-  __shared__ uint32_t n_found[2], at_found[2];
-  const int sl = blockIdx.y;
-  const int64_t r = a.row0 + blockIdx.x;
-  row_ws& ws = wss[blockIdx.x];
-  const row_set s = rs_load(a, r);
-  const uint32_t best = best_of(ws, slices);
-  if (best == 0) return;
-  const row_mass rm = rm_make(best, s, shift);
-  if (threadIdx.x == 0) bins[0] = -1, bins[1] = 0, bins[2] = -1, n_found[0] = 0, n_found[1] = 0;
-  // where top-p ends, and between which masses the draw falls
-  constexpr int PB = SB_BINS / SR_THREADS;
-  unsigned long long m[PB], before[PB];
+  constexpr int PB = SB_BINS / THREADS;
+  if (threadIdx.x == 0) bins[0] = -1, bins[1] = 0, bins[2] = -1;
+  unsigned long long m[PB];
 #pragma unroll
   for (int i = 0; i < PB; ++i) m[i] = ws.hist_m[threadIdx.x * PB + i];
-  const unsigned long long total = scan_bins<SR_THREADS>(m, before, red);
-  const bool known = !rm.greedy && !(COUNT && (unsigned long long)s.k < ws.count);  // (otherwise the total itself is not known yet)
+  const unsigned long long total = scan_bins<THREADS>(m, before, red);
+  const bool known = s.temperature != 0.0f && !(COUNT && (unsigned long long)s.k < ws.count);  // (otherwise the total itself is not known yet)
   if (known) {
     const unsigned long long border = border_of(s.top_p, total);
     const bool cuts = s.top_p < 1.0f && border < total;
@@ -1356,8 +1370,7 @@ __global__ __launch_bounds__(SR_THREADS) void k_row_collect(sample_args a, row_w
         if (before[i] < border && before[i] + m[i] >= border) bins[0] = threadIdx.x * PB + i, range[0] = border, range[1] = before[i] + m[i];
     }
     __syncthreads();
-    const unsigned long long most = max(ws.above, (unsigned long long)rm.scale);
-    const float u = a.u[r * a.ld_u];
+    const unsigned long long most = max(ws.above, 1ull << shift);
     const unsigned long long w0 = want_of(u, min(range[0], most)), w1 = want_of(u, min(range[1], most));
 #pragma unroll
     for (int i = 0; i < PB; ++i) {
@@ -1366,17 +1379,65 @@ __global__ __launch_bounds__(SR_THREADS) void k_row_collect(sample_args a, row_w
     }
   }
   __syncthreads();
-  const int b1 = bins[0], lo = bins[1], hi = bins[2];
-  if (sl == 0 && threadIdx.x == 0) ws.b1 = b1, ws.b2_lo = lo, ws.b2_hi = hi;
+  return {bins[0], bins[1], bins[2], total};
+}
+template <int THREADS>
+__device__ __forceinline__ void keep_bins(row_ws& ws, const row_bins& b, const unsigned long long (&before)[SB_BINS / THREADS]) {
+  constexpr int PB = SB_BINS / THREADS;
+  if (threadIdx.x == 0) ws.b1 = b.b1, ws.b2_lo = b.lo, ws.b2_hi = b.hi, ws.total = b.total;
+#pragma unroll
+  for (int i = 0; i < PB; ++i) {
+    if ((int)threadIdx.x * PB + i == b.b1) ws.before[0] = before[i];
+    if ((int)threadIdx.x * PB + i == b.lo) ws.before[1] = before[i];
+  }
+}
+template <bool COUNT>
+__global__ __launch_bounds__(SL_THREADS) void k_row_bins(sample_args a, row_ws* __restrict__ wss, int shift) {
+  const int64_t r = a.row0 + blockIdx.x;
+  row_ws& ws = wss[blockIdx.x];
+  unsigned long long before[SB_BINS / SL_THREADS];
+  const row_bins b = find_bins<SL_THREADS, COUNT>(ws, rs_load(a, r), a.u[r * a.ld_u], shift, before);
+  keep_bins<SL_THREADS>(ws, b, before);
+}
+
+// (FIND: every workgroup finds the bins itself, where one launch less is more)
+template <class T, bool COUNT, bool FIND>
+__global__ __launch_bounds__(SR_THREADS) void k_row_collect(sample_args a, row_ws* __restrict__ wss, int slices, int shift) {
+  __shared__ unsigned long long found[2][RC_FOUND];
+  __shared__ uint32_t n_found[2], at_found[2];
+  const int sl = blockIdx.y;
+  const int64_t r = a.row0 + blockIdx.x;
+  row_ws& ws = wss[blockIdx.x];
+  const row_set s = rs_load(a, r);
+  const uint32_t best = best_of(ws, slices);
+  if (best == 0) return;
+  const row_mass rm = rm_make(best, s, shift, nullptr);
+  if (threadIdx.x < 2) n_found[threadIdx.x] = 0;
+  __syncthreads();
+  row_bins bins;
+  if constexpr (FIND) {
+    unsigned long long before[SB_BINS / SR_THREADS];
+    bins = find_bins<SR_THREADS, COUNT>(ws, s, a.u[r * a.ld_u], shift, before);
+    if (sl == 0) keep_bins<SR_THREADS>(ws, bins, before);
+  } else {
+    bins = {ws.b1, ws.b2_lo, ws.b2_hi, 0};
+  }
+  const int b1 = bins.b1, lo = bins.lo, hi = bins.hi;
   if (b1 < 0 && hi < lo) return;
+  // between which scores these bins lie, half a bin more on either side, and a float's step: all others are passed over by comparisons
+  auto above = [&](int bin) __attribute__((always_inline)) { return nextafterf((float)((double)rm.best + (1.0 - bin) / rm.c), INFINITY); };
+  auto below = [&](int bin) __attribute__((always_inline)) { return bin == SB_BINS - 1 ? -INFINITY : nextafterf((float)((double)rm.best - (1.0 + bin) / rm.c), -INFINITY); };
+  const float high1 = b1 < 0 ? -INFINITY : above(b1), low1 = b1 < 0 ? INFINITY : below(b1), high2 = hi < lo ? -INFINITY : above(lo), low2 = hi < lo ? INFINITY : below(hi);
   int begin, end;
   slice_of(s.len, gridDim.y, sl, begin, end);
   scan_row<T>((const T*)a.scores + r * a.ld, begin, end, threadIdx.x, SR_THREADS, [&](int j, const rp_vec<T, PIECE<T>>& v, int) __attribute__((always_inline)) {
 #pragma unroll
     for (int i = 0; i < PIECE<T>; ++i) {
-      const uint32_t k = key_of(rp_to_f32(v.v[i]));
+      const float x = rp_to_f32(v.v[i]);
+      if (!((x >= low1 && x <= high1) || (x >= low2 && x <= high2))) continue;
+      const uint32_t k = key_of(x);
       if (k == 0) continue;
-      const int b = rm.bin(rm.log2_of(score_of(k)));
+      const int b = rm.bin(rm.t_of(score_of(k)));
       const unsigned long long entry = ((unsigned long long)k << 32) | (uint32_t) ~(j + i);
       auto put = [&](int which) __attribute__((always_inline)) {
         uint32_t at = atomicAdd(&n_found[which], 1u);
@@ -1399,7 +1460,7 @@ __global__ __launch_bounds__(SR_THREADS) void k_row_collect(sample_args a, row_w
 
 // A list of at most 256 candidates, ranked by four waves: sorted[] and the cumulative masses with those in front of the list, and each one's own.
 struct ranked_list {
-  unsigned long long runs[256], sorted[256], cum[256], own[256], sum[4], before;
+  unsigned long long runs[256], sorted[256], cum[256], own[256], sum[4];
 };
 // the first rank whose cumulative mass reaches the target (n if none); a whole wave
 __device__ __forceinline__ int rank_reaching(const ranked_list& l, int n, unsigned long long target, int lane) {
@@ -1414,6 +1475,7 @@ __device__ __forceinline__ int rank_reaching(const ranked_list& l, int n, unsign
 
 template <class T, bool COUNT>
 __global__ __launch_bounds__(SL_THREADS) void k_row_draw(sample_args a, const row_ws* __restrict__ wss, int slices, int shift) {
+  __shared__ double powers[SB_PER];
   __shared__ union {
     seek_shared seek;
     ranked_list two[2];
@@ -1433,36 +1495,24 @@ __global__ __launch_bounds__(SL_THREADS) void k_row_draw(sample_args a, const ro
     }
     return;
   }
-  const row_mass rm = rm_make(best, s, shift);
+  const row_mass rm = rm_make(best, s, shift, powers);
   const int b1 = ws.b1, b2_lo = ws.b2_lo, b2_hi = ws.b2_hi;
   const int n1 = b1 >= 0 && ws.n_list[0] <= SB_CAP ? (int)ws.n_list[0] : -1;
   const int n2 = b2_hi >= b2_lo && ws.n_list[1] <= SB_CAP ? (int)ws.n_list[1] : -1;
   const int which = wave >> 2, t = threadIdx.x & 255;  // (waves 0 - 3: the first list, 4 - 7: the second one)
   unsigned long long e = t;
   if (which < 2 && t < (which == 0 ? n1 : n2)) e = ws.list[which][t];
-  unsigned long long incl = 0, own = 0, m[SEEK_PB], bm[SEEK_PB], c[SEEK_PB], bc[SEEK_PB];
-#pragma unroll
-  for (int i = 0; i < SEEK_PB; ++i) {
-    m[i] = ws.hist_m[threadIdx.x * SEEK_PB + i];
-    c[i] = COUNT ? ws.hist_c[threadIdx.x * SEEK_PB + i] : 0u;
-    bc[i] = 0;
-  }
-  unsigned long long total = scan_bins<SL_THREADS>(m, bm, red64);
+  __syncthreads();
   const unsigned long long most = max(ws.above, (unsigned long long)rm.scale);
   const bool cut_by_count = COUNT && (unsigned long long)s.k < ws.count;
   // the common case - both lists are there and short: four waves each, side by side
   if (!cut_by_count && !rm.greedy && (b1 < 0 || (n1 >= 1 && n1 <= 256)) && n2 >= 1 && n2 <= 256) {
-#pragma unroll
-    for (int i = 0; i < SEEK_PB; ++i) {
-      if ((int)threadIdx.x * SEEK_PB + i == b1) sh.two[0].before = bm[i];
-      if ((int)threadIdx.x * SEEK_PB + i == b2_lo) sh.two[1].before = bm[i];
-    }
     const bool on = which == 1 || (which == 0 && b1 >= 0);
     ranked_list& mine = sh.two[which & 1];
     const int rank = rank_256(e, mine.runs, mine.sorted, t, on);
-    unsigned long long own = 0, cum = 0;
+    unsigned long long own = 0, cum = 0, before = ws.before[which & 1];
     if (on) {  // (this thread's entry, where it belongs)
-      own = rank < (which == 0 ? n1 : n2) ? rm.mass(rm.log2_of(score_of((uint32_t)(e >> 32)))) : 0ull;
+      own = rank < (which == 0 ? n1 : n2) ? rm.mass(rm.t_of(score_of((uint32_t)(e >> 32)))) : 0ull;
       mine.own[rank] = own;
     }
     __syncthreads();
@@ -1472,15 +1522,15 @@ __global__ __launch_bounds__(SL_THREADS) void k_row_draw(sample_args a, const ro
     }
     __syncthreads();
     if (on) {
-      cum += mine.before;
+      cum += before;
 #pragma unroll
       for (int w = 0; w < 3; ++w) cum += w < (wave & 3) ? mine.sum[w] : 0ull;
       mine.cum[t] = cum;
     }
     __syncthreads();
     if (wave != 0) return;
-    unsigned long long kept = total;
-    if (b1 >= 0) kept = sh.two[0].cum[min(rank_reaching(sh.two[0], n1, border_of(s.top_p, total), lane), n1 - 1)];
+    unsigned long long kept = ws.total;
+    if (b1 >= 0) kept = sh.two[0].cum[min(rank_reaching(sh.two[0], n1, border_of(s.top_p, kept), lane), n1 - 1)];
     kept = min(kept, most);
     const int at_rank = min(rank_reaching(sh.two[1], n2, want_of(a.u[r * a.ld_u], kept), lane), n2 - 1);
     if (lane == 0) {
@@ -1491,6 +1541,14 @@ __global__ __launch_bounds__(SL_THREADS) void k_row_draw(sample_args a, const ro
     }
     return;
   }
+  unsigned long long incl = 0, own = 0, m[SEEK_PB], bm[SEEK_PB], c[SEEK_PB], bc[SEEK_PB];
+#pragma unroll
+  for (int i = 0; i < SEEK_PB; ++i) {
+    m[i] = ws.hist_m[threadIdx.x * SEEK_PB + i];
+    c[i] = COUNT ? ws.hist_c[threadIdx.x * SEEK_PB + i] : 0u;
+    bc[i] = 0;
+  }
+  unsigned long long total = scan_bins<SL_THREADS>(m, bm, red64);
   if (cut_by_count) {
     scan_bins<SL_THREADS>(c, bc, red64);
     seek<T>(p, s.len, rm, m, bm, c, bc, true, (unsigned long long)s.k, sh.seek, nullptr, -1, 0, -1, &incl, &own);
@@ -1599,7 +1657,15 @@ extern "C" int rphip_sample(rphip_ctx* ctx, void* stream, int64_t rows, int64_t 
             RP_LAUNCHED();
             k_row_hist<T, COUNT><<<dim3(n, slices), SR_THREADS, 0, st>>>(a, ws, shift);
             RP_LAUNCHED();
-            k_row_collect<T, COUNT><<<dim3(n, slices), SR_THREADS, 0, st>>>(a, ws, slices, shift);
+            // few rows, or one slice a row: a launch (3 - 4 us) costs more than finding the bins in every slice (one row of 100000: 25.6 us
+            // against 28.4; 512 of 2000: 39 against 46; but 128 rows of 100000 95 against 85)
+            if (n <= 8 || slices == 1) {
+              k_row_collect<T, COUNT, true><<<dim3(n, slices), SR_THREADS, 0, st>>>(a, ws, slices, shift);
+            } else {
+              k_row_bins<COUNT><<<n, SL_THREADS, 0, st>>>(a, ws, shift);
+              RP_LAUNCHED();
+              k_row_collect<T, COUNT, false><<<dim3(n, slices), SR_THREADS, 0, st>>>(a, ws, slices, shift);
+            }
             RP_LAUNCHED();
             k_row_draw<T, COUNT><<<n, SL_THREADS, 0, st>>>(a, ws, slices, shift);
             RP_LAUNCHED();
