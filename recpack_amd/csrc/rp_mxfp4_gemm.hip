@@ -470,6 +470,199 @@ __global__ __launch_bounds__(256) void k_mxg_rows(const T* __restrict__ a, int64
     }
 }
 
+// ---- small products ------------------------------------------------------------------------------------------------------------------
+// One launch, no workspace: a workgroup takes 16 x 64 of C (4-bit A: 32 x 32), its eight waves every eighth chunk of K each, operands from memory into registers
+// as a lane hands them to the matrix instruction (A cut or its scales taken there), a chunk ahead; the waves' sums are joined in LDS
+// in wave order.  A is read once per tile column and W once per tile row, so this is for products whose time is launches and latency.
+constexpr int SD_WAVES = 8;
+constexpr int sd_tm(int planes) { return planes ? 1 : 2; }  // (cutting A is most of the work: 16 rows of A to 64 of W)
+constexpr int sd_tn(int planes) { return planes ? 4 : 2; }
+
+typedef unsigned int u32x2 __attribute__((ext_vector_type(2)));
+__device__ __forceinline__ void swap16(uint32_t& x, uint32_t& y) {
+  const u32x2 r = __builtin_amdgcn_permlane16_swap(x, y, false, false);
+  x = r.x, y = r.y;
+}
+__device__ __forceinline__ void swap32(uint32_t& x, uint32_t& y) {
+  const u32x2 r = __builtin_amdgcn_permlane32_swap(x, y, false, false);
+  x = r.x, y = r.y;
+}
+// eight elements to planes; one with an infinity or a NaN among them (in any lane) the careful way
+template <int P>
+__device__ __forceinline__ void cut8(const float (&v)[8], bf16x8 (&out)[P]) {
+  uint32_t top = 0;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) top = max(top, __float_as_uint(v[e]) << 1);
+  i32x4 q[P];
+  if (__any(top >= 0xff000000u)) {
+    uint16_t h[8][P];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) cut_planes<P>(v[e], h[e]);
+#pragma unroll
+    for (int pl = 0; pl < P; ++pl)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) q[pl][e] = (int)(h[2 * e][pl] | (uint32_t)h[2 * e + 1][pl] << 16);
+  } else {
+    float r[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) r[e] = v[e];
+#pragma unroll
+    for (int pl = 0; pl < P; ++pl) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) q[pl][e] = (int)__builtin_amdgcn_perm(__float_as_uint(r[2 * e + 1]), __float_as_uint(r[2 * e]), 0x07060302u);  // (the high halves)
+      if (pl + 1 < P) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) r[e] -= __uint_as_float(__float_as_uint(r[e]) & 0xffff0000u);
+      }
+    }
+  }
+#pragma unroll
+  for (int pl = 0; pl < P; ++pl) out[pl] = __builtin_bit_cast(bf16x8, q[pl]);
+}
+template <class T, class OT, int P>
+__global__ __launch_bounds__(64 * SD_WAVES) void k_mxg_direct(const T* __restrict__ a, int64_t lda, const uint8_t* __restrict__ as, int64_t ldas, int M, int N, int K, int nb,
+                                                              const uint8_t* __restrict__ w, int64_t ldw, const uint8_t* __restrict__ ws, int64_t ldws, OT* __restrict__ c,
+                                                              int64_t ldc, int gx) {
+  constexpr int TM = sd_tm(P), TN = sd_tn(P);
+  __shared__ f32x4 part[SD_WAVES][TM * TN][64];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), fr = lane & 15, fg = lane >> 4;
+  const int m0 = (int)(blockIdx.x / gx) * TM * 16, n0 = (int)(blockIdx.x % gx) * TN * 16, nc = (nb + 3) / 4;
+  const T* ap[TM];
+  const uint8_t* asp[TM];
+  const uint8_t* wp[TN];
+  const uint8_t* wsp[TN];
+#pragma unroll
+  for (int i = 0; i < TM; ++i) {  // (rows past the matrices: the last one again; not stored)
+    const int64_t m = min(m0 + i * 16 + fr, M - 1);
+    ap[i] = a + m * lda;
+    if (P == 0) asp[i] = as + m * ldas;
+  }
+#pragma unroll
+  for (int j = 0; j < TN; ++j) {
+    const int64_t n = min(n0 + j * 16 + fr, N - 1);
+    wp[j] = w + n * ldw;
+    wsp[j] = ws + n * ldws;
+  }
+  f32x4 acc[TM][TN];
+#pragma unroll
+  for (int i = 0; i < TM; ++i)
+#pragma unroll
+    for (int j = 0; j < TN; ++j) acc[i][j] = f32x4{0, 0, 0, 0};
+  rp_vec<T, 8> av[2][TM][P > 0 ? 4 : 1];
+  uint4 aq[2][TM], wq[2][TN];
+  uint32_t sa[2][TM], sw[2][TN];
+  auto fetch = [&](auto tag, int ch) __attribute__((always_inline)) {
+    constexpr int S = decltype(tag)::value;
+    const int b = ch * 4 + fg, bb = min(b, nb - 1);  // (a block past the row: scale 2^-127 meets zeros of A, or its like)
+#pragma unroll
+    for (int j = 0; j < TN; ++j) {
+      wq[S][j] = *(const uint4*)(wp[j] + (int64_t)bb * 16);
+      sw[S][j] = b < nb ? wsp[j][bb] : 0u;
+    }
+#pragma unroll
+    for (int i = 0; i < TM; ++i) {
+      if constexpr (P == 0) {
+        aq[S][i] = *(const uint4*)(ap[i] + (int64_t)bb * 16);
+        sa[S][i] = b < nb ? asp[i][bb] : 0u;
+      } else {
+#pragma unroll
+        for (int s = 0; s < 4; ++s) {
+          const int64_t k = (int64_t)ch * KC + s * 32 + fg * 8;
+          if (k + 8 <= K) av[S][i][s] = rp_load_vec<T, 8>(ap[i] + k);
+          else {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) av[S][i][s].v[e] = k + e < K ? ap[i][k + e] : (T)0.0f;
+          }
+        }
+      }
+    }
+  };
+  auto add = [&](auto tag) __attribute__((always_inline)) {
+    constexpr int S = decltype(tag)::value;
+    if constexpr (P == 0) {
+#pragma unroll
+      for (int j = 0; j < TN; ++j) {
+        const i32x8 wf = {(int)wq[S][j].x, (int)wq[S][j].y, (int)wq[S][j].z, (int)wq[S][j].w, 0, 0, 0, 0};
+#pragma unroll
+        for (int i = 0; i < TM; ++i) {
+          const i32x8 af = {(int)aq[S][i].x, (int)aq[S][i].y, (int)aq[S][i].z, (int)aq[S][i].w, 0, 0, 0, 0};
+          acc[i][j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(wf, af, acc[i][j], 4, 4, 0, (int)sw[S][j], 0, (int)sa[S][i]);
+        }
+      }
+    } else {
+      // step s takes the elements 32 s + 8 g .. of the chunk (A's loads then share lines): of W, dword g of block s, which lane group s holds
+      uint32_t wd[TN][4], sc[TN][4];
+#pragma unroll
+      for (int j = 0; j < TN; ++j) {
+        wd[j][0] = wq[S][j].x, wd[j][1] = wq[S][j].y, wd[j][2] = wq[S][j].z, wd[j][3] = wq[S][j].w;
+        swap16(wd[j][0], wd[j][1]);
+        swap16(wd[j][2], wd[j][3]);
+        swap32(wd[j][0], wd[j][2]);
+        swap32(wd[j][1], wd[j][3]);
+        sc[j][0] = sc[j][1] = sw[S][j] << 23;
+        swap16(sc[j][0], sc[j][1]);
+        sc[j][2] = sc[j][0], sc[j][3] = sc[j][1];
+        swap32(sc[j][0], sc[j][2]);
+        swap32(sc[j][1], sc[j][3]);
+      }
+#pragma unroll
+      for (int s = 0; s < 4; ++s) {
+        bf16x8 wf[TN];
+#pragma unroll
+        for (int j = 0; j < TN; ++j) wf[j] = codes_bf16(wd[j][s], __uint_as_float(sc[j][s]));
+#pragma unroll
+        for (int i = 0; i < TM; ++i) {
+          float v[8];
+#pragma unroll
+          for (int e = 0; e < 8; ++e) v[e] = rp_to_f32(av[S][i][s].v[e]);
+          bf16x8 af[P];
+          cut8<P>(v, af);
+#pragma unroll
+          for (int pl = 0; pl < P; ++pl)
+#pragma unroll
+            for (int j = 0; j < TN; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(wf[j], af[pl], acc[i][j], 0, 0, 0);
+        }
+      }
+    }
+  };
+  using set0 = std::integral_constant<int, 0>;
+  using set1 = std::integral_constant<int, 1>;
+  int ch = wave;
+  if (ch < nc) {
+    fetch(set0{}, ch);
+    for (; ch < nc; ch += 2 * SD_WAVES) {
+      fetch(set1{}, min(ch + SD_WAVES, nc - 1));
+      add(set0{});
+      if (ch + SD_WAVES >= nc) break;
+      fetch(set0{}, min(ch + 2 * SD_WAVES, nc - 1));
+      add(set1{});
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < TM; ++i)
+#pragma unroll
+    for (int j = 0; j < TN; ++j) part[wave][i * TN + j][lane] = acc[i][j];
+  __syncthreads();
+  // a lane holds four neighbouring columns n of one row m
+  if (wave >= TM * TN) return;
+  f32x4 t = part[0][wave][lane];
+#pragma unroll
+  for (int q = 1; q < SD_WAVES; ++q) t += part[q][wave][lane];
+  const int m = m0 + wave / TN * 16 + fr, n = n0 + wave % TN * 16 + fg * 4;
+  if (m >= M) return;
+  OT* o = c + (int64_t)m * ldc + n;
+  if (n + 4 <= N) {
+    rp_vec<OT, 4> v;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v.v[e] = rp_from_f32<OT>(t[e]);
+    rp_store_vec<OT, 4>(o, v);
+  } else {
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      if (n + e < N) o[e] = rp_from_f32<OT>(t[e]);
+  }
+}
+
 // split K: the parts in order, one rounding
 template <class OT>
 __global__ __launch_bounds__(256) void k_mxg_join(const float* __restrict__ part, int split, int M, int N, OT* __restrict__ c, int64_t ldc) {
@@ -482,7 +675,8 @@ __global__ __launch_bounds__(256) void k_mxg_join(const float* __restrict__ part
 
 struct plan {
   int planes = 0, split = 1, nc = 0, nq = 0;
-  bool rows = false;  // few rows of A: k_mxg_rows
+  bool rows = false;    // few rows of A: k_mxg_rows
+  bool direct = false;  // small: k_mxg_direct
   int bm = 16, bn = 64;
   int64_t plane_bytes = 0, a_scale_bytes = 0, w_scale_bytes = 0, part_bytes = 0;
   int64_t total() const { return plane_bytes + a_scale_bytes + w_scale_bytes + part_bytes; }
@@ -497,6 +691,12 @@ plan make_plan(int n_cu, int64_t M, int64_t N, int64_t K, int32_t a_type) {
   // the vector unit's form: f32 105 us against 120 at M = 4, 16 bits 63 against 91 at M = 2 (but 110 at 4)
   p.rows = p.planes != 0 && M <= (p.planes == 3 ? 4 : 2) && K > 0;
   if (p.rows) return p;
+  // small products, by tiles and by what a tile's latency comes to: f32 97 x 1999 x 2003 13.7 us against 20.2, bf16 256 x 2000 x 2000 16.5
+  // against 17.6; but bf16 64 x 2000 x 8000 26 against 21, 128 x 4000 x 4000 32 against 22, 1000 x 1000 x 1000 29 against 18.  4-bit (with
+  // A's quantising): 1000 x 1000 x 1000 24 against 28, 16 x 16000 x 8000 25 against 28; but 300 x 8000 x 1000 41 against 27.
+  const int64_t small = rp_cdiv(M, 16 * sd_tm(p.planes)) * rp_cdiv(N, 16 * sd_tn(p.planes)), latency = small * (p.nc + 8);
+  p.direct = K > 0 && (p.planes ? small <= 2 * n_cu && p.nc <= 32 && latency <= 48 * n_cu : p.nc <= 128 && latency <= 140 * n_cu);
+  if (p.direct) return p;
   auto tiles = [&](int bm, int bn) { return std::max<int64_t>(rp_cdiv(M, bm) * rp_cdiv(N, bn), 1); };
   auto rounds = [&](int bm, int bn, int per_cu) { return rp_cdiv(tiles(bm, bn), per_cu * n_cu); };
   if (p.planes) {
@@ -612,6 +812,23 @@ extern "C" int rphip_mxfp4_gemm_nt(rphip_ctx* ctx, void* stream, int64_t M, int6
         return RPHIP_OK;
       });
     });
+  if (p.direct) {
+    const int gx = (int)rp_cdiv(N, 16 * sd_tn(p.planes));
+    const unsigned grid = (unsigned)(gx * rp_cdiv(M, 16 * sd_tm(p.planes)));
+    return rp_by_type(c_type, [&](auto ct) -> int {
+      using OT = typename decltype(ct)::T;
+      auto go = [&](auto kernel, auto type) {
+        kernel<<<grid, 64 * SD_WAVES, 0, st>>>((const decltype(type)*)A_dev, lda, a_scales_dev, ld_a_scales, (int)M, (int)N, (int)K, g.nb, w_codes_dev, ld_w, w_scales_dev, ld_w_scales,
+                                               (OT*)C_dev, ldc, gx);
+      };
+      if (a_type == RPHIP_BF16) go(k_mxg_direct<__bf16, OT, 1>, __bf16{});
+      else if (a_type == RPHIP_F16) go(k_mxg_direct<_Float16, OT, 2>, _Float16{});
+      else if (a_type == RPHIP_F32) go(k_mxg_direct<float, OT, 3>, 0.0f);
+      else go(k_mxg_direct<uint8_t, OT, 0>, uint8_t{0});
+      RP_LAUNCHED();
+      return RPHIP_OK;
+    });
+  }
   if (p.nc) {
     const int64_t w_units = rp_cdiv(N, 16) * p.nq * 64, wg_w = rp_cdiv(w_units, 256);
     const int64_t a_units = p.planes ? rp_cdiv(M, 16) * p.nc : rp_cdiv(M, 16) * p.nq * 64, wg_a = p.planes ? a_units : rp_cdiv(a_units, 256);

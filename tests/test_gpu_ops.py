@@ -484,7 +484,9 @@ def values_gpu(ops, ctx, m):
     (torch.bfloat16, 2050, 8200, 257), (torch.float16, 2050, 8200, 90),                                     # 256 x 256
     (torch.bfloat16, 130, 20001, 8100), (torch.float32, 200, 9001, 4000),                                   # 128 x 128, K in parts
     (torch.bfloat16, 33, 3001, 6000), (torch.float16, 64, 999, 9000), (torch.float32, 9, 2000, 5001), (torch.float32, 4, 5003, 7001),
-    ("mxfp4", 4000, 4200, 300), ("mxfp4", 600, 3001, 1000), ("mxfp4", 200, 1999, 5000), ("mxfp4", 20, 700, 9000)])
+    ("mxfp4", 4000, 4200, 300), ("mxfp4", 600, 3001, 1000), ("mxfp4", 200, 1999, 5000), ("mxfp4", 20, 700, 9000),
+    ("mxfp4", 20, 40001, 3000), ("mxfp4", 300, 8001, 2000), ("mxfp4", 1000, 8000, 3000), ("mxfp4", 500, 3001, 5000), ("mxfp4", 90, 1501, 17000),
+    (torch.bfloat16, 16, 2001, 4200), (torch.float16, 300, 5003, 1000), (torch.float32, 40, 4001, 4096), (torch.bfloat16, 500, 1001, 3999)])
 def test_product_large(ctx, ops, dtype, m, n, k):
     g = torch.Generator(device="cuda").manual_seed(m + n + k)
     a = torch.randn(m, k, device="cuda", generator=g)
