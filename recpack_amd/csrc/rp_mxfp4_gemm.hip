@@ -2,8 +2,11 @@
 // C ABI: include/recpack_hip.h, rphip_mxfp4_gemm_nt.
 //
 // 16- and 32-bit A: every element of W is a bf16 number exactly (two significant bits times a power of two), and every element of A a
-// sum of one (bf16), two (f16: 8 + 3 bits) or three (f32: 8 + 8 + 8 bits) of them, so the product runs on v_mfma_f32_16x16x32_bf16
-// with exact operands; the planes of A are cut once into a workspace, W is converted in registers.
+// sum of one (bf16) or three (f32: 8 + 8 + 8 bits) of them, so the product runs on v_mfma_f32_16x16x32_bf16 with exact operands; the
+// planes of A are cut once into a workspace, W is converted in registers.  f16 A runs on v_mfma_f32_16x16x32_f16 as it is: a row of W
+// relative to the power of two of its largest block is a row of f16 numbers exactly as long as its blocks' scales lie within 2^36 of each other
+// (subnormals included), and its sums are scaled back as they are stored.  Rows of W that span more are found beforehand and their part
+// of C is computed again with f16 as two bf16 planes (8 + 3 bits).
 // MXFP4 A: v_mfma_scale_f32_16x16x128_f8f6f4, which takes codes and scales as they are.
 #include "rp_ops.h"
 
@@ -13,6 +16,8 @@
 namespace {
 
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef int i32x8 __attribute__((ext_vector_type(8)));
 typedef int i32x4 __attribute__((ext_vector_type(4)));
@@ -62,7 +67,10 @@ __device__ __forceinline__ void cut_fragment(const T* __restrict__ a, int64_t ld
   }
   uint16_t h[8][P];
 #pragma unroll
-  for (int i = 0; i < 8; ++i) cut_planes<P>(v[i], h[i]);
+  for (int i = 0; i < 8; ++i) {
+    if constexpr (std::is_same<T, _Float16>::value) h[i][0] = __builtin_bit_cast(uint16_t, (_Float16)v[i]);  // (as it is: P = 1)
+    else cut_planes<P>(v[i], h[i]);
+  }
   uint4* o = (uint4*)(out + (frag * P * 4 + s) * 512) + lane;
 #pragma unroll
   for (int pl = 0; pl < P; ++pl) {
@@ -90,11 +98,60 @@ __device__ __forceinline__ void pack_scales(const uint8_t* __restrict__ s, int64
   out[unit] = w;
 }
 
+// The same for W beside f16 A, a workgroup to 16 rows: scales relative to the row's largest one, which becomes 2^HALF_TOP (6 * 2^13 is an f16
+// number); top[] keeps the largest, wide[block] says whether a row has an element that f16 does not hold then.
+constexpr int HALF_TOP = 13, HALF_SPAN = 36;  // (.5 * 2^(13 - 36) = 2^-24, the least f16 number)
+__device__ __forceinline__ void pack_scales_half(const uint8_t* __restrict__ s, int64_t lds, const uint8_t* __restrict__ codes, int64_t ldc, int rows, int nb, int nq, int64_t rb,
+                                                 uint32_t* __restrict__ out, uint8_t* __restrict__ top, uint8_t* __restrict__ wide) {
+  __shared__ uint32_t best[16], lost;
+  const int t = threadIdx.x, row = t >> 4;
+  if (t < 16) best[t] = 0;
+  if (t == 0) lost = 0;
+  __syncthreads();
+  const int64_t r = min(rb * 16 + row, (int64_t)rows - 1);
+  uint32_t m = 0;
+  for (int b = t & 15; b < nb; b += 16) {
+    const uint32_t v = s[r * lds + b];
+    m = max(m, v == 255u ? 0u : v);
+  }
+  atomicMax(&best[row], m);
+  __syncthreads();
+  for (int u = t; u < nq * 64; u += 256) {
+    const int lane = u & 63, b = (u >> 6) * 16 + (lane >> 4);
+    const int64_t rr = min(rb * 16 + (lane & 15), (int64_t)rows - 1);
+    const int e = (int)best[lane & 15];
+    uint32_t w = 0;
+#pragma unroll
+    for (int cc = 0; cc < 4; ++cc) {
+      if (b + cc * 4 >= nb) break;
+      const int v = s[rr * lds + b + cc * 4], span = e - v;
+      if (v != 255 && span > HALF_SPAN) {
+        const uint4 q = *(const uint4*)(codes + rr * ldc + (int64_t)(b + cc * 4) * 16);
+        if (((q.x | q.y | q.z | q.w) & 0x77777777u) != 0) lost = 1;  // (blocks of zeros lose nothing; codes behind the last column are 0)
+      }
+      w |= (uint32_t)(v == 255 ? 255 : max(127 + HALF_TOP - span, 0)) << (8 * cc);
+    }
+    out[rb * nq * 64 + u] = w;
+  }
+  __syncthreads();
+  if (t < 16) top[rb * 16 + t] = (uint8_t)best[t];
+  if (t == 0) wide[rb] = (uint8_t)lost;
+}
+
 // One launch for all of them: workgroups [0, wg_w) pack W's scales, the others cut A (P > 0) or pack A's scales.
+struct half_args {  // (f16 A only)
+  const uint8_t* codes;
+  int64_t ldc;
+  uint8_t *top, *wide;
+};
 template <class T, int P>
 __global__ __launch_bounds__(256) void k_mxg_prepare(const uint8_t* __restrict__ ws, int64_t ldws, int N, int nb, int nq, int64_t w_units, uint32_t* __restrict__ w_out,
-                                                     unsigned wg_w, const T* __restrict__ a, int64_t lda, int M, int K, int nc, int64_t a_units, void* __restrict__ a_out) {
+                                                     unsigned wg_w, const T* __restrict__ a, int64_t lda, int M, int K, int nc, int64_t a_units, void* __restrict__ a_out, half_args half) {
   if (blockIdx.x < wg_w) {
+    if constexpr (std::is_same<T, _Float16>::value) {
+      pack_scales_half(ws, ldws, half.codes, half.ldc, N, nb, nq, blockIdx.x, w_out, half.top, half.wide);
+      return;
+    }
     const int64_t unit = (int64_t)blockIdx.x * 256 + threadIdx.x;
     if (unit < w_units) pack_scales(ws, ldws, N, nb, nq, unit, w_out);
     return;
@@ -116,11 +173,18 @@ __device__ __forceinline__ bf16x8 codes_bf16(uint32_t w, float s) {
   return r;
 }
 
+__device__ __forceinline__ f16x8 codes_f16(uint32_t w, float s) {
+  const f16x2 a = __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, s, 0), b = __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, s, 1);
+  const f16x2 c = __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, s, 2), d = __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, s, 3);
+  return f16x8{a.x, a.y, b.x, b.y, c.x, c.y, d.x, d.y};
+}
+
 struct gemm_args {
   int M, N, nb, nc, nq;      // nb: blocks of a row of W (and of an MXFP4 A); nc: chunks; nq: groups of four chunks
   const uint8_t* planes;     // 16-bit form of A
   const uint8_t* a_codes; int64_t lda; const uint32_t* a_scales;  // MXFP4 A (scales in the workspace form)
   const uint8_t* w; int64_t ldw; const uint32_t* w_scales;
+  const uint8_t* w_top;      // f16 A: the largest scale of each row of W (padded to 16 rows)
   void* c; int64_t ldc;
   float* part;               // split K: partial sums [split][M][N]
   int split;
@@ -155,9 +219,20 @@ __device__ __forceinline__ void wait_loads_and_meet() {
 }
 
 // D = W fragment x A fragment: a lane holds four neighbouring columns n of one row m.
-template <class OT, int TM, int TN>
-__device__ __forceinline__ void store_tile(const gemm_args& g, const f32x4 (&acc)[TM][TN], int m0, int n0, int lane) {
+template <class OT, int TM, int TN, bool HALF = false>
+__device__ __forceinline__ void store_tile(const gemm_args& g, f32x4 (&acc)[TM][TN], int m0, int n0, int lane) {
   const int z = blockIdx.y;
+  if constexpr (HALF) {
+#pragma unroll
+    for (int j = 0; j < TN; ++j) {
+      const int n = n0 + j * 16 + (lane >> 4) * 4;
+      const uint32_t top = n < g.N ? *(const uint32_t*)(g.w_top + n) : 0u;
+#pragma unroll
+      for (int i = 0; i < TM; ++i)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc[i][j][e] = ldexpf(acc[i][j][e], (int)((top >> (8 * e)) & 255u) - 127 - HALF_TOP);
+    }
+  }
 #pragma unroll
   for (int i = 0; i < TM; ++i) {
     const int m = m0 + i * 16 + (lane & 15);
@@ -199,7 +274,7 @@ __device__ __forceinline__ void store_tile(const gemm_args& g, const f32x4 (&acc
 // 16-bit form.  Tile BM x BN, WM x WN waves.  A in a ring of three stages, each the half of a plane of a chunk (two of its four steps),
 // requested two stages ahead; W's codes and scales in two slots, a chunk ahead, converted in registers once per plane and wave (4 conversions
 // per 8 codes against TM matrix instructions that use them).
-template <class OT, int P, int BM, int BN, int WM, int WN>
+template <class OT, int P, bool HALF, int BM, int BN, int WM, int WN>
 __global__ __launch_bounds__(WM * WN * 64) void k_mxg_bf16(gemm_args g) {
   constexpr int WAVES = WM * WN, TM = BM / WM / 16, TN = BN / WN / 16, RING = 3;
   constexpr int STAGE = BM * 128, D = BM / 8 / WAVES;                // A: bytes of a stage, KB a wave requests of it
@@ -271,14 +346,21 @@ __global__ __launch_bounds__(WM * WN * 64) void k_mxg_bf16(gemm_args g) {
         const uint8_t* st = ring + stage * STAGE + lane * 16;
 #pragma unroll
         for (int s = 0; s < 2; ++s) {
-          bf16x8 wf[TN];
+          using frag = typename std::conditional<HALF, f16x8, bf16x8>::type;
+          frag wf[TN];
 #pragma unroll
-          for (int j = 0; j < TN; ++j) wf[j] = codes_bf16((uint32_t)wq[j][h * 2 + s], __uint_as_float(sc[j]));
+          for (int j = 0; j < TN; ++j) {
+            if constexpr (HALF) wf[j] = codes_f16((uint32_t)wq[j][h * 2 + s], __uint_as_float(sc[j]));
+            else wf[j] = codes_bf16((uint32_t)wq[j][h * 2 + s], __uint_as_float(sc[j]));
+          }
 #pragma unroll
           for (int i = 0; i < TM; ++i) {
-            const bf16x8 af = *(const bf16x8*)(st + ((wm + i) * 2 + s) * 1024);
+            const frag af = *(const frag*)(st + ((wm + i) * 2 + s) * 1024);
 #pragma unroll
-            for (int j = 0; j < TN; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(wf[j], af, acc[i][j], 0, 0, 0);
+            for (int j = 0; j < TN; ++j) {
+              if constexpr (HALF) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(wf[j], af, acc[i][j], 0, 0, 0);
+              else acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(wf[j], af, acc[i][j], 0, 0, 0);
+            }
           }
         }
         stage = stage == 2 ? 0 : stage + 1;
@@ -286,7 +368,7 @@ __global__ __launch_bounds__(WM * WN * 64) void k_mxg_bf16(gemm_args g) {
     }
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // (the trailing requests write LDS)
   }
-  store_tile<OT, TM, TN>(g, acc, m0 + wm * 16, tn * BN + wn * 16, lane);
+  store_tile<OT, TM, TN, HALF>(g, acc, m0 + wm * 16, tn * BN + wn * 16, lane);
 }
 
 // 4-bit form: codes of both operands in two slots, a stage (two chunks of both) ahead; scales in two slots of four chunks.  A piece is
@@ -522,144 +604,153 @@ __device__ __forceinline__ void cut8(const float (&v)[8], bf16x8 (&out)[P]) {
 template <class T, class OT, int P>
 __global__ __launch_bounds__(64 * SD_WAVES) void k_mxg_direct(const T* __restrict__ a, int64_t lda, const uint8_t* __restrict__ as, int64_t ldas, int M, int N, int K, int nb,
                                                               const uint8_t* __restrict__ w, int64_t ldw, const uint8_t* __restrict__ ws, int64_t ldws, OT* __restrict__ c,
-                                                              int64_t ldc, int gx) {
+                                                              int64_t ldc, const uint8_t* __restrict__ wide) {
   constexpr int TM = sd_tm(P), TN = sd_tn(P);
   __shared__ f32x4 part[SD_WAVES][TM * TN][64];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), fr = lane & 15, fg = lane >> 4;
-  const int m0 = (int)(blockIdx.x / gx) * TM * 16, n0 = (int)(blockIdx.x % gx) * TN * 16, nc = (nb + 3) / 4;
-  const T* ap[TM];
-  const uint8_t* asp[TM];
-  const uint8_t* wp[TN];
-  const uint8_t* wsp[TN];
+  const int n0 = (int)blockIdx.x * TN * 16, nc = (nb + 3) / 4;
+  if (wide) {  // (f16 A, after the product: only columns that f16 does not hold)
+    bool any = false;
 #pragma unroll
-  for (int i = 0; i < TM; ++i) {  // (rows past the matrices: the last one again; not stored)
-    const int64_t m = min(m0 + i * 16 + fr, M - 1);
-    ap[i] = a + m * lda;
-    if (P == 0) asp[i] = as + m * ldas;
+    for (int j = 0; j < TN; ++j) any = any || (n0 + j * 16 < N && wide[n0 / 16 + j] != 0);
+    if (!any) return;
   }
+  for (int m0 = (int)blockIdx.y * TM * 16; m0 < M; m0 += (int)gridDim.y * TM * 16) {
+    const T* ap[TM];
+    const uint8_t* asp[TM];
+    const uint8_t* wp[TN];
+    const uint8_t* wsp[TN];
 #pragma unroll
-  for (int j = 0; j < TN; ++j) {
-    const int64_t n = min(n0 + j * 16 + fr, N - 1);
-    wp[j] = w + n * ldw;
-    wsp[j] = ws + n * ldws;
-  }
-  f32x4 acc[TM][TN];
-#pragma unroll
-  for (int i = 0; i < TM; ++i)
-#pragma unroll
-    for (int j = 0; j < TN; ++j) acc[i][j] = f32x4{0, 0, 0, 0};
-  rp_vec<T, 8> av[2][TM][P > 0 ? 4 : 1];
-  uint4 aq[2][TM], wq[2][TN];
-  uint32_t sa[2][TM], sw[2][TN];
-  auto fetch = [&](auto tag, int ch) __attribute__((always_inline)) {
-    constexpr int S = decltype(tag)::value;
-    const int b = ch * 4 + fg, bb = min(b, nb - 1);  // (a block past the row: scale 2^-127 meets zeros of A, or its like)
-#pragma unroll
-    for (int j = 0; j < TN; ++j) {
-      wq[S][j] = *(const uint4*)(wp[j] + (int64_t)bb * 16);
-      sw[S][j] = b < nb ? wsp[j][bb] : 0u;
+    for (int i = 0; i < TM; ++i) {  // (rows past the matrices: the last one again; not stored)
+      const int64_t m = min(m0 + i * 16 + fr, M - 1);
+      ap[i] = a + m * lda;
+      if (P == 0) asp[i] = as + m * ldas;
     }
 #pragma unroll
-    for (int i = 0; i < TM; ++i) {
-      if constexpr (P == 0) {
-        aq[S][i] = *(const uint4*)(ap[i] + (int64_t)bb * 16);
-        sa[S][i] = b < nb ? asp[i][bb] : 0u;
-      } else {
+    for (int j = 0; j < TN; ++j) {
+      const int64_t n = min(n0 + j * 16 + fr, N - 1);
+      wp[j] = w + n * ldw;
+      wsp[j] = ws + n * ldws;
+    }
+    f32x4 acc[TM][TN];
 #pragma unroll
-        for (int s = 0; s < 4; ++s) {
-          const int64_t k = (int64_t)ch * KC + s * 32 + fg * 8;
-          if (k + 8 <= K) av[S][i][s] = rp_load_vec<T, 8>(ap[i] + k);
-          else {
+    for (int i = 0; i < TM; ++i)
 #pragma unroll
-            for (int e = 0; e < 8; ++e) av[S][i][s].v[e] = k + e < K ? ap[i][k + e] : (T)0.0f;
+      for (int j = 0; j < TN; ++j) acc[i][j] = f32x4{0, 0, 0, 0};
+    rp_vec<T, 8> av[2][TM][P > 0 ? 4 : 1];
+    uint4 aq[2][TM], wq[2][TN];
+    uint32_t sa[2][TM], sw[2][TN];
+    auto fetch = [&](auto tag, int ch) __attribute__((always_inline)) {
+      constexpr int S = decltype(tag)::value;
+      const int b = ch * 4 + fg, bb = min(b, nb - 1);  // (a block past the row: scale 2^-127 meets zeros of A, or its like)
+#pragma unroll
+      for (int j = 0; j < TN; ++j) {
+        wq[S][j] = *(const uint4*)(wp[j] + (int64_t)bb * 16);
+        sw[S][j] = b < nb ? wsp[j][bb] : 0u;
+      }
+#pragma unroll
+      for (int i = 0; i < TM; ++i) {
+        if constexpr (P == 0) {
+          aq[S][i] = *(const uint4*)(ap[i] + (int64_t)bb * 16);
+          sa[S][i] = b < nb ? asp[i][bb] : 0u;
+        } else {
+#pragma unroll
+          for (int s = 0; s < 4; ++s) {
+            const int64_t k = (int64_t)ch * KC + s * 32 + fg * 8;
+            if (k + 8 <= K) av[S][i][s] = rp_load_vec<T, 8>(ap[i] + k);
+            else {
+#pragma unroll
+              for (int e = 0; e < 8; ++e) av[S][i][s].v[e] = k + e < K ? ap[i][k + e] : (T)0.0f;
+            }
           }
         }
       }
-    }
-  };
-  auto add = [&](auto tag) __attribute__((always_inline)) {
-    constexpr int S = decltype(tag)::value;
-    if constexpr (P == 0) {
+    };
+    auto add = [&](auto tag) __attribute__((always_inline)) {
+      constexpr int S = decltype(tag)::value;
+      if constexpr (P == 0) {
 #pragma unroll
-      for (int j = 0; j < TN; ++j) {
-        const i32x8 wf = {(int)wq[S][j].x, (int)wq[S][j].y, (int)wq[S][j].z, (int)wq[S][j].w, 0, 0, 0, 0};
+        for (int j = 0; j < TN; ++j) {
+          const i32x8 wf = {(int)wq[S][j].x, (int)wq[S][j].y, (int)wq[S][j].z, (int)wq[S][j].w, 0, 0, 0, 0};
 #pragma unroll
-        for (int i = 0; i < TM; ++i) {
-          const i32x8 af = {(int)aq[S][i].x, (int)aq[S][i].y, (int)aq[S][i].z, (int)aq[S][i].w, 0, 0, 0, 0};
-          acc[i][j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(wf, af, acc[i][j], 4, 4, 0, (int)sw[S][j], 0, (int)sa[S][i]);
+          for (int i = 0; i < TM; ++i) {
+            const i32x8 af = {(int)aq[S][i].x, (int)aq[S][i].y, (int)aq[S][i].z, (int)aq[S][i].w, 0, 0, 0, 0};
+            acc[i][j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(wf, af, acc[i][j], 4, 4, 0, (int)sw[S][j], 0, (int)sa[S][i]);
+          }
+        }
+      } else {
+        // step s takes the elements 32 s + 8 g .. of the chunk (A's loads then share lines): of W, dword g of block s, which lane group s holds
+        uint32_t wd[TN][4], sc[TN][4];
+#pragma unroll
+        for (int j = 0; j < TN; ++j) {
+          wd[j][0] = wq[S][j].x, wd[j][1] = wq[S][j].y, wd[j][2] = wq[S][j].z, wd[j][3] = wq[S][j].w;
+          swap16(wd[j][0], wd[j][1]);
+          swap16(wd[j][2], wd[j][3]);
+          swap32(wd[j][0], wd[j][2]);
+          swap32(wd[j][1], wd[j][3]);
+          sc[j][0] = sc[j][1] = sw[S][j] << 23;
+          swap16(sc[j][0], sc[j][1]);
+          sc[j][2] = sc[j][0], sc[j][3] = sc[j][1];
+          swap32(sc[j][0], sc[j][2]);
+          swap32(sc[j][1], sc[j][3]);
+        }
+#pragma unroll
+        for (int s = 0; s < 4; ++s) {
+          bf16x8 wf[TN];
+#pragma unroll
+          for (int j = 0; j < TN; ++j) wf[j] = codes_bf16(wd[j][s], __uint_as_float(sc[j][s]));
+#pragma unroll
+          for (int i = 0; i < TM; ++i) {
+            float v[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[e] = rp_to_f32(av[S][i][s].v[e]);
+            bf16x8 af[P];
+            cut8<P>(v, af);
+#pragma unroll
+            for (int pl = 0; pl < P; ++pl)
+#pragma unroll
+              for (int j = 0; j < TN; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(wf[j], af[pl], acc[i][j], 0, 0, 0);
+          }
         }
       }
-    } else {
-      // step s takes the elements 32 s + 8 g .. of the chunk (A's loads then share lines): of W, dword g of block s, which lane group s holds
-      uint32_t wd[TN][4], sc[TN][4];
-#pragma unroll
-      for (int j = 0; j < TN; ++j) {
-        wd[j][0] = wq[S][j].x, wd[j][1] = wq[S][j].y, wd[j][2] = wq[S][j].z, wd[j][3] = wq[S][j].w;
-        swap16(wd[j][0], wd[j][1]);
-        swap16(wd[j][2], wd[j][3]);
-        swap32(wd[j][0], wd[j][2]);
-        swap32(wd[j][1], wd[j][3]);
-        sc[j][0] = sc[j][1] = sw[S][j] << 23;
-        swap16(sc[j][0], sc[j][1]);
-        sc[j][2] = sc[j][0], sc[j][3] = sc[j][1];
-        swap32(sc[j][0], sc[j][2]);
-        swap32(sc[j][1], sc[j][3]);
-      }
-#pragma unroll
-      for (int s = 0; s < 4; ++s) {
-        bf16x8 wf[TN];
-#pragma unroll
-        for (int j = 0; j < TN; ++j) wf[j] = codes_bf16(wd[j][s], __uint_as_float(sc[j][s]));
-#pragma unroll
-        for (int i = 0; i < TM; ++i) {
-          float v[8];
-#pragma unroll
-          for (int e = 0; e < 8; ++e) v[e] = rp_to_f32(av[S][i][s].v[e]);
-          bf16x8 af[P];
-          cut8<P>(v, af);
-#pragma unroll
-          for (int pl = 0; pl < P; ++pl)
-#pragma unroll
-            for (int j = 0; j < TN; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(wf[j], af[pl], acc[i][j], 0, 0, 0);
-        }
+    };
+    using set0 = std::integral_constant<int, 0>;
+    using set1 = std::integral_constant<int, 1>;
+    int ch = wave;
+    if (ch < nc) {
+      fetch(set0{}, ch);
+      for (; ch < nc; ch += 2 * SD_WAVES) {
+        fetch(set1{}, min(ch + SD_WAVES, nc - 1));
+        add(set0{});
+        if (ch + SD_WAVES >= nc) break;
+        fetch(set0{}, min(ch + 2 * SD_WAVES, nc - 1));
+        add(set1{});
       }
     }
-  };
-  using set0 = std::integral_constant<int, 0>;
-  using set1 = std::integral_constant<int, 1>;
-  int ch = wave;
-  if (ch < nc) {
-    fetch(set0{}, ch);
-    for (; ch < nc; ch += 2 * SD_WAVES) {
-      fetch(set1{}, min(ch + SD_WAVES, nc - 1));
-      add(set0{});
-      if (ch + SD_WAVES >= nc) break;
-      fetch(set0{}, min(ch + 2 * SD_WAVES, nc - 1));
-      add(set1{});
+#pragma unroll
+    for (int i = 0; i < TM; ++i)
+#pragma unroll
+      for (int j = 0; j < TN; ++j) part[wave][i * TN + j][lane] = acc[i][j];
+    __syncthreads();
+    // a lane holds four neighbouring columns n of one row m
+    const int m = m0 + wave / TN * 16 + fr, n = n0 + wave % TN * 16 + fg * 4;
+    if (wave < TM * TN && m < M) {
+      f32x4 t = part[0][wave][lane];
+#pragma unroll
+      for (int q = 1; q < SD_WAVES; ++q) t += part[q][wave][lane];
+      OT* o = c + (int64_t)m * ldc + n;
+      if (n + 4 <= N) {
+        rp_vec<OT, 4> v;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v.v[e] = rp_from_f32<OT>(t[e]);
+        rp_store_vec<OT, 4>(o, v);
+      } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (n + e < N) o[e] = rp_from_f32<OT>(t[e]);
+      }
     }
-  }
-#pragma unroll
-  for (int i = 0; i < TM; ++i)
-#pragma unroll
-    for (int j = 0; j < TN; ++j) part[wave][i * TN + j][lane] = acc[i][j];
-  __syncthreads();
-  // a lane holds four neighbouring columns n of one row m
-  if (wave >= TM * TN) return;
-  f32x4 t = part[0][wave][lane];
-#pragma unroll
-  for (int q = 1; q < SD_WAVES; ++q) t += part[q][wave][lane];
-  const int m = m0 + wave / TN * 16 + fr, n = n0 + wave % TN * 16 + fg * 4;
-  if (m >= M) return;
-  OT* o = c + (int64_t)m * ldc + n;
-  if (n + 4 <= N) {
-    rp_vec<OT, 4> v;
-#pragma unroll
-    for (int e = 0; e < 4; ++e) v.v[e] = rp_from_f32<OT>(t[e]);
-    rp_store_vec<OT, 4>(o, v);
-  } else {
-#pragma unroll
-    for (int e = 0; e < 4; ++e)
-      if (n + e < N) o[e] = rp_from_f32<OT>(t[e]);
+    __syncthreads();
   }
 }
 
@@ -677,15 +768,17 @@ struct plan {
   int planes = 0, split = 1, nc = 0, nq = 0;
   bool rows = false;    // few rows of A: k_mxg_rows
   bool direct = false;  // small: k_mxg_direct
+  bool half = false;    // f16 A as it is
   int bm = 16, bn = 64;
-  int64_t plane_bytes = 0, a_scale_bytes = 0, w_scale_bytes = 0, part_bytes = 0;
-  int64_t total() const { return plane_bytes + a_scale_bytes + w_scale_bytes + part_bytes; }
+  int64_t plane_bytes = 0, a_scale_bytes = 0, w_scale_bytes = 0, top_bytes = 0, wide_bytes = 0, part_bytes = 0;
+  int64_t total() const { return plane_bytes + a_scale_bytes + w_scale_bytes + top_bytes + wide_bytes + part_bytes; }
 };
 
 // Which tile, and into how many parts K is split: by rounds of workgroups over the CUs.  Measured on W of 20000 x 20000 unless said.
 plan make_plan(int n_cu, int64_t M, int64_t N, int64_t K, int32_t a_type) {
   plan p;
-  p.planes = a_type == RPHIP_BF16 ? 1 : a_type == RPHIP_F16 ? 2 : a_type == RPHIP_F32 ? 3 : 0;
+  p.planes = a_type == RPHIP_BF16 || a_type == RPHIP_F16 ? 1 : a_type == RPHIP_F32 ? 3 : 0;
+  p.half = a_type == RPHIP_F16;
   p.nc = (int)rp_cdiv(K, KC);
   p.nq = (int)rp_cdiv(p.nc, 4);
   // the vector unit's form: f32 105 us against 120 at M = 4, 16 bits 63 against 91 at M = 2 (but 110 at 4)
@@ -728,6 +821,8 @@ plan make_plan(int n_cu, int64_t M, int64_t N, int64_t K, int32_t a_type) {
   p.plane_bytes = room(rp_cdiv(M, 16) * p.nc * p.planes * 4096);
   p.a_scale_bytes = p.planes ? 0 : room(rp_cdiv(M, 16) * p.nq * 256);
   p.w_scale_bytes = room(rp_cdiv(N, 16) * p.nq * 256);
+  p.top_bytes = p.half ? room(rp_cdiv(N, 16) * 16) : 0;
+  p.wide_bytes = p.half ? room(rp_cdiv(N, 16)) : 0;
   p.part_bytes = p.split > 1 ? M * N * 4 * p.split : 0;
   return p;
 }
@@ -748,11 +843,11 @@ int launch_fp4(const gemm_args& g, hipStream_t st) {
   return launch_tiles<BM, BN>(k_mxg_fp4<OT, BM, BN, WM, WN>, g, WM * WN * 64, 2 * (BM + BN) * 128 + 2 * (BM + BN) * 16, st);
 }
 template <class OT, int BM, int BN, int WM, int WN>
-int launch_bf16(const gemm_args& g, int planes, hipStream_t st) {
+int launch_bf16(const gemm_args& g, int planes, bool half, hipStream_t st) {
   constexpr int threads = WM * WN * 64, lds = 3 * BM * 128 + 2 * BN * 64 + 2 * BN * 16;
-  if (planes == 1) return launch_tiles<BM, BN>(k_mxg_bf16<OT, 1, BM, BN, WM, WN>, g, threads, lds, st);
-  if (planes == 2) return launch_tiles<BM, BN>(k_mxg_bf16<OT, 2, BM, BN, WM, WN>, g, threads, lds, st);
-  return launch_tiles<BM, BN>(k_mxg_bf16<OT, 3, BM, BN, WM, WN>, g, threads, lds, st);
+  if (half) return launch_tiles<BM, BN>(k_mxg_bf16<OT, 1, true, BM, BN, WM, WN>, g, threads, lds, st);
+  if (planes == 1) return launch_tiles<BM, BN>(k_mxg_bf16<OT, 1, false, BM, BN, WM, WN>, g, threads, lds, st);
+  return launch_tiles<BM, BN>(k_mxg_bf16<OT, 3, false, BM, BN, WM, WN>, g, threads, lds, st);
 }
 
 int check_sizes(const char* who, int64_t M, int64_t N, int64_t K) {
@@ -797,7 +892,10 @@ extern "C" int rphip_mxfp4_gemm_nt(rphip_ctx* ctx, void* stream, int64_t M, int6
   g.planes = (const uint8_t*)ws;
   g.a_codes = (const uint8_t*)A_dev, g.lda = lda, g.a_scales = (const uint32_t*)(ws + p.plane_bytes);
   g.w = w_codes_dev, g.ldw = ld_w, g.w_scales = (const uint32_t*)(ws + p.plane_bytes + p.a_scale_bytes);
-  g.c = C_dev, g.ldc = ldc, g.part = (float*)(ws + p.plane_bytes + p.a_scale_bytes + p.w_scale_bytes), g.split = p.split;
+  uint8_t* top = (uint8_t*)ws + p.plane_bytes + p.a_scale_bytes + p.w_scale_bytes;
+  uint8_t* wide = top + p.top_bytes;
+  g.w_top = top;
+  g.c = C_dev, g.ldc = ldc, g.part = (float*)(wide + p.wide_bytes), g.split = p.split;
   if (p.rows)
     return rp_by_type(a_type, [&](auto at) -> int {
       return rp_by_type(c_type, [&](auto ct) -> int {
@@ -812,35 +910,34 @@ extern "C" int rphip_mxfp4_gemm_nt(rphip_ctx* ctx, void* stream, int64_t M, int6
         return RPHIP_OK;
       });
     });
-  if (p.direct) {
-    const int gx = (int)rp_cdiv(N, 16 * sd_tn(p.planes));
-    const unsigned grid = (unsigned)(gx * rp_cdiv(M, 16 * sd_tm(p.planes)));
+  // the direct form: the whole product, or (wide) what f16 did not hold
+  auto direct = [&](auto kernel, auto type, auto out, int planes, const uint8_t* flags) -> int {
+    const unsigned gx = (unsigned)rp_cdiv(N, 16 * sd_tn(planes)), gy = (unsigned)rp_cdiv(M, 16 * sd_tm(planes));
+    kernel<<<dim3(gx, flags ? std::min(gy, 16u) : gy), 64 * SD_WAVES, 0, st>>>((const decltype(type)*)A_dev, lda, a_scales_dev, ld_a_scales, (int)M, (int)N, (int)K, g.nb, w_codes_dev,
+                                                                               ld_w, w_scales_dev, ld_w_scales, (decltype(out)*)C_dev, ldc, flags);
+    RP_LAUNCHED();
+    return RPHIP_OK;
+  };
+  if (p.direct)
     return rp_by_type(c_type, [&](auto ct) -> int {
       using OT = typename decltype(ct)::T;
-      auto go = [&](auto kernel, auto type) {
-        kernel<<<grid, 64 * SD_WAVES, 0, st>>>((const decltype(type)*)A_dev, lda, a_scales_dev, ld_a_scales, (int)M, (int)N, (int)K, g.nb, w_codes_dev, ld_w, w_scales_dev, ld_w_scales,
-                                               (OT*)C_dev, ldc, gx);
-      };
-      if (a_type == RPHIP_BF16) go(k_mxg_direct<__bf16, OT, 1>, __bf16{});
-      else if (a_type == RPHIP_F16) go(k_mxg_direct<_Float16, OT, 2>, _Float16{});
-      else if (a_type == RPHIP_F32) go(k_mxg_direct<float, OT, 3>, 0.0f);
-      else go(k_mxg_direct<uint8_t, OT, 0>, uint8_t{0});
-      RP_LAUNCHED();
-      return RPHIP_OK;
+      if (a_type == RPHIP_BF16) return direct(k_mxg_direct<__bf16, OT, 1>, __bf16{}, OT{}, 1, nullptr);
+      if (a_type == RPHIP_F16) return direct(k_mxg_direct<_Float16, OT, 2>, _Float16{}, OT{}, 2, nullptr);
+      if (a_type == RPHIP_F32) return direct(k_mxg_direct<float, OT, 3>, 0.0f, OT{}, 3, nullptr);
+      return direct(k_mxg_direct<uint8_t, OT, 0>, uint8_t{0}, OT{}, 0, nullptr);
     });
-  }
   if (p.nc) {
-    const int64_t w_units = rp_cdiv(N, 16) * p.nq * 64, wg_w = rp_cdiv(w_units, 256);
+    const int64_t w_units = rp_cdiv(N, 16) * p.nq * 64, wg_w = p.half ? rp_cdiv(N, 16) : rp_cdiv(w_units, 256);
     const int64_t a_units = p.planes ? rp_cdiv(M, 16) * p.nc : rp_cdiv(M, 16) * p.nq * 64, wg_a = p.planes ? a_units : rp_cdiv(a_units, 256);
     if ((wg_w + wg_a) * 256 >= ((int64_t)1 << 32))
       RP_FAIL(RPHIP_ELIMIT, "mxfp4_gemm_nt: %lld x %lld x %lld: more 16-row blocks than one launch prepares (split M or N)", (long long)M, (long long)N, (long long)K);
     auto go = [&](auto kernel, auto type, const void* a, int64_t ld, void* o) {
       using T = decltype(type);
       kernel<<<(unsigned)(wg_w + wg_a), 256, 0, st>>>(w_scales_dev, ld_w_scales, (int)N, g.nb, p.nq, w_units, (uint32_t*)g.w_scales, (unsigned)wg_w, (const T*)a, ld, (int)M,
-                                                     (int)K, p.nc, a_units, o);
+                                                     (int)K, p.nc, a_units, o, half_args{w_codes_dev, ld_w, top, wide});
     };
     if (a_type == RPHIP_BF16) go(k_mxg_prepare<__bf16, 1>, __bf16{}, A_dev, lda, (void*)g.planes);
-    else if (a_type == RPHIP_F16) go(k_mxg_prepare<_Float16, 2>, _Float16{}, A_dev, lda, (void*)g.planes);
+    else if (a_type == RPHIP_F16) go(k_mxg_prepare<_Float16, 1>, _Float16{}, A_dev, lda, (void*)g.planes);
     else if (a_type == RPHIP_F32) go(k_mxg_prepare<float, 3>, 0.0f, A_dev, lda, (void*)g.planes);
     else go(k_mxg_prepare<uint8_t, 0>, uint8_t{0}, a_scales_dev, ld_a_scales, (void*)g.a_scales);
     RP_LAUNCHED();
@@ -853,16 +950,17 @@ extern "C" int rphip_mxfp4_gemm_nt(rphip_ctx* ctx, void* stream, int64_t M, int6
       else if (p.bm == 128) RP_TRY((launch_fp4<OT, 128, 128, 2, 2>(g, st)));
       else RP_TRY((launch_fp4<OT, 256, 256, 2, 4>(g, st)));
     } else {
-      if (p.bm == 16) RP_TRY((launch_bf16<OT, 16, 64, 1, 2>(g, p.planes, st)));
-      else if (p.bm == 64) RP_TRY((launch_bf16<OT, 64, 64, 2, 2>(g, p.planes, st)));
-      else if (p.bm == 128 && p.bn == 128) RP_TRY((launch_bf16<OT, 128, 128, 2, 2>(g, p.planes, st)));
-      else if (p.bm == 128) RP_TRY((launch_bf16<OT, 128, 256, 2, 4>(g, p.planes, st)));
-      else RP_TRY((launch_bf16<OT, 256, 256, 2, 4>(g, p.planes, st)));
+      if (p.bm == 16) RP_TRY((launch_bf16<OT, 16, 64, 1, 2>(g, p.planes, p.half, st)));
+      else if (p.bm == 64) RP_TRY((launch_bf16<OT, 64, 64, 2, 2>(g, p.planes, p.half, st)));
+      else if (p.bm == 128 && p.bn == 128) RP_TRY((launch_bf16<OT, 128, 128, 2, 2>(g, p.planes, p.half, st)));
+      else if (p.bm == 128) RP_TRY((launch_bf16<OT, 128, 256, 2, 4>(g, p.planes, p.half, st)));
+      else RP_TRY((launch_bf16<OT, 256, 256, 2, 4>(g, p.planes, p.half, st)));
     }
     if (p.split > 1) {
       k_mxg_join<OT><<<(unsigned)rp_cdiv(M * N, 256), 256, 0, st>>>(g.part, p.split, g.M, g.N, (OT*)C_dev, ldc);
       RP_LAUNCHED();
     }
+    if (p.half && p.nc) return direct(k_mxg_direct<_Float16, OT, 2>, _Float16{}, OT{}, 2, wide);
     return RPHIP_OK;
   });
 }

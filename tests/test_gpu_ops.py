@@ -216,6 +216,48 @@ def test_product_not_finite(ctx, ops):
     assert got[keep][:, [c for c in range(70) if c != 11]].isfinite().all()
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("m,n,k", [(40, 5000, 5000), (300, 9001, 700), (700, 6003, 1000)])
+def test_product_scales_far_apart(ctx, ops, dtype, m, n, k):
+    """Rows of W whose blocks differ by 2^35 .. 2^200, rows of A that meet only the small ones; zero blocks and NaN blocks among them."""
+    g = gen(m)
+    w = random_mxfp4(ops, n, k, 2)
+    w.scales.fill_(130)
+    for row, block, scale in ((3, 2, 130 - 35), (7, 3, 130 - 36), (9, 3, 130 - 37), (20, 1, 60), (1000, 5, 254 - 2), (1001, 5, 0), (n - 1, 3, 90), (n - 2, 7, 0)):
+        w.scales[row, block] = scale
+    w.codes[1001, 5 * 16:6 * 16] = 0  # (a block of zeros)
+    w.scales[2000, 4] = 255
+    a = torch.randn(m, k, generator=g)
+    for r in range(8):  # row r of A: nothing but block r
+        a[r] = 0
+        a[r, r * 32:r * 32 + 32] = torch.randn(32, generator=g)
+    a = a.to(dtype).cuda()
+    W = values_gpu(ops, ctx, w)
+    A = a.double()
+    got = ops.mxfp4_gemm_nt(ctx, a, w, dtype=torch.float32).double()
+    W[2000, 128:160] = math.nan
+    want, size = A @ W.t(), A.abs() @ W.abs().t()
+    # (a block of 6 x 2^125 times a standard normal number passes float32's largest, 2^128: such sums are no numbers in any order)
+    fits = ~(size >= 2.0 ** 127)
+    assert torch.equal(got.isnan() & fits, want.isnan()) and bool(got[:, 2000].isnan().all()) and int((~fits).sum()) <= m
+    terms = k * {torch.float32: 3, torch.float16: 2, torch.bfloat16: 1}[dtype]
+    bound = 8 * math.sqrt(terms) * 2.0 ** -23 * size + torch.finfo(torch.float32).tiny
+    assert bool((((got - want).abs() <= bound) | want.isnan() | ~fits).all())
+
+
+def test_product_not_finite_large(ctx, ops):
+    a = torch.randn(40, 5000, generator=gen(1))
+    a[3, 9], a[5, 50], a[6, 0] = math.inf, math.nan, -math.inf
+    w = random_mxfp4(ops, 5000, 5000, 8)
+    w.scales[11, 2] = 255
+    for dtype in TYPES:
+        x = a.to(dtype).cuda()
+        got, want = ops.mxfp4_gemm_nt(ctx, x, w), x.double() @ values_gpu(ops, ctx, w).t()
+        want[:, 11] = math.nan
+        for v in (torch.isnan, torch.isposinf, torch.isneginf):
+            assert torch.equal(v(got), v(want))
+
+
 def test_product_strides(ctx, ops):
     big = torch.randn(90, 301, generator=gen(2)).cuda()
     a = big[1:78, 3:204]
