@@ -189,22 +189,36 @@ struct gemm_args {
   float* part;               // split K: partial sums [split][M][N]
   int split;
   int gx, gy, blocked;       // tiles, and whether the grid runs in blocks of 4 x 8
+  int first, parts, n_tail;  // the last, incomplete round: its first block (tile), the parts of K its tiles are cut into (0: not this), its tiles
 };
 
 // Workgroups go to the 8 XCDs round-robin and an XCD runs 32 of them at a time; those 32 become a block of 4 tile rows x 8 tile columns,
 // so that an XCD's L2 serves 12 operand panels for 32 tiles.  Grids of fewer than 256 such tiles, or of less than four rows, go row by
 // row: blocks would leave XCDs idle.
-__device__ __forceinline__ bool tile_of(const gemm_args& g, int& tm, int& tn) {
-  if (!g.blocked) {
-    tm = (int)blockIdx.x / g.gx;
-    tn = (int)blockIdx.x % g.gx;
-    return true;
-  }
-  const unsigned L = blockIdx.x, x = L & 7u, s8 = L >> 3, beta = s8 >> 5, pp = s8 & 31u;
-  const unsigned nbc = ((unsigned)g.gx + 7) / 8, gb = beta * 8u + x, row = gb / nbc, col = gb - row * nbc;
+struct tile_at {
+  int tm, tn, z, parts, nth;  // which part of K, of how many; the tile's number in the last round
+};
+__device__ __forceinline__ bool tile_of_block(const gemm_args& g, unsigned block, unsigned pp, int& tm, int& tn) {
+  const unsigned nbc = ((unsigned)g.gx + 7) / 8, row = block / nbc, col = block - row * nbc;
   tm = (int)(row * 4 + pp / 8);
   tn = (int)(col * 8 + pp % 8);
   return tm < g.gy && tn < g.gx;
+}
+__device__ __forceinline__ bool tile_of(const gemm_args& g, tile_at& at) {
+  const unsigned L = blockIdx.x, cut = g.parts ? (unsigned)g.parts : 1u;
+  at.parts = g.parts ? g.parts : g.split;
+  if (!g.blocked) {
+    const unsigned tile = g.first + L / cut;
+    at.z = g.parts ? (int)(L % cut) : (int)blockIdx.y;
+    at.nth = (int)(L / cut);
+    at.tm = (int)(tile / g.gx);
+    at.tn = (int)(tile % g.gx);
+    return true;
+  }
+  const unsigned x = L & 7u, s8 = L >> 3, unit = (s8 >> 5) * 8u + x, pp = s8 & 31u;
+  at.z = g.parts ? (int)(unit % cut) : (int)blockIdx.y;
+  at.nth = (int)(unit / cut * 32 + pp);
+  return tile_of_block(g, g.first + unit / cut, pp, at.tm, at.tn) && (g.parts == 0 || at.nth < g.n_tail);
 }
 
 __device__ __forceinline__ void dma16(const uint8_t* from, uint8_t* to) {
@@ -219,9 +233,9 @@ __device__ __forceinline__ void wait_loads_and_meet() {
 }
 
 // D = W fragment x A fragment: a lane holds four neighbouring columns n of one row m.
-template <class OT, int TM, int TN, bool HALF = false>
-__device__ __forceinline__ void store_tile(const gemm_args& g, f32x4 (&acc)[TM][TN], int m0, int n0, int lane) {
-  const int z = blockIdx.y;
+template <class OT, int BM, int BN, int TM, int TN, bool HALF = false>
+__device__ __forceinline__ void store_tile(const gemm_args& g, const tile_at& at, f32x4 (&acc)[TM][TN], int wm, int wn, int lane) {
+  const int m0 = at.tm * BM + wm * 16, n0 = at.tn * BN + wn * 16, z = at.z;
   if constexpr (HALF) {
 #pragma unroll
     for (int j = 0; j < TN; ++j) {
@@ -232,6 +246,14 @@ __device__ __forceinline__ void store_tile(const gemm_args& g, f32x4 (&acc)[TM][
 #pragma unroll
         for (int e = 0; e < 4; ++e) acc[i][j][e] = ldexpf(acc[i][j][e], (int)((top >> (8 * e)) & 255u) - 127 - HALF_TOP);
     }
+  }
+  if (g.parts) {  // (whole tiles: k_mxg_join_tail leaves out what lies beyond C)
+    float* o = g.part + ((int64_t)z * g.n_tail + at.nth) * (BM * BN) + (wm * 16 + (lane & 15)) * BN + wn * 16 + (lane >> 4) * 4;
+#pragma unroll
+    for (int i = 0; i < TM; ++i)
+#pragma unroll
+      for (int j = 0; j < TN; ++j) *(f32x4*)(o + i * 16 * BN + j * 16) = acc[i][j];
+    return;
   }
 #pragma unroll
   for (int i = 0; i < TM; ++i) {
@@ -284,16 +306,16 @@ __global__ __launch_bounds__(WM * WN * 64) void k_mxg_bf16(gemm_args g) {
   static_assert(D * WAVES * 8 == BM && DW * WAVES * 16 == BN && SLANES <= 64, "every wave requests the same number of pieces");
   extern __shared__ __attribute__((aligned(1024))) uint8_t ring[];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  int tm, tn;
-  if (!tile_of(g, tm, tn)) return;
+  tile_at at;
+  if (!tile_of(g, at)) return;
+  const int tm = at.tm, tn = at.tn;
   const int m0 = tm * BM, wm = (wave / WN) * TM, wn = (wave % WN) * TN;  // (wm, wn in fragments of the tile)
   f32x4 acc[TM][TN];
 #pragma unroll
   for (int i = 0; i < TM; ++i)
 #pragma unroll
     for (int j = 0; j < TN; ++j) acc[i][j] = f32x4{0, 0, 0, 0};
-  const int z = blockIdx.y;
-  const int c0 = (int)((int64_t)g.nc * z / g.split), c1 = (int)((int64_t)g.nc * (z + 1) / g.split);
+  const int c0 = (int)((int64_t)g.nc * at.z / at.parts), c1 = (int)((int64_t)g.nc * (at.z + 1) / at.parts);
   const int t0 = c0 * P * 2, t1 = c1 * P * 2;
   const int mblocks = (g.M + 15) / 16, nblocks = (g.N + 15) / 16;
   const uint8_t* asrc[D];
@@ -368,7 +390,7 @@ __global__ __launch_bounds__(WM * WN * 64) void k_mxg_bf16(gemm_args g) {
     }
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // (the trailing requests write LDS)
   }
-  store_tile<OT, TM, TN, HALF>(g, acc, m0 + wm * 16, tn * BN + wn * 16, lane);
+  store_tile<OT, BM, BN, TM, TN, HALF>(g, at, acc, wm, wn, lane);
 }
 
 // 4-bit form: codes of both operands in two slots, a stage (two chunks of both) ahead; scales in two slots of four chunks.  A piece is
@@ -381,16 +403,16 @@ __global__ __launch_bounds__(WM * WN * 64) void k_mxg_fp4(gemm_args g) {
   static_assert(D * WAVES * 8 == BM + BN && SLANES <= 64, "every wave requests the same number of pieces");
   extern __shared__ __attribute__((aligned(1024))) uint8_t ring[];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  int tm, tn;
-  if (!tile_of(g, tm, tn)) return;
+  tile_at at;
+  if (!tile_of(g, at)) return;
+  const int tm = at.tm, tn = at.tn;
   const int wm = (wave / WN) * TM, wn = (wave % WN) * TN;  // (in fragments of the tile)
   f32x4 acc[TM][TN];
 #pragma unroll
   for (int i = 0; i < TM; ++i)
 #pragma unroll
     for (int j = 0; j < TN; ++j) acc[i][j] = f32x4{0, 0, 0, 0};
-  const int z = blockIdx.y;
-  const int q0 = (int)((int64_t)g.nq * z / g.split), q1 = (int)((int64_t)g.nq * (z + 1) / g.split);
+  const int q0 = (int)((int64_t)g.nq * at.z / at.parts), q1 = (int)((int64_t)g.nq * (at.z + 1) / at.parts);
   const int s0 = q0 * 2, s1 = min(q1 * 2, (g.nc + 1) / 2);  // stages: two chunks
   const int mblocks = (g.M + 15) / 16, nblocks = (g.N + 15) / 16;
   // a piece: 8 rows x 128 bytes; row r's block j of the stage lies at j ^ (r & 7)
@@ -458,7 +480,7 @@ __global__ __launch_bounds__(WM * WN * 64) void k_mxg_fp4(gemm_args g) {
     }
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // (the trailing requests write LDS)
   }
-  store_tile<OT, TM, TN>(g, acc, tm * BM + wm * 16, tn * BN + wn * 16, lane);
+  store_tile<OT, BM, BN, TM, TN>(g, at, acc, wm, wn, lane);
 }
 
 // ---- few rows of A -------------------------------------------------------------------------------------------------------------------
@@ -764,15 +786,69 @@ __global__ __launch_bounds__(256) void k_mxg_join(const float* __restrict__ part
   c[i / N * ldc + i % N] = rp_from_f32<OT>(s);
 }
 
+// the last round's tiles: the parts in order, one rounding
+template <class OT, int BM, int BN>
+__global__ __launch_bounds__(256) void k_mxg_join_tail(gemm_args g) {
+  int tm, tn;
+  const int nth = blockIdx.x;
+  if (g.blocked) {
+    if (!tile_of_block(g, (unsigned)(g.first + nth / 32), (unsigned)nth & 31u, tm, tn)) return;
+  } else {
+    tm = (g.first + nth) / g.gx, tn = (g.first + nth) % g.gx;
+  }
+  const int i = (int)blockIdx.y * 256 + threadIdx.x, m = tm * BM + i / (BN / 4), n = tn * BN + i % (BN / 4) * 4;
+  if (m >= g.M || n >= g.N) return;
+  f32x4 t = f32x4{0, 0, 0, 0};
+  for (int z = 0; z < g.parts; ++z) t += *(const f32x4*)(g.part + ((int64_t)z * g.n_tail + nth) * (BM * BN) + (int64_t)i * 4);
+  OT* o = (OT*)g.c + (int64_t)m * g.ldc + n;
+  if (n + 4 <= g.N) {
+    rp_vec<OT, 4> v;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v.v[e] = rp_from_f32<OT>(t[e]);
+    rp_store_vec<OT, 4>(o, v);
+  } else {
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      if (n + e < g.N) o[e] = rp_from_f32<OT>(t[e]);
+  }
+}
+
 struct plan {
   int planes = 0, split = 1, nc = 0, nq = 0;
   bool rows = false;    // few rows of A: k_mxg_rows
   bool direct = false;  // small: k_mxg_direct
   bool half = false;    // f16 A as it is
+  int first = 0, parts = 0, n_tail = 0;  // the last round of tiles (gemm_args)
   int bm = 16, bn = 64;
   int64_t plane_bytes = 0, a_scale_bytes = 0, w_scale_bytes = 0, top_bytes = 0, wide_bytes = 0, part_bytes = 0;
   int64_t total() const { return plane_bytes + a_scale_bytes + w_scale_bytes + top_bytes + wide_bytes + part_bytes; }
 };
+
+struct tile_grid {
+  int gx, gy;
+  bool blocked;
+  int64_t blocks, tiles;
+};
+tile_grid grid_of(int64_t M, int64_t N, int bm, int bn) {
+  tile_grid t;
+  t.gx = (int)rp_cdiv(N, bn), t.gy = (int)rp_cdiv(M, bm);
+  t.tiles = (int64_t)t.gx * t.gy;
+  t.blocked = t.gy >= 4 && t.tiles >= 256;
+  t.blocks = rp_cdiv(t.gx, 8) * rp_cdiv(t.gy, 4);
+  return t;
+}
+
+// Tiles of one workgroup to a CU: an incomplete round of them behind complete ones is cut along K, as often as it leaves CUs idle
+// (bf16 1500 x 12000 x 12000 538 -> 445 us; f16 2048 x 20000 x 20000, two and a half rounds: 1.71 -> 1.51 ms).  hundredths: the rounds' time.
+struct last_round {
+  int first, parts, n_tail;
+  int64_t hundredths;
+};
+last_round last_round_of(int n_cu, const tile_grid& t, int nc) {
+  const int64_t units = t.blocked ? t.blocks : t.tiles, round = t.blocked ? std::max(n_cu / 32, 1) : n_cu, rest = units % round;
+  const int64_t parts = rest && units > round ? std::max<int64_t>(1, std::min<int64_t>({round / rest, nc / 16, 8})) : 1;
+  return {(int)(units - rest), (int)parts, (int)(t.blocked ? rest * 32 : rest), units / round * 100 + (rest ? 100 / parts : 0)};
+}
 
 // Which tile, and into how many parts K is split: by rounds of workgroups over the CUs.  Measured on W of 20000 x 20000 unless said.
 plan make_plan(int n_cu, int64_t M, int64_t N, int64_t K, int32_t a_type) {
@@ -792,6 +868,7 @@ plan make_plan(int n_cu, int64_t M, int64_t N, int64_t K, int32_t a_type) {
   if (p.direct) return p;
   auto tiles = [&](int bm, int bn) { return std::max<int64_t>(rp_cdiv(M, bm) * rp_cdiv(N, bn), 1); };
   auto rounds = [&](int bm, int bn, int per_cu) { return rp_cdiv(tiles(bm, bn), per_cu * n_cu); };
+  auto hundredths = [&](int bm, int bn) { return last_round_of(n_cu, grid_of(M, N, bm, bn), p.nc).hundredths; };
   if (p.planes) {
     const int64_t steps = (int64_t)p.nc * p.planes * 2;
     int per_cu = 1;  // workgroups a CU should see when K is split: small tiles wait for memory together
@@ -800,7 +877,7 @@ plan make_plan(int n_cu, int64_t M, int64_t N, int64_t K, int32_t a_type) {
     } else if (M > 128 && tiles(128, 256) >= n_cu) {
       // a 128 x 256 tile takes 0.57 of a 256 x 256 one (527 and 302 us a round); three planes do not fit the larger one's registers
       p.bn = 256;
-      p.bm = p.planes == 3 || rounds(128, 256, 1) * 57 < rounds(256, 256, 1) * 100 ? 128 : 256;
+      p.bm = p.planes == 3 || hundredths(128, 256) * 57 < hundredths(256, 256) * 100 ? 128 : 256;
     } else if (M > 64 && tiles(128, 128) * steps >= 40000) {
       p.bm = 128, p.bn = 128, per_cu = 5;  // (M = 128: 157 us in eight parts, 199 with 64 x 64 tiles; 1000 x 3000 x 3000: 39 against 36)
     } else {
@@ -811,7 +888,7 @@ plan make_plan(int n_cu, int64_t M, int64_t N, int64_t K, int32_t a_type) {
     p.split = (int)std::max<int64_t>(1, std::min<int64_t>({(per_cu * (int64_t)n_cu + n / 2) / n, steps / 24, 16}));
   } else {
     // a round of 64 x 64 tiles (four a CU), 128 x 128 (two), 256 x 256 (one) takes 34, 45, 58 us at K = 8000
-    const int64_t t64 = rounds(64, 64, 4) * 58, t128 = rounds(128, 128, 2) * 76, t256 = rounds(256, 256, 1) * 100;
+    const int64_t t64 = rounds(64, 64, 4) * 58, t128 = rounds(128, 128, 2) * 76, t256 = hundredths(256, 256);
     p.bm = M <= 32 ? 32 : t64 <= t128 && t64 <= t256 ? 64 : t128 <= t256 ? 128 : 256;
     p.bn = p.bm;
     const int64_t n = tiles(p.bm, p.bn);
@@ -824,30 +901,49 @@ plan make_plan(int n_cu, int64_t M, int64_t N, int64_t K, int32_t a_type) {
   p.top_bytes = p.half ? room(rp_cdiv(N, 16) * 16) : 0;
   p.wide_bytes = p.half ? room(rp_cdiv(N, 16)) : 0;
   p.part_bytes = p.split > 1 ? M * N * 4 * p.split : 0;
+  if (p.split == 1 && p.bn == 256) {
+    const last_round l = last_round_of(n_cu, grid_of(M, N, p.bm, p.bn), p.nc);
+    if (l.parts > 1) {
+      p.first = l.first, p.parts = l.parts, p.n_tail = l.n_tail;
+      p.part_bytes = (int64_t)p.parts * p.n_tail * p.bm * p.bn * 4;
+    }
+  }
   return p;
 }
 
-template <int BM, int BN, class Kernel>
+template <class OT, int BM, int BN, class Kernel>
 int launch_tiles(Kernel kernel, gemm_args g, int threads, int lds, hipStream_t st) {
-  g.gx = (int)rp_cdiv(g.N, BN), g.gy = (int)rp_cdiv(g.M, BM);
-  g.blocked = g.gy >= 4 && (int64_t)g.gx * g.gy >= 256;
-  const int64_t blocks = rp_cdiv(g.gx, 8) * rp_cdiv(g.gy, 4), tiles = g.blocked ? rp_cdiv(blocks, 8) * 8 * 32 : (int64_t)g.gx * g.gy;
-  if (tiles * threads >= ((int64_t)1 << 32)) RP_FAIL(RPHIP_ELIMIT, "mxfp4_gemm_nt: %d x %d is more than a launch takes", g.M, g.N);
+  const tile_grid t = grid_of(g.M, g.N, BM, BN);
+  g.gx = t.gx, g.gy = t.gy, g.blocked = t.blocked;
+  auto workgroups = [&](int64_t units) { return t.blocked ? rp_cdiv(units, 8) * 8 * 32 : units; };
+  const gemm_args tail = g;
+  const int64_t units = t.blocked ? t.blocks : t.tiles, whole = g.parts ? g.first : units;
+  if (workgroups(units) * threads >= ((int64_t)1 << 32)) RP_FAIL(RPHIP_ELIMIT, "mxfp4_gemm_nt: %d x %d is more than a launch takes", g.M, g.N);
   if (lds > 64 * 1024) RP_HIP(hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, lds));
-  kernel<<<dim3((unsigned)tiles, (unsigned)g.split), threads, lds, st>>>(g);
+  g.first = g.parts = 0;
+  kernel<<<dim3((unsigned)workgroups(whole), (unsigned)g.split), threads, lds, st>>>(g);
   RP_LAUNCHED();
+  if constexpr (BN == 256) {
+    if (tail.parts) {
+      kernel<<<(unsigned)workgroups((units - whole) * tail.parts), threads, lds, st>>>(tail);
+      RP_LAUNCHED();
+      k_mxg_join_tail<OT, BM, BN><<<dim3((unsigned)tail.n_tail, BM * BN / 4 / 256), 256, 0, st>>>(tail);
+      RP_LAUNCHED();
+    }
+  }
   return RPHIP_OK;
 }
 template <class OT, int BM, int BN, int WM, int WN>
 int launch_fp4(const gemm_args& g, hipStream_t st) {
-  return launch_tiles<BM, BN>(k_mxg_fp4<OT, BM, BN, WM, WN>, g, WM * WN * 64, 2 * (BM + BN) * 128 + 2 * (BM + BN) * 16, st);
+  return launch_tiles<OT, BM, BN>(k_mxg_fp4<OT, BM, BN, WM, WN>, g, WM * WN * 64, 2 * (BM + BN) * 128 + 2 * (BM + BN) * 16, st);
 }
 template <class OT, int BM, int BN, int WM, int WN>
 int launch_bf16(const gemm_args& g, int planes, bool half, hipStream_t st) {
   constexpr int threads = WM * WN * 64, lds = 3 * BM * 128 + 2 * BN * 64 + 2 * BN * 16;
-  if (half) return launch_tiles<BM, BN>(k_mxg_bf16<OT, 1, true, BM, BN, WM, WN>, g, threads, lds, st);
-  if (planes == 1) return launch_tiles<BM, BN>(k_mxg_bf16<OT, 1, false, BM, BN, WM, WN>, g, threads, lds, st);
-  return launch_tiles<BM, BN>(k_mxg_bf16<OT, 3, false, BM, BN, WM, WN>, g, threads, lds, st);
+  if (half) return launch_tiles<OT, BM, BN>(k_mxg_bf16<OT, 1, true, BM, BN, WM, WN>, g, threads, lds, st);
+  if (planes == 1) return launch_tiles<OT, BM, BN>(k_mxg_bf16<OT, 1, false, BM, BN, WM, WN>, g, threads, lds, st);
+  if constexpr (BM * BN < 256 * 256) return launch_tiles<OT, BM, BN>(k_mxg_bf16<OT, 3, false, BM, BN, WM, WN>, g, threads, lds, st);
+  RP_FAIL(RPHIP_EINVAL, "mxfp4_gemm_nt: no such tile");
 }
 
 int check_sizes(const char* who, int64_t M, int64_t N, int64_t K) {
@@ -896,6 +992,7 @@ extern "C" int rphip_mxfp4_gemm_nt(rphip_ctx* ctx, void* stream, int64_t M, int6
   uint8_t* wide = top + p.top_bytes;
   g.w_top = top;
   g.c = C_dev, g.ldc = ldc, g.part = (float*)(wide + p.wide_bytes), g.split = p.split;
+  g.first = p.first, g.parts = p.parts, g.n_tail = p.n_tail;
   if (p.rows)
     return rp_by_type(a_type, [&](auto at) -> int {
       return rp_by_type(c_type, [&](auto ct) -> int {

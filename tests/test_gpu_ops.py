@@ -528,6 +528,8 @@ def values_gpu(ops, ctx, m):
     (torch.bfloat16, 33, 3001, 6000), (torch.float16, 64, 999, 9000), (torch.float32, 9, 2000, 5001), (torch.float32, 4, 5003, 7001),
     ("mxfp4", 4000, 4200, 300), ("mxfp4", 600, 3001, 1000), ("mxfp4", 200, 1999, 5000), ("mxfp4", 20, 700, 9000),
     ("mxfp4", 20, 40001, 3000), ("mxfp4", 300, 8001, 2000), ("mxfp4", 1000, 8000, 3000), ("mxfp4", 500, 3001, 5000), ("mxfp4", 90, 1501, 17000),
+    (torch.bfloat16, 1500, 12001, 4200), (torch.float16, 2001, 12000, 4200), (torch.float32, 1500, 12001, 4200), ("mxfp4", 1500, 12003, 8300),  # the last round in parts
+    (torch.bfloat16, 300, 30002, 4200), (torch.float16, 300, 30001, 4300), (torch.float32, 300, 30001, 4200), ("mxfp4", 700, 30001, 8300),
     (torch.bfloat16, 16, 2001, 4200), (torch.float16, 300, 5003, 1000), (torch.float32, 40, 4001, 4096), (torch.bfloat16, 500, 1001, 3999)])
 def test_product_large(ctx, ops, dtype, m, n, k):
     g = torch.Generator(device="cuda").manual_seed(m + n + k)
