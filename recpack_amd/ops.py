@@ -58,16 +58,18 @@ def _matrix(name, t):
     """A two-dimensional tensor whose rows are contiguous (copied if they are not), and its leading dimension."""
     if t.dim() != 2:
         raise ValueError(f"{name}: two dimensions expected, got {tuple(t.shape)}")
+    if t.is_contiguous():  # (the usual case first: a small call is as long as its checks)
+        return t, t.size(1)
     if not _rows_ok(t):
         t = t.contiguous()
     return t, t.stride(0) if t.shape[0] > 1 and t.stride(0) > t.shape[1] else t.shape[1]
 
 
-def _output(ctx, out, rows, cols, dtype):
-    """The given output, checked, or a new one; with its leading dimension and element type."""
+def _output(ctx, out, rows, cols, dtype, near):
+    """The given output, checked, or a new one on the device of the tensor ``near``; with its leading dimension and element type."""
     if out is None:
         code = _type_of("dtype", dtype)
-        return torch.empty((rows, cols), dtype=dtype, device=f"cuda:{ctx.device}"), max(cols, 1), code
+        return near.new_empty((rows, cols), dtype=dtype), cols or 1, code
     _on(ctx, "out", out)
     code = _type_of("out", out.dtype)
     if tuple(out.shape) != (rows, cols):
@@ -77,9 +79,9 @@ def _output(ctx, out, rows, cols, dtype):
     return out, max(out.stride(0) if rows > 1 else 0, cols, 1), code
 
 
-def _scratch(ctx, size):
+def _scratch(size, near):
     """Scratch memory of a call: torch's allocator keeps it with the stream, and with the graph a call is captured into."""
-    return torch.empty(size, dtype=torch.uint8, device=f"cuda:{ctx.device}") if size else None
+    return near.new_empty(size, dtype=torch.uint8) if size else None
 
 
 class MXFP4:
@@ -112,7 +114,7 @@ class MXFP4:
         codes = torch.empty((rows, line), dtype=torch.uint8, device=device)
         m = cls.__new__(cls)
         m.codes, m.cols = codes[:, :width] if line != width else codes, cols
-        m.scales = torch.empty((rows, blocks), dtype=torch.uint8, device=device)
+        m.scales = codes.new_empty((rows, blocks))
         return m
 
     @property
@@ -129,18 +131,21 @@ class MXFP4:
 
     def _args(self):
         c, s = self.codes, self.scales
-        many = c.shape[0] > 1 and c.shape[1] > 0
-        return c.data_ptr(), c.stride(0) if many else c.shape[1], s.data_ptr(), s.stride(0) if many else s.shape[1]
+        rows, width = c.shape
+        if rows > 1 and width:
+            return c.data_ptr(), c.stride(0), s.data_ptr(), s.stride(0)
+        return c.data_ptr(), width, s.data_ptr(), s.size(1)
 
 
 def mxfp4_quantize(ctx, x: torch.Tensor, transpose: bool = False, out: MXFP4 | None = None) -> MXFP4:
     """The rows of ``x`` (with ``transpose`` its columns: the result is that of ``x.T``) in MXFP4 (rphip_mxfp4_quantize)."""
     _on(ctx, "x", x)
     code = _type_of("x", x.dtype)
-    if x.dim() == 2 and x.shape[0] > 1 and x.shape[1] > 1 and x.stride(0) == 1 and x.stride(1) >= x.shape[0]:
+    if not x.is_contiguous() and x.dim() == 2 and x.shape[0] > 1 and x.shape[1] > 1 and x.stride(0) == 1 and x.stride(1) >= x.shape[0]:
         x, transpose = x.t(), not transpose  # a transposed view: its columns are contiguous
     x, ldx = _matrix("x", x)
-    rows, cols = (x.shape[1], x.shape[0]) if transpose else x.shape
+    m, n = x.shape
+    rows, cols = (n, m) if transpose else (m, n)
     if out is None:
         out = MXFP4.empty(rows, cols, x.device)
     elif out.shape != (rows, cols):
@@ -148,16 +153,17 @@ def mxfp4_quantize(ctx, x: torch.Tensor, transpose: bool = False, out: MXFP4 | N
     else:
         _on(ctx, "out", out.codes)
     codes, ldc, scales, lds = out._args()
-    _lib.check(ctx.lib.rphip_mxfp4_quantize(ctx.handle, _stream(ctx), x.shape[0], x.shape[1], x.data_ptr(), code, ldx, 1 if transpose else 0, codes, ldc, scales, lds))
+    _lib.check(ctx.lib.rphip_mxfp4_quantize(ctx.handle, _stream(ctx), m, n, x.data_ptr(), code, ldx, 1 if transpose else 0, codes, ldc, scales, lds))
     return out
 
 
 def mxfp4_dequantize(ctx, m: MXFP4, dtype: torch.dtype = torch.float32, out: torch.Tensor | None = None) -> torch.Tensor:
     """The values of a quantised matrix (exact in float32; rounded once otherwise)."""
     _on(ctx, "m", m.codes)
-    out, ldo, code = _output(ctx, out, m.codes.shape[0], m.cols, dtype)
+    rows = m.codes.size(0)
+    out, ldo, code = _output(ctx, out, rows, m.cols, dtype, m.codes)
     codes, ldc, scales, lds = m._args()
-    _lib.check(ctx.lib.rphip_mxfp4_dequantize(ctx.handle, _stream(ctx), m.codes.shape[0], m.cols, codes, ldc, scales, lds, out.data_ptr(), code, ldo))
+    _lib.check(ctx.lib.rphip_mxfp4_dequantize(ctx.handle, _stream(ctx), rows, m.cols, codes, ldc, scales, lds, out.data_ptr(), code, ldo))
     return out
 
 
@@ -179,10 +185,10 @@ def mxfp4_gemm_nt(ctx, a, w: MXFP4, dtype: torch.dtype | None = None, out: torch
     (m, k), n = a.shape, w.codes.shape[0]
     if k != w.cols:
         raise ValueError(f"a {(m, k)} and w {w.shape}: the second dimensions must be equal")
-    out, ldo, code = _output(ctx, out, m, n, dtype)
+    out, ldo, code = _output(ctx, out, m, n, dtype, w.codes)
     size = C.c_int64()
     _lib.check(ctx.lib.rphip_mxfp4_gemm_nt_workspace(ctx.handle, m, n, k, a_type, C.byref(size)))
-    ws = _scratch(ctx, size.value)
+    ws = _scratch(size.value, w.codes)
     wc, ldw, wsc, ldws = w._args()
     _lib.check(ctx.lib.rphip_mxfp4_gemm_nt(ctx.handle, _stream(ctx), m, n, k, a_ptr, a_type, lda, a_scales, ldas, wc, ldw, wsc, ldws, out.data_ptr(), code, ldo, _ptr(ws),
                                            size.value))
@@ -211,7 +217,7 @@ def mxfp4_scores(ctx, indptr: torch.Tensor, indices: torch.Tensor, w: MXFP4, wei
         weights = _vector(ctx, "weights", weights, nnz, torch.float32)
     if item_keep is not None:
         item_keep = _vector(ctx, "item_keep", item_keep.view(torch.uint8) if item_keep.dtype == torch.bool else item_keep, w.cols, torch.uint8)
-    out, ldo, code = _output(ctx, out, users, w.cols, dtype)
+    out, ldo, code = _output(ctx, out, users, w.cols, dtype, w.codes)
     codes, ldc, scales, lds = w._args()
     _lib.check(ctx.lib.rphip_mxfp4_scores(ctx.handle, _stream(ctx), users, nnz, indptr.data_ptr(), indices.data_ptr(), _ptr(weights), w.codes.shape[0], w.cols, codes, ldc,
                                           scales, lds, 1 if exclude_history else 0, _ptr(item_keep), out.data_ptr(), code, ldo))
@@ -255,12 +261,12 @@ def sample(ctx, scores: torch.Tensor, u: torch.Tensor, temperature=1.0, top_k=0,
     if top_k_per_row is not None:
         top_k_per_row = _vector(ctx, "top_k_per_row", top_k_per_row, rows, torch.int32)
         p.top_k_dev = top_k_per_row.data_ptr()
-    idx = torch.empty((rows, draws), dtype=torch.int32, device=scores.device)
-    prob = torch.empty((rows, draws), dtype=torch.float32, device=scores.device)
-    nnz = torch.empty(rows, dtype=torch.int32, device=scores.device)
+    idx = u.new_empty((rows, draws), dtype=torch.int32)
+    prob = u.new_empty((rows, draws))
+    nnz = u.new_empty(rows, dtype=torch.int32)
     size = C.c_int64()
     _lib.check(ctx.lib.rphip_sample_workspace(ctx.handle, rows, width, draws, int(top_k), C.byref(size)))
-    ws = _scratch(ctx, size.value)
+    ws = _scratch(size.value, scores)
     _lib.check(ctx.lib.rphip_sample(ctx.handle, _stream(ctx), rows, width, scores.data_ptr(), code, ld, _ptr(lengths), _ptr(ids), ld_ids, draws, u.data_ptr(), ldu,
                                     C.byref(p), idx.data_ptr(), prob.data_ptr(), nnz.data_ptr(), _ptr(ws), size.value))
     return idx, prob, nnz
