@@ -138,7 +138,8 @@ __device__ __forceinline__ void pack_scales_half(const uint8_t* __restrict__ s, 
   if (t == 0) wide[rb] = (uint8_t)lost;
 }
 
-// One launch for all of them: workgroups [0, wg_w) pack W's scales, the others cut A (P > 0) or pack A's scales.
+// One launch for all of them: workgroups [0, wg_w) pack W's scales, the others cut A (P > 0) or pack A's scales.  2048 x 20000 of A in f16 and
+// the scales of 20000 x 20000 of W: 52 us of 1.37 ms (once a call: 4 bytes an element of A and 2 a scale, read and written).
 struct half_args {  // (f16 A only)
   const uint8_t* codes;
   int64_t ldc;
@@ -295,7 +296,8 @@ __device__ __forceinline__ void store_tile(const gemm_args& g, const tile_at& at
 
 // 16-bit form.  Tile BM x BN, WM x WN waves.  A in a ring of three stages, each the half of a plane of a chunk (two of its four steps),
 // requested two stages ahead; W's codes and scales in two slots, a chunk ahead, converted in registers once per plane and wave (4 conversions
-// per 8 codes against TM matrix instructions that use them).
+// per 8 codes against TM matrix instructions that use them).  Bound by the matrix pipe as far as it is fed: 2048 x 20000 x 20000 f16 1.37 ms
+// (1.2 PF, with preparing), bf16 1.4, f32 3.7 (three planes: 1.3 PF); a bf16 library product of that size takes 1.07 to 1.26 ms.
 template <class OT, int P, bool HALF, int BM, int BN, int WM, int WN>
 __global__ __launch_bounds__(WM * WN * 64) void k_mxg_bf16(gemm_args g) {
   constexpr int WAVES = WM * WN, TM = BM / WM / 16, TN = BN / WN / 16, RING = 3;
@@ -394,7 +396,8 @@ __global__ __launch_bounds__(WM * WN * 64) void k_mxg_bf16(gemm_args g) {
 }
 
 // 4-bit form: codes of both operands in two slots, a stage (two chunks of both) ahead; scales in two slots of four chunks.  A piece is
-// eight rows of 128 bytes: 64 bytes a row and chunk fetched every cache line twice (1.16 -> 0.98 ms at 4096 x 20000 x 20000).
+// eight rows of 128 bytes: 64 bytes a row and chunk fetched every cache line twice (1.16 -> 0.98 ms at 4096 x 20000 x 20000).  Bound by the
+// requests' latency beside the matrix pipe (two stages of 64 KB are all that LDS holds beside one workgroup): 3.8 PF there.
 template <class OT, int BM, int BN, int WM, int WN>
 __global__ __launch_bounds__(WM * WN * 64) void k_mxg_fp4(gemm_args g) {
   constexpr int WAVES = WM * WN, TM = BM / WM / 16, TN = BN / WN / 16;
@@ -488,7 +491,7 @@ __global__ __launch_bounds__(WM * WN * 64) void k_mxg_fp4(gemm_args g) {
 // multiply-adds in float32 per element (no planes, no workspace).  A wave takes GV_ROWS rows of W at once, a lane every 64th MX block of
 // them: 1 KB contiguous per row and step.  The four waves of a workgroup share A's 2048 elements of a step in LDS as float32, in
 // the order [16 bytes of a block][block]: a lane reads its block without bank conflicts (from memory, 64 - 128 bytes apart, these reads
-// took longer than W: 80 us instead of 48 at 1 x 20000 x 20000 in f32).
+// took longer than W: 80 us instead of 48 at 1 x 20000 x 20000 in f32).  Bound by W's bytes: 45 us, 4.7 TB/s.
 constexpr int GV_ROWS = 4;
 template <class T, class OT, int M>
 __global__ __launch_bounds__(256) void k_mxg_rows(const T* __restrict__ a, int64_t lda, int m_real, int N, int K, int nb, const uint8_t* __restrict__ w, int64_t ldw,
@@ -577,7 +580,8 @@ __global__ __launch_bounds__(256) void k_mxg_rows(const T* __restrict__ a, int64
 // ---- small products ------------------------------------------------------------------------------------------------------------------
 // One launch, no workspace: a workgroup takes 16 x 64 of C (4-bit A: 32 x 32), its eight waves every eighth chunk of K each, operands from memory into registers
 // as a lane hands them to the matrix instruction (A cut or its scales taken there), a chunk ahead; the waves' sums are joined in LDS
-// in wave order.  A is read once per tile column and W once per tile row, so this is for products whose time is launches and latency.
+// in wave order.  A is read once per tile column and W once per tile row, so this is for products whose time is launches and latency:
+// 97 x 1999 x 2003 in f32 12 us, three launches of the tiles' form 20.
 constexpr int SD_WAVES = 8;
 constexpr int sd_tm(int planes) { return planes ? 1 : 2; }  // (cutting A is most of the work: 16 rows of A to 64 of W)
 constexpr int sd_tn(int planes) { return planes ? 4 : 2; }
@@ -857,7 +861,7 @@ plan make_plan(int n_cu, int64_t M, int64_t N, int64_t K, int32_t a_type) {
   p.half = a_type == RPHIP_F16;
   p.nc = (int)rp_cdiv(K, KC);
   p.nq = (int)rp_cdiv(p.nc, 4);
-  // the vector unit's form: f32 105 us against 120 at M = 4, 16 bits 63 against 91 at M = 2 (but 110 at 4)
+  // the vector unit's form: f32 104 us against 118 at M = 4, 16 bits 72 against 90 to 108 at M = 2 (but 105 to 116 against 89 to 108 at 3)
   p.rows = p.planes != 0 && M <= (p.planes == 3 ? 4 : 2) && K > 0;
   if (p.rows) return p;
   // small products, by tiles and by what a tile's latency comes to: f32 97 x 1999 x 2003 13.7 us against 20.2, bf16 256 x 2000 x 2000 16.5
