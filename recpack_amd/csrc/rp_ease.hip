@@ -2021,6 +2021,8 @@ int rp_spd_inverse(rphip_ctx* ctx, float* A, int n_pad, long long ld, int* info_
   if (n22_issued < n_inv_panels) {
     RP_HIP(hipEventRecord(e_panel, st));  // (the factor is complete)
     RP_HIP(hipStreamWaitEvent(s2, e_panel, 0));
+    // (the chains share T2: those of the first panels may still be running on s4 where the factorisation has little left behind them)
+    if (n22_issued > 0) RP_HIP(hipStreamWaitEvent(s2, n22_ev.v[n22_issued - 1], 0));
   }
   // diagnostic (RP_INV_TRACE=1): where the inverse's main stream spends its time, summed over the panels
   std::vector<hipEvent_t> iv_ev;
