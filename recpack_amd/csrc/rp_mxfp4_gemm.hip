@@ -396,8 +396,9 @@ __global__ __launch_bounds__(WM * WN * 64) void k_mxg_bf16(gemm_args g) {
 }
 
 // 4-bit form: codes of both operands in two slots, a stage (two chunks of both) ahead; scales in two slots of four chunks.  A piece is
-// eight rows of 128 bytes: 64 bytes a row and chunk fetched every cache line twice (1.16 -> 0.98 ms at 4096 x 20000 x 20000).  Bound by the
-// requests' latency beside the matrix pipe (two stages of 64 KB are all that LDS holds beside one workgroup): 3.8 PF there.
+// eight rows of 128 bytes: 64 bytes a row and chunk fetched every cache line twice (1.16 -> 0.98 ms at 4096 x 20000 x 20000).  Bound by
+// the operands' way into LDS: a CU takes 64 KB a stage in 2.1 us, where its matrix instructions take 0.9 (3.8 PF there; 128 x 256 tiles three
+// stages deep, half again the bytes, are 17 % slower).
 template <class OT, int BM, int BN, int WM, int WN>
 __global__ __launch_bounds__(WM * WN * 64) void k_mxg_fp4(gemm_args g) {
   constexpr int WAVES = WM * WN, TM = BM / WM / 16, TN = BN / WN / 16;
