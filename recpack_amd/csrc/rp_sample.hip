@@ -72,9 +72,6 @@ __device__ __forceinline__ uint32_t key_of(float x) {
 }
 __device__ __forceinline__ float score_of(uint32_t key) { return __uint_as_float(key & 0x80000000u ? key & 0x7fffffffu : ~key); }
 
-// log of a mass relative to the best score; equal scores give 0 (+inf among them)
-__device__ __forceinline__ double z_of(float x, float best, double inv_t_num) { return x == best ? 0.0 : ((double)x - (double)best) / inv_t_num; }
-
 // ---- exchanges inside a wave: in the vector unit where it can (data-parallel moves, lane swaps), no LDS round trips -----------------
 template <int CTRL, int ROWS = 0xf>
 __device__ __forceinline__ uint32_t dpp(uint32_t v) {  // lanes without a source get 0
