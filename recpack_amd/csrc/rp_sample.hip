@@ -21,7 +21,6 @@ constexpr int SB_PER = 128;
 constexpr int SB_CAP = 2048;         // entries of a list collected ahead
 constexpr int RC_FOUND = 512;        // ... of a workgroup's own part of them, in LDS
 constexpr int SR_THREADS = 256;      // threads of a workgroup that takes a slice of a row
-constexpr int64_t STRIP = 1024;      // rows whose workspace exists at a time (whole-row form: 58 KB each)
 
 struct sample_args {
   int64_t rows, ld, ld_ids, ld_u;
@@ -991,7 +990,7 @@ __global__ __launch_bounds__(SL_THREADS, 8) void k_sample_topk(sample_args a) {
 // Masses of a row's candidates relative to its best score, by t = 128 log2(mass) (0 for the best score, +inf among them; -8000 where next to
 // nothing is left).  Its nearest whole number is the bin; 2^(t / 128) is a power of two from a table of 128, times a polynomial of degree 4
 // on +-ln2 / 256 (remainder < 2^-49 relative); as whole numbers of 2^-shift (shift <= 50: the add of 2^52 rounds).  Some 20 instructions; a
-// series of degree 11 and the conversion to 64 bits took 40 (k_row_hist on 512 rows of 100000: 99 us, 84 so).
+// series of degree 11 and the conversion to 64 bits took 40 (this pass over 512 rows of 100000: 99 us, 84 so).
 struct row_mass {
   float best;
   double c;      // 128 log2(e) / temperature
@@ -1252,16 +1251,15 @@ __device__ __forceinline__ int seek(const T* p, int len, const row_mass& rm, con
   return (int)sh.found;
 }
 
-// The whole-row form runs in four or five launches, three of them with a row's slices spread over workgroups:
+// The whole-row form: for few wide rows in four or five launches, three of them with a row's slices spread over workgroups,
 //   best     the slices' best scores; clears the row's workspace
 //   hist     masses and counts per bin (fixed point: the order of the atomics does not matter)
-//   bins     the bin where top-p ends and the bins where the draw can fall (known up to one bin's mass); few rows: inside collect
+//   bins     the bin where top-p ends and the bins where the draw can fall (known up to one bin's mass); very few rows: inside collect
 //   collect  the candidates of these bins
 //   draw     one workgroup: the exact end of the kept prefix, then the draw
-// Read three times, from memory once where it fits the caches.  (The last slice of hist in the place of bins needs a fence in every
-// workgroup that writes its XCD's cache back: 16 us instead of 7 for one row, 350 instead of 80 for 512.)  One row of 100000: 25 us, four
-// launches one after the other; 512 rows in f32 197 us, best 52, hist 84, bins 8, collect 37, draw 17 (each pass over 205 MB takes 43 at the
-// rate of a copy; hist is bound by the vector unit and the LDS atomics).
+// otherwise the same in one launch (k_row_one).  Read three times, from memory once where it fits the caches.  (The last slice of hist in the
+// place of bins needs a fence in every workgroup that writes its XCD's cache back: 16 us instead of 7 for one row.)  One row of 100000: 25
+// us, four launches one after the other.
 __device__ __forceinline__ void slice_of(int len, int slices, int s, int& begin, int& end) {
   const int64_t pieces = ((int64_t)len + 7) / 8;
   begin = (int)(pieces * s / slices * 8);
@@ -1402,6 +1400,18 @@ __global__ __launch_bounds__(SL_THREADS) void k_row_bins(sample_args a, row_ws* 
   keep_bins<SL_THREADS>(ws, b, before);
 }
 
+// between which scores the bins b1 and lo .. hi lie, half a bin more on either side, and a float's step: all others are passed over by
+// comparisons
+struct row_ranges {
+  float low1, high1, low2, high2;
+  __device__ __forceinline__ bool holds(float x) const { return (x >= low1 && x <= high1) || (x >= low2 && x <= high2); }
+};
+__device__ __forceinline__ row_ranges ranges_of(const row_mass& rm, const row_bins& b) {
+  auto above = [&](int bin) __attribute__((always_inline)) { return nextafterf((float)((double)rm.best + (1.0 - bin) / rm.c), INFINITY); };
+  auto below = [&](int bin) __attribute__((always_inline)) { return bin == SB_BINS - 1 ? -INFINITY : nextafterf((float)((double)rm.best - (1.0 + bin) / rm.c), -INFINITY); };
+  return {b.b1 < 0 ? INFINITY : below(b.b1), b.b1 < 0 ? -INFINITY : above(b.b1), b.hi < b.lo ? INFINITY : below(b.hi), b.hi < b.lo ? -INFINITY : above(b.lo)};
+}
+
 // (FIND: every workgroup finds the bins itself, where one launch less is more)
 template <class T, bool COUNT, bool FIND>
 __global__ __launch_bounds__(SR_THREADS) void k_row_collect(sample_args a, row_ws* __restrict__ wss, int slices, int shift) {
@@ -1426,17 +1436,14 @@ __global__ __launch_bounds__(SR_THREADS) void k_row_collect(sample_args a, row_w
   }
   const int b1 = bins.b1, lo = bins.lo, hi = bins.hi;
   if (b1 < 0 && hi < lo) return;
-  // between which scores these bins lie, half a bin more on either side, and a float's step: all others are passed over by comparisons
-  auto above = [&](int bin) __attribute__((always_inline)) { return nextafterf((float)((double)rm.best + (1.0 - bin) / rm.c), INFINITY); };
-  auto below = [&](int bin) __attribute__((always_inline)) { return bin == SB_BINS - 1 ? -INFINITY : nextafterf((float)((double)rm.best - (1.0 + bin) / rm.c), -INFINITY); };
-  const float high1 = b1 < 0 ? -INFINITY : above(b1), low1 = b1 < 0 ? INFINITY : below(b1), high2 = hi < lo ? -INFINITY : above(lo), low2 = hi < lo ? INFINITY : below(hi);
+  const row_ranges ranges = ranges_of(rm, bins);
   int begin, end;
   slice_of(s.len, gridDim.y, sl, begin, end);
   scan_row<T>((const T*)a.scores + r * a.ld, begin, end, threadIdx.x, SR_THREADS, [&](int j, const rp_vec<T, PIECE<T>>& v, int) __attribute__((always_inline)) {
 #pragma unroll
     for (int i = 0; i < PIECE<T>; ++i) {
       const float x = rp_to_f32(v.v[i]);
-      if (!((x >= low1 && x <= high1) || (x >= low2 && x <= high2))) continue;
+      if (!ranges.holds(x)) continue;
       const uint32_t k = key_of(x);
       if (k == 0) continue;
       const int b = rm.bin(rm.t_of(score_of(k)));
@@ -1475,29 +1482,22 @@ __device__ __forceinline__ int rank_reaching(const ranked_list& l, int n, unsign
   return at;
 }
 
+union draw_shared {
+  seek_shared seek;
+  ranked_list two[2];
+};
+__device__ __forceinline__ void nothing_drawn(const sample_args& a, int64_t r) {
+  if (threadIdx.x == 0) {
+    a.idx[r] = -1;
+    a.prob[r] = 0.0f;
+    if (a.nnz) a.nnz[r] = 0;
+  }
+}
+// the draw from what was collected; a workgroup of SL_THREADS
 template <class T, bool COUNT>
-__global__ __launch_bounds__(SL_THREADS) void k_row_draw(sample_args a, const row_ws* __restrict__ wss, int slices, int shift) {
-  __shared__ double powers[SB_PER];
-  __shared__ union {
-    seek_shared seek;
-    ranked_list two[2];
-  } sh;
+__device__ __forceinline__ void draw_row(const sample_args& a, int64_t r, const row_set& s, const T* p, const row_mass& rm, const row_ws& ws, draw_shared& sh) {
   __shared__ unsigned long long red64[SL_THREADS / 64];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int64_t r = a.row0 + blockIdx.x;
-  const row_ws& ws = wss[blockIdx.x];
-  const row_set s = rs_load(a, r);
-  const T* p = (const T*)a.scores + r * a.ld;
-  const uint32_t best = best_of(ws, slices);
-  if (best == 0) {  // nothing to draw from
-    if (threadIdx.x == 0) {
-      a.idx[r] = -1;
-      a.prob[r] = 0.0f;
-      if (a.nnz) a.nnz[r] = 0;
-    }
-    return;
-  }
-  const row_mass rm = rm_make(best, s, shift, powers);
   const int b1 = ws.b1, b2_lo = ws.b2_lo, b2_hi = ws.b2_hi;
   const int n1 = b1 >= 0 && ws.n_list[0] <= SB_CAP ? (int)ws.n_list[0] : -1;
   const int n2 = b2_hi >= b2_lo && ws.n_list[1] <= SB_CAP ? (int)ws.n_list[1] : -1;
@@ -1574,12 +1574,108 @@ __global__ __launch_bounds__(SL_THREADS) void k_row_draw(sample_args a, const ro
   }
 }
 
+template <class T, bool COUNT>
+__global__ __launch_bounds__(SL_THREADS) void k_row_draw(sample_args a, const row_ws* __restrict__ wss, int slices, int shift) {
+  __shared__ double powers[SB_PER];
+  __shared__ draw_shared sh;
+  const int64_t r = a.row0 + blockIdx.x;
+  const row_ws& ws = wss[blockIdx.x];
+  const row_set s = rs_load(a, r);
+  const uint32_t best = best_of(ws, slices);
+  if (best == 0) return nothing_drawn(a, r);
+  const row_mass rm = rm_make(best, s, shift, powers);
+  draw_row<T, COUNT>(a, r, s, (const T*)a.scores + r * a.ld, rm, ws, sh);
+}
+
+// ... all of it in one launch, a workgroup to a row, its workspace in LDS (118 KB: one to a CU).  Bound by the vector unit (some 25 instructions
+// in 64 bits a score and the LDS atomics) and by what one workgroup has under way: 512 rows of 100000 in f32 156 us, where reading them takes 43.
+struct one_shared {
+  row_ws ws;
+  draw_shared draw;
+};
+template <class T, bool COUNT>
+__global__ __launch_bounds__(SL_THREADS) void k_row_one(sample_args a, int shift) {
+  extern __shared__ __attribute__((aligned(16))) char one_lds[];
+  __shared__ double powers[SB_PER];
+  __shared__ uint32_t red[SL_THREADS / 64];
+  __shared__ unsigned long long red64[SL_THREADS / 64];
+  row_ws& ws = ((one_shared*)one_lds)->ws;
+  const int64_t r = a.row0 + blockIdx.x;
+  const row_set s = rs_load(a, r);
+  const T* p = (const T*)a.scores + r * a.ld;
+  const float u = a.u[r * a.ld_u];
+  uint32_t best = 0;
+  scan_row<T>(p, 0, s.len, threadIdx.x, SL_THREADS, [&](int, const rp_vec<T, PIECE<T>>& v, int) __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < PIECE<T>; ++i) best = max(best, key_of(rp_to_f32(v.v[i])));
+  });
+  for (int i = threadIdx.x; i < SB_BINS; i += SL_THREADS) {
+    ws.hist_m[i] = 0;
+    if (COUNT) ws.hist_c[i] = 0;
+  }
+  if (threadIdx.x < 2) ws.n_list[threadIdx.x] = 0;
+  best = block_max_u32<SL_THREADS>(best, red);
+  if (best == 0) return nothing_drawn(a, r);
+  const row_mass rm = rm_make(best, s, shift, powers);
+  __syncthreads();
+  unsigned long long above = 0, count = 0;
+  const double least = (double)s.min_p;
+  scan_row<T>(p, 0, s.len, threadIdx.x, SL_THREADS, [&](int, const rp_vec<T, PIECE<T>>& v, int) __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < PIECE<T>; ++i) {
+      const uint32_t k = key_of(rp_to_f32(v.v[i]));
+      if (k == 0) continue;
+      const double t = rm.t_of(score_of(k)), e = rm.part(t);
+      const unsigned long long m = rm.whole(e);
+      const int b = rm.bin(t);
+      if (m) atomicAdd(&ws.hist_m[b], m);
+      if (COUNT) {
+        atomicAdd(&ws.hist_c[b], 1u);
+        ++count;
+      }
+      if (e >= least) above += m;
+    }
+  });
+  above = block_sum_u64<SL_THREADS>(above, red64);
+  if (COUNT) count = block_sum_u64<SL_THREADS>(count, red64);
+  if (threadIdx.x == 0) ws.above = above, ws.count = count;
+  __syncthreads();
+  unsigned long long before[SB_BINS / SL_THREADS];
+  const row_bins bins = find_bins<SL_THREADS, COUNT>(ws, s, u, shift, before);
+  keep_bins<SL_THREADS>(ws, bins, before);
+  if (bins.b1 >= 0 || bins.hi >= bins.lo) {
+    const row_ranges ranges = ranges_of(rm, bins);
+    scan_row<T>(p, 0, s.len, threadIdx.x, SL_THREADS, [&](int j, const rp_vec<T, PIECE<T>>& v, int) __attribute__((always_inline)) {
+#pragma unroll
+      for (int i = 0; i < PIECE<T>; ++i) {
+        const float x = rp_to_f32(v.v[i]);
+        if (!ranges.holds(x)) continue;
+        const uint32_t k = key_of(x);
+        if (k == 0) continue;
+        const int b = rm.bin(rm.t_of(score_of(k)));
+        const unsigned long long entry = ((unsigned long long)k << 32) | (uint32_t) ~(j + i);
+        auto put = [&](int which) __attribute__((always_inline)) {
+          const uint32_t at = atomicAdd(&ws.n_list[which], 1u);
+          if (at < SB_CAP) ws.list[which][at] = entry;
+        };
+        if (b == bins.b1) put(0);
+        if (b >= bins.lo && b <= bins.hi) put(1);
+      }
+    });
+  }
+  __syncthreads();
+  draw_row<T, COUNT>(a, r, s, p, rm, ws, ((one_shared*)one_lds)->draw);
+}
+
 // which form a call takes, and its workspace
 enum sample_form { FORM_WAVE, FORM_LISTS, FORM_ROWS };
 sample_form form_of(int64_t width, int64_t k) { return width <= RPS_SHORT ? FORM_WAVE : k <= RPS_SHORT ? FORM_LISTS : FORM_ROWS; }
+// One workgroup to a row and launch, or slices of few wide rows over the card: 1 x 12000 20 us against 28, 256 x 12000 23 against 56, 64 x 50000 42
+// against 58, 512 x 100000 156 against 190; but 1 x 50000 37 against 28 and 16 x 100000 65 against 41 (f32).
+bool one_launch(int64_t rows, int64_t width) { return width <= 20000 || rows >= 64; }
 int64_t workspace_of(int64_t rows, int64_t width, int64_t k) {
   switch (form_of(width, k)) {
-    case FORM_ROWS: return std::min(rows, STRIP) * (int64_t)sizeof(row_ws);
+    case FORM_ROWS: return one_launch(rows, width) ? 0 : rows * (int64_t)sizeof(row_ws);
     default: return 0;
   }
 }
@@ -1648,30 +1744,36 @@ extern "C" int rphip_sample(rphip_ctx* ctx, void* stream, int64_t rows, int64_t 
         }
         return RPHIP_OK;
       default: {
-        // slices of a row: about eight workgroups per CU in all, of no fewer than 1024 scores
-        const int slices = (int)std::max<int64_t>(1, std::min<int64_t>({8 * (int64_t)ctx->n_cu / std::min<int64_t>(rows, STRIP), width / 1024, 64}));
         auto go = [&](auto by_count) -> int {
           constexpr bool COUNT = decltype(by_count)::value;
-          for (a.row0 = 0; a.row0 < rows; a.row0 += STRIP) {
-            const unsigned n = (unsigned)std::min<int64_t>(STRIP, rows - a.row0);
-            row_ws* ws = (row_ws*)workspace_dev;
-            k_row_best<T><<<dim3(n, slices), SR_THREADS, 0, st>>>(a, ws);
-            RP_LAUNCHED();
-            k_row_hist<T, COUNT><<<dim3(n, slices), SR_THREADS, 0, st>>>(a, ws, shift);
-            RP_LAUNCHED();
-            // few rows, or one slice a row: a launch (3 - 4 us) costs more than finding the bins in every slice (one row of 100000: 25.6 us
-            // against 28.4; 512 of 2000: 39 against 46; but 128 rows of 100000 95 against 85)
-            if (n <= 8 || slices == 1) {
-              k_row_collect<T, COUNT, true><<<dim3(n, slices), SR_THREADS, 0, st>>>(a, ws, slices, shift);
-            } else {
-              k_row_bins<COUNT><<<n, SL_THREADS, 0, st>>>(a, ws, shift);
+          if (one_launch(rows, width)) {
+            RP_HIP(hipFuncSetAttribute((const void*)k_row_one<T, COUNT>, hipFuncAttributeMaxDynamicSharedMemorySize, (int)sizeof(one_shared)));
+            for (a.row0 = 0; a.row0 < rows; a.row0 += 1 << 20) {
+              k_row_one<T, COUNT><<<(unsigned)std::min<int64_t>(1 << 20, rows - a.row0), SL_THREADS, sizeof(one_shared), st>>>(a, shift);
               RP_LAUNCHED();
-              k_row_collect<T, COUNT, false><<<dim3(n, slices), SR_THREADS, 0, st>>>(a, ws, slices, shift);
             }
-            RP_LAUNCHED();
-            k_row_draw<T, COUNT><<<n, SL_THREADS, 0, st>>>(a, ws, slices, shift);
-            RP_LAUNCHED();
+            return RPHIP_OK;
           }
+          // slices of a row: about eight workgroups per CU in all, of no fewer than 1024 scores
+          const unsigned n = (unsigned)rows;
+          const int slices = (int)std::max<int64_t>(1, std::min<int64_t>({8 * (int64_t)ctx->n_cu / rows, width / 1024, 64}));
+          row_ws* ws = (row_ws*)workspace_dev;
+          k_row_best<T><<<dim3(n, slices), SR_THREADS, 0, st>>>(a, ws);
+          RP_LAUNCHED();
+          k_row_hist<T, COUNT><<<dim3(n, slices), SR_THREADS, 0, st>>>(a, ws, shift);
+          RP_LAUNCHED();
+          // very few rows: a launch (3 - 4 us) costs more than finding the bins in every slice (one row of 100000: 25.6 us against 28.4; 16 rows 46
+          // against 42)
+          if (n <= 8) {
+            k_row_collect<T, COUNT, true><<<dim3(n, slices), SR_THREADS, 0, st>>>(a, ws, slices, shift);
+          } else {
+            k_row_bins<COUNT><<<n, SL_THREADS, 0, st>>>(a, ws, shift);
+            RP_LAUNCHED();
+            k_row_collect<T, COUNT, false><<<dim3(n, slices), SR_THREADS, 0, st>>>(a, ws, slices, shift);
+          }
+          RP_LAUNCHED();
+          k_row_draw<T, COUNT><<<n, SL_THREADS, 0, st>>>(a, ws, slices, shift);
+          RP_LAUNCHED();
           return RPHIP_OK;
         };
         return params->top_k > 0 ? go(std::true_type{}) : go(std::false_type{});

@@ -481,6 +481,24 @@ def test_sample_close_scores(ctx, ops, width, top_k, apart):
     check_sample(ctx, ops, x, torch.rand(6, n, generator=g), temperature=0.05, top_k=top_k, top_p=0.9)
 
 
+@pytest.mark.parametrize("rows,width", [(1, 30001), (3, 40000), (12, 30001), (63, 20001), (64, 30001), (70, 1500), (2, 20000), (300, 2050)])
+@pytest.mark.parametrize("top_k", [0, 1025, 5000])
+def test_sample_whole_rows(ctx, ops, rows, width, top_k):
+    """One draw from a long prefix: few wide rows over many workgroups, otherwise a workgroup to a row; rows without candidates among them."""
+    g = gen(rows + width + top_k)
+    x = torch.randn(rows, width, generator=g) * 2
+    x[torch.rand(rows, width, generator=g) < 0.1] = -math.inf
+    if rows > 2:
+        x[1] = math.nan
+        x[2, 7:] = -math.inf
+    u = torch.rand(rows, 1, generator=g)
+    k = min(top_k, width)
+    check_sample(ctx, ops, x, u, temperature=0.8, top_k=k, top_p=0.9, min_p=0.001)
+    check_sample(ctx, ops, x, u, temperature=torch.rand(rows, generator=g) + 0.3, top_k=k)
+    check_sample(ctx, ops, x.half(), u, temperature=0.0, top_k=k)
+    check_sample(ctx, ops, torch.round(x), u, temperature=1.0, top_k=k, top_p=0.5)  # thousands of equal scores
+
+
 def test_sample_far_below(ctx, ops):
     """Candidates far below the best one: by value in one coarse bin, drawn after the rest is gone."""
     x = torch.cat([torch.tensor([[50.0, 49.0]]), torch.randn(1, 30000, generator=gen(0)) - 400], 1)
