@@ -591,7 +591,8 @@ int rphip_mxfp4_scores(rphip_ctx* ctx, void* stream, int64_t n_users, int64_t nn
  * exceeds u[d] times their total; prob = its share of that total (the propensity of the draw).  u in [0, 1) (values outside are moved to
  * the nearest end, NaN to 0).  temperature 0: the first k in rank order, prob 1; top_p, min_p and u are not used.
  * Out: idx (index, or ids[row, index]; -1 where nothing was left), prob (0 there), nnz = number drawn (may be NULL): rows x draws and
- * rows, contiguous.  Masses are summed in 64 bits; the result does not depend on the launch.
+ * rows, contiguous.  Masses are summed in 64 bits; where a prefix may be longer than 1024, each as a whole number that holds it to 2^-45 of itself at
+ * 100 000 scores and to 2^-32 at 2^30 (a mass below 2^-32 of the best one's: to that much of 2^-32).  The result does not depend on the launch.
  * params: scalars, or one value per row where a device array is given (values out of range are moved into it; top_k_dev needs top_k > 0 as
  * its upper bound, entries <= 0 mean that bound).  draws > 1 needs min(top_k, width) <= 1024. */
 typedef struct rphip_sample_params {

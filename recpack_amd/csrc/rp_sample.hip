@@ -3,7 +3,7 @@
 //
 // Candidates are ranked by (score descending, index ascending); everything below works on that order.  The kept set is a prefix of it,
 // a draw inverts the cumulative mass along it.  Whole numbers come out, so sums next to a border decide: masses are float64 (short
-// lists) or 64-bit fixed point (whole rows, where the order of the adds must not matter), never float32.
+// lists) or whole numbers of 64 bits (whole rows, where the order of the adds must not matter), never float32.
 #include "rp_ops.h"
 
 #include <algorithm>
@@ -109,6 +109,8 @@ __device__ __forceinline__ double lane_f64(double v, int src) {
 __device__ __forceinline__ unsigned long long lane_u64(unsigned long long v, int src) {
   return ((unsigned long long)lane_u32((uint32_t)(v >> 32), src) << 32) | lane_u32((uint32_t)v, src);
 }
+__device__ __forceinline__ double wave_scan(double v) { return wave_scan_f64(v); }
+__device__ __forceinline__ unsigned long long wave_scan(unsigned long long v) { return wave_scan_u64(v); }
 typedef unsigned int u32x2 __attribute__((ext_vector_type(2)));
 template <int M>
 __device__ __forceinline__ uint32_t xor_lane(uint32_t v, int lane) {
@@ -987,19 +989,27 @@ __global__ __launch_bounds__(SL_THREADS, 8) void k_sample_topk(sample_args a) {
 }
 
 // ---- whole rows, any prefix, one draw ------------------------------------------------------------------------------------------------
-// Masses of a row's candidates relative to its best score, by t = 128 log2(mass) (0 for the best score, +inf among them; -8000 where next to
-// nothing is left).  Its nearest whole number is the bin; 2^(t / 128) is a power of two from a table of 128, times a polynomial of degree 4
-// on +-ln2 / 256 (remainder < 2^-49 relative); as whole numbers of 2^-shift (shift <= 50: the add of 2^52 rounds).  Some 20 instructions; a
-// series of degree 11 and the conversion to 64 bits took 40 (this pass over 512 rows of 100000: 99 us, 84 so).
+// Masses of a row's candidates relative to its best score, by t = 128 log2(mass) (0 for the best score, +inf among them; -16000 where nothing
+// is left).  Its nearest whole number is the bin; 2^(t / 128) is a power of two from a table of 128, times a polynomial of degree 4
+// on +-ln2 / 256 (remainder < 2^-49 relative).  Some 20 instructions; a series of degree 11 and the conversion to 64 bits took 40 (this pass over 512
+// rows of 100000: 99 us, 84 so).
+// A bin's are added up as whole numbers, so that no order matters, in a unit of its octave (the power of two at or above the bin): 2^-(shift +
+// octave).  In one unit for all of them the tail of a very wide row would round away (2^25 masses of 2^-37); so each is kept to 2^-(shift + 1) of
+// itself, 2^-45 at 100000 scores and 2^-32 at 2^30, down to 2^-32 of the best one's, and to 2^-(shift + 33) of that below (the last bin): the
+// sums are right to 2^-31 at any width.  A bin's sum fits 64 bits (width * 2^(shift + 1) <= 2^62); the sums along the bins are float64, always
+// added in the same order.
+constexpr int SB_OCTAVES = SB_BINS / SB_PER;
+__device__ __forceinline__ int octave_of(int bin) { return (bin + SB_PER - 1) / SB_PER; }
 struct row_mass {
   float best;
   double c;      // 128 log2(e) / temperature
+  int shift;
   double scale;  // 2^shift
   bool greedy;
   const double* powers;  // 2^(j / 128), in LDS
-  __device__ __forceinline__ double t_of(float x) const { return x == best ? 0.0 : greedy ? -8000.0 : fmax(((double)x - (double)best) * c, -8000.0); }
+  __device__ __forceinline__ double t_of(float x) const { return x == best ? 0.0 : greedy ? -16000.0 : fmax(((double)x - (double)best) * c, -16000.0); }
   __device__ __forceinline__ int bin(double t) const { return min(-(int)rint(t), SB_BINS - 1); }
-  __device__ __forceinline__ double part(double t) const {
+  __device__ __forceinline__ double in_octave(double t) const {  // the mass times 2^octave: 1 .. 2, less in the last bin
     constexpr double L = 0.69314718055994530942 / SB_PER;
     const double n = rint(t), f = t - n;
     const int i = (int)n;
@@ -1007,11 +1017,26 @@ struct row_mass {
     q = fma(q, f, in_scalar(L * L / 2.0));
     q = fma(q, f, in_scalar(L));
     q = fma(q, f, 1.0);
-    return ldexp(powers[i & (SB_PER - 1)], i >> 7) * q;
+    return ldexp(powers[i & (SB_PER - 1)], min((i >> 7) + SB_OCTAVES, 0)) * q;
   }
-  __device__ __forceinline__ unsigned long long whole(double part) const { return (unsigned long long)__double_as_longlong(fma(part, scale, 0x1p52)) ^ 0x4330000000000000ull; }
-  __device__ __forceinline__ unsigned long long mass(double t) const { return whole(part(t)); }
+  __device__ __forceinline__ double value(double t) const { return ldexp(in_octave(t), -octave_of(bin(t))); }
+  // (shift <= 50: the add of 2^52 rounds)
+  __device__ __forceinline__ unsigned long long whole(double in_octave) const { return (unsigned long long)__double_as_longlong(fma(in_octave, scale, 0x1p52)) ^ 0x4330000000000000ull; }
+  __device__ __forceinline__ unsigned long long mass(double t) const { return whole(in_octave(t)); }
+  __device__ __forceinline__ double sum(unsigned long long masses, int bin) const { return ldexp((double)masses, -shift - octave_of(bin)); }
+  __device__ __forceinline__ double kept(double t) const { return sum(mass(t), bin(t)); }  // the mass as it is added up
 };
+// The bins around min_p: every candidate in front of them has more than min_p of the best one's mass, those behind them have less; `above` adds up
+// those inside that have as much, in units of 2^-(shift + unit).  (A logarithm in float32 is off by less than a hundredth of a bin.)  No min_p: none.
+struct near_bins {
+  int first, last, unit;
+  __device__ __forceinline__ bool holds(int b) const { return b >= first && b <= last; }
+};
+__device__ __forceinline__ near_bins near_of(const row_mass& rm, float min_p) {
+  if (!(min_p > 0.0f)) return {SB_BINS, -1, 0};
+  const int b = rm.bin(fmax((double)(SB_PER * __builtin_amdgcn_logf(min_p)), -16000.0)), first = max(b - 1, 0);
+  return {first, min(b + 1, SB_BINS - 1), min(octave_of(first) + 1, SB_OCTAVES)};
+}
 // (every thread of the workgroup; a barrier has to follow; without `powers` for t and bins only)
 __device__ __forceinline__ row_mass rm_make(uint32_t best, const row_set& s, int shift, double* powers) {
   if (powers && threadIdx.x < SB_PER) powers[threadIdx.x] = 2.0 * exp2_le0((double)threadIdx.x / SB_PER - 1.0);
@@ -1019,6 +1044,7 @@ __device__ __forceinline__ row_mass rm_make(uint32_t best, const row_set& s, int
   rm.best = score_of(best);
   rm.greedy = s.temperature == 0.0f;
   rm.c = rm.greedy ? 1.0 : 1.4426950408889634074 * SB_PER / (double)s.temperature;
+  rm.shift = shift;
   rm.scale = ldexp(1.0, shift);
   rm.powers = powers;
   return rm;
@@ -1027,8 +1053,8 @@ __device__ __forceinline__ row_mass rm_make(uint32_t best, const row_set& s, int
 // a row's part of the workspace
 struct row_ws {
   unsigned long long hist_m[SB_BINS];  // masses per bin
-  unsigned long long above, count;     // mass of the candidates with at least min_p of the best one's mass; candidates
-  unsigned long long total, before[2]; // all mass; the masses in front of the lists' bins
+  unsigned long long above, count;     // mass of the candidates of the bins around min_p that reach it (near_bins); candidates
+  double total, most, before[2];       // all mass; that of the candidates that reach min_p; the masses in front of the lists' bins
   unsigned long long list[2][SB_CAP];  // candidates of bin b1 (where top-p ends) and of the bins b2 (where the draw can fall)
   uint32_t hist_c[SB_BINS];            // candidates per bin
   uint32_t n_list[2];
@@ -1038,73 +1064,102 @@ struct row_ws {
 
 struct seek_shared {
   unsigned long long list[SL_CAP];
-  unsigned long long red64[SL_THREADS / 64];
-  unsigned long long before64, mass64;
+  double red64[SL_THREADS / 64];
+  double before64;
   uint32_t red32[SL_THREADS / 64];
   uint32_t n_list, before32, bin, digit, found;
   unsigned long long hist_m[256];
   uint32_t hist_c[256];
 };
 
-// Cumulative masses (and counts) over the bins, thread t owning the bins [t PB, (t + 1) PB): before[] are the sums in front of them.
+// Cumulative masses or counts over the bins, four to a thread (in rounds, if the workgroup has fewer than 1024): bin_at(i) starts at before[i] and
+// ends where the next one starts, at end(before, i).  The adds come in the same order whatever the number of threads.
 template <int THREADS>
-__device__ __forceinline__ unsigned long long scan_bins(const unsigned long long (&v)[SB_BINS / THREADS], unsigned long long (&before)[SB_BINS / THREADS],
-                                                        unsigned long long* red) {
-  unsigned long long own = 0;
+struct bin_sums {
+  static constexpr int ROUNDS = SB_BINS / 4 / THREADS, N = ROUNDS * 4;
+  static __device__ __forceinline__ int bin_at(int i) { return ((i >> 2) * THREADS + (int)threadIdx.x) * 4 + (i & 3); }
+  template <class V> using sums = V[ROUNDS * 5];  // (a round: four bins, and the end of the last one)
+  template <class V>
+  static __device__ __forceinline__ const V& start(const sums<V>& before, int i) { return before[(i >> 2) * 5 + (i & 3)]; }
+  template <class V>
+  static __device__ __forceinline__ const V& end(const sums<V>& before, int i) { return before[(i >> 2) * 5 + (i & 3) + 1]; }
+  // value(bin) -> V; returns the total.  red: SB_BINS / 256 entries
+  template <class V, class F>
+  static __device__ __forceinline__ V scan(F&& value, sums<V>& before, V* red) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    V incl[ROUNDS];
 #pragma unroll
-  for (int i = 0; i < SB_BINS / THREADS; ++i) own += v[i];
-  const unsigned long long incl = wave_scan_u64(own);
-  const int wave = threadIdx.x >> 6;
-  __syncthreads();
-  if ((threadIdx.x & 63) == 63) red[wave] = incl;
-  __syncthreads();
-  unsigned long long run = incl - own, total = 0;
+    for (int q = 0; q < ROUNDS; ++q) {
+      V run = 0;
 #pragma unroll
-  for (int w = 0; w < THREADS / 64; ++w) {
-    run += w < wave ? red[w] : 0ull;
-    total += red[w];
+      for (int i = 0; i < 4; ++i) {
+        before[q * 5 + i] = run;
+        run += value(bin_at(q * 4 + i));
+      }
+      incl[q] = wave_scan(run);
+    }
+    __syncthreads();
+#pragma unroll
+    for (int q = 0; q < ROUNDS; ++q)
+      if (lane == 63) red[q * (THREADS / 64) + wave] = incl[q];
+    __syncthreads();
+    V at[ROUNDS] = {}, total = 0;
+#pragma unroll
+    for (int w = 0; w < SB_BINS / 256; ++w) {
+#pragma unroll
+      for (int q = 0; q < ROUNDS; ++q) at[q] = w == q * (THREADS / 64) + wave ? total : at[q];
+      total += red[w];
+    }
+#pragma unroll
+    for (int q = 0; q < ROUNDS; ++q) {
+      const V first = at[q] + below(incl[q], lane), last = at[q] + incl[q];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) before[q * 5 + i] = min(first + before[q * 5 + i], last);  // (rounding: no bin ends before it starts)
+      before[q * 5 + 4] = last;
+    }
+    return total;
   }
-#pragma unroll
-  for (int i = 0; i < SB_BINS / THREADS; ++i) {
-    before[i] = run;
-    run += v[i];
+  static __device__ __forceinline__ double below(double v, int lane) {
+    const double t = __shfl_up(v, 1);
+    return lane > 0 ? t : 0.0;
   }
-  return total;
-}
+  static __device__ __forceinline__ unsigned long long below(unsigned long long v, int lane) {
+    const unsigned long long t = __shfl_up(v, 1);
+    return lane > 0 ? t : 0ull;
+  }
+};
 
-__device__ __forceinline__ unsigned long long border_of(float top_p, unsigned long long total) { return max((unsigned long long)ceil((double)top_p * (double)total), 1ull); }
-__device__ __forceinline__ unsigned long long want_of(float u, unsigned long long kept) {
+// what a cumulative mass has to reach: top_p of the total; more than u of what is kept (u < 1)
+__device__ __forceinline__ double border_of(float top_p, double total) { return fmax((double)top_p * total, DBL_MIN); }
+__device__ __forceinline__ double want_of(float u, double kept) {
   u = u > 0.0f ? fminf(u, 0x1.fffffep-1f) : 0.0f;
-  return min((unsigned long long)floor((double)u * (double)kept) + 1ull, kept);
+  return fmin(nextafter((double)u * kept, (double)INFINITY), kept);
 }
 
 // First candidate in rank order with (by_count: rank + 1 >= target; otherwise: cumulative mass up to and with it >= target).
-// m / bm: this thread's bins and the masses before them, c / bc: the same in counts (by_count only).  ahead / n_ahead: the candidates of
-// the bins lo .. hi, if they were collected (n_ahead >= 0).  Returns its index (-1: none) and, in *incl / *own, the cumulative mass with it
-// and its own.
-constexpr int SEEK_PB = SB_BINS / SL_THREADS;
+// bm / bc: the masses and counts (by_count only) in front of this thread's bins.  ahead / n_ahead: the candidates of the bins lo .. hi, if they
+// were collected (n_ahead >= 0).  Returns its index (-1: none) and, in *incl, the cumulative mass with it.
+using seek_sums = bin_sums<SL_THREADS>;
 template <class T>
-__device__ __forceinline__ int seek(const T* p, int len, const row_mass& rm, const unsigned long long (&m)[SEEK_PB], const unsigned long long (&bm)[SEEK_PB],
-                                    const unsigned long long (&c)[SEEK_PB], const unsigned long long (&bc)[SEEK_PB], bool by_count, unsigned long long target,
-                                    seek_shared& sh, const unsigned long long* ahead, int n_ahead, int lo, int hi, unsigned long long* incl, unsigned long long* own) {
+__device__ __forceinline__ int seek(const T* p, int len, const row_mass& rm, const seek_sums::sums<double>& bm, const seek_sums::sums<unsigned long long>& bc, bool by_count,
+                                    double target, int count, seek_shared& sh, const unsigned long long* ahead, int n_ahead, int lo, int hi, double* incl) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   if (threadIdx.x == 0) sh.bin = SB_BINS, sh.n_list = 0, sh.found = 0xffffffffu;
   __syncthreads();
 #pragma unroll
-  for (int i = 0; i < SEEK_PB; ++i) {
-    const unsigned long long run = by_count ? bc[i] : bm[i], step = by_count ? c[i] : m[i];
-    if (run < target && run + step >= target) sh.bin = threadIdx.x * SEEK_PB + i;
-  }
+  for (int i = 0; i < seek_sums::N; ++i)
+    if (by_count ? bc[i] < (unsigned long long)count && bc[i + 1] >= (unsigned long long)count : bm[i] < target && bm[i + 1] >= target)
+      atomicMin(&sh.bin, (uint32_t)seek_sums::bin_at(i));  // (rounding can let two neighbours end at the same mass)
   __syncthreads();
   const bool have = n_ahead >= 0 && (int)sh.bin >= lo && (int)sh.bin <= hi;  // (never by count)
 #pragma unroll
-  for (int i = 0; i < SEEK_PB; ++i)
-    if ((int)threadIdx.x * SEEK_PB + i == (have ? lo : (int)sh.bin)) sh.before64 = bm[i], sh.before32 = (uint32_t)bc[i];
+  for (int i = 0; i < seek_sums::N; ++i)
+    if (seek_sums::bin_at(i) == (have ? lo : (int)sh.bin)) sh.before64 = bm[i], sh.before32 = (uint32_t)bc[i];
   __syncthreads();
   const int b = (int)sh.bin;
   if (b >= SB_BINS) return -1;
-  unsigned long long mass_before = sh.before64;
-  unsigned long long count_before = sh.before32;
+  double mass_before = sh.before64;
+  int count_before = (int)sh.before32;
   int n = n_ahead;
   if (have && n > 256) {
     for (int i = threadIdx.x; i < n; i += SL_THREADS) sh.list[i] = ahead[i];
@@ -1129,27 +1184,25 @@ __device__ __forceinline__ int seek(const T* p, int len, const row_mass& rm, con
 #pragma unroll
       for (int i = 0; i < 4; ++i) e[i] = i * 64 + lane < n ? from[i * 64 + lane] : 0ull;
       rank_row<4>(e, sh.list, lane);
-      unsigned long long run = mass_before;
+      double run = mass_before;
       bool looking = true;
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const int rank = i * 64 + lane;
-        const unsigned long long mine = rank < n ? rm.mass(rm.t_of(score_of((uint32_t)(sh.list[rank] >> 32)))) : 0ull;
-        const unsigned long long cum = run + wave_scan_u64(mine);
-        const unsigned long long pass = __ballot(rank < n && (by_count ? count_before + rank + 1 == target : cum >= target));
+        const double cum = run + wave_scan(rank < n ? rm.kept(rm.t_of(score_of((uint32_t)(sh.list[rank] >> 32)))) : 0.0);
+        const unsigned long long pass = __ballot(rank < n && (by_count ? count_before + rank + 1 == count : cum >= target || rank == n - 1));  // (rounding: the last one)
         if (looking && pass) {
           const int who = (int)__ffsll((long long)pass) - 1;
           looking = false;
-          if (lane == who) sh.found = (uint32_t)rank, sh.before64 = cum, sh.mass64 = mine;
+          if (lane == who) sh.found = (uint32_t)rank, sh.before64 = cum;
         }
-        run = lane_u64(cum, 63);
+        run = lane_f64(cum, 63);
       }
     }
     __syncthreads();
     const uint32_t f = sh.found;
     const unsigned long long got = f == 0xffffffffu ? 0ull : sh.list[f];
     *incl = sh.before64;
-    *own = sh.mass64;
     __syncthreads();
     return f == 0xffffffffu ? -1 : (int)~(uint32_t)got;
   }
@@ -1161,36 +1214,31 @@ __device__ __forceinline__ int seek(const T* p, int len, const row_mass& rm, con
     // cumulative sums along the sorted list: 1024 entries at a time
     for (int i0 = 0; i0 < n; i0 += SL_THREADS) {
       const int i = i0 + threadIdx.x;
-      const unsigned long long mine = i < n ? rm.mass(rm.t_of(score_of((uint32_t)(sh.list[i] >> 32)))) : 0ull;
-      const unsigned long long s = wave_scan_u64(mine);
+      const double s = wave_scan(i < n ? rm.kept(rm.t_of(score_of((uint32_t)(sh.list[i] >> 32)))) : 0.0);
       __syncthreads();
       if (lane == 63) sh.red64[wave] = s;
       __syncthreads();
-      unsigned long long off = mass_before, all = 0;
+      double off = mass_before, all = 0.0;
       for (int w = 0; w < SL_THREADS / 64; ++w) {
-        off += w < wave ? sh.red64[w] : 0ull;
+        off += w < wave ? sh.red64[w] : 0.0;
         all += sh.red64[w];
       }
-      const unsigned long long cum = off + s;
-      const bool hit = i < n && (by_count ? count_before + i + 1 == target : cum >= target && cum - mine < target);
-      if (hit) {
-        sh.found = (uint32_t)i;
-        sh.before64 = cum;
-        sh.mass64 = mine;
-      }
+      const double cum = off + s;
+      if (i < n && (by_count ? count_before + i + 1 == count : cum >= target || i == n - 1)) atomicMin(&sh.found, (uint32_t)i);
       __syncthreads();
+      if (sh.found == (uint32_t)i) sh.before64 = cum;
       if (sh.found != 0xffffffffu) break;
       mass_before += all;
     }
+    __syncthreads();
     const uint32_t f = sh.found;
     const unsigned long long got = f == 0xffffffffu ? 0ull : sh.list[f];
     *incl = sh.before64;
-    *own = sh.mass64;
     __syncthreads();
     return f == 0xffffffffu ? -1 : (int)~(uint32_t)got;
   }
   // a bin of thousands: radix descent over the keys inside it, then the ties by index
-  uint32_t prefix = 0;
+  uint32_t prefix = 0, ties = 1;
   for (int shift = 24; shift >= 0; shift -= 8) {
     __syncthreads();
     for (int i = threadIdx.x; i < 256; i += SL_THREADS) sh.hist_m[i] = 0, sh.hist_c[i] = 0;
@@ -1206,27 +1254,30 @@ __device__ __forceinline__ int seek(const T* p, int len, const row_mass& rm, con
     }
     __syncthreads();
     if (threadIdx.x == 0) {
-      unsigned long long cc = count_before, mm = mass_before;
-      int d = 255;
-      for (; d > 0; --d) {
-        if (by_count ? cc + sh.hist_c[d] >= target : mm + sh.hist_m[d] >= target) break;
-        cc += sh.hist_c[d];
-        mm += sh.hist_m[d];
+      int cc = count_before, digit = 0, cc_at = cc;
+      double mm = mass_before, mm_at = mm;
+      for (int d = 255; d >= 0; --d) {  // (rounding may let none reach a target at the bin's end: the last one with candidates)
+        if (sh.hist_c[d] == 0) continue;
+        digit = d, cc_at = cc, mm_at = mm;
+        cc += (int)sh.hist_c[d];
+        mm += rm.sum(sh.hist_m[d], b);
+        if (by_count ? cc >= count : mm >= target) break;
       }
-      sh.digit = d;
-      sh.before32 = (uint32_t)cc;
-      sh.before64 = mm;
+      sh.digit = digit;
+      sh.before32 = (uint32_t)cc_at;
+      sh.before64 = mm_at;
     }
     __syncthreads();
     prefix |= sh.digit << shift;
-    count_before = sh.before32;
+    count_before = (int)sh.before32;
     mass_before = sh.before64;
+    ties = sh.hist_c[sh.digit];
   }
-  const unsigned long long each = rm.mass(rm.t_of(score_of(prefix)));
+  const double each = rm.kept(rm.t_of(score_of(prefix)));
   // the ordinal among the equal scores
-  const unsigned long long nth = by_count ? target - count_before : each ? (target - mass_before + each - 1) / each : 1ull;
-  *incl = mass_before + nth * each;
-  *own = each;
+  const double nth_of = each > 0.0 ? fmin(fmax(ceil((target - mass_before) / each), 1.0), (double)ties) : 1.0;
+  const unsigned long long nth = by_count ? (unsigned long long)(count - count_before) : (unsigned long long)nth_of;
+  *incl = mass_before + (double)nth * each;
   __syncthreads();
   if (threadIdx.x == 0) sh.found = 0xffffffffu, sh.n_list = 0;
   __syncthreads();
@@ -1314,12 +1365,13 @@ __global__ __launch_bounds__(SR_THREADS) void k_row_hist(sample_args a, row_ws* 
   slice_of(s.len, slices, sl, begin, end);
   unsigned long long above = 0, count = 0;
   const double least = (double)s.min_p;
+  const near_bins near = near_of(rm, s.min_p);
   scan_row<T>((const T*)a.scores + r * a.ld, begin, end, threadIdx.x, SR_THREADS, [&](int, const rp_vec<T, PIECE<T>>& v, int) __attribute__((always_inline)) {
 #pragma unroll
     for (int i = 0; i < PIECE<T>; ++i) {
       const uint32_t k = key_of(rp_to_f32(v.v[i]));
       if (k == 0) continue;
-      const double t = rm.t_of(score_of(k)), e = rm.part(t);
+      const double t = rm.t_of(score_of(k)), e = rm.in_octave(t);
       const unsigned long long m = rm.whole(e);
       const int b = rm.bin(t);
       if (m) atomicAdd(&hist_m[b], m);
@@ -1327,7 +1379,7 @@ __global__ __launch_bounds__(SR_THREADS) void k_row_hist(sample_args a, row_ws* 
         atomicAdd(&hist_c[b], 1u);
         ++count;
       }
-      if (e >= least) above += m;
+      if (near.holds(b) && ldexp(e, -octave_of(b)) >= least) above += m << (near.unit - octave_of(b));
     }
   });
   above = block_sum_u64<SR_THREADS>(above, red);
@@ -1346,57 +1398,67 @@ __global__ __launch_bounds__(SR_THREADS) void k_row_hist(sample_args a, row_ws* 
 // where top-p ends, and between which masses the draw falls: every thread of the workgroup
 struct row_bins {
   int b1, lo, hi;
-  unsigned long long total;
+  double total, most;
 };
 template <int THREADS, bool COUNT>
-__device__ __forceinline__ row_bins find_bins(const row_ws& ws, const row_set& s, float u, int shift, unsigned long long (&before)[SB_BINS / THREADS]) {
-  __shared__ unsigned long long red[THREADS / 64], range[2];
+__device__ __forceinline__ row_bins find_bins(const row_ws& ws, const row_mass& rm, const row_set& s, float u, const near_bins& near,
+                                              typename bin_sums<THREADS>::template sums<double>& before) {
+  using B = bin_sums<THREADS>;
+  __shared__ double red[SB_BINS / 256], range[2], ahead;
   __shared__ int bins[3];
-  constexpr int PB = SB_BINS / THREADS;
-  if (threadIdx.x == 0) bins[0] = -1, bins[1] = 0, bins[2] = -1;
-  unsigned long long m[PB];
+  if (threadIdx.x == 0) bins[0] = -1, bins[1] = SB_BINS, bins[2] = -1;
+  const double total = B::template scan<double>([&](int b) __attribute__((always_inline)) { return rm.sum(ws.hist_m[b], b); }, before, red);
 #pragma unroll
-  for (int i = 0; i < PB; ++i) m[i] = ws.hist_m[threadIdx.x * PB + i];
-  const unsigned long long total = scan_bins<THREADS>(m, before, red);
+  for (int i = 0; i < B::N; ++i)
+    if (B::bin_at(i) == near.first) ahead = B::start(before, i);
+  __syncthreads();
+  const double most = near.last < 0 ? total : ahead + ldexp((double)ws.above, -rm.shift - near.unit);
   const bool known = s.temperature != 0.0f && !(COUNT && (unsigned long long)s.k < ws.count);  // (otherwise the total itself is not known yet)
   if (known) {
-    const unsigned long long border = border_of(s.top_p, total);
+    const double border = border_of(s.top_p, total);
     const bool cuts = s.top_p < 1.0f && border < total;
     if (threadIdx.x == 0) range[0] = range[1] = total;
     __syncthreads();
     if (cuts) {
 #pragma unroll
-      for (int i = 0; i < PB; ++i)
-        if (before[i] < border && before[i] + m[i] >= border) bins[0] = threadIdx.x * PB + i, range[0] = border, range[1] = before[i] + m[i];
+      for (int i = 0; i < B::N; ++i)
+        if (B::start(before, i) < border && B::end(before, i) >= border) atomicMax(&bins[0], B::bin_at(i));  // (rounding can let two neighbours end at the same mass)
     }
     __syncthreads();
-    const unsigned long long most = max(ws.above, 1ull << shift);
-    const unsigned long long w0 = want_of(u, min(range[0], most)), w1 = want_of(u, min(range[1], most));
 #pragma unroll
-    for (int i = 0; i < PB; ++i) {
-      if (before[i] < w0 && before[i] + m[i] >= w0) bins[1] = threadIdx.x * PB + i;
-      if (before[i] < w1 && before[i] + m[i] >= w1) bins[2] = threadIdx.x * PB + i;
+    for (int i = 0; i < B::N; ++i)
+      if (B::bin_at(i) == bins[0]) range[0] = border, range[1] = B::end(before, i);
+    __syncthreads();
+    const double w0 = want_of(u, fmin(range[0], most)), w1 = want_of(u, fmin(range[1], most));
+#pragma unroll
+    for (int i = 0; i < B::N; ++i) {
+      if (B::start(before, i) < w0 && B::end(before, i) >= w0) atomicMin(&bins[1], B::bin_at(i));
+      if (B::start(before, i) < w1 && B::end(before, i) >= w1) atomicMax(&bins[2], B::bin_at(i));
     }
   }
   __syncthreads();
-  return {bins[0], bins[1], bins[2], total};
+  return {bins[0], bins[1], bins[2], total, most};
 }
 template <int THREADS>
-__device__ __forceinline__ void keep_bins(row_ws& ws, const row_bins& b, const unsigned long long (&before)[SB_BINS / THREADS]) {
-  constexpr int PB = SB_BINS / THREADS;
-  if (threadIdx.x == 0) ws.b1 = b.b1, ws.b2_lo = b.lo, ws.b2_hi = b.hi, ws.total = b.total;
+__device__ __forceinline__ void keep_bins(row_ws& ws, const row_bins& b, const typename bin_sums<THREADS>::template sums<double>& before) {
+  using B = bin_sums<THREADS>;
+  if (threadIdx.x == 0) ws.b1 = b.b1, ws.b2_lo = b.lo, ws.b2_hi = b.hi, ws.total = b.total, ws.most = b.most;
 #pragma unroll
-  for (int i = 0; i < PB; ++i) {
-    if ((int)threadIdx.x * PB + i == b.b1) ws.before[0] = before[i];
-    if ((int)threadIdx.x * PB + i == b.lo) ws.before[1] = before[i];
+  for (int i = 0; i < B::N; ++i) {
+    if (B::bin_at(i) == b.b1) ws.before[0] = B::start(before, i);
+    if (B::bin_at(i) == b.lo) ws.before[1] = B::start(before, i);
   }
 }
 template <bool COUNT>
-__global__ __launch_bounds__(SL_THREADS) void k_row_bins(sample_args a, row_ws* __restrict__ wss, int shift) {
+__global__ __launch_bounds__(SL_THREADS) void k_row_bins(sample_args a, row_ws* __restrict__ wss, int slices, int shift) {
   const int64_t r = a.row0 + blockIdx.x;
   row_ws& ws = wss[blockIdx.x];
-  unsigned long long before[SB_BINS / SL_THREADS];
-  const row_bins b = find_bins<SL_THREADS, COUNT>(ws, rs_load(a, r), a.u[r * a.ld_u], shift, before);
+  const row_set s = rs_load(a, r);
+  const uint32_t best = best_of(ws, slices);
+  if (best == 0) return;
+  bin_sums<SL_THREADS>::sums<double> before;
+  const row_mass rm = rm_make(best, s, shift, nullptr);
+  const row_bins b = find_bins<SL_THREADS, COUNT>(ws, rm, s, a.u[r * a.ld_u], near_of(rm, s.min_p), before);
   keep_bins<SL_THREADS>(ws, b, before);
 }
 
@@ -1428,11 +1490,11 @@ __global__ __launch_bounds__(SR_THREADS) void k_row_collect(sample_args a, row_w
   __syncthreads();
   row_bins bins;
   if constexpr (FIND) {
-    unsigned long long before[SB_BINS / SR_THREADS];
-    bins = find_bins<SR_THREADS, COUNT>(ws, s, a.u[r * a.ld_u], shift, before);
+    bin_sums<SR_THREADS>::sums<double> before;
+    bins = find_bins<SR_THREADS, COUNT>(ws, rm, s, a.u[r * a.ld_u], near_of(rm, s.min_p), before);
     if (sl == 0) keep_bins<SR_THREADS>(ws, bins, before);
   } else {
-    bins = {ws.b1, ws.b2_lo, ws.b2_hi, 0};
+    bins = {ws.b1, ws.b2_lo, ws.b2_hi, 0, 0};
   }
   const int b1 = bins.b1, lo = bins.lo, hi = bins.hi;
   if (b1 < 0 && hi < lo) return;
@@ -1469,10 +1531,11 @@ __global__ __launch_bounds__(SR_THREADS) void k_row_collect(sample_args a, row_w
 
 // A list of at most 256 candidates, ranked by four waves: sorted[] and the cumulative masses with those in front of the list, and each one's own.
 struct ranked_list {
-  unsigned long long runs[256], sorted[256], cum[256], own[256], sum[4];
+  unsigned long long runs[256], sorted[256];
+  double cum[256], own[256], sum[4];
 };
 // the first rank whose cumulative mass reaches the target (n if none); a whole wave
-__device__ __forceinline__ int rank_reaching(const ranked_list& l, int n, unsigned long long target, int lane) {
+__device__ __forceinline__ int rank_reaching(const ranked_list& l, int n, double target, int lane) {
   int at = n;
 #pragma unroll
   for (int i = 3; i >= 0; --i) {
@@ -1496,7 +1559,8 @@ __device__ __forceinline__ void nothing_drawn(const sample_args& a, int64_t r) {
 // the draw from what was collected; a workgroup of SL_THREADS
 template <class T, bool COUNT>
 __device__ __forceinline__ void draw_row(const sample_args& a, int64_t r, const row_set& s, const T* p, const row_mass& rm, const row_ws& ws, draw_shared& sh) {
-  __shared__ unsigned long long red64[SL_THREADS / 64];
+  __shared__ double red_m[SB_BINS / 256];
+  __shared__ unsigned long long red_c[SB_BINS / 256];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int b1 = ws.b1, b2_lo = ws.b2_lo, b2_hi = ws.b2_hi;
   const int n1 = b1 >= 0 && ws.n_list[0] <= SB_CAP ? (int)ws.n_list[0] : -1;
@@ -1505,71 +1569,67 @@ __device__ __forceinline__ void draw_row(const sample_args& a, int64_t r, const 
   unsigned long long e = t;
   if (which < 2 && t < (which == 0 ? n1 : n2)) e = ws.list[which][t];
   __syncthreads();
-  const unsigned long long most = max(ws.above, (unsigned long long)rm.scale);
+  const double most = ws.most;
   const bool cut_by_count = COUNT && (unsigned long long)s.k < ws.count;
   // the common case - both lists are there and short: four waves each, side by side
   if (!cut_by_count && !rm.greedy && (b1 < 0 || (n1 >= 1 && n1 <= 256)) && n2 >= 1 && n2 <= 256) {
     const bool on = which == 1 || (which == 0 && b1 >= 0);
     ranked_list& mine = sh.two[which & 1];
     const int rank = rank_256(e, mine.runs, mine.sorted, t, on);
-    unsigned long long own = 0, cum = 0, before = ws.before[which & 1];
-    if (on) {  // (this thread's entry, where it belongs)
-      own = rank < (which == 0 ? n1 : n2) ? rm.mass(rm.t_of(score_of((uint32_t)(e >> 32)))) : 0ull;
-      mine.own[rank] = own;
-    }
+    double cum = 0.0;
+    const double before = ws.before[which & 1];
+    // (this thread's entry, where it belongs)
+    if (on) mine.own[rank] = rank < (which == 0 ? n1 : n2) ? rm.kept(rm.t_of(score_of((uint32_t)(e >> 32)))) : 0.0;
     __syncthreads();
     if (on) {
-      cum = wave_scan_u64(mine.own[t]);
+      cum = wave_scan(mine.own[t]);
       if (lane == 63) mine.sum[wave & 3] = cum;
     }
     __syncthreads();
     if (on) {
       cum += before;
 #pragma unroll
-      for (int w = 0; w < 3; ++w) cum += w < (wave & 3) ? mine.sum[w] : 0ull;
+      for (int w = 0; w < 3; ++w) cum += w < (wave & 3) ? mine.sum[w] : 0.0;
       mine.cum[t] = cum;
     }
     __syncthreads();
     if (wave != 0) return;
-    unsigned long long kept = ws.total;
+    double kept = ws.total;
     if (b1 >= 0) kept = sh.two[0].cum[min(rank_reaching(sh.two[0], n1, border_of(s.top_p, kept), lane), n1 - 1)];
-    kept = min(kept, most);
+    kept = fmin(kept, most);
     const int at_rank = min(rank_reaching(sh.two[1], n2, want_of(a.u[r * a.ld_u], kept), lane), n2 - 1);
     if (lane == 0) {
-      const int at = (int)~(uint32_t)sh.two[1].sorted[at_rank];
+      const unsigned long long entry = sh.two[1].sorted[at_rank];
+      const int at = (int)~(uint32_t)entry;
       a.idx[r] = a.ids ? a.ids[r * a.ld_ids + at] : at;
-      a.prob[r] = (float)((double)sh.two[1].own[at_rank] / (double)kept);
+      a.prob[r] = (float)(rm.value(rm.t_of(score_of((uint32_t)(entry >> 32)))) / kept);
       if (a.nnz) a.nnz[r] = 1;
     }
     return;
   }
-  unsigned long long incl = 0, own = 0, m[SEEK_PB], bm[SEEK_PB], c[SEEK_PB], bc[SEEK_PB];
-#pragma unroll
-  for (int i = 0; i < SEEK_PB; ++i) {
-    m[i] = ws.hist_m[threadIdx.x * SEEK_PB + i];
-    c[i] = COUNT ? ws.hist_c[threadIdx.x * SEEK_PB + i] : 0u;
-    bc[i] = 0;
-  }
-  unsigned long long total = scan_bins<SL_THREADS>(m, bm, red64);
+  double incl = 0.0;
+  seek_sums::sums<double> bm;
+  seek_sums::sums<unsigned long long> bc = {};
+  double total = seek_sums::scan<double>([&](int b) __attribute__((always_inline)) { return rm.sum(ws.hist_m[b], b); }, bm, red_m);
   if (cut_by_count) {
-    scan_bins<SL_THREADS>(c, bc, red64);
-    seek<T>(p, s.len, rm, m, bm, c, bc, true, (unsigned long long)s.k, sh.seek, nullptr, -1, 0, -1, &incl, &own);
+    seek_sums::scan<unsigned long long>([&](int b) __attribute__((always_inline)) { return (unsigned long long)ws.hist_c[b]; }, bc, red_c);
+    seek<T>(p, s.len, rm, bm, bc, true, 0.0, s.k, sh.seek, nullptr, -1, 0, -1, &incl);
     total = incl;
   }
-  unsigned long long kept = total;
+  double kept = total;
   if (s.top_p < 1.0f && !rm.greedy) {
-    const unsigned long long border = border_of(s.top_p, total);
+    const double border = border_of(s.top_p, total);
     if (border < kept) {
-      seek<T>(p, s.len, rm, m, bm, c, bc, false, border, sh.seek, ws.list[0], n1, b1, b1, &incl, &own);
+      seek<T>(p, s.len, rm, bm, bc, false, border, 0, sh.seek, ws.list[0], n1, b1, b1, &incl);
       kept = incl;
     }
   }
-  if (!rm.greedy) kept = min(kept, most);
-  const unsigned long long want = rm.greedy ? 1ull : want_of(a.u[r * a.ld_u], kept);
-  const int at = seek<T>(p, s.len, rm, m, bm, c, bc, false, want, sh.seek, ws.list[1], n2, b2_lo, b2_hi, &incl, &own);
+  if (!rm.greedy) kept = fmin(kept, most);
+  const double want = rm.greedy ? DBL_MIN : want_of(a.u[r * a.ld_u], kept);
+  const int at = seek<T>(p, s.len, rm, bm, bc, false, want, 0, sh.seek, ws.list[1], n2, b2_lo, b2_hi, &incl);
   if (threadIdx.x == 0) {
     a.idx[r] = at < 0 ? -1 : a.ids ? a.ids[r * a.ld_ids + at] : at;
-    a.prob[r] = at < 0 ? 0.0f : rm.greedy ? 1.0f : (float)((double)own / (double)kept);
+    a.prob[r] = at < 0 ? 0.0f : rm.greedy ? 1.0f : (float)(rm.value(rm.t_of(rp_to_f32(p[at]))) / kept);
     if (a.nnz) a.nnz[r] = at < 0 ? 0 : 1;
   }
 }
@@ -1587,8 +1647,8 @@ __global__ __launch_bounds__(SL_THREADS) void k_row_draw(sample_args a, const ro
   draw_row<T, COUNT>(a, r, s, (const T*)a.scores + r * a.ld, rm, ws, sh);
 }
 
-// ... all of it in one launch, a workgroup to a row, its workspace in LDS (118 KB: one to a CU).  Bound by the vector unit (some 25 instructions
-// in 64 bits a score and the LDS atomics) and by what one workgroup has under way: 512 rows of 100000 in f32 156 us, where reading them takes 43.
+// ... all of it in one launch, a workgroup to a row, its workspace in LDS (151 KB with the draw's: one to a CU).  Bound by the vector unit (some 25 instructions
+// in 64 bits a score and the LDS atomics) and by what one workgroup has under way: 512 rows of 100000 in f32 164 us, where reading them takes 43.
 struct one_shared {
   row_ws ws;
   draw_shared draw;
@@ -1620,12 +1680,13 @@ __global__ __launch_bounds__(SL_THREADS) void k_row_one(sample_args a, int shift
   __syncthreads();
   unsigned long long above = 0, count = 0;
   const double least = (double)s.min_p;
+  const near_bins near = near_of(rm, s.min_p);
   scan_row<T>(p, 0, s.len, threadIdx.x, SL_THREADS, [&](int, const rp_vec<T, PIECE<T>>& v, int) __attribute__((always_inline)) {
 #pragma unroll
     for (int i = 0; i < PIECE<T>; ++i) {
       const uint32_t k = key_of(rp_to_f32(v.v[i]));
       if (k == 0) continue;
-      const double t = rm.t_of(score_of(k)), e = rm.part(t);
+      const double t = rm.t_of(score_of(k)), e = rm.in_octave(t);
       const unsigned long long m = rm.whole(e);
       const int b = rm.bin(t);
       if (m) atomicAdd(&ws.hist_m[b], m);
@@ -1633,15 +1694,15 @@ __global__ __launch_bounds__(SL_THREADS) void k_row_one(sample_args a, int shift
         atomicAdd(&ws.hist_c[b], 1u);
         ++count;
       }
-      if (e >= least) above += m;
+      if (near.holds(b) && ldexp(e, -octave_of(b)) >= least) above += m << (near.unit - octave_of(b));
     }
   });
   above = block_sum_u64<SL_THREADS>(above, red64);
   if (COUNT) count = block_sum_u64<SL_THREADS>(count, red64);
   if (threadIdx.x == 0) ws.above = above, ws.count = count;
   __syncthreads();
-  unsigned long long before[SB_BINS / SL_THREADS];
-  const row_bins bins = find_bins<SL_THREADS, COUNT>(ws, s, u, shift, before);
+  bin_sums<SL_THREADS>::sums<double> before;
+  const row_bins bins = find_bins<SL_THREADS, COUNT>(ws, rm, s, u, near, before);
   keep_bins<SL_THREADS>(ws, bins, before);
   if (bins.b1 >= 0 || bins.hi >= bins.lo) {
     const row_ranges ranges = ranges_of(rm, bins);
@@ -1719,7 +1780,7 @@ extern "C" int rphip_sample(rphip_ctx* ctx, void* stream, int64_t rows, int64_t 
                    params->temperature_dev, params->top_p_dev, params->min_p_dev, params->top_k_dev, idx_dev, prob_dev, nnz_dev, 0};
   int bits = 0;
   while (((int64_t)1 << bits) < width) ++bits;
-  const int shift = 61 - bits;  // the row's masses add up to at most width * 2^shift
+  const int shift = 61 - bits;  // (row_mass: 31 .. 50)
   return rp_by_type(type, [&](auto tag) -> int {
     using T = typename decltype(tag)::T;
     const hipStream_t st = (hipStream_t)stream;
@@ -1767,7 +1828,7 @@ extern "C" int rphip_sample(rphip_ctx* ctx, void* stream, int64_t rows, int64_t 
           if (n <= 8) {
             k_row_collect<T, COUNT, true><<<dim3(n, slices), SR_THREADS, 0, st>>>(a, ws, slices, shift);
           } else {
-            k_row_bins<COUNT><<<n, SL_THREADS, 0, st>>>(a, ws, shift);
+            k_row_bins<COUNT><<<n, SL_THREADS, 0, st>>>(a, ws, slices, shift);
             RP_LAUNCHED();
             k_row_collect<T, COUNT, false><<<dim3(n, slices), SR_THREADS, 0, st>>>(a, ws, slices, shift);
           }

@@ -1,0 +1,125 @@
+"""The 4-bit and sampling operators where rounding decides: far tails of wide rows, exact products in every tile shape, sums that must not depend on the batch."""
+import decimal
+import math
+
+import numpy as np
+import pytest
+import torch
+
+from test_gpu_ops import check_sample, gen
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def ctx():
+    from recpack_amd import get_context
+
+    return get_context(0)
+
+
+@pytest.fixture(scope="module")
+def ops():
+    from recpack_amd import ops
+
+    return ops
+
+
+# ---- sampling: one best score and a flat tail far below ---------------------------------------------------------------------------------
+
+def tail_draw(width, at, below, u, top_p=1.0, top_k=0):
+    """The draw from a best score at index `at` and width - 1 equal ones `below` it, in 60 decimal digits: (index, probability)."""
+    with decimal.localcontext(decimal.Context(prec=60)):
+        D = decimal.Decimal
+        m = (-D(below)).exp()
+        n = min(top_k or width, width)  # kept ranks: the best one and n - 1 of the tail
+        if top_p < 1:
+            n = min(n, max(1, 1 + math.ceil((D(top_p) * (1 + (n - 1) * m) - 1) / m)))
+        kept = 1 + (n - 1) * m
+        want = (D(u) * kept - 1) / m
+        if want < 0:
+            return at, float(1 / kept)
+        # a draw within a hundredth of a candidate from the border between two says nothing (a mass is right to 2^-32 of itself, 2^25 of them to 2^-7)
+        assert D("0.01") < want % 1 < D("0.99"), want % 1
+        k = int(want)
+        return (k if k < at else k + 1), float(m / kept)
+
+
+TAILS = [(100_000, 26.0, 1.0), (100_000, 13.0, 0.5), (30_001, 24.5, 1.0), (2 ** 20 + 1, 28.0, 1.0), (2 ** 20 + 1, 30.0, 1.0)]
+
+
+@pytest.mark.parametrize("width,below,temperature", TAILS)
+@pytest.mark.parametrize("rows", [1, 12, 64])
+def test_sample_from_a_far_tail(ctx, ops, width, below, temperature, rows):
+    """A tail of 1e-7 of the mass, an item of which has 1e-12: drawn by uniforms next to 1, with the item's own probability."""
+    at = width // 3
+    x = torch.full((width,), -below)
+    x[at] = 0.0
+    us = [1 - 2.0 ** -24, 1 - 2.0 ** -23, 1 - 3 * 2.0 ** -24, 0.5]
+    x, u = x.cuda().expand(rows, width).contiguous(), torch.tensor([us[r % 4] for r in range(rows)]).view(rows, 1).cuda()
+    for setting in (dict(), dict(top_p=1 - 2.0 ** -23), dict(top_k=width - 5), dict(min_p=1e-14)):
+        idx, prob, n = ops.sample(ctx, x, u, temperature=temperature, **setting)
+        want = [tail_draw(width, at, below / temperature, us[r % 4], setting.get("top_p", 1.0), setting.get("top_k", 0)) for r in range(min(rows, 4))]
+        assert idx.view(-1).tolist() == [want[r % 4][0] for r in range(rows)]
+        # the masses' sum is right to 2^-31, a mass to 2^-45; one rounding to float32
+        np.testing.assert_allclose(prob.view(-1).double().cpu().numpy(), [want[r % 4][1] for r in range(rows)], rtol=2.0 ** -24 + 2.0 ** -30)
+        assert (n == 1).all()
+    idx, prob, _ = ops.sample(ctx, x, u, temperature=temperature, min_p=1e-9)  # (the tail is below it)
+    assert (idx == at).all() and (prob == 1).all()
+
+
+def test_sample_from_the_tail_of_a_very_wide_row(ctx, ops):
+    """2^25 items 25.75 below the best one have 2.2e-4 of the mass together."""
+    width, below, at = 2 ** 25 + 7, 25.75, 12_345
+    x = torch.full((1, width), -below, device="cuda")
+    x[0, at] = 0.0
+    for u in (0.25, 1 - 2.0 ** -12 + 2.0 ** -14, 1 - 2.0 ** -13, 1 - 2.0 ** -24):
+        for setting in (dict(), dict(top_p=1 - 2.0 ** -14), dict(top_k=2 ** 24)):
+            idx, prob, _ = ops.sample(ctx, x, torch.tensor([[u]], device="cuda"), **setting)
+            want = tail_draw(width, at, below, u, setting.get("top_p", 1.0), setting.get("top_k", 0))
+            assert int(idx) == want[0]
+            assert abs(float(prob) - want[1]) <= want[1] * (2.0 ** -24 + 2.0 ** -30)
+
+
+@pytest.mark.parametrize("below", [5.0, 18.0, 23.0, 40.0])
+def test_sample_from_a_tail_of_different_scores(ctx, ops, below):
+    """The same with a tail of different scores, in extended precision: index and probability."""
+    width = 100_000
+    x = torch.randn(1, width, generator=gen(3)) - below
+    x[0, 77] = 0.0
+    order = np.argsort(-x[0].double().numpy(), kind="stable")
+    m = np.exp(x[0].numpy().astype(np.longdouble)[order])
+    c = np.cumsum(m)
+    for u in (0.1, 0.9, 1 - 2.0 ** -12, 1 - 2.0 ** -20, 1 - 2.0 ** -23, 1 - 2.0 ** -24):
+        k = int(np.searchsorted(c, np.longdouble(u) * c[-1], side="right"))
+        idx, prob, _ = ops.sample(ctx, x.cuda(), torch.tensor([[u]], device="cuda"))
+        assert int(idx) == order[k]
+        assert abs(float(prob) - float(m[k] / c[-1])) <= float(m[k] / c[-1]) * (2.0 ** -24 + 2.0 ** -30)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("top_k", [0, 3000])
+def test_sample_alone_and_among_others(ctx, ops, dtype, top_k):
+    """Few rows (slices of them) and many (a workgroup each): the same draws, bit for bit."""
+    x = (torch.randn(70, 30_001, generator=gen(1)) * 4).to(dtype).cuda()
+    u = torch.rand(70, 1, generator=gen(2)).cuda()
+    for setting in (dict(), dict(temperature=0.3, top_p=0.9), dict(temperature=2.0, min_p=0.003)):
+        many = ops.sample(ctx, x, u, top_k=top_k, **setting)
+        for part in (slice(0, 1), slice(5, 25)):
+            for a, b in zip(many, ops.sample(ctx, x[part], u[part], top_k=top_k, **setting)):
+                assert torch.equal(a[part], b)
+
+
+@pytest.mark.parametrize("rows", [3, 70])
+def test_sample_min_p_on_a_border(ctx, ops, rows):
+    """Scores whose mass is min_p, a step above and a step below it, in bins on either side of an octave's end."""
+    width = 25_000
+    for octaves in (1, 3, 31, 32, 40):
+        x = torch.full((rows, width), -70.0)
+        x[:, 5] = 0.0
+        edge = np.float32(-octaves * math.log(2))
+        for i, v in enumerate((np.nextafter(edge, np.float32(0)), edge, np.nextafter(edge, np.float32(-99)), edge * np.float32(1.004), edge * np.float32(0.996))):
+            x[:, 100 + 50 * i] = float(v)
+        u = torch.linspace(0, 1, rows).view(rows, 1) * (1 - 2.0 ** -24)
+        check_sample(ctx, ops, x, u, min_p=2.0 ** -octaves)
+        check_sample(ctx, ops, x, u, min_p=float(np.nextafter(np.float32(2.0 ** -octaves), np.float32(0))))
