@@ -576,7 +576,7 @@ int rphip_mxfp4_gemm_nt(rphip_ctx* ctx, void* stream, int64_t M, int64_t N, int6
 /* Scores of histories against a quantised item-item matrix W (rows x cols, blocks along the columns): X @ similarity_matrix_
  * (recpack/algorithms/base.py:248) for n_users CSR rows,
  *   out[u, :] = sum over e in [indptr[u], indptr[u + 1]) of weights[e] * W[indices[e], :]     (weights NULL: 1)
- * in float32, one rounding to out_type.  Repeated entries count as often as they stand; entries outside [0, rows) count nothing and
+ * in float32, one rounding to out_type; a user's scores are the same bits alone and among any others.  Repeated entries count as often as they stand; entries outside [0, rows) count nothing and
  * indptr is read no further than nnz.  exclude_history != 0 (needs rows = cols; history removal of pipelines/pipeline.py:174-175): the
  * history's own items get -inf.  item_keep (cols bytes, NULL = all): items with 0 get -inf (postprocessing/filters.py:58-101). */
 int rphip_mxfp4_scores(rphip_ctx* ctx, void* stream, int64_t n_users, int64_t nnz, const int32_t* indptr_dev, const int32_t* indices_dev,

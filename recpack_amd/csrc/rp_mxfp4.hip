@@ -188,9 +188,9 @@ extern "C" int rphip_mxfp4_dequantize(rphip_ctx* ctx, void* stream, int64_t rows
 
 // ---- scores of histories -----------------------------------------------------------------------------------------------------------
 // out[u, :] = sum over the entries e of user u of w_e * W[idx_e, :], in f32.  The rows of a history are contiguous and their blocks run along
-// the output.  A workgroup takes (user, 2048 columns); its waves take groups of four entries in turn and add their sums up in wave order
-// (the result does not depend on the launch).
-constexpr int MXS_COLS = 64 * RP_MX;
+// the output.  A workgroup of four waves takes (user, 2048 columns).  The order of the adds does not depend on the number of users: a user's
+// scores are the same bits alone and in any batch.
+constexpr int MXS_COLS = 64 * RP_MX, MXS_WAVES = 4;
 
 // Which user and column tile.  Workgroups go to the 8 XCDs round-robin: while eight tiles are left each XCD takes one of them for all
 // users, so that its L2 meets every history's pieces (1 KB) of the popular rows; the remaining tiles go through the XCDs together.
@@ -213,16 +213,19 @@ struct mxs_chunk {
   float wgt;
 };
 template <bool WEIGHTED>
-__device__ __forceinline__ mxs_chunk mxs_entries(const int32_t* __restrict__ indices, const float* __restrict__ weights, int64_t e0, int64_t e1, int rows, bool mark, int c0,
-                                                 uint32_t* drop, int lane) {
-  mxs_chunk k = {-1, 0, 0.0f};
-  const int n = (int)min((int64_t)64, e1 - e0);
-  if (lane < n) {
+__device__ __forceinline__ mxs_chunk mxs_load(const int32_t* __restrict__ indices, const float* __restrict__ weights, int64_t e0, int64_t e1, int lane) {
+  mxs_chunk k = {-1, (int)min((int64_t)64, max(e1 - e0, (int64_t)0)), 0.0f};  // (m: entries)
+  if (lane < k.m) {
     k.idx = indices[e0 + lane];
-    if ((unsigned)k.idx >= (unsigned)rows) k.idx = -1;
     if (WEIGHTED) k.wgt = weights[e0 + lane];
-    if (mark && k.idx >= c0 && k.idx < c0 + MXS_COLS) atomicOr(&drop[(k.idx - c0) >> 5], 1u << (k.idx & 31));
   }
+  return k;
+}
+template <bool WEIGHTED>
+__device__ __forceinline__ mxs_chunk mxs_entries(mxs_chunk k, int rows, bool mark, int c0, uint32_t* drop, int lane) {  // (m: entries that count)
+  const int n = k.m;
+  if ((unsigned)k.idx >= (unsigned)rows) k.idx = -1;
+  if (mark && k.idx >= c0 && k.idx < c0 + MXS_COLS) atomicOr(&drop[(k.idx - c0) >> 5], 1u << (k.idx & 31));
   const unsigned long long good = __ballot(k.idx >= 0);
   k.m = (int)__popcll(good);
   if (k.m < n) {
@@ -237,25 +240,25 @@ __device__ __forceinline__ mxs_chunk mxs_entries(const int32_t* __restrict__ ind
 // history rows, the 16 columns of its right operand 16 MX blocks of them as they lie in memory (lane (block, row): 16 bytes and a
 // scale), its left operand a one per output row that picks one element of the 32.  Two such selections turn four rows' blocks into
 // 16 x 32 sums without a conversion: 64 elements a cycle and SIMD against 5 - 7 converted and added in the vector unit.  The selection
-// is laid out so that a lane ends with 8 neighbouring columns of its block.  Bound by the rows' bytes: 1024 histories of 50 against 50000 x
-// 50000 226 us, where each row read once and the scores written take 177 at the rate of a copy (238 us with the tiles in any order, 257 with
+// is laid out so that a lane ends with 8 neighbouring columns of its block.  A wave takes 512 of the 2048 columns and all entries, in their order, up to
+// 64 under way together (one wave for all columns, eight entries under way: 64 histories of 100 against 20000 x 20000 29 us, 16 so).  Bound by the rows'
+// bytes: 1024 histories of 50 against 50000 x 50000 230 us, where each row read once and the scores written take 177 at the rate of a copy (238 us with the tiles in any order, 257 with
 // the sums in the vector unit).
 typedef int mxs_i32x8 __attribute__((ext_vector_type(8)));
 typedef int mxs_i32x4 __attribute__((ext_vector_type(4)));
-constexpr int MXS_GROUPS = MXS_COLS / 512;  // fragments of 16 blocks
-template <class T, int WAVES>
-__global__ __launch_bounds__(64 * WAVES) void k_mx_scores_sum(const int32_t* __restrict__ indptr, const int32_t* __restrict__ indices, int64_t nnz, int rows, int cols, int nb,
+template <class T>
+__global__ __launch_bounds__(64 * MXS_WAVES) void k_mx_scores_sum(const int32_t* __restrict__ indptr, const int32_t* __restrict__ indices, int64_t nnz, int rows, int cols, int nb,
                                                               const uint8_t* __restrict__ codes, int64_t ldc, const uint8_t* __restrict__ scales, int64_t lds, int exclude,
                                                               const uint8_t* __restrict__ keep, T* __restrict__ out, int64_t ldo, int64_t user0, unsigned users, int tiles) {
+  constexpr int STEPS = 8;  // groups of four entries: half a chunk
   __shared__ uint32_t drop[64];  // bit c of word l: column 32 l + c of the tile gets -inf
-  __shared__ rp_f32x4 sums[WAVES > 1 ? WAVES * MXS_GROUPS * 2 * 64 : 1];
-  const int lane = threadIdx.x & 63, wave = WAVES > 1 ? __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) : 0;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int fr = lane & 15, fg = lane >> 4;
   unsigned user;
   int tile;
   mxs_task(users, tiles, user, tile);
   const int64_t u = user0 + user;
-  const int b0 = tile * 64;
+  const int b = tile * 64 + wave * 16 + fr;  // this lane's block
   if (wave == 0) drop[lane] = 0;
   __syncthreads();
   // left operand: output row q (this lane's fr) of half h picks element (q >> 2) * 8 + h * 4 + (q & 3) of every group's 32; code of 1.0: 2
@@ -266,111 +269,90 @@ __global__ __launch_bounds__(64 * WAVES) void k_mx_scores_sum(const int32_t* __r
 #pragma unroll
     for (int w = 0; w < 8; ++w) pick[h][w] = w == j / 8 ? 2 << (j % 8 * 4) : 0;
   }
-  rp_f32x4 acc[MXS_GROUPS][2];
-#pragma unroll
-  for (int q = 0; q < MXS_GROUPS; ++q)
-#pragma unroll
-    for (int h = 0; h < 2; ++h) acc[q][h] = rp_f32x4{0, 0, 0, 0};
-  int64_t co[MXS_GROUPS];  // this lane's blocks (past the row: the last one; not stored)
-#pragma unroll
-  for (int q = 0; q < MXS_GROUPS; ++q) co[q] = min(b0 + q * 16 + fr, nb - 1);
+  rp_f32x4 acc[2] = {{0, 0, 0, 0}, {0, 0, 0, 0}};
+  const int64_t at = min(b, nb - 1);  // (past the row: the last one; not stored)
   const int64_t e1 = min((int64_t)indptr[u + 1], nnz);
-  for (int64_t e0 = max((int64_t)indptr[u], (int64_t)0); e0 < e1; e0 += 64) {
-    const mxs_chunk ch = mxs_entries<false>(indices, nullptr, e0, e1, rows, exclude && wave == 0, tile * MXS_COLS, drop, lane);
-    mxs_i32x4 w[2][MXS_GROUPS];
-    int sc[2][MXS_GROUPS];
-    auto fetch = [&](auto tag, int k) __attribute__((always_inline)) {  // entries k .. k + 3, one a lane group; past the end: zeros
+  int64_t e0 = max((int64_t)indptr[u], (int64_t)0);
+  mxs_chunk next = mxs_load<false>(indices, nullptr, e0, e1, lane);
+  for (; e0 < e1; e0 += 64) {
+    const mxs_chunk ch = mxs_entries<false>(next, rows, exclude && wave == 0, tile * MXS_COLS, drop, lane);
+    next = mxs_load<false>(indices, nullptr, e0 + 64, e1, lane);
+    mxs_i32x4 w[2][STEPS];
+    int sc[2][STEPS];
+    auto fetch = [&](auto tag, int k0) __attribute__((always_inline)) {  // entries k .. k + 3, one a lane group; past the end: zeros
       constexpr int S = decltype(tag)::value;
-      const int64_t row = __shfl(ch.idx, (k + fg) & 63);
-      const bool there = k + fg < ch.m;
 #pragma unroll
-      for (int q = 0; q < MXS_GROUPS; ++q) {
-        w[S][q] = mxs_i32x4{0, 0, 0, 0};
-        sc[S][q] = 0;
-        if (there) {
-          w[S][q] = *(const mxs_i32x4*)(codes + row * ldc + co[q] * 16);
-          sc[S][q] = scales[row * lds + co[q]];
+      for (int t = 0; t < STEPS; ++t) {
+        const int k = k0 + t * 4;
+        const int64_t row = __shfl(ch.idx, (k + fg) & 63);
+        w[S][t] = mxs_i32x4{0, 0, 0, 0};
+        sc[S][t] = 0;
+        if (k + fg < ch.m) {
+          w[S][t] = *(const mxs_i32x4*)(codes + row * ldc + at * 16);
+          sc[S][t] = scales[row * lds + at];
         }
       }
     };
-    auto add = [&](auto tag) __attribute__((always_inline)) {
+    auto add = [&](auto tag, int k0) __attribute__((always_inline)) {
       constexpr int S = decltype(tag)::value;
 #pragma unroll
-      for (int q = 0; q < MXS_GROUPS; ++q) {
-        const mxs_i32x8 v = {w[S][q].x, w[S][q].y, w[S][q].z, w[S][q].w, 0, 0, 0, 0};
+      for (int t = 0; t < STEPS; ++t) {
+        if (k0 + t * 4 >= ch.m) break;
+        const mxs_i32x8 v = {w[S][t].x, w[S][t].y, w[S][t].z, w[S][t].w, 0, 0, 0, 0};
 #pragma unroll
-        for (int h = 0; h < 2; ++h) acc[q][h] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(pick[h], v, acc[q][h], 4, 4, 0, 127, 0, sc[S][q]);
+        for (int h = 0; h < 2; ++h) acc[h] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(pick[h], v, acc[h], 4, 4, 0, 127, 0, sc[S][t]);
       }
     };
-    constexpr int STEP = 4 * WAVES;
     using set0 = std::integral_constant<int, 0>;
     using set1 = std::integral_constant<int, 1>;
-    int k = wave * 4;
-    if (k < ch.m) {
-      fetch(set0{}, k);
-      for (; k < ch.m; k += 2 * STEP) {
-        fetch(set1{}, k + STEP);
-        add(set0{});
-        fetch(set0{}, k + 2 * STEP);
-        add(set1{});
+    if (ch.m > 0) {  // (both sets once; written without the loop they take more registers than four waves a SIMD leave)
+      fetch(set0{}, 0);
+      for (int k = 0; k < ch.m; k += 8 * STEPS) {
+        fetch(set1{}, k + 4 * STEPS);
+        add(set0{}, k);
+        if (k + 8 * STEPS < ch.m) fetch(set0{}, k + 8 * STEPS);
+        add(set1{}, k + 4 * STEPS);
       }
     }
-  }
-  // lane (fr, fg): columns 8 fg .. 8 fg + 7 of the blocks 16 q + fr
-  if (WAVES > 1) {
-#pragma unroll
-    for (int q = 0; q < MXS_GROUPS; ++q)
-#pragma unroll
-      for (int h = 0; h < 2; ++h) sums[((wave * MXS_GROUPS + q) * 2 + h) * 64 + lane] = acc[q][h];
   }
   __syncthreads();
+  // lane (fr, fg): columns 8 fg .. 8 fg + 7 of its block
+  if (b >= nb) return;
+  const int c = b * RP_MX + fg * 8, left = min(8, cols - c);
+  uint32_t gone = drop[wave * 16 + fr] >> (fg * 8);
+  if (keep)
+    for (int i = 0; i < left; ++i) gone |= keep[c + i] ? 0u : 1u << i;
+  float v[8];
 #pragma unroll
-  for (int q = 0; q < MXS_GROUPS; ++q) {
-    if (WAVES > 1) {
-      if (q % WAVES != wave) continue;  // (the waves share the fragments out)
+  for (int i = 0; i < 8; ++i) v[i] = (gone >> i) & 1 ? -INFINITY : acc[i >> 2][i & 3];
+  T* p = out + u * ldo + c;
+  if (left == 8) {
+    rp_vec<T, 8> t;
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        acc[q][h] = sums[q * 2 * 64 + h * 64 + lane];
+    for (int i = 0; i < 8; ++i) t.v[i] = rp_from_f32<T>(v[i]);
+    rp_store_vec<T, 8>(p, t);
+  } else {
 #pragma unroll
-        for (int o = 1; o < WAVES; ++o) acc[q][h] += sums[((o * MXS_GROUPS + q) * 2 + h) * 64 + lane];
-      }
-    }
-    const int b = b0 + q * 16 + fr;
-    if (b >= nb) continue;
-    const int c = b * RP_MX + fg * 8, left = min(8, cols - c);
-    uint32_t gone = drop[q * 16 + fr] >> (fg * 8);
-    float v[8];
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      v[i] = acc[q][i >> 2][i & 3];
-      if (((gone >> i) & 1) || (keep && i < left && !keep[c + i])) v[i] = -INFINITY;
-    }
-    T* p = out + u * ldo + c;
-    if (left == 8) {
-      rp_vec<T, 8> t;
-#pragma unroll
-      for (int i = 0; i < 8; ++i) t.v[i] = rp_from_f32<T>(v[i]);
-      rp_store_vec<T, 8>(p, t);
-    } else {
-#pragma unroll
-      for (int i = 0; i < 8; ++i)
-        if (i < left) p[i] = rp_from_f32<T>(v[i]);
-    }
+    for (int i = 0; i < 8; ++i)
+      if (i < left) p[i] = rp_from_f32<T>(v[i]);
   }
 }
 
 // Weighted histories in the vector unit: a lane owns one block of 32 columns of every row and keeps its 32 sums in registers, half a
 // conversion and one multiply-add per element; four rows in flight while four are added.  (The matrix pipe would take five planes per weight.)
+// The waves take groups of four entries in turn and add their sums up in wave order, however many users there are: waves that share the
+// columns out instead convert as much and address four times as many rows (251 histories of 100 against 20000 x 20000: 72 us); one wave alone is
+// a little faster where there are many users (1024 histories of 50 against 50000 x 50000: 257 us, 274 so), and sums in another order.
 // Bound by the gathered pieces: 251 histories of 100 against 20000 x 20000 in bf16 47 us, 266 MB at 5.6 TB/s (117 MB of rows are different ones, but
 // an XCD meets a row again when its L2 has long seen others).
-template <class T, int WAVES>
-__global__ __launch_bounds__(64 * WAVES) void k_mx_scores_weighted(const int32_t* __restrict__ indptr, const int32_t* __restrict__ indices, const float* __restrict__ weights,
+template <class T>
+__global__ __launch_bounds__(64 * MXS_WAVES) void k_mx_scores_weighted(const int32_t* __restrict__ indptr, const int32_t* __restrict__ indices, const float* __restrict__ weights,
                                                           int64_t nnz, int rows, int cols, int nb, const uint8_t* __restrict__ codes, int64_t ldc,
                                                           const uint8_t* __restrict__ scales, int64_t lds, int exclude, const uint8_t* __restrict__ keep,
                                                           T* __restrict__ out, int64_t ldo, int64_t user0, unsigned users, int tiles) {
   __shared__ uint32_t drop[64];  // bit c of word l: column 32 l + c of the tile gets -inf
-  __shared__ float sums[WAVES > 1 ? WAVES * 32 * 64 : 1];
-  const int lane = threadIdx.x & 63, wave = WAVES > 1 ? __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) : 0;
+  __shared__ float sums[MXS_WAVES * 32 * 64];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   unsigned user;
   int tile;
   mxs_task(users, tiles, user, tile);
@@ -385,8 +367,11 @@ __global__ __launch_bounds__(64 * WAVES) void k_mx_scores_weighted(const int32_t
   const uint8_t* cbase = codes + (int64_t)b * 16;
   const uint8_t* sbase = scales + b;
   const int64_t e1 = min((int64_t)indptr[u + 1], nnz);
-  for (int64_t e0 = max((int64_t)indptr[u], (int64_t)0); e0 < e1; e0 += 64) {
-    const mxs_chunk ch = mxs_entries<true>(indices, weights, e0, e1, rows, exclude && wave == 0, c0, drop, lane);
+  int64_t e0 = max((int64_t)indptr[u], (int64_t)0);
+  mxs_chunk next = mxs_load<true>(indices, weights, e0, e1, lane);
+  for (; e0 < e1; e0 += 64) {
+    const mxs_chunk ch = mxs_entries<true>(next, rows, exclude && wave == 0, c0, drop, lane);
+    next = mxs_load<true>(indices, weights, e0 + 64, e1, lane);
     const int idx = ch.idx, m = ch.m;
     const float wgt = ch.wgt;
     uint4 w[2][4];
@@ -417,7 +402,7 @@ __global__ __launch_bounds__(64 * WAVES) void k_mx_scores_weighted(const int32_t
         }
       }
     };
-    constexpr int STEP = 4 * WAVES;
+    constexpr int STEP = 4 * MXS_WAVES;
     int k = wave * 4;
     if (k < m) {
       fetch(std::integral_constant<int, 0>{}, k);
@@ -433,55 +418,31 @@ __global__ __launch_bounds__(64 * WAVES) void k_mx_scores_weighted(const int32_t
   const int c = b * RP_MX;
   const int left = min(RP_MX, cols - c);
   T* p = out + u * ldo + c;
-  if constexpr (WAVES > 1) {
-    // a lane of wave w ends with the columns [w * PC, (w + 1) * PC) of its block
-    constexpr int PC = 32 / WAVES;
+  // a lane of wave w ends with the columns [w * PC, (w + 1) * PC) of its block
+  constexpr int PC = 32 / MXS_WAVES;
 #pragma unroll
-    for (int i = 0; i < 32; ++i) sums[(wave * 32 + i) * 64 + lane] = acc[i];
-    __syncthreads();
-    if (!mine) return;
-    const uint32_t gone = drop[lane];
-    float v[PC];
+  for (int i = 0; i < 32; ++i) sums[(wave * 32 + i) * 64 + lane] = acc[i];
+  __syncthreads();
+  if (!mine) return;
+  const uint32_t gone = drop[lane];
+  float v[PC];
 #pragma unroll
-    for (int i = 0; i < PC; ++i) {
-      const int col = wave * PC + i;
-      v[i] = 0.0f;
+  for (int i = 0; i < PC; ++i) {
+    const int col = wave * PC + i;
+    v[i] = 0.0f;
 #pragma unroll
-      for (int o = 0; o < WAVES; ++o) v[i] += sums[(o * 32 + col) * 64 + lane];
-      if (((gone >> col) & 1) || (keep && col < left && !keep[c + col])) v[i] = -INFINITY;
-    }
-    if (left == RP_MX) {
-      rp_vec<T, PC> t;
+    for (int o = 0; o < MXS_WAVES; ++o) v[i] += sums[(o * 32 + col) * 64 + lane];
+    if (((gone >> col) & 1) || (keep && col < left && !keep[c + col])) v[i] = -INFINITY;
+  }
+  if (left == RP_MX) {
+    rp_vec<T, PC> t;
 #pragma unroll
-      for (int i = 0; i < PC; ++i) t.v[i] = rp_from_f32<T>(v[i]);
-      rp_store_vec<T, PC>(p + wave * PC, t);
-    } else {
-#pragma unroll
-      for (int i = 0; i < PC; ++i)
-        if (wave * PC + i < left) p[wave * PC + i] = rp_from_f32<T>(v[i]);
-    }
+    for (int i = 0; i < PC; ++i) t.v[i] = rp_from_f32<T>(v[i]);
+    rp_store_vec<T, PC>(p + wave * PC, t);
   } else {
-    __syncthreads();
-    if (!mine) return;
-    uint32_t gone = drop[lane];
-    if (keep)
-      for (int i = 0; i < left; ++i) gone |= keep[c + i] ? 0u : 1u << i;
 #pragma unroll
-    for (int i = 0; i < 32; ++i)
-      if ((gone >> i) & 1) acc[i] = -INFINITY;
-    if (left == RP_MX) {
-#pragma unroll
-      for (int g = 0; g < 4; ++g) {
-        rp_vec<T, 8> t;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) t.v[i] = rp_from_f32<T>(acc[g * 8 + i]);
-        rp_store_vec<T, 8>(p + g * 8, t);
-      }
-    } else {
-#pragma unroll
-      for (int i = 0; i < 32; ++i)
-        if (i < left) p[i] = rp_from_f32<T>(acc[i]);
-    }
+    for (int i = 0; i < PC; ++i)
+      if (wave * PC + i < left) p[wave * PC + i] = rp_from_f32<T>(v[i]);
   }
 }
 
@@ -505,27 +466,16 @@ extern "C" int rphip_mxfp4_scores(rphip_ctx* ctx, void* stream, int64_t n_users,
     using T = typename decltype(tag)::T;
     const hipStream_t st = (hipStream_t)stream;
     const int64_t strip = std::max<int64_t>(1, ((int64_t)1 << 22) / tiles);  // (users of a launch: below 2^32 threads)
-    auto go = [&](auto waves) -> int {
-      constexpr int WV = decltype(waves)::value;
-      for (int64_t u0 = 0; u0 < n_users; u0 += strip) {
-        const unsigned users = (unsigned)std::min(strip, n_users - u0);
-        const unsigned grid = users * (unsigned)tiles;
-        if (weights_dev)
-          k_mx_scores_weighted<T, WV><<<grid, 64 * WV, 0, st>>>(indptr_dev, indices_dev, weights_dev, nnz, (int)rows, (int)cols, nb, codes_dev, ld_codes, scales_dev, ld_scales,
-                                                                exclude_history, item_keep_dev, (T*)out_dev, ld_out, u0, users, (int)tiles);
-        else
-          k_mx_scores_sum<T, WV><<<grid, 64 * WV, 0, st>>>(indptr_dev, indices_dev, nnz, (int)rows, (int)cols, nb, codes_dev, ld_codes, scales_dev, ld_scales, exclude_history,
-                                                           item_keep_dev, (T*)out_dev, ld_out, u0, users, (int)tiles);
-        RP_LAUNCHED();
-      }
-      return RPHIP_OK;
-    };
-    // few (user, tile) pairs: more waves to each.  64 users x 20000: 17 us with 8 or 4 waves, 26 with one (weighted 24, 27, 36); 251 x 20000
-    // weighted: 52 with four, 71 with one, 66 with eight; 1024 x 50000: 226 with one, 245 with four
-    using std::integral_constant;
-    const int64_t groups = n_users * tiles;
-    if (groups <= 4 * ctx->n_cu) return go(integral_constant<int, 8>{});
-    if (groups <= 32 * ctx->n_cu) return go(integral_constant<int, 4>{});
-    return go(integral_constant<int, 1>{});
+    for (int64_t u0 = 0; u0 < n_users; u0 += strip) {
+      const unsigned users = (unsigned)std::min(strip, n_users - u0), grid = users * (unsigned)tiles;
+      if (weights_dev)
+        k_mx_scores_weighted<T><<<grid, 64 * MXS_WAVES, 0, st>>>(indptr_dev, indices_dev, weights_dev, nnz, (int)rows, (int)cols, nb, codes_dev, ld_codes, scales_dev, ld_scales,
+                                                                 exclude_history, item_keep_dev, (T*)out_dev, ld_out, u0, users, (int)tiles);
+      else
+        k_mx_scores_sum<T><<<grid, 64 * MXS_WAVES, 0, st>>>(indptr_dev, indices_dev, nnz, (int)rows, (int)cols, nb, codes_dev, ld_codes, scales_dev, ld_scales, exclude_history,
+                                                            item_keep_dev, (T*)out_dev, ld_out, u0, users, (int)tiles);
+      RP_LAUNCHED();
+    }
+    return RPHIP_OK;
   });
 }

@@ -123,3 +123,57 @@ def test_sample_min_p_on_a_border(ctx, ops, rows):
         u = torch.linspace(0, 1, rows).view(rows, 1) * (1 - 2.0 ** -24)
         check_sample(ctx, ops, x, u, min_p=2.0 ** -octaves)
         check_sample(ctx, ops, x, u, min_p=float(np.nextafter(np.float32(2.0 ** -octaves), np.float32(0))))
+
+
+# ---- scores: the same bits alone and in any batch -----------------------------------------------------------------------------------------
+
+def wide_mxfp4(ops, rows, cols, seed, lo, hi):
+    nb = -(-cols // 32)
+    codes = torch.randint(0, 256, (rows, nb * 16), generator=gen(seed), dtype=torch.uint8)
+    if cols % 2:
+        codes[:, cols // 2] &= 15
+    codes[:, (cols + 1) // 2:] = 0
+    return ops.MXFP4(codes.cuda(), torch.randint(lo, hi, (rows, nb), generator=gen(seed + 1), dtype=torch.uint8).cuda(), cols)
+
+
+def batch_of(histories, times):
+    """CSR of the given histories, one after the other, `times` times."""
+    counts = torch.tensor([len(h) for h in histories] * times)
+    indptr = torch.zeros(len(counts) + 1, dtype=torch.int32)
+    indptr[1:] = counts.cumsum(0)
+    return indptr.cuda(), torch.cat([torch.cat(histories)] * times).cuda()
+
+
+@pytest.mark.parametrize("weighted", [False, True])
+@pytest.mark.parametrize("items,times", [(2500, 700), (4101, 500), (12_300, 250)])
+@pytest.mark.parametrize("lo,hi", [(117, 126), (0, 8), (3, 200)])
+def test_scores_do_not_depend_on_the_batch(ctx, ops, weighted, items, times, lo, hi):
+    """Few users (four waves to a tile of columns) and many (one): sums of many entries, bit for bit; within the bound of float32 sums."""
+    w = wide_mxfp4(ops, items, items, items, lo, hi)
+    sizes = [1, 3, 37, 64, 65, 133, 300, 9]
+    histories = [torch.randint(0, items, (n,), generator=gen(n), dtype=torch.int32) for n in sizes]
+    histories[3][::7] = -1  # (entries that count nothing move the others together)
+    indptr, indices = batch_of(histories, times)
+    one = torch.randn(sum(sizes), generator=gen(5)).cuda() if weighted else None
+    kw = dict(exclude_history=True) if items == 2500 else {}
+    got = ops.mxfp4_scores(ctx, indptr, indices, w, weights=None if one is None else one.repeat(times), **kw)
+    few_ptr, few_indices = batch_of(histories, 1)
+    few = ops.mxfp4_scores(ctx, few_ptr, few_indices, w, weights=one, **kw)
+    assert torch.equal(got.view(times, len(sizes), items)[[0, 1, times - 1]].contiguous(), few.expand(3, -1, -1).contiguous())
+    at = 0
+    lut = torch.tensor([0, .5, 1, 1.5, 2, 3, 4, 6, 0, -.5, -1, -1.5, -2, -3, -4, -6], dtype=torch.float64)
+    for u, h in enumerate(histories):
+        part = None if one is None else one[at:at + len(h)]
+        alone = ops.mxfp4_scores(ctx, torch.tensor([0, len(h)], dtype=torch.int32).cuda(), h.cuda(), w, weights=part, **kw)
+        assert torch.equal(alone[0], few[u])
+        h, f = h.long(), torch.ones(len(h), dtype=torch.float64) if part is None else part.double().cpu()
+        h, f = h[h >= 0], f[h >= 0]
+        codes = w.codes.cpu()[h].long()
+        V = torch.stack((lut[codes & 15], lut[codes >> 4]), -1).view(len(h), -1) * torch.exp2(w.scales.cpu()[h].double() - 127).repeat_interleave(32, 1)
+        want, size = (f[:, None] * V).sum(0)[:items], (f[:, None] * V).abs().sum(0)[:items]
+        # n adds (and products), each off by at most half a step of at most the sum of the magnitudes (or of float32's least number)
+        bound = (len(h) + 1) * (2.0 ** -23 * size + 2.0 ** -149)
+        gone = torch.isneginf(alone[0].cpu())
+        assert bool((((alone[0].double().cpu() - want).abs() <= bound) | gone).all())
+        assert int(gone.sum()) == (len(set(h.tolist())) if kw else 0)
+        at += sizes[u]
