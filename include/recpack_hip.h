@@ -568,7 +568,7 @@ int rphip_mxfp4_dequantize(rphip_ctx* ctx, void* stream, int64_t rows, int64_t c
  * own type otherwise; none for few rows or a small product), or RPHIP_MXFP4 (A_dev = codes, lda in bytes, a_scales; ignored otherwise).
  * Sums in float32, one rounding to c_type; not finite where a value of W is not (scales 253 and 254, which quantising does not make, reach
  * past float32).  f16 A: 16 rows of W take longer if the scales of one of them lie more than 2^36 apart.
- * M <= 65 535 * 16, N <= 2^28. */
+ * M <= 65 535 * 16, N <= 2^28, any K that memory holds. */
 int rphip_mxfp4_gemm_nt_workspace(rphip_ctx* ctx, int64_t M, int64_t N, int64_t K, int32_t a_type, int64_t* bytes_out);
 int rphip_mxfp4_gemm_nt(rphip_ctx* ctx, void* stream, int64_t M, int64_t N, int64_t K, const void* A_dev, int32_t a_type, int64_t lda,
                         const uint8_t* a_scales_dev, int64_t ld_a_scales, const uint8_t* w_codes_dev, int64_t ld_w, const uint8_t* w_scales_dev,
@@ -577,7 +577,7 @@ int rphip_mxfp4_gemm_nt(rphip_ctx* ctx, void* stream, int64_t M, int64_t N, int6
  * (recpack/algorithms/base.py:248) for n_users CSR rows,
  *   out[u, :] = sum over e in [indptr[u], indptr[u + 1]) of weights[e] * W[indices[e], :]     (weights NULL: 1)
  * in float32, one rounding to out_type; a user's scores are the same bits alone and among any others.  Repeated entries count as often as they stand; entries outside [0, rows) count nothing and
- * indptr is read no further than nnz.  exclude_history != 0 (needs rows = cols; history removal of pipelines/pipeline.py:174-175): the
+ * indptr is read no further than nnz.  cols <= 65 535 * 2 048.  exclude_history != 0 (needs rows = cols; history removal of pipelines/pipeline.py:174-175): the
  * history's own items get -inf.  item_keep (cols bytes, NULL = all): items with 0 get -inf (postprocessing/filters.py:58-101). */
 int rphip_mxfp4_scores(rphip_ctx* ctx, void* stream, int64_t n_users, int64_t nnz, const int32_t* indptr_dev, const int32_t* indices_dev,
                        const float* weights_dev, int64_t rows, int64_t cols, const uint8_t* codes_dev, int64_t ld_codes, const uint8_t* scales_dev,

@@ -138,7 +138,7 @@ __device__ __forceinline__ void pack_scales_half(const uint8_t* __restrict__ s, 
   if (t == 0) wide[rb] = (uint8_t)lost;
 }
 
-// One launch for all of them: workgroups [0, wg_w) pack W's scales, the others cut A (P > 0) or pack A's scales.  2048 x 20000 of A in f16 and
+// One launch for all of them (2^23 workgroups at a time, from wg0): workgroups [0, wg_w) pack W's scales, the others cut A (P > 0) or pack A's scales.  2048 x 20000 of A in f16 and
 // the scales of 20000 x 20000 of W: 52 us of 1.37 ms (once a call: 4 bytes an element of A and 2 a scale, read and written).
 struct half_args {  // (f16 A only)
   const uint8_t* codes;
@@ -147,17 +147,19 @@ struct half_args {  // (f16 A only)
 };
 template <class T, int P>
 __global__ __launch_bounds__(256) void k_mxg_prepare(const uint8_t* __restrict__ ws, int64_t ldws, int N, int nb, int nq, int64_t w_units, uint32_t* __restrict__ w_out,
-                                                     unsigned wg_w, const T* __restrict__ a, int64_t lda, int M, int K, int nc, int64_t a_units, void* __restrict__ a_out, half_args half) {
-  if (blockIdx.x < wg_w) {
+                                                     int64_t wg0, int64_t wg_w, const T* __restrict__ a, int64_t lda, int M, int K, int nc, int64_t a_units,
+                                                     void* __restrict__ a_out, half_args half) {
+  int64_t wg = wg0 + blockIdx.x;
+  if (wg < wg_w) {
     if constexpr (std::is_same<T, _Float16>::value) {
-      pack_scales_half(ws, ldws, half.codes, half.ldc, N, nb, nq, blockIdx.x, w_out, half.top, half.wide);
+      pack_scales_half(ws, ldws, half.codes, half.ldc, N, nb, nq, wg, w_out, half.top, half.wide);
       return;
     }
-    const int64_t unit = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    const int64_t unit = wg * 256 + threadIdx.x;
     if (unit < w_units) pack_scales(ws, ldws, N, nb, nq, unit, w_out);
     return;
   }
-  const int64_t wg = blockIdx.x - wg_w;
+  wg -= wg_w;
   if constexpr (P > 0) {
     if (wg < a_units) cut_fragment<T, P>(a, lda, M, K, nc, wg, threadIdx.x >> 6, threadIdx.x & 63, (uint16_t*)a_out);
   } else {
@@ -1003,13 +1005,16 @@ extern "C" int rphip_mxfp4_gemm_nt(rphip_ctx* ctx, void* stream, int64_t M, int6
       return rp_by_type(c_type, [&](auto ct) -> int {
         using T = typename decltype(at)::T;
         using OT = typename decltype(ct)::T;
-        const unsigned grid = (unsigned)rp_cdiv(N, 4 * GV_ROWS);
-        auto go = [&](auto kernel) { kernel<<<grid, 256, 0, st>>>((const T*)A_dev, lda, (int)M, (int)N, (int)K, g.nb, w_codes_dev, ld_w, w_scales_dev, ld_w_scales, (OT*)C_dev, ldc); };
-        if (M == 1) go(k_mxg_rows<T, OT, 1>);
-        else if (M == 2) go(k_mxg_rows<T, OT, 2>);
-        else go(k_mxg_rows<T, OT, 4>);
-        RP_LAUNCHED();
-        return RPHIP_OK;
+        auto go = [&](auto kernel) -> int {
+          for (int64_t n0 = 0; n0 < N; n0 += (int64_t)1 << 27) {  // (a launch takes less than 2^32 threads)
+            const int n = (int)std::min<int64_t>(N - n0, (int64_t)1 << 27);
+            kernel<<<(unsigned)rp_cdiv(n, 4 * GV_ROWS), 256, 0, st>>>((const T*)A_dev, lda, (int)M, n, (int)K, g.nb, w_codes_dev + n0 * ld_w, ld_w,
+                                                                      w_scales_dev + n0 * ld_w_scales, ld_w_scales, (OT*)C_dev + n0, ldc);
+            RP_LAUNCHED();
+          }
+          return RPHIP_OK;
+        };
+        return M == 1 ? go(k_mxg_rows<T, OT, 1>) : M == 2 ? go(k_mxg_rows<T, OT, 2>) : go(k_mxg_rows<T, OT, 4>);
       });
     });
   // the direct form: the whole product, or (wide) what f16 did not hold
@@ -1031,18 +1036,20 @@ extern "C" int rphip_mxfp4_gemm_nt(rphip_ctx* ctx, void* stream, int64_t M, int6
   if (p.nc) {
     const int64_t w_units = rp_cdiv(N, 16) * p.nq * 64, wg_w = p.half ? rp_cdiv(N, 16) : rp_cdiv(w_units, 256);
     const int64_t a_units = p.planes ? rp_cdiv(M, 16) * p.nc : rp_cdiv(M, 16) * p.nq * 64, wg_a = p.planes ? a_units : rp_cdiv(a_units, 256);
-    if ((wg_w + wg_a) * 256 >= ((int64_t)1 << 32))
-      RP_FAIL(RPHIP_ELIMIT, "mxfp4_gemm_nt: %lld x %lld x %lld: more 16-row blocks than one launch prepares (split M or N)", (long long)M, (long long)N, (long long)K);
-    auto go = [&](auto kernel, auto type, const void* a, int64_t ld, void* o) {
+    auto go = [&](auto kernel, auto type, const void* a, int64_t ld, void* o) -> int {
       using T = decltype(type);
-      kernel<<<(unsigned)(wg_w + wg_a), 256, 0, st>>>(w_scales_dev, ld_w_scales, (int)N, g.nb, p.nq, w_units, (uint32_t*)g.w_scales, (unsigned)wg_w, (const T*)a, ld, (int)M,
-                                                     (int)K, p.nc, a_units, o, half_args{w_codes_dev, ld_w, top, wide});
+      for (int64_t wg0 = 0; wg0 < wg_w + wg_a; wg0 += (int64_t)1 << 23) {
+        kernel<<<(unsigned)std::min<int64_t>(wg_w + wg_a - wg0, (int64_t)1 << 23), 256, 0, st>>>(w_scales_dev, ld_w_scales, (int)N, g.nb, p.nq, w_units, (uint32_t*)g.w_scales, wg0,
+                                                                                               wg_w, (const T*)a, ld, (int)M, (int)K, p.nc, a_units, o,
+                                                                                               half_args{w_codes_dev, ld_w, top, wide});
+        RP_LAUNCHED();
+      }
+      return RPHIP_OK;
     };
-    if (a_type == RPHIP_BF16) go(k_mxg_prepare<__bf16, 1>, __bf16{}, A_dev, lda, (void*)g.planes);
-    else if (a_type == RPHIP_F16) go(k_mxg_prepare<_Float16, 1>, _Float16{}, A_dev, lda, (void*)g.planes);
-    else if (a_type == RPHIP_F32) go(k_mxg_prepare<float, 3>, 0.0f, A_dev, lda, (void*)g.planes);
-    else go(k_mxg_prepare<uint8_t, 0>, uint8_t{0}, a_scales_dev, ld_a_scales, (void*)g.a_scales);
-    RP_LAUNCHED();
+    if (a_type == RPHIP_BF16) RP_TRY(go(k_mxg_prepare<__bf16, 1>, __bf16{}, A_dev, lda, (void*)g.planes));
+    else if (a_type == RPHIP_F16) RP_TRY(go(k_mxg_prepare<_Float16, 1>, _Float16{}, A_dev, lda, (void*)g.planes));
+    else if (a_type == RPHIP_F32) RP_TRY(go(k_mxg_prepare<float, 3>, 0.0f, A_dev, lda, (void*)g.planes));
+    else RP_TRY(go(k_mxg_prepare<uint8_t, 0>, uint8_t{0}, a_scales_dev, ld_a_scales, (void*)g.a_scales));
   }
   return rp_by_type(c_type, [&](auto tag) -> int {
     using OT = typename decltype(tag)::T;

@@ -177,3 +177,23 @@ def test_scores_do_not_depend_on_the_batch(ctx, ops, weighted, items, times, lo,
         assert bool((((alone[0].double().cpu() - want).abs() <= bound) | gone).all())
         assert int(gone.sum()) == (len(set(h.tolist())) if kw else 0)
         at += sizes[u]
+
+
+# ---- products: the documented limits -------------------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("m,dtype", [(1, torch.float32), (2, torch.bfloat16), (4, torch.float32), (5, torch.float16)])
+def test_product_with_the_most_rows_of_w(ctx, ops, m, dtype):
+    """N = 2^28, more workgroups of 16 rows than a launch takes: the rows at the ends and where the launches meet are those of a small product."""
+    n, k = 2 ** 28, 32
+    w = ops.MXFP4.empty(n, k, "cuda")
+    w.codes.random_(generator=torch.Generator(device="cuda").manual_seed(m))
+    w.scales.random_(120, 127, generator=torch.Generator(device="cuda").manual_seed(9))
+    a = torch.randn(m, k, generator=gen(m)).to(dtype).cuda()
+    got = ops.mxfp4_gemm_nt(ctx, a, w)
+    at = torch.tensor([0, 1, 63, 2 ** 26 + 5, 2 ** 27 - 1, 2 ** 27, 2 ** 27 + 17, 2 ** 28 - 17, 2 ** 28 - 16, 2 ** 28 - 1], device="cuda")
+    few = ops.mxfp4_dequantize(ctx, ops.MXFP4(w.codes[at].contiguous(), w.scales[at].contiguous(), k)).double()
+    want, size = a.double() @ few.t(), a.double().abs() @ few.t().abs()
+    # 32 products in three planes at most, a step (2^-23) of the magnitudes' sum each at most; one rounding
+    assert bool(((got[:, at].double() - want).abs() <= 96 * 2.0 ** -23 * size + torch.finfo(dtype).eps / 2 * want.abs()).all())
+    for part in got.view(-1).split(2 ** 28):
+        assert bool(part.isfinite().all())
