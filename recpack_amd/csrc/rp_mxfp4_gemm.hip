@@ -5,8 +5,8 @@
 // sum of one (bf16) or three (f32: 8 + 8 + 8 bits) of them, so the product runs on v_mfma_f32_16x16x32_bf16 with exact operands; the
 // planes of A are cut once into a workspace, W is converted in registers.  f16 A runs on v_mfma_f32_16x16x32_f16 as it is: a row of W
 // relative to the power of two of its largest block is a row of f16 numbers exactly as long as its blocks' scales lie within 2^36 of each other
-// (subnormals included), and its sums are scaled back as they are stored.  Rows of W that span more are found beforehand and their part
-// of C is computed again with f16 as two bf16 planes (8 + 3 bits).
+// (subnormals included), and its sums are scaled back as they are stored.  Rows of W that span more are found beforehand and their
+// columns of C are computed again with f16 as two bf16 planes (8 + 3 bits).
 // MXFP4 A: v_mfma_scale_f32_16x16x128_f8f6f4, which takes codes and scales as they are.
 #include "rp_ops.h"
 
@@ -30,7 +30,8 @@ constexpr int KC = 128;  // K of a chunk: four MX blocks
 // bf16 instruction and (g, 32 elements) for the 4-bit one - the same for both operands, which is all a product asks - so a lane's 16
 // code bytes are one MX block with one scale in either kernel.
 
-// by truncation: the high part never overflows, each remainder is exact
+// by truncation: the high part never overflows, each remainder is exact down to 2^-133, bf16's least number (of an f32 element below 2^-110 the
+// bits under that are left out)
 template <int P>
 __device__ __forceinline__ void cut_planes(float x, uint16_t (&h)[P]) {
   const uint32_t b = __float_as_uint(x);
@@ -99,10 +100,10 @@ __device__ __forceinline__ void pack_scales(const uint8_t* __restrict__ s, int64
 }
 
 // The same for W beside f16 A, a workgroup to 16 rows: scales relative to the row's largest one, which becomes 2^HALF_TOP (6 * 2^13 is an f16
-// number); top[] keeps the largest, wide[block] says whether a row has an element that f16 does not hold then.
+// number); top[] keeps the largest, wide[block] has a bit for each row with an element that f16 does not hold then.
 constexpr int HALF_TOP = 13, HALF_SPAN = 36;  // (.5 * 2^(13 - 36) = 2^-24, the least f16 number)
 __device__ __forceinline__ void pack_scales_half(const uint8_t* __restrict__ s, int64_t lds, const uint8_t* __restrict__ codes, int64_t ldc, int rows, int nb, int nq, int64_t rb,
-                                                 uint32_t* __restrict__ out, uint8_t* __restrict__ top, uint8_t* __restrict__ wide) {
+                                                 uint32_t* __restrict__ out, uint8_t* __restrict__ top, uint16_t* __restrict__ wide) {
   __shared__ uint32_t best[16], lost;
   const int t = threadIdx.x, row = t >> 4;
   if (t < 16) best[t] = 0;
@@ -127,7 +128,7 @@ __device__ __forceinline__ void pack_scales_half(const uint8_t* __restrict__ s, 
       const int v = s[rr * lds + b + cc * 4], span = e - v;
       if (v != 255 && span > HALF_SPAN) {
         const uint4 q = *(const uint4*)(codes + rr * ldc + (int64_t)(b + cc * 4) * 16);
-        if (((q.x | q.y | q.z | q.w) & 0x77777777u) != 0) lost = 1;  // (blocks of zeros lose nothing; codes behind the last column are 0)
+        if (((q.x | q.y | q.z | q.w) & 0x77777777u) != 0) atomicOr(&lost, 1u << (lane & 15));  // (blocks of zeros lose nothing; codes behind the last column are 0)
       }
       w |= (uint32_t)(v == 255 ? 255 : max(127 + HALF_TOP - span, 0)) << (8 * cc);
     }
@@ -135,7 +136,7 @@ __device__ __forceinline__ void pack_scales_half(const uint8_t* __restrict__ s, 
   }
   __syncthreads();
   if (t < 16) top[rb * 16 + t] = (uint8_t)best[t];
-  if (t == 0) wide[rb] = (uint8_t)lost;
+  if (t == 0) wide[rb] = (uint16_t)lost;
 }
 
 // One launch for all of them (2^23 workgroups at a time, from wg0): workgroups [0, wg_w) pack W's scales, the others cut A (P > 0) or pack A's scales.  2048 x 20000 of A in f16 and
@@ -143,7 +144,8 @@ __device__ __forceinline__ void pack_scales_half(const uint8_t* __restrict__ s, 
 struct half_args {  // (f16 A only)
   const uint8_t* codes;
   int64_t ldc;
-  uint8_t *top, *wide;
+  uint8_t* top;
+  uint16_t* wide;
 };
 template <class T, int P>
 __global__ __launch_bounds__(256) void k_mxg_prepare(const uint8_t* __restrict__ ws, int64_t ldws, int N, int nb, int nq, int64_t w_units, uint32_t* __restrict__ w_out,
@@ -633,12 +635,12 @@ __device__ __forceinline__ void cut8(const float (&v)[8], bf16x8 (&out)[P]) {
 template <class T, class OT, int P>
 __global__ __launch_bounds__(64 * SD_WAVES) void k_mxg_direct(const T* __restrict__ a, int64_t lda, const uint8_t* __restrict__ as, int64_t ldas, int M, int N, int K, int nb,
                                                               const uint8_t* __restrict__ w, int64_t ldw, const uint8_t* __restrict__ ws, int64_t ldws, OT* __restrict__ c,
-                                                              int64_t ldc, const uint8_t* __restrict__ wide) {
+                                                              int64_t ldc, const uint16_t* __restrict__ wide) {
   constexpr int TM = sd_tm(P), TN = sd_tn(P);
   __shared__ f32x4 part[SD_WAVES][TM * TN][64];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), fr = lane & 15, fg = lane >> 4;
   const int n0 = (int)blockIdx.x * TN * 16, nc = (nb + 3) / 4;
-  if (wide) {  // (f16 A, after the product: only columns that f16 does not hold)
+  if (wide) {  // (f16 A, after the product: only columns that f16 does not hold; the others of their tiles stay as they are)
     bool any = false;
 #pragma unroll
     for (int j = 0; j < TN; ++j) any = any || (n0 + j * 16 < N && wide[n0 / 16 + j] != 0);
@@ -768,7 +770,8 @@ __global__ __launch_bounds__(64 * SD_WAVES) void k_mxg_direct(const T* __restric
 #pragma unroll
       for (int q = 1; q < SD_WAVES; ++q) t += part[q][wave][lane];
       OT* o = c + (int64_t)m * ldc + n;
-      if (n + 4 <= N) {
+      const uint32_t mine = wide ? (n < N ? (uint32_t)wide[n >> 4] >> (n & 15) : 0u) & 15u : 15u;
+      if (n + 4 <= N && mine == 15u) {
         rp_vec<OT, 4> v;
 #pragma unroll
         for (int e = 0; e < 4; ++e) v.v[e] = rp_from_f32<OT>(t[e]);
@@ -776,7 +779,7 @@ __global__ __launch_bounds__(64 * SD_WAVES) void k_mxg_direct(const T* __restric
       } else {
 #pragma unroll
         for (int e = 0; e < 4; ++e)
-          if (n + e < N) o[e] = rp_from_f32<OT>(t[e]);
+          if (n + e < N && ((mine >> e) & 1)) o[e] = rp_from_f32<OT>(t[e]);
       }
     }
     __syncthreads();
@@ -906,7 +909,7 @@ plan make_plan(int n_cu, int64_t M, int64_t N, int64_t K, int32_t a_type) {
   p.a_scale_bytes = p.planes ? 0 : room(rp_cdiv(M, 16) * p.nq * 256);
   p.w_scale_bytes = room(rp_cdiv(N, 16) * p.nq * 256);
   p.top_bytes = p.half ? room(rp_cdiv(N, 16) * 16) : 0;
-  p.wide_bytes = p.half ? room(rp_cdiv(N, 16)) : 0;
+  p.wide_bytes = p.half ? room(rp_cdiv(N, 16) * 2) : 0;
   p.part_bytes = p.split > 1 ? M * N * 4 * p.split : 0;
   if (p.split == 1 && p.bn == 256) {
     const last_round l = last_round_of(n_cu, grid_of(M, N, p.bm, p.bn), p.nc);
@@ -996,9 +999,9 @@ extern "C" int rphip_mxfp4_gemm_nt(rphip_ctx* ctx, void* stream, int64_t M, int6
   g.a_codes = (const uint8_t*)A_dev, g.lda = lda, g.a_scales = (const uint32_t*)(ws + p.plane_bytes);
   g.w = w_codes_dev, g.ldw = ld_w, g.w_scales = (const uint32_t*)(ws + p.plane_bytes + p.a_scale_bytes);
   uint8_t* top = (uint8_t*)ws + p.plane_bytes + p.a_scale_bytes + p.w_scale_bytes;
-  uint8_t* wide = top + p.top_bytes;
+  uint16_t* wide = (uint16_t*)(top + p.top_bytes);
   g.w_top = top;
-  g.c = C_dev, g.ldc = ldc, g.part = (float*)(wide + p.wide_bytes), g.split = p.split;
+  g.c = C_dev, g.ldc = ldc, g.part = (float*)((char*)wide + p.wide_bytes), g.split = p.split;
   g.first = p.first, g.parts = p.parts, g.n_tail = p.n_tail;
   if (p.rows)
     return rp_by_type(a_type, [&](auto at) -> int {
@@ -1018,7 +1021,7 @@ extern "C" int rphip_mxfp4_gemm_nt(rphip_ctx* ctx, void* stream, int64_t M, int6
       });
     });
   // the direct form: the whole product, or (wide) what f16 did not hold
-  auto direct = [&](auto kernel, auto type, auto out, int planes, const uint8_t* flags) -> int {
+  auto direct = [&](auto kernel, auto type, auto out, int planes, const uint16_t* flags) -> int {
     const unsigned gx = (unsigned)rp_cdiv(N, 16 * sd_tn(planes)), gy = (unsigned)rp_cdiv(M, 16 * sd_tm(planes));
     kernel<<<dim3(gx, flags ? std::min(gy, 16u) : gy), 64 * SD_WAVES, 0, st>>>((const decltype(type)*)A_dev, lda, a_scales_dev, ld_a_scales, (int)M, (int)N, (int)K, g.nb, w_codes_dev,
                                                                                ld_w, w_scales_dev, ld_w_scales, (decltype(out)*)C_dev, ldc, flags);

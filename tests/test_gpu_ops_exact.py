@@ -197,3 +197,56 @@ def test_product_with_the_most_rows_of_w(ctx, ops, m, dtype):
     assert bool(((got[:, at].double() - want).abs() <= 96 * 2.0 ** -23 * size + torch.finfo(dtype).eps / 2 * want.abs()).all())
     for part in got.view(-1).split(2 ** 28):
         assert bool(part.isfinite().all())
+
+
+def normal_mxfp4(ops, n, k, seed, scale=127):
+    w = wide_mxfp4(ops, n, k, seed, 0, 1)
+    w.scales.fill_(scale)
+    return w
+
+
+@pytest.mark.parametrize("m,n,k", [(40, 5003, 5000), (300, 9001, 700), (9, 2000, 9000)])
+def test_product_f16_rows_beside_a_wide_one(ctx, ops, m, n, k):
+    """Rows of W beside one whose scales lie more than 2^36 apart: their sums are the same bits as without it; that row's are right."""
+    a = torch.randn(m, k, generator=gen(m)).half().cuda()
+    w = normal_mxfp4(ops, n, k, 4)
+    rows = [3, 16, 700, 702, 703, n - 1]
+    w.codes[rows, :16] = 0  # (a block of zeros: it takes any scale without a change)
+    without = ops.mxfp4_gemm_nt(ctx, a, w, dtype=torch.float32)
+    w.codes[rows, 0] = 0x21  # 0.5 and 1.0, once 2^-40 of the others
+    w.scales[rows, 0] = 127 - 40
+    with_them = ops.mxfp4_gemm_nt(ctx, a, w, dtype=torch.float32)
+    others = [r for r in range(n) if r not in rows]
+    assert torch.equal(with_them[:, others], without[:, others])
+    few = ops.mxfp4_dequantize(ctx, ops.MXFP4(w.codes[rows].contiguous(), w.scales[rows].contiguous(), k)).double()
+    want, size = a.double() @ few.t(), a.double().abs() @ few.t().abs()
+    assert bool(((with_them[:, rows].double() - want).abs() <= 8 * math.sqrt(2 * k) * 2.0 ** -23 * size).all())
+    # a row of A that meets nothing but the small block: exact
+    one = torch.zeros(m, k)
+    one[:, 0], one[:, 1] = torch.arange(m) + 1.0, 0.25
+    got = ops.mxfp4_gemm_nt(ctx, one.half().cuda(), w, dtype=torch.float32)[:, rows].cpu()
+    assert torch.equal(got, ((one[:, :1] * 0.5 + 0.25) * 2.0 ** -40).expand(-1, len(rows)))
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("m,n,k", [(2, 64, 64), (16, 64, 64), (40, 5000, 5000)])
+def test_product_from_the_least_to_the_largest_number(ctx, ops, dtype, m, n, k):
+    """One element per row of A, of every power of two, against 1 and 2^100: exact; below 2^-110 a float32 element may lose the bits under 2^-133."""
+    i = torch.arange(m)
+    for scale in (127, 227):
+        w = normal_mxfp4(ops, n, k, 1, scale)
+        w.codes.zero_()
+        w.codes[i, i // 2] = torch.where(i % 2 == 0, 2, 32).to(torch.uint8).cuda()  # 1.0 on the diagonal
+        a = torch.zeros(m, k, dtype=dtype, device="cuda")
+        g = gen(m + scale)
+        for e in range(-149, 128):
+            v = (torch.randint(1 << 23, 1 << 24, (m,), generator=g).double() * 2.0 ** (e - 23)).to(dtype)
+            if not bool(v.isfinite().all()):
+                continue
+            a[i, i] = v.cuda()
+            got = ops.mxfp4_gemm_nt(ctx, a, w, dtype=torch.float32).diagonal()[:m].cpu()
+            want = (v.double() * 2.0 ** (scale - 127)).float()
+            if dtype == torch.float32 and e < -110:
+                assert bool(((got.double() - want.double()).abs() <= 2.0 ** (-133 + scale - 127)).all())
+            else:
+                assert torch.equal(got, want)
