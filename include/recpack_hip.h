@@ -565,9 +565,10 @@ int rphip_mxfp4_dequantize(rphip_ctx* ctx, void* stream, int64_t rows, int64_t c
                            const uint8_t* scales_dev, int64_t ld_scales, void* out_dev, int32_t out_type, int64_t ld_out);
 /* C[M,N] = A[M,K] W[N,K]^T, W in MXFP4 with its blocks along K: dense rows (user profiles) against a quantised matrix, beside
  * rphip_gemm_nt_f32.  A: RPHIP_F32 / F16 / BF16 with every product exact (a copy of A in the workspace: three bf16 planes for f32, one of A's
- * own type otherwise; none for few rows or a small product), or RPHIP_MXFP4 (A_dev = codes, lda in bytes, a_scales; ignored otherwise).
+ * own type otherwise; none for few rows or a small product; of f32 elements below 2^-110 the bits under 2^-133 may be left out: bf16's planes
+ * end there), or RPHIP_MXFP4 (A_dev = codes, lda in bytes, a_scales; ignored otherwise).
  * Sums in float32, one rounding to c_type; not finite where a value of W is not (scales 253 and 254, which quantising does not make, reach
- * past float32).  f16 A: 16 rows of W take longer if the scales of one of them lie more than 2^36 apart.
+ * past float32).  f16 A: a row of W whose scales lie more than 2^36 apart is computed a second time (in a tile of 64 rows: longer).
  * M <= 65 535 * 16, N <= 2^28, any K that memory holds. */
 int rphip_mxfp4_gemm_nt_workspace(rphip_ctx* ctx, int64_t M, int64_t N, int64_t K, int32_t a_type, int64_t* bytes_out);
 int rphip_mxfp4_gemm_nt(rphip_ctx* ctx, void* stream, int64_t M, int64_t N, int64_t K, const void* A_dev, int32_t a_type, int64_t lda,

@@ -168,8 +168,8 @@ def mxfp4_dequantize(ctx, m: MXFP4, dtype: torch.dtype = torch.float32, out: tor
 
 
 def mxfp4_gemm_nt(ctx, a, w: MXFP4, dtype: torch.dtype | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
-    """``a @ w.T`` with a quantised ``w`` [N, K] and ``a`` [M, K] a float32 / float16 / bfloat16 tensor (its products are exact) or itself
-    :class:`MXFP4`.  Sums in float32; the result in ``dtype`` (default: that of ``a``, float32 for MXFP4)."""
+    """``a @ w.T`` with a quantised ``w`` [N, K] and ``a`` [M, K] a float32 / float16 / bfloat16 tensor (its products are exact; of float32
+    elements below 2^-110 the bits under 2^-133 may be left out) or itself :class:`MXFP4`.  Sums in float32; the result in ``dtype`` (default: that of ``a``, float32 for MXFP4)."""
     _on(ctx, "w", w.codes)
     if isinstance(a, MXFP4):
         _on(ctx, "a", a.codes)
