@@ -250,3 +250,60 @@ def test_product_from_the_least_to_the_largest_number(ctx, ops, dtype, m, n, k):
                 assert bool(((got.double() - want.double()).abs() <= 2.0 ** (-133 + scale - 127)).all())
             else:
                 assert torch.equal(got, want)
+
+
+EVERY_TILE = [
+    (torch.float32, 1, 3000, 2048), (torch.float32, 4, 5003, 7001), (torch.bfloat16, 2, 2001, 4100), (torch.float16, 1, 3000, 5000),  # few rows
+    (torch.float32, 97, 1999, 2003), (torch.bfloat16, 64, 1000, 1000), (torch.float16, 33, 2000, 2000),                              # one launch
+    (torch.float32, 9, 2000, 5001), (torch.float16, 16, 20001, 5000), (torch.bfloat16, 16, 2001, 4200),                              # 16 x 64, K in parts
+    (torch.bfloat16, 33, 3001, 6000), (torch.float16, 64, 999, 9000), (torch.float32, 40, 4001, 4096), (torch.float32, 64, 9000, 9000),  # 64 x 64
+    (torch.bfloat16, 130, 20001, 8100), (torch.float32, 200, 9001, 4000), (torch.float16, 300, 8001, 8001),                          # 128 x 128, K in parts
+    (torch.bfloat16, 1100, 8010, 200), (torch.float16, 1100, 8010, 330), (torch.float32, 1100, 8010, 130),                           # 128 x 256
+    (torch.bfloat16, 2050, 8200, 257), (torch.float16, 2050, 8200, 90),                                                              # 256 x 256
+    (torch.bfloat16, 1500, 12001, 4200), (torch.float16, 2001, 12000, 4200), (torch.float32, 1500, 12001, 4200), (torch.float16, 300, 30001, 4300),  # the last round in parts
+    ("mxfp4", 20, 700, 9000), ("mxfp4", 30, 40001, 3000), ("mxfp4", 90, 1501, 17000), ("mxfp4", 200, 1999, 5000), ("mxfp4", 600, 3001, 1000), ("mxfp4", 1000, 8000, 3000),
+    ("mxfp4", 4000, 4200, 300), ("mxfp4", 1500, 12003, 8300)]
+
+
+@pytest.mark.parametrize("dtype,m,n,k", EVERY_TILE)
+def test_product_is_exact_in_every_tile(ctx, ops, dtype, m, n, k):
+    """One element per row of A: C holds its products with a column of W, bit for bit.  (A plane of A left out, a fragment or a part of K in
+    another's place or added twice changes nearly all of them; the bounds of sums over K would let a lost third plane pass.)"""
+    g = gen(m + n + k)
+    at = torch.randint(0, k, (m,), generator=g)
+    at[0], at[-1] = 0, k - 1
+    if m > 40:
+        at[1:40] = torch.arange(k - 40, k - 1)
+    i = torch.arange(m)
+    w = wide_mxfp4(ops, n, k, n + k, 110, 146)  # (within 2^36: f16 in one pass)
+    lut = torch.tensor([0, .5, 1, 1.5, 2, 3, 4, 6, -0.0, -.5, -1, -1.5, -2, -3, -4, -6], device="cuda")
+    sign = torch.randint(0, 2, (m,), generator=g) * 2.0 - 1
+
+    def column(q, rows, cols):  # the values at (rows, cols), one column for each
+        byte = q.codes[rows, cols // 2].long()
+        return lut[torch.where(cols % 2 == 0, byte & 15, byte >> 4)] * torch.exp2(q.scales[rows, cols // 32].float() - 127)
+
+    if dtype == "mxfp4":
+        a = wide_mxfp4(ops, m, k, m, 100, 150)
+        a.codes.zero_()
+        a.codes[i, at // 2] = (torch.randint(1, 8, (m,), generator=g) << (at % 2 * 4)).to(torch.uint8).cuda()
+        v = column(a, i.cuda(), at.cuda())
+    else:
+        bits = {torch.float32: 24, torch.float16: 11, torch.bfloat16: 8}[dtype]
+        v = (torch.randint(1 << (bits - 1), 1 << bits, (m,), generator=g) | (0x8001 if bits == 24 else 1)).double() * torch.exp2(torch.randint(-14, 5, (m,), generator=g).double() + 1 - bits) * sign
+        a = torch.zeros(m, k, dtype=dtype)
+        a[i, at] = v.to(dtype)
+        assert torch.equal(a[i, at].double(), v)
+        if dtype == torch.float32:
+            w.codes.copy_(torch.tensor([1, 2, 4, 6, 9, 10, 12, 14], dtype=torch.uint8, device="cuda")[w.codes.long() & 7] * 17)  # powers of two
+            w.codes[:, (k + 1) // 2:] = 0
+            if k % 2:
+                w.codes[:, k // 2] &= 15
+            # two planes of bf16 do not hold any of these elements
+            high = (v.float().view(torch.int32) & -65536).view(torch.float32)
+            rest = ((v.float() - high).view(torch.int32) & -65536).view(torch.float32)
+            assert bool((high + rest != v.float()).all())
+        a, v = a.cuda(), v.float().cuda()
+    want = v[:, None] * column(w, torch.arange(n, device="cuda")[None, :], at.cuda()[:, None].expand(m, n))
+    assert int((want != 0).sum()) > m * n // 2
+    assert torch.equal(ops.mxfp4_gemm_nt(ctx, a, w, dtype=torch.float32), want)
