@@ -16,6 +16,19 @@ from recpack_amd.algorithms import EASE, Algorithm, draw_uniforms, get_context, 
 CHUNK_BYTES = 1 << 30  # scores of a chunk of users on the device
 
 
+def entries_by_row(X, in_order: bool):
+    """Row pointers and column indices of the stored entries of a sparse matrix, by rows, none of them joined; ``in_order``: as they stand, which
+    is by rows in a CSR matrix only."""
+    if X.format == "csr":
+        return X.indptr, X.indices[:X.indptr[-1]]
+    if in_order:
+        raise ValueError(f"weights go with the stored entries of a CSR matrix, X is {X.format}")
+    coo = X.tocoo()
+    indptr = np.zeros(X.shape[0] + 1, dtype=np.int64)
+    np.cumsum(np.bincount(coo.row, minlength=X.shape[0]), out=indptr[1:])
+    return indptr, coo.col[np.argsort(coo.row, kind="stable")]
+
+
 class CompressedEASE(Algorithm):
     """EASE (recpack/algorithms/ease.py:19-109) whose fitted matrix is kept in MXFP4 (:mod:`recpack_amd.ops`) instead of float32.
 
@@ -111,27 +124,30 @@ class CompressedEASE(Algorithm):
 
     # ---- answers ----------------------------------------------------------------------------------------------------------------------
     def scores(self, X: sp.csr_matrix, exclude_history: bool = False, item_keep=None, weights=None, dtype=None, out=None):
-        """Scores of histories as a torch tensor [users, items] on the GPU: X @ similarity_matrix_ (base.py:248) with the entries of the CSR
-        ``X`` counted once each, or ``weights`` (one number per stored entry, in its order) times.  ``exclude_history`` / ``item_keep``: those
-        items get -inf."""
+        """Scores of histories as a torch tensor [users, items] on the GPU: X @ similarity_matrix_ (base.py:248) with the stored entries of the
+        sparse ``X`` counted once each (repeated ones as often as they stand), or ``weights`` (CSR only: one number per stored entry, in its order)
+        times.  ``exclude_history`` / ``item_keep``: those items get -inf."""
         import torch
 
         from recpack_amd import ops
 
         rows, _ = self._matrices()
+        if not sp.issparse(X):
+            raise TypeError(f"X: a scipy sparse matrix is expected, got {type(X).__name__}")
         if X.shape[1] != self.n_items_:
             raise ValueError(f"X has {X.shape[1]} items, the model {self.n_items_}")
+        indptr, indices = entries_by_row(X, weights is not None)
         ctx = get_context()
         device = f"cuda:{ctx.device}"
 
         def put(a, t):
             return torch.from_numpy(np.ascontiguousarray(a, dtype=t)).to(device)
 
-        if X.indptr[-1] > np.iinfo(np.int32).max:
+        if len(indices) > np.iinfo(np.int32).max:
             raise ValueError("more than 2^31 stored entries: pass the users in parts")
         keep = None if item_keep is None else put(np.asarray(item_keep) != 0, np.uint8)
         w = None if weights is None else put(weights, np.float32)
-        return ops.mxfp4_scores(ctx, put(X.indptr, np.int32), put(X.indices, np.int32), rows, weights=w, exclude_history=exclude_history, item_keep=keep,
+        return ops.mxfp4_scores(ctx, put(indptr, np.int32), put(indices, np.int32), rows, weights=w, exclude_history=exclude_history, item_keep=keep,
                                 dtype=dtype or torch.float32, out=out)
 
     def profile_scores(self, profiles, dtype=None):

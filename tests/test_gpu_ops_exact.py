@@ -307,3 +307,21 @@ def test_product_is_exact_in_every_tile(ctx, ops, dtype, m, n, k):
     want = v[:, None] * column(w, torch.arange(n, device="cuda")[None, :], at.cuda()[:, None].expand(m, n))
     assert int((want != 0).sum()) > m * n // 2
     assert torch.equal(ops.mxfp4_gemm_nt(ctx, a, w, dtype=torch.float32), want)
+
+
+# ---- the compressed model's inputs -------------------------------------------------------------------------------------------------------------
+
+def test_scores_of_every_sparse_format():
+    import scipy.sparse as sp
+
+    from recpack_amd import EASE
+    from recpack_amd.synth import powerlaw_csr
+
+    X = powerlaw_csr(90, 90, 0.1, seed=3).to_scipy()
+    model = EASE(l2=10.0).fit(X).compress()
+    want = model.scores(X, exclude_history=True)
+    for kind in ("csc", "coo", "lil"):
+        assert torch.allclose(model.scores(X.asformat(kind), exclude_history=True), want, rtol=1e-5, atol=1e-6)  # (entries of a row in another order)
+    assert torch.equal(model.scores(sp.csr_array(X), exclude_history=True), want)
+    with pytest.raises(ValueError, match="CSR"):
+        model.scores(X.tocsc(), weights=np.ones(X.nnz))
