@@ -2,7 +2,8 @@
 
 Every function takes the :class:`recpack_amd._lib.Context` of the tensors' device first and runs on torch's current stream of that
 device; nothing is copied to the host or waited for, so the calls can be captured into a graph.  Outputs may be given (``out=``);
-otherwise they are allocated.  There is no backward pass: a fitted model is compressed and answered from, not trained through.
+otherwise they are allocated.  There is no backward pass: a fitted model is compressed and answered from, not trained through
+(tensors that require a gradient are refused while gradients are recorded).
 """
 from __future__ import annotations
 
@@ -33,11 +34,13 @@ if hasattr(torch._C, "_cuda_getCurrentRawStream"):  # (the same value without a 
 
 
 def _on(ctx, name, t):
-    """``t`` is a tensor on the context's GPU."""
+    """``t`` is a tensor on the context's GPU that nobody expects a gradient of."""
     if not isinstance(t, torch.Tensor):
         raise TypeError(f"{name}: a torch tensor is expected, got {type(t).__name__}")
     if t.get_device() != ctx.device:
         raise ValueError(f"{name} is on {t.device}, the context on cuda:{ctx.device}")
+    if t.requires_grad and torch.is_grad_enabled():
+        raise ValueError(f"{name} requires a gradient, and there is no backward pass: detach it, or call under torch.no_grad()")
 
 
 def _type_of(name, dtype):

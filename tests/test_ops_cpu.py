@@ -111,3 +111,25 @@ def test_tensors_are_checked():
                 (torch.zeros(4, 40, dtype=torch.uint8)[:, :32], scales, 64), (torch.zeros(4, 48, dtype=torch.uint8)[:, 8:40], scales, 64)):
         with pytest.raises(ValueError):
             ops.MXFP4(*bad)
+
+
+class OnTheHost:
+    """A context whose device is the tensors' own (-1: none), for checks that come after the device's."""
+
+    device, handle, lib = -1, None, None
+
+
+def test_gradients_are_refused():
+    ctx, x, w = OnTheHost(), torch.zeros(4, 64, requires_grad=True), torch.zeros(5, requires_grad=True)
+    plain, m = torch.zeros(4, 64), ops.MXFP4(torch.zeros(64, 32, dtype=torch.uint8), torch.zeros(64, 2, dtype=torch.uint8), 64)
+    indptr, indices = torch.tensor([0, 2, 5], dtype=torch.int32), torch.zeros(5, dtype=torch.int32)
+    calls = [("x", lambda: ops.mxfp4_quantize(ctx, x)), ("x", lambda: ops.mxfp4_quantize(ctx, x * 2)), ("a", lambda: ops.mxfp4_gemm_nt(ctx, x, m)),
+             ("weights", lambda: ops.mxfp4_scores(ctx, indptr, indices, m, weights=w)), ("scores", lambda: ops.sample(ctx, x, plain[:, :1])),
+             ("temperature", lambda: ops.sample(ctx, plain, plain[:, :1], temperature=w[:4])), ("out", lambda: ops.mxfp4_dequantize(ctx, m, out=torch.zeros(64, 64, requires_grad=True)))]
+    for name, call in calls:
+        with pytest.raises(ValueError, match=f"^{name} requires a gradient"):
+            call()
+    with torch.no_grad():  # (past the check: the stand-in has no library)
+        with pytest.raises(Exception) as e:
+            ops.mxfp4_quantize(ctx, x)
+        assert "gradient" not in str(e.value)
