@@ -252,7 +252,8 @@ def sample(ctx, scores: torch.Tensor, u: torch.Tensor, temperature=1.0, top_k=0,
         if ids.dtype != torch.int32 or tuple(ids.shape) != (rows, width):
             raise ValueError(f"ids: int32 {(rows, width)} expected, got {ids.dtype} {tuple(ids.shape)}")
         ids, ld_ids = _matrix("ids", ids)
-    p = _lib.SampleParams(1.0, 1.0, 0.0, int(top_k))
+    top_k = max(-1, min(int(top_k), 2**31 - 1))  # (the library's argument has 32 bits; beyond the width it means all, below 0 it is refused)
+    p = _lib.SampleParams(1.0, 1.0, 0.0, top_k)
     keep = []  # (copies of strided settings live until the call is made)
     for name, v in (("temperature", temperature), ("top_p", top_p), ("min_p", min_p)):
         if isinstance(v, torch.Tensor):
@@ -268,7 +269,7 @@ def sample(ctx, scores: torch.Tensor, u: torch.Tensor, temperature=1.0, top_k=0,
     prob = u.new_empty((rows, draws))
     nnz = u.new_empty(rows, dtype=torch.int32)
     size = C.c_int64()
-    _lib.check(ctx.lib.rphip_sample_workspace(ctx.handle, rows, width, draws, int(top_k), C.byref(size)))
+    _lib.check(ctx.lib.rphip_sample_workspace(ctx.handle, rows, width, draws, top_k, C.byref(size)))
     ws = _scratch(size.value, scores)
     _lib.check(ctx.lib.rphip_sample(ctx.handle, _stream(ctx), rows, width, scores.data_ptr(), code, ld, _ptr(lengths), _ptr(ids), ld_ids, draws, u.data_ptr(), ldu,
                                     C.byref(p), idx.data_ptr(), prob.data_ptr(), nnz.data_ptr(), _ptr(ws), size.value))

@@ -133,3 +133,23 @@ def test_gradients_are_refused():
         with pytest.raises(Exception) as e:
             ops.mxfp4_quantize(ctx, x)
         assert "gradient" not in str(e.value)
+
+
+class Recorder:
+    """Stands in for the library: notes what it is asked for, and refuses it."""
+
+    def __init__(self):
+        self.asked = []
+
+    def rphip_sample_workspace(self, handle, rows, width, draws, top_k, size):
+        self.asked.append(top_k)
+        return _lib.RPHIP_EINVAL
+
+
+@pytest.mark.parametrize("top_k,passed", [(0, 0), (7, 7), (2**31 - 1, 2**31 - 1), (2**32 + 5, 2**31 - 1), (10**30, 2**31 - 1), (-1, -1), (5 - 2**32, -1)])
+def test_top_k_of_more_than_32_bits(top_k, passed):
+    ctx = OnTheHost()
+    ctx.lib = Recorder()
+    with pytest.raises(_lib.RecpackHipError):
+        ops.sample(ctx, torch.zeros(4, 64), torch.zeros(4, 1), top_k=top_k)
+    assert ctx.lib.asked == [passed]
