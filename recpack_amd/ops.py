@@ -96,6 +96,8 @@ class MXFP4:
     def __init__(self, codes: torch.Tensor, scales: torch.Tensor, cols: int):
         blocks = -(-int(cols) // BLOCK)
         for name, t, width in (("codes", codes, blocks * 16), ("scales", scales, blocks)):
+            if not isinstance(t, torch.Tensor):
+                raise TypeError(f"{name}: a torch tensor is expected, got {type(t).__name__}")
             if t.dtype != torch.uint8 or t.dim() != 2 or t.shape[1] != width:
                 raise ValueError(f"{name}: uint8 [rows, {width}] expected for {cols} columns, got {t.dtype} {tuple(t.shape)}")
             if not _rows_ok(t):
@@ -212,6 +214,7 @@ def mxfp4_scores(ctx, indptr: torch.Tensor, indices: torch.Tensor, w: MXFP4, wei
     uint8 [cols]): items with 0 get -inf."""
     _on(ctx, "w", w.codes)
     _on(ctx, "indptr", indptr)
+    _on(ctx, "indices", indices)
     if indptr.dim() != 1 or indptr.shape[0] < 1:
         raise ValueError(f"indptr: one dimension of users + 1 expected, got {tuple(indptr.shape)}")
     users, nnz = indptr.shape[0] - 1, indices.numel()
@@ -219,6 +222,7 @@ def mxfp4_scores(ctx, indptr: torch.Tensor, indices: torch.Tensor, w: MXFP4, wei
     if weights is not None:
         weights = _vector(ctx, "weights", weights, nnz, torch.float32)
     if item_keep is not None:
+        _on(ctx, "item_keep", item_keep)
         item_keep = _vector(ctx, "item_keep", item_keep.view(torch.uint8) if item_keep.dtype == torch.bool else item_keep, w.cols, torch.uint8)
     out, ldo, code = _output(ctx, out, users, w.cols, dtype, w.codes)
     codes, ldc, scales, lds = w._args()

@@ -153,3 +153,13 @@ def test_top_k_of_more_than_32_bits(top_k, passed):
     with pytest.raises(_lib.RecpackHipError):
         ops.sample(ctx, torch.zeros(4, 64), torch.zeros(4, 1), top_k=top_k)
     assert ctx.lib.asked == [passed]
+
+
+def test_what_is_no_tensor_is_a_type_error():
+    ctx, m = OnTheHost(), ops.MXFP4(torch.zeros(64, 32, dtype=torch.uint8), torch.zeros(64, 2, dtype=torch.uint8), 64)
+    indptr, indices = torch.tensor([0, 1], dtype=torch.int32), torch.zeros(1, dtype=torch.int32)
+    for name, call in (("indices", lambda: ops.mxfp4_scores(ctx, indptr, [0], m)), ("item_keep", lambda: ops.mxfp4_scores(ctx, indptr, indices, m, item_keep=[1] * 64)),
+                       ("weights", lambda: ops.mxfp4_scores(ctx, indptr, indices, m, weights=[1.0])), ("indptr", lambda: ops.mxfp4_scores(ctx, [0, 1], indices, m)),
+                       ("codes", lambda: ops.MXFP4([0], m.scales, 64)), ("u", lambda: ops.sample(ctx, torch.zeros(1, 4), [[0.5]]))):
+        with pytest.raises(TypeError, match=f"^{name}: a torch tensor"):
+            call()
