@@ -180,7 +180,8 @@ class CompressedEASE(Algorithm):
         return s.masked_fill_(s == 0, -np.inf)
 
     def predict_topk(self, X, K: int, exclude_history: bool = False, exclude_items=None, select_items=None) -> sp.csr_matrix:
-        """The K best scores per user, as ``ItemSimilarityMatrixAlgorithm.predict_topk`` returns them (K <= 1024 or all items)."""
+        """The K best scores per user, as ``ItemSimilarityMatrixAlgorithm.predict_topk`` returns them (K <= 1024; a small catalogue's number of items
+        takes a larger K's place)."""
         import torch
 
         from recpack_amd import ops
