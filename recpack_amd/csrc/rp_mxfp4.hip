@@ -343,7 +343,7 @@ __global__ __launch_bounds__(64 * MXS_WAVES) void k_mx_scores_sum(const int32_t*
 // The waves take groups of four entries in turn and add their sums up in wave order, however many users there are: waves that share the
 // columns out instead convert as much and address four times as many rows (251 histories of 100 against 20000 x 20000: 72 us); one wave alone is
 // a little faster where there are many users (1024 histories of 50 against 50000 x 50000: 257 us, 274 so), and sums in another order.
-// Bound by the gathered pieces: 251 histories of 100 against 20000 x 20000 in bf16 47 us, 266 MB at 5.6 TB/s (117 MB of rows are different ones, but
+// Bound by the gathered pieces: 251 histories of 100 against 20000 x 20000 in bf16 48 us, 266 MB at 5.5 TB/s (117 MB of rows are different ones, but
 // an XCD meets a row again when its L2 has long seen others).
 template <class T>
 __global__ __launch_bounds__(64 * MXS_WAVES) void k_mx_scores_weighted(const int32_t* __restrict__ indptr, const int32_t* __restrict__ indices, const float* __restrict__ weights,

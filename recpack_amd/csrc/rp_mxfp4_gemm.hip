@@ -401,8 +401,10 @@ __global__ __launch_bounds__(WM * WN * 64) void k_mxg_bf16(gemm_args g) {
 
 // 4-bit form: codes of both operands in two slots, a stage (two chunks of both) ahead; scales in two slots of four chunks.  A piece is
 // eight rows of 128 bytes: 64 bytes a row and chunk fetched every cache line twice (1.16 -> 0.98 ms at 4096 x 20000 x 20000).  Bound by
-// the operands' way into LDS: a CU takes 64 KB a stage in 2.1 us, where its matrix instructions take 0.9 (3.8 PF there; 128 x 256 tiles three
-// stages deep, half again the bytes, are 17 % slower).
+// how little its two halves overlap: two normal matrices, quantised, 4096 x 20000 x 20000 take 917 us with the scales' packing; without the
+// requests, so matrix instructions and the reads of LDS alone, 726; requests and reads without matrix instructions 668; every stage from one
+// panel that stays in the L2 827.  The matrix pipe is busy in half of the cycles: a stage's requests are waited for completely, one stage after they were made.
+// (128 x 256 tiles three stages deep, half again the bytes: 17 % slower.)
 template <class OT, int BM, int BN, int WM, int WN>
 __global__ __launch_bounds__(WM * WN * 64) void k_mxg_fp4(gemm_args g) {
   constexpr int WAVES = WM * WN, TM = BM / WM / 16, TN = BN / WN / 16;
@@ -867,7 +869,8 @@ plan make_plan(int n_cu, int64_t M, int64_t N, int64_t K, int32_t a_type) {
   p.half = a_type == RPHIP_F16;
   p.nc = (int)rp_cdiv(K, KC);
   p.nq = (int)rp_cdiv(p.nc, 4);
-  // the vector unit's form: f32 104 us against 118 at M = 4, 16 bits 72 against 90 to 108 at M = 2 (but 105 to 116 against 89 to 108 at 3)
+  // the vector unit's form: f32 99 us against 118 at M = 4, 16 bits 73 against 91 (bf16) and 108 (f16) at M = 2 (but 108 against 90 and 106 against 107
+  // at 3)
   p.rows = p.planes != 0 && M <= (p.planes == 3 ? 4 : 2) && K > 0;
   if (p.rows) return p;
   // small products, by tiles and by what a tile's latency comes to: f32 97 x 1999 x 2003 13.7 us against 20.2, bf16 256 x 2000 x 2000 16.5
@@ -889,7 +892,7 @@ plan make_plan(int n_cu, int64_t M, int64_t N, int64_t K, int32_t a_type) {
       p.bn = 256;
       p.bm = p.planes == 3 || hundredths(128, 256) * 57 < hundredths(256, 256) * 100 ? 128 : 256;
     } else if (M > 64 && tiles(128, 128) * steps >= 40000) {
-      p.bm = 128, p.bn = 128, per_cu = 5;  // (M = 128: 157 us in eight parts, 199 with 64 x 64 tiles; 1000 x 3000 x 3000: 39 against 36)
+      p.bm = 128, p.bn = 128, per_cu = 5;  // (bf16, M = 128: 160 us in eight parts, 202 with 64 x 64 tiles; 1000 x 3000 x 3000, 64 x 64: 37)
     } else {
       p.bm = 64, p.bn = 64, per_cu = 4;
     }

@@ -457,8 +457,8 @@ __device__ __forceinline__ void rank_keys(const uint32_t (&key)[PER], unsigned l
   __builtin_amdgcn_wave_barrier();
 }
 
-// One wave per row: up to 64 * PER scores in registers, sorted there.  Bound by the vector unit: 8192 rows of 200, ten draws, 24 us, of which
-// the draws are 6; the bytes would take 3.  8192 rows of 1000 (PER = 16), twenty draws: 107 us.
+// One wave per row: up to 64 * PER scores in registers, sorted there.  Bound by the vector unit, which is busy in 92 % of the cycles: 8192 rows of 200, ten
+// draws, 24 us, of which the draws are 6; the bytes would take 3.  8192 rows of 1000 (PER = 16), twenty draws: 107 us.
 template <class T, int PER>
 __global__ __launch_bounds__(256) void k_sample_wave(sample_args a) {
   __shared__ unsigned long long sorted[4][64 * PER];
@@ -1648,7 +1648,7 @@ __global__ __launch_bounds__(SL_THREADS) void k_row_draw(sample_args a, const ro
 }
 
 // ... all of it in one launch, a workgroup to a row, its workspace in LDS (151 KB with the draw's: one to a CU).  Bound by the vector unit (some 25 instructions
-// in 64 bits a score and the LDS atomics) and by what one workgroup has under way: 512 rows of 100000 in f32 164 us, where reading them takes 43.
+// in 64 bits a score and the LDS atomics) and by what one workgroup has under way: 512 rows of 100000 in f32 165 us, where reading them takes 43.
 struct one_shared {
   row_ws ws;
   draw_shared draw;
@@ -1731,8 +1731,8 @@ __global__ __launch_bounds__(SL_THREADS) void k_row_one(sample_args a, int shift
 // which form a call takes, and its workspace
 enum sample_form { FORM_WAVE, FORM_LISTS, FORM_ROWS };
 sample_form form_of(int64_t width, int64_t k) { return width <= RPS_SHORT ? FORM_WAVE : k <= RPS_SHORT ? FORM_LISTS : FORM_ROWS; }
-// One workgroup to a row and launch, or slices of few wide rows over the card: 1 x 12000 20 us against 28, 256 x 12000 23 against 56, 64 x 50000 42
-// against 58, 512 x 100000 156 against 190; but 1 x 50000 37 against 28 and 16 x 100000 65 against 41 (f32).
+// One workgroup to a row and launch, or slices of few wide rows over the card: 1 x 12000 20 us against 26, 256 x 12000 22 against 61, 64 x 50000 42
+// against 62, 512 x 100000 165 against 198; but 1 x 50000 37 against 25 and 16 x 100000 67 against 43 (f32).
 bool one_launch(int64_t rows, int64_t width) { return width <= 20000 || rows >= 64; }
 int64_t workspace_of(int64_t rows, int64_t width, int64_t k) {
   switch (form_of(width, k)) {
@@ -1823,8 +1823,8 @@ extern "C" int rphip_sample(rphip_ctx* ctx, void* stream, int64_t rows, int64_t 
           RP_LAUNCHED();
           k_row_hist<T, COUNT><<<dim3(n, slices), SR_THREADS, 0, st>>>(a, ws, shift);
           RP_LAUNCHED();
-          // very few rows: a launch (3 - 4 us) costs more than finding the bins in every slice (one row of 100000: 25.6 us against 28.4; 16 rows 46
-          // against 42)
+          // very few rows: a launch (3 - 4 us) costs more than finding the bins in every slice (one row of 100000: 25.2 us against 26.5; 8 rows the same,
+          // 16 rows 44 against 42)
           if (n <= 8) {
             k_row_collect<T, COUNT, true><<<dim3(n, slices), SR_THREADS, 0, st>>>(a, ws, slices, shift);
           } else {
