@@ -325,3 +325,96 @@ def test_scores_of_every_sparse_format():
     assert torch.equal(model.scores(sp.csr_array(X), exclude_history=True), want)
     with pytest.raises(ValueError, match="CSR"):
         model.scores(X.tocsc(), weights=np.ones(X.nnz))
+
+
+# ---- calls that other tests do not make ------------------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("rows,width", [(1, 100_000), (3, 30_001), (20, 30_001), (70, 5_000)])
+@pytest.mark.parametrize("top_k", [0, 2000])
+def test_draws_from_long_prefixes_captured(ctx, ops, rows, width, top_k):
+    """Every form of the whole-row draw in a graph, replayed on other scores, settings and uniforms."""
+    x, u = torch.empty(rows, width, device="cuda"), torch.empty(rows, 1, device="cuda")
+    t, p, m = (torch.empty(rows, device="cuda") for _ in range(3))
+
+    def fill(turn):
+        g = gen(turn)
+        x.copy_(torch.randn(rows, width, generator=g) * (1 + 5 * turn))
+        if turn == 2:
+            x[0] = -math.inf  # (a row without candidates, after rows with some)
+        for v, lo, size in ((u, 0.0, 1.0), (t, 0.3, 1.0), (p, 0.5, 0.5), (m, 0.0, 1e-3)):
+            v.copy_(torch.rand(v.shape, generator=g) * size + lo)
+        u.clamp_(max=1 - 2.0 ** -24)
+
+    def call():
+        return ops.sample(ctx, x, u, temperature=t, top_k=top_k, top_p=p, min_p=m)
+
+    fill(0)
+    call()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = call()
+    for turn in range(5):
+        fill(turn)
+        want = [v.clone() for v in call()]
+        for v in out:
+            v.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        for a, b in zip(out, want):
+            assert torch.equal(a, b)
+
+
+def test_scores_captured_with_other_histories(ctx, ops):
+    """Row pointers are read when the graph runs: shorter, longer and empty histories in the same buffers."""
+    items, users, room = 3000, 40, 4000
+    w = wide_mxfp4(ops, items, items, 1, 117, 126)
+    indptr, indices, weights = torch.zeros(users + 1, dtype=torch.int32, device="cuda"), torch.zeros(room, dtype=torch.int32, device="cuda"), torch.zeros(room, device="cuda")
+
+    def call():
+        return [ops.mxfp4_scores(ctx, indptr, indices, w, exclude_history=True), ops.mxfp4_scores(ctx, indptr, indices, w, weights=weights, dtype=torch.bfloat16)]
+
+    call()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = call()
+    for turn in range(4):
+        g = gen(turn)
+        counts = torch.randint(0, (1, 30, 100, 2)[turn], (users,), generator=g)
+        indptr[1:] = counts.cumsum(0).cuda()
+        indices.copy_(torch.randint(0, items, (room,), generator=g, dtype=torch.int32))
+        weights.copy_(torch.randn(room, generator=g))
+        want = [v.clone() for v in call()]
+        for v in out:
+            v.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        for a, b in zip(out, want):
+            assert torch.equal(a, b)
+
+
+def test_scores_without_entries(ctx, ops):
+    w = wide_mxfp4(ops, 700, 700, 2, 117, 126)
+    none = torch.zeros(0, dtype=torch.int32, device="cuda")
+    keep = torch.arange(700, device="cuda") % 3 > 0
+    for weights in (None, torch.zeros(0, device="cuda")):
+        got = ops.mxfp4_scores(ctx, torch.zeros(6, dtype=torch.int32, device="cuda"), none, w, weights=weights, exclude_history=True, item_keep=keep)
+        assert bool((got[:, keep] == 0).all()) and bool(torch.isneginf(got[:, ~keep]).all())
+
+
+def test_products_on_two_streams_at_once(ctx, ops):
+    """Two products of different plans and the draws of long prefixes under way together: each has its own scratch memory."""
+    w = wide_mxfp4(ops, 9000, 5000, 3, 117, 126)
+    a = [torch.randn(m, 5000, generator=gen(m)).cuda() for m in (60, 300)]
+    x, u = torch.randn(4, 60_000, generator=gen(9)).cuda(), torch.rand(4, 1, generator=gen(8)).cuda()
+    calls = [lambda: ops.mxfp4_gemm_nt(ctx, a[0], w), lambda: ops.mxfp4_gemm_nt(ctx, a[1].half(), w), lambda: ops.sample(ctx, x, u, top_p=0.9)[0]]
+    want = [c().clone() for c in calls]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in calls]
+    got = []
+    for _ in range(5):
+        for s, c in zip(streams, calls):
+            with torch.cuda.stream(s):
+                got.append(c())
+    torch.cuda.synchronize()
+    for i, v in enumerate(got):
+        assert torch.equal(v, want[i % len(calls)])
